@@ -269,6 +269,101 @@ int ltx_op_attention(ltx_ctx* ctx, const void* q, const void* k, const void* v, 
 int ltx_op_dequant(ltx_ctx* ctx, const int8_t* q, const void* scales, int scale_f16, int N, int K, float* out32,
                    void* out16, int mode, void* stream);
 
+/* No counterpart in the reference. ltx_op_linear_q8 with 4-bit weights, for few
+ * rows (the projections of single tokens): y[M][N] = a[M][K] . (q s)^T (+ bias)
+ * with optional GELU-tanh. q [N][K / 2]: two weights a byte, the even k in the
+ * low nibble, two's complement (-8 .. 7); scales [N][K / 128] f32 or f16. Modes
+ * F16 and BF16: a 16-bit, y f32 (out_f32) or 16-bit; F32: a and y f32, a taken as
+ * three exact bf16 planes. The weights are exact operands, a group's scale
+ * multiplies its f32 sum. No scratch: calls may overlap and be captured. Refused:
+ * M, N or K not positive, K no multiple of 128, a or q not on 16 bytes, scales,
+ * bias or y not aligned to their types, an unknown mode, more than 1,048,560 rows. */
+int ltx_op_linear_q4(ltx_ctx* ctx, const void* a, const uint8_t* q, const void* scales, int scale_f16,
+                     const float* bias, void* y, int out_f32, int M, int N, int K, int gelu, int mode,
+                     void* stream);
+
+/* ---- a key/value cache in 4 bits ---------------------------------------- */
+
+/* No counterpart in the reference: for streamed generation, where the keys and
+ * values of earlier frames or tokens stay for every block. A cache is a pool of
+ * `pages` pages of LTX_KV_PAGE_TOKENS tokens, each with `kv_heads` heads of
+ * LTX_HEAD_DIM dims of k and of v, 136 bytes a token and head (512 in 16 bits).
+ * Which page holds which tokens of which sequence is the caller's page table.
+ *
+ * Form: 32 consecutive dims share a power of two 2^e and are held as e2m1
+ * numbers (0, 0.5, 1, 1.5, 2, 3, 4, 6, signed), x / 2^e rounded to the nearest,
+ * ties to the even code, beyond 6 to 6. With A the group's largest magnitude, e =
+ * floor(log2 A) - 2, one more where A > 7 2^e, limited to -23 .. 13 (mode F16) or
+ * -125 .. 125 (BF16), so that what a code stands for is a number of the mode's
+ * type. A group with a value that is not finite reads back as NaN.
+ *
+ * `mode` (LTX_MODE_F16 or LTX_MODE_BF16) is the type of k, v, q and the outputs of
+ * every call on the cache. Pages start as zeros. */
+#define LTX_KV_PAGE_TOKENS 64
+typedef struct ltx_kv_cache ltx_kv_cache;
+int ltx_kv_cache_create(ltx_ctx* ctx, int mode, int kv_heads, int pages, ltx_kv_cache** out);
+/* Waits for the device; before the context is destroyed. */
+void ltx_kv_cache_free(ltx_ctx* ctx, ltx_kv_cache* cache);
+/* Device bytes held by the cache. */
+uint64_t ltx_kv_cache_bytes(const ltx_kv_cache* cache);
+
+/* The sequences of a call. row_start, kv_len and pages are device memory, read
+ * when the call runs: a captured call follows what they hold at each replay.
+ * Sequence b has rows row_start[b] .. row_start[b + 1] - 1 of the call's k, v, q
+ * and out (row_start NULL: row b alone, rows == nseq) and kv_len[b] keys in all;
+ * its n rows are the last n of these positions, and position p lies in row p % 64
+ * of page pages[b * max_pages + p / 64]. row_start ascends from 0 on within 0 ..
+ * rows; kv_len is taken as at most 64 max_pages. Rows behind the last sequence are
+ * left as they were, and so are the cache's other rows. A page index outside the
+ * pool is not followed: the row is not written, or read as zeros, or the page's
+ * keys take no part in the attention, and it is counted (ltx_kv_cache_faults).
+ * The host checks what it can see: nseq and max_pages (at most 2^24) positive,
+ * rows not negative (0: nothing to do), pointers, heads, and that rows of k, v, q
+ * and out start on 16 bytes with strides (in elements) that are multiples of 8 and
+ * not shorter than a row. */
+typedef struct ltx_kv_batch {
+    int nseq, rows;
+    const int32_t* row_start;
+    const int32_t* kv_len;
+    const int32_t* pages;
+    int max_pages;
+} ltx_kv_batch;
+
+/* The count of bad pages (once a row in ltx_op_kv_write and ltx_op_kv_read, once a
+ * page and tile of rows in ltx_op_kv_attention) since creation or the last reset.
+ * Waits for `stream`. */
+int ltx_kv_cache_faults(ltx_ctx* ctx, ltx_kv_cache* cache, void* stream, uint64_t* count, int reset);
+
+/* Quantises the batch's rows of k and v [rows][kv_heads * 128] (ldk and ldv
+ * elements apart: slices of fused q|k|v rows will do) to their positions. Rows at
+ * positions below 0 (more rows than keys) are left out. Two rows of one call on one
+ * place (a page twice in the table) leave a mixture of the two there. */
+int ltx_op_kv_write(ltx_ctx* ctx, ltx_kv_cache* cache, const ltx_kv_batch* batch, const void* k, int64_t ldk,
+                    const void* v, int64_t ldv, void* stream);
+/* What the cache holds of the batch's rows, as the mode's type (row_start with
+ * n = kv_len reads whole sequences). Rows at positions below 0 read as zeros. */
+int ltx_op_kv_read(ltx_ctx* ctx, const ltx_kv_cache* cache, const ltx_kv_batch* batch, void* k, int64_t ldk, void* v,
+                   int64_t ldv, void* stream);
+
+/* Attention of the batch's rows over their sequences' keys in the cache (write
+ * the rows' own k and v first): q and out [rows][heads * 128], query head j on the
+ * cached head j / (heads / kv_heads); scores q . k / sqrt(128); causal: a row sees
+ * the keys up to its own position, else all kv_len; glog [rows][heads] f32 or NULL,
+ * the gate of ltx_op_attention. A row that sees no key gives zeros; a row that
+ * sees a token with a value of v (or k) that is not finite in that head gives NaN,
+ * and one that does not is untouched by it. f32 statistics and sums, weights
+ * rounded to 16 bits. Results do not depend on other calls' timing.
+ * Keys are split over workgroups, whose partial results lie in `work`: device
+ * memory of ltx_op_kv_attention_workspace bytes (for the batch's nseq, rows and
+ * max_pages), not used by two calls at once; for calls that are captured. NULL:
+ * scratch of the context, as in ltx_op_attention (a call being captured, or one
+ * that finds no memory, does not split). */
+int ltx_op_kv_attention_workspace(ltx_ctx* ctx, const ltx_kv_cache* cache, const ltx_kv_batch* batch, int heads,
+                                  uint64_t* bytes);
+int ltx_op_kv_attention(ltx_ctx* ctx, const ltx_kv_cache* cache, const ltx_kv_batch* batch, const void* q,
+                        int64_t ldq, int heads, int causal, const float* glog, void* out, int64_t ldo, void* work,
+                        uint64_t work_bytes, void* stream);
+
 /* ---- host utilities ---------------------------------------------------- */
 
 /* 3D RoPE tables, host f64 (ltx/block_conformance.zig:87-126). grid

@@ -1,0 +1,199 @@
+// The 4-bit key/value cache: its handle, rows written and read back, attention.
+#include <cstring>
+
+#include "ltx_internal.hpp"
+
+struct ltx_kv_cache {
+    int device = 0, mode = 0, kv_heads = 0, pages = 0;
+    // blocks [pages][kv_heads], then the count of bad pages, then a flag a page
+    ltx::DevBuf buf;
+    size_t blocks = 0;
+    uint8_t* data() const { return (uint8_t*)buf.p; }
+    unsigned long long* bad() const { return (unsigned long long*)((char*)buf.p + blocks); }
+    uint32_t* flags() const { return (uint32_t*)((char*)buf.p + blocks + 256); }
+};
+
+namespace ltx {
+namespace {
+
+constexpr int kTile = 16;          // columns of an item (k_kv.hip)
+constexpr int kLeastPages = 4;     // pages of a run, at least
+constexpr int kTargetItems = 1024; // items of all cached heads that a call aims at: four workgroups a CU
+constexpr int kMaxPages = 1 << 24; // of a table: positions stay in 31 bits
+
+// Checks of a batch that need no device value; rows == 0 is an empty call.
+LtxKvBatchArgs batch_args(const ltx_ctx* c, const ltx_kv_cache* k, const ltx_kv_batch* b) {
+    if (!k || !b) throw Error("NULL argument");
+    if (k->device != c->device) throw Error("the cache is on another device than the context");
+    if (b->nseq <= 0 || b->rows < 0) throw Error("bad batch: nseq must be positive, rows not negative");
+    if (b->max_pages <= 0 || b->max_pages > kMaxPages) throw Error("bad batch: max_pages must be 1 .. 2^24");
+    if (!b->kv_len || !b->pages) throw Error("bad batch: kv_len and pages are needed");
+    if (!b->row_start && b->rows != b->nseq) throw Error("bad batch: without row_start, rows must equal nseq");
+    return LtxKvBatchArgs{k->data(), k->flags(), k->bad(),     b->row_start, b->kv_len,
+                          b->pages,  b->nseq,    b->rows, b->max_pages, k->pages, k->kv_heads};
+}
+
+void check_rows(const void* p, int64_t ld, int width, int rows, const char* what) {
+    if (rows == 0) return;
+    if (!p) throw Error(std::string(what) + " is NULL");
+    if (ld < width || ld % 8 || ((uintptr_t)p & 15))
+        throw Error(std::string(what) + ": rows must start on 16 bytes and be at least as long as their values");
+}
+
+// One launch over the rows: `write` or read.
+void kv_rows(ltx_ctx* c, const ltx_kv_cache* k, const ltx_kv_batch* b, void* kp, int64_t ldk, void* vp, int64_t ldv,
+             bool write, hipStream_t st) {
+    LtxKvRowsArgs a{batch_args(c, k, b), kp, vp, ldk, ldv};
+    const int width = k->kv_heads * LTX_HD;
+    check_rows(kp, ldk, width, b->rows, "k");
+    check_rows(vp, ldv, width, b->rows, "v");
+    if (b->rows == 0) return;
+    HIPC(hipSetDevice(c->device));
+    const bool f16 = k->mode == LTX_MODE_F16;
+    c->launch(write ? (f16 ? "ltx_kv_write_f16" : "ltx_kv_write_bf16") : (f16 ? "ltx_kv_read_f16" : "ltx_kv_read_bf16"),
+              (unsigned)(((size_t)b->rows + 15) / 16), k->kv_heads, 1, 256, &a, st);
+}
+
+struct AttnPlan {
+    int slots = 0, items = 0;
+    size_t bytes = 0;  // of partial results
+};
+
+AttnPlan attn_plan(const ltx_kv_cache* k, const ltx_kv_batch* b, int heads, bool split) {
+    const int64_t group = heads / k->kv_heads;
+    const int64_t tiles = (int64_t)b->rows * group / kTile + b->nseq;
+    AttnPlan p;
+    if (split && b->max_pages > kLeastPages) p.slots = (kTargetItems + k->kv_heads - 1) / k->kv_heads;
+    // the grids' limit, 2^32 threads along x
+    if (tiles + p.slots >= 1 << 24 || b->rows >= 1 << 24) throw Error("too many rows for one call");
+    p.items = (int)(tiles + p.slots);
+    if (p.slots) p.bytes = (size_t)p.items * k->kv_heads * kTile * (LTX_HD + 2) * sizeof(float);
+    return p;
+}
+
+void check_heads(const ltx_kv_cache* k, int heads) {
+    if (heads <= 0 || heads % k->kv_heads) throw Error("heads must be a positive multiple of the cache's");
+    if (heads > 65535) throw Error("heads must be at most 65535");
+}
+
+}  // namespace
+}  // namespace ltx
+
+extern "C" {
+
+int ltx_kv_cache_create(ltx_ctx* c, int mode, int kv_heads, int pages, ltx_kv_cache** out) {
+    LTX_GUARD(c, {
+        if (!c || !out) throw ltx::Error("NULL argument");
+        *out = nullptr;
+        if (mode != LTX_MODE_F16 && mode != LTX_MODE_BF16)
+            throw ltx::Error("a 4-bit cache has a 16-bit mode, F16 or BF16");
+        if (kv_heads <= 0 || kv_heads > 65535 || pages <= 0) throw ltx::Error("bad cache shape");
+        if ((int64_t)pages * LTX_KV_PAGE > 0x7fffffff) throw ltx::Error("a cache holds at most 2^25 - 1 pages");
+        HIPC(hipSetDevice(c->device));
+        ltx_kv_cache* k = new ltx_kv_cache();
+        try {
+            k->device = c->device;
+            k->mode = mode;
+            k->kv_heads = kv_heads;
+            k->pages = pages;
+            k->blocks = (size_t)pages * kv_heads * LTX_KV_BLOCK;
+            k->buf.alloc(k->blocks + 256 + (size_t)pages * 4);
+            // zeros: no page holds a code of a non-finite value before it is written
+            HIPC(hipMemset(k->buf.p, 0, k->buf.bytes));
+        } catch (...) {
+            delete k;
+            throw;
+        }
+        *out = k;
+    })
+}
+
+void ltx_kv_cache_free(ltx_ctx* c, ltx_kv_cache* k) {
+    if (!k) return;
+    (void)hipSetDevice(k->device);
+    (void)hipDeviceSynchronize();
+    (void)c;
+    delete k;
+}
+
+uint64_t ltx_kv_cache_bytes(const ltx_kv_cache* k) { return k ? k->buf.bytes : 0; }
+
+int ltx_kv_cache_faults(ltx_ctx* c, ltx_kv_cache* k, void* stream, uint64_t* count, int reset) {
+    LTX_GUARD(c, {
+        if (!c || !k || !count) throw ltx::Error("NULL argument");
+        HIPC(hipSetDevice(c->device));
+        HIPC(hipStreamSynchronize((hipStream_t)stream));
+        unsigned long long v = 0;
+        HIPC(hipMemcpy(&v, k->bad(), sizeof(v), hipMemcpyDeviceToHost));
+        *count = v;
+        if (reset) {
+            v = 0;
+            HIPC(hipMemcpy(k->bad(), &v, sizeof(v), hipMemcpyHostToDevice));
+        }
+    })
+}
+
+int ltx_op_kv_write(ltx_ctx* c, ltx_kv_cache* cache, const ltx_kv_batch* batch, const void* k, int64_t ldk,
+                    const void* v, int64_t ldv, void* stream) {
+    LTX_GUARD(c, {
+        if (!c) throw ltx::Error("NULL context");
+        ltx::kv_rows(c, cache, batch, (void*)k, ldk, (void*)v, ldv, true, (hipStream_t)stream);
+    })
+}
+
+int ltx_op_kv_read(ltx_ctx* c, const ltx_kv_cache* cache, const ltx_kv_batch* batch, void* k, int64_t ldk, void* v,
+                   int64_t ldv, void* stream) {
+    LTX_GUARD(c, {
+        if (!c) throw ltx::Error("NULL context");
+        ltx::kv_rows(c, cache, batch, k, ldk, v, ldv, false, (hipStream_t)stream);
+    })
+}
+
+int ltx_op_kv_attention_workspace(ltx_ctx* c, const ltx_kv_cache* cache, const ltx_kv_batch* batch, int heads,
+                                  uint64_t* bytes) {
+    LTX_GUARD(c, {
+        if (!c || !bytes) throw ltx::Error("NULL argument");
+        ltx::batch_args(c, cache, batch);
+        ltx::check_heads(cache, heads);
+        *bytes = ltx::attn_plan(cache, batch, heads, true).bytes;
+    })
+}
+
+int ltx_op_kv_attention(ltx_ctx* c, const ltx_kv_cache* cache, const ltx_kv_batch* batch, const void* q, int64_t ldq,
+                        int heads, int causal, const float* glog, void* out, int64_t ldo, void* work,
+                        uint64_t work_bytes, void* stream) {
+    LTX_GUARD(c, {
+        if (!c) throw ltx::Error("NULL context");
+        LtxKvAttnArgs a{};
+        a.b = ltx::batch_args(c, cache, batch);
+        ltx::check_heads(cache, heads);
+        ltx::check_rows(q, ldq, heads * LTX_HD, batch->rows, "q");
+        ltx::check_rows(out, ldo, heads * LTX_HD, batch->rows, "out");
+        if ((uintptr_t)work & 15) throw ltx::Error("work must start on 16 bytes");
+        ltx::AttnPlan p = ltx::attn_plan(cache, batch, heads, true);
+        if (work && work_bytes < p.bytes) throw ltx::Error("work is smaller than ltx_op_kv_attention_workspace says");
+        if (batch->rows == 0) return LTX_OK;
+        HIPC(hipSetDevice(c->device));
+        hipStream_t st = (hipStream_t)stream;
+        ltx::ScratchUse use(c->op_scratch, st);
+        if (p.bytes && !work && !(work = use.take(p.bytes))) p = ltx::attn_plan(cache, batch, heads, false);
+        a.q = q;
+        a.out = out;
+        a.glog = glog;
+        a.part = (float*)work;
+        a.ldq = ldq;
+        a.ldo = ldo;
+        a.heads = heads;
+        a.group = heads / cache->kv_heads;
+        a.causal = causal != 0;
+        a.slots = p.slots;
+        a.items = p.items;
+        a.scale_log2 = 0.12751743f;  // log2(e) / sqrt(128)
+        const bool f16 = cache->mode == LTX_MODE_F16;
+        c->launch(f16 ? "ltx_kv_attn_f16" : "ltx_kv_attn_bf16", p.items, cache->kv_heads, 1, 256, &a, st);
+        if (p.slots)
+            c->launch(f16 ? "ltx_kv_join_f16" : "ltx_kv_join_bf16", batch->rows, (heads + 3) / 4, 1, 256, &a, st);
+    })
+}
+
+}  // extern "C"

@@ -1,0 +1,499 @@
+// A key/value cache held in 4 bits: rows written into it, read back, and
+// attended to.
+//
+// Form. Groups of 32 dims of a row and head share a power of two 2^e, their
+// values are e2m1 numbers (0, 0.5, 1, 1.5, 2, 3, 4, 6, signed). With A the
+// largest magnitude of the group, e = floor(log2 A) - 2, one more where A > 7 2^e
+// (what rounds past 6): 19.0 dB of signal to noise on normal values, against 18.8
+// without that step. Both are limited so that 0.5 2^e and 6 2^e are finite numbers
+// of the cache's 16-bit type: every code then stands for a value that type holds
+// exactly, and gfx950's conversions (v_cvt_scalef32_pk_f16_fp4 and _bf16_fp4, one
+// instruction a pair) give the MFMA operands without a rounding. They read only
+// the scale's exponent bits, so a scale byte anywhere in a word becomes one with a
+// single shift. A group that holds a non-finite value has scale code 255, which
+// they turn into NaN.
+#include <type_traits>
+
+#include "ltx_device.h"
+#include "ltx_kv_index.h"
+
+template <typename T>
+struct Fp4;
+template <>
+struct Fp4<_Float16> {
+    static constexpr int lo = 127 - 23, hi = 127 + 13;
+    template <int B>
+    static __device__ __forceinline__ uint32_t pair(uint32_t w, float s) {
+        return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, s, B));
+    }
+};
+template <>
+struct Fp4<__bf16> {
+    static constexpr int lo = 127 - 125, hi = 127 + 125;
+    template <int B>
+    static __device__ __forceinline__ uint32_t pair(uint32_t w, float s) {
+        return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, s, B));
+    }
+};
+
+// The scale whose code is byte i of w, as the conversions read it: the code at
+// bits 30 .. 23 (the bits around it take no part).
+__device__ __forceinline__ float scale_of(uint32_t w, int i) {
+    return __builtin_bit_cast(float, i == 0 ? w << 23 : i == 1 ? w << 15 : i == 2 ? w << 7 : w >> 1);
+}
+
+// ---- the batch ----------------------------------------------------------------
+// The sequences of rows row0 .. row0 + 3, each lane that of row0 + sub (nseq or
+// more: of none). All 64 lanes call it with one row0.
+__device__ __forceinline__ int kv_find(const LtxKvBatchArgs& a, int row0, int sub) {
+    if (!a.row_start) return row0 + sub;
+    const int lane = threadIdx.x & 63;
+    int b = 0;
+    for (int base = 0; base < a.nseq; base += 64) {
+        const int e = base + lane < a.nseq ? a.row_start[base + lane + 1] : 0x7fffffff;
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            const int c = __popcll(__builtin_amdgcn_ballot_w64(e <= row0 + j));
+            if (j == sub) b += c;
+        }
+    }
+    return b;
+}
+
+// The block of (row's position, head), and its key within the page; NULL where the
+// row is in no sequence, before the first position, or on no page of the pool.
+__device__ __forceinline__ uint8_t* kv_place(const LtxKvBatchArgs& a, int row, int b, int head, int& key) {
+    if (row >= a.rows || b >= a.nseq) return nullptr;
+    const int pos = kv_position(kv_seq(a, b), row);
+    if (pos < 0) return nullptr;
+    const int page = kv_page(a, b, pos / LTX_KV_PAGE);
+    if (!kv_in_pool(a, page)) {
+        if (head == 0 && (threadIdx.x & 15) == 0) atomicAdd(a.bad, 1ull);
+        return nullptr;
+    }
+    key = pos % LTX_KV_PAGE;
+    return a.data + kv_block(a, page, head);
+}
+
+__device__ __forceinline__ uint32_t quad_max(uint32_t x) {  // over lanes 4 j .. 4 j + 3
+    x = max(x, (uint32_t)__builtin_amdgcn_mov_dpp((int)x, 0xB1, 0xf, 0xf, true));
+    return max(x, (uint32_t)__builtin_amdgcn_mov_dpp((int)x, 0x4E, 0xf, 0xf, true));
+}
+
+// Eight consecutive dims of a row -> their codes, and the scale code of their
+// group (four lanes hold its 32 dims).
+template <typename T>
+__device__ __forceinline__ uint32_t kv_encode(u32x4 w, uint32_t& code) {
+    float x[8];
+    uint32_t top = 0;
+#pragma unroll
+    for (int e = 0; e < 8; e++) {
+        x[e] = Op<T>::to_f32((uint16_t)(w[e >> 1] >> (16 * (e & 1))));
+        top = max(top, __builtin_bit_cast(uint32_t, x[e]) & 0x7fffffffu);
+    }
+    top = quad_max(top);
+    const int e = (int)(top >> 23) - 2 + ((top & 0x7fffffu) > 0x600000u ? 1 : 0);
+    code = top >= 0x7f800000u ? 255u : (uint32_t)min(max(e, Fp4<T>::lo), Fp4<T>::hi);
+    if (code == 255u) return 0u;
+    const float s = __builtin_bit_cast(float, code << 23);
+    uint32_t q = 0;
+    q = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(q, x[0], x[1], s, 0);
+    q = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(q, x[2], x[3], s, 1);
+    q = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(q, x[4], x[5], s, 2);
+    q = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(q, x[6], x[7], s, 3);
+    return q;
+}
+
+// Rows into the cache and out of it: a wave takes four rows of a head, 16 lanes of
+// eight dims each. Four positions of a quad are 256 consecutive bytes of V codes.
+template <typename T, bool WRITE>
+__device__ void kv_rows(const LtxKvRowsArgs& a) {
+    const int lane = threadIdx.x & 63, o = lane & 15, sub = lane >> 4;
+    const int row0 = 4 * (4 * blockIdx.x + (threadIdx.x >> 6)), row = row0 + sub, head = blockIdx.y;
+    const int b = kv_find(a.b, row0, sub);
+    int key = 0;
+    uint8_t* blk = kv_place(a.b, row, b, head, key);
+    const int t = key >> 4, r = key & 15;
+    uint16_t* k = (uint16_t*)a.k + (size_t)row * a.ldk + head * LTX_HD + 8 * o;
+    uint16_t* v = (uint16_t*)a.v + (size_t)row * a.ldv + head * LTX_HD + 8 * o;
+    const uint32_t ck = 1024 * t + 64 * r + 4 * o, sk = LTX_KV_KS + 16 * r + 4 * (o >> 2) + t;
+    const uint32_t cv = LTX_KV_V + 1024 * t + 16 * (16 * (r >> 2) + o) + 4 * (r & 3);
+    const uint32_t sv = LTX_KV_VS + 64 * (o >> 2) + 16 * (r >> 2) + 4 * t + (r & 3);
+    if (WRITE) {
+        const u32x4 zero = {0, 0, 0, 0};
+        const u32x4 wk = blk ? *(const u32x4*)k : zero, wv = blk ? *(const u32x4*)v : zero;
+        uint32_t ek, ev;
+        const uint32_t qk = kv_encode<T>(wk, ek), qv = kv_encode<T>(wv, ev);
+        if (!blk) return;
+        *(uint32_t*)(blk + ck) = qk;
+        *(uint32_t*)(blk + cv) = qv;
+        if ((o & 3) == 0) {
+            blk[sk] = (uint8_t)ek;
+            blk[sv] = (uint8_t)ev;
+            if (ek == 255u || ev == 255u)
+                a.b.flags[(size_t)(blk - a.b.data) / LTX_KV_BLOCK / a.b.kvh] = 1u;
+        }
+    } else {
+        // rows of a sequence that are on no page read as zeros; rows of none stay
+        if (row >= a.b.rows || b >= a.b.nseq) return;
+        const KvSeq s = kv_seq(a.b, b);
+        if (row < s.s0 || row >= s.s0 + s.n) return;
+        u32x4 wk = {0, 0, 0, 0}, wv = {0, 0, 0, 0};
+        if (blk) {
+            const uint32_t qk = *(const uint32_t*)(blk + ck), qv = *(const uint32_t*)(blk + cv);
+            const float fk = __builtin_bit_cast(float, (uint32_t)blk[sk] << 23);
+            const float fv = __builtin_bit_cast(float, (uint32_t)blk[sv] << 23);
+            wk = u32x4{Fp4<T>::template pair<0>(qk, fk), Fp4<T>::template pair<1>(qk, fk),
+                       Fp4<T>::template pair<2>(qk, fk), Fp4<T>::template pair<3>(qk, fk)};
+            wv = u32x4{Fp4<T>::template pair<0>(qv, fv), Fp4<T>::template pair<1>(qv, fv),
+                       Fp4<T>::template pair<2>(qv, fv), Fp4<T>::template pair<3>(qv, fv)};
+        }
+        *(u32x4*)k = wk;
+        *(u32x4*)v = wv;
+    }
+}
+
+#define KV_ROWS(NAME, T, WRITE) \
+    extern "C" __global__ void __launch_bounds__(256) NAME(const LtxKvRowsArgs a) { kv_rows<T, WRITE>(a); }
+KV_ROWS(ltx_kv_write_f16, _Float16, true)
+KV_ROWS(ltx_kv_write_bf16, __bf16, true)
+KV_ROWS(ltx_kv_read_f16, _Float16, false)
+KV_ROWS(ltx_kv_read_bf16, __bf16, false)
+
+// ---- attention ------------------------------------------------------------------
+// Items. The rows of a sequence times the query heads of a cached head are its
+// columns c = i * group + g; a tile is `tile` of them. Its keys are split into runs
+// of `per` pages, the same for all sequences: as many as make about `slots` items of
+// a cached head in all. Every wave works the split out from the batch's lengths, so
+// lengths may change behind one launch (a graph's), and a table may be wider than
+// what is in use. Items: sequence by sequence, tile by tile, run by run.
+struct KvItem {
+    int b, tile, run;
+    KvSeq s;
+};
+
+__device__ __forceinline__ uint64_t wave_sum(uint64_t v) {
+    for (int o = 32; o > 0; o >>= 1) v += __shfl_xor((unsigned long long)v, o, 64);
+    return v;
+}
+
+// pages a run, at least `least`
+__device__ __forceinline__ int kv_per(const LtxKvAttnArgs& a, int tile, int least) {
+    if (a.slots == 0) return KV_NO_SPLIT;
+    const int lane = threadIdx.x & 63;
+    uint64_t w = 0;
+    if (a.b.nseq == 1) {
+        const KvSeq s = kv_seq(a.b, 0);
+        w = (uint64_t)kv_tiles(s.n, a.group, tile) * kv_pages(s.L);
+    } else {
+        for (int b = lane; b < a.b.nseq; b += 64) {
+            const KvSeq s = kv_seq(a.b, b);
+            w += (uint64_t)kv_tiles(s.n, a.group, tile) * kv_pages(s.L);
+        }
+        w = wave_sum(w);
+    }
+    return kv_per_of(w, a.slots, least);
+}
+
+// The item's sequence, tile and run; false: there is none.
+__device__ __forceinline__ bool kv_item(const LtxKvAttnArgs& a, int tile, int per, int item, KvItem& it) {
+    if (a.b.nseq == 1) {
+        it.b = 0;
+    } else {
+        const int lane = threadIdx.x & 63;
+        it.b = -1;
+        for (int base = 0; base < a.b.nseq; base += 64) {
+            int c = 0;
+            if (base + lane < a.b.nseq) {
+                const KvSeq s = kv_seq(a.b, base + lane);
+                c = kv_tiles(s.n, a.group, tile) * kv_runs(kv_pages(s.L), per);
+            }
+            int sum = c;
+            for (int o = 1; o < 64; o <<= 1) {
+                const int up = __shfl_up(sum, o, 64);
+                if (lane >= o) sum += up;
+            }
+            const uint64_t here = __builtin_amdgcn_ballot_w64(item < sum && item >= sum - c);
+            if (here) {
+                const int l = __builtin_ctzll(here);
+                it.b = base + l;
+                item -= __shfl(sum - c, l, 64);
+                break;
+            }
+            item -= __shfl(sum, 63, 64);
+        }
+        it.b = __builtin_amdgcn_readfirstlane(it.b);
+        item = __builtin_amdgcn_readfirstlane(item);
+        if (it.b < 0) return false;
+    }
+    it.s = kv_seq(a.b, it.b);
+    const int runs = kv_runs(kv_pages(it.s.L), per);
+    it.tile = item / runs;
+    it.run = item - it.tile * runs;
+    return it.tile < kv_tiles(it.s.n, a.group, tile);
+}
+
+__device__ __forceinline__ float kv_quad_max(float x) {  // over lanes l, l ^ 16, l ^ 32, l ^ 48
+    const uint32_t u = __builtin_bit_cast(uint32_t, x);
+    const auto r = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+    x = fmaxf(__builtin_bit_cast(float, (uint32_t)r[0]), __builtin_bit_cast(float, (uint32_t)r[1]));
+    const uint32_t w = __builtin_bit_cast(uint32_t, x);
+    const auto q = __builtin_amdgcn_permlane32_swap(w, w, false, false);
+    return fmaxf(__builtin_bit_cast(float, (uint32_t)q[0]), __builtin_bit_cast(float, (uint32_t)q[1]));
+}
+
+#define KV_TILE 16
+#define KV_LEAST 4  // pages of a run, one a wave
+
+// Few columns: a workgroup takes 16 columns and a run of pages, a page a wave in
+// turn, everything in registers. Scores transposed, S^T = K . Q^T, and O^T = V^T .
+// P^T (v_mfma_f32_16x16x32), so that a column's statistics lie in the four lanes
+// l % 16 + 16 j and P^T comes straight from the S^T accumulators. The orders in
+// which dims and keys are summed are free: lane (r, h) = (l % 16, l / 16) holds
+// dims 32 h .. + 31 of key 16 t + r (one 16-byte load and one scale), and for V dims
+// 8 r .. + 7 of the keys 16 t + 4 h + i that its scores belong to, 16 scales in one
+// load. MFMA db of O^T has dim 8 r + db in row r.
+template <typename T>
+__device__ void kv_attn(const LtxKvAttnArgs& a) {
+    typedef typename Op<T>::v8 v8;
+    __shared__ __attribute__((aligned(16))) float so[4][KV_TILE][LTX_HD + 4];
+    __shared__ float sm[4][KV_TILE], sl[4][KV_TILE];
+    const int tid = threadIdx.x, lane = tid & 63, r = lane & 15, h = lane >> 4;
+    const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int kh = blockIdx.y;
+    const int per = kv_per(a, KV_TILE, KV_LEAST);
+    KvItem it;
+    if (!kv_item(a, KV_TILE, per, blockIdx.x, it)) return;
+    const int limit = kv_tile_limit(a.causal, it.s, a.group, it.tile, KV_TILE), np = kv_pages(limit);
+    const int p0 = it.run * per, p1 = min(np, p0 + min(per, np));
+    if (it.run > 0 && p0 >= np) return;
+
+    // this lane's column: row, query head, keys it sees
+    const int64_t ncol = (int64_t)it.s.n * a.group;
+    const int64_t c0 = (int64_t)it.tile * KV_TILE;
+    const int cols = (int)min((int64_t)KV_TILE, ncol - c0);
+    const int64_t c = min(c0 + r, ncol - 1);
+    const int row = (int)(c / a.group), head = kh * a.group + (int)(c % a.group);
+    const int mine = kv_limit(a.causal, it.s, row);
+    const int all = kv_limit(a.causal, it.s, (int)(c0 / a.group));  // keys that every column sees
+    v8 qf[4];
+    const uint16_t* Q = (const uint16_t*)a.q + (size_t)(it.s.s0 + row) * a.ldq + (size_t)head * LTX_HD + 32 * h;
+#pragma unroll
+    for (int j = 0; j < 4; j++) qf[j] = __builtin_bit_cast(v8, *(const u32x4*)(Q + 8 * j));
+
+    f32x4 o[8];
+#pragma unroll
+    for (int db = 0; db < 8; db++) o[db] = f32x4{0};
+    float m = -__builtin_inff(), l = 0.f;
+    const float C = a.scale_log2;
+    for (int p = p0 + w; p < p1; p += 4) {
+        int page = __builtin_amdgcn_readfirstlane(kv_page(a.b, it.b, p));
+        const bool none = !kv_in_pool(a.b, page);
+        if (none) {  // a page outside the pool: its keys are left out
+            if (lane == 0 && kh == 0) atomicAdd(a.b.bad, 1ull);
+            page = 0;
+        }
+        const uint8_t* blk = a.b.data + kv_block(a.b, page, kh);
+        const uint32_t flag = a.b.flags[page];
+        u32x4 kc[4], vc[4];
+#pragma unroll
+        for (int t = 0; t < 4; t++) {
+            kc[t] = *(const u32x4*)(blk + 1024 * t + 64 * r + 16 * h);
+            vc[t] = *(const u32x4*)(blk + LTX_KV_V + 1024 * t + 16 * lane);
+        }
+        const uint32_t ks = *(const uint32_t*)(blk + LTX_KV_KS + 16 * r + 4 * h);
+        u32x4 vs = *(const u32x4*)(blk + LTX_KV_VS + 64 * (r >> 2) + 16 * h);
+
+        f32x4 s[4];
+#pragma unroll
+        for (int t = 0; t < 4; t++) {
+            const float f = scale_of(ks, t);
+            s[t] = f32x4{0};
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const uint32_t x = kc[t][j];
+                const u32x4 d = {Fp4<T>::template pair<0>(x, f), Fp4<T>::template pair<1>(x, f),
+                                 Fp4<T>::template pair<2>(x, f), Fp4<T>::template pair<3>(x, f)};
+                s[t] = Op<T>::mfma16(__builtin_bit_cast(v8, d), qf[j], s[t]);
+            }
+        }
+        if (flag) {
+            // values of V that are not finite: the scores of their keys become NaN
+            // (a row that sees such a key is NaN, one that does not is untouched),
+            // the values zero
+            uint32_t bits = 0;
+#pragma unroll
+            for (int t = 0; t < 4; t++)
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+                    if (((vs[t] >> (8 * i)) & 255u) == 255u) {
+                        bits |= 1u << (4 * t + i);
+                        vs[t] &= ~(255u << (8 * i));
+                    }
+            bits |= __shfl_xor(bits, 4, 64);
+            bits |= __shfl_xor(bits, 8, 64);
+#pragma unroll
+            for (int t = 0; t < 4; t++)
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+                    if (bits & (1u << (4 * t + i))) s[t][i] = __builtin_nanf("");
+        }
+        if (none || (p + 1) * LTX_KV_PAGE > all) {
+            const int left = none ? 0 : mine - p * LTX_KV_PAGE - 4 * h;
+#pragma unroll
+            for (int t = 0; t < 4; t++)
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+                    if (16 * t + i >= left) s[t][i] = -__builtin_inff();
+        }
+        float mx = s[0][0];
+#pragma unroll
+        for (int t = 0; t < 4; t++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) mx = fmaxf(mx, s[t][i]);
+        mx = kv_quad_max(mx) * C;
+        if (__builtin_amdgcn_ballot_w64(mx > m) != 0) {
+            const float mn = fmaxf(m, mx);
+            const float corr = mn == -__builtin_inff() ? 1.0f : __builtin_amdgcn_exp2f(m - mn);
+            m = mn;
+            l *= corr;
+#pragma unroll
+            for (int db = 0; db < 8; db++) o[db] *= corr;
+        }
+        const float mz = m == -__builtin_inff() ? 0.f : m;
+        uint32_t pw[4][2];
+#pragma unroll
+        for (int t = 0; t < 4; t++) {
+            float e[4];
+#pragma unroll
+            for (int i = 0; i < 4; i++) e[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][i], C, -mz));
+            // the sum takes the rounded weights, as the products do
+            pw[t][0] = Op<T>::cvt2(e[0], e[1]);
+            pw[t][1] = Op<T>::cvt2(e[2], e[3]);
+            l = Op<T>::sum2(pw[t][1], Op<T>::sum2(pw[t][0], l));
+        }
+#pragma unroll
+        for (int cc = 0; cc < 2; cc++) {
+            const v8 pf = __builtin_bit_cast(v8, (u32x4){pw[2 * cc][0], pw[2 * cc][1], pw[2 * cc + 1][0],
+                                                         pw[2 * cc + 1][1]});
+            auto two = [&](auto B) {  // dims 8 r + 2 B and + 1: eight keys each
+                constexpr int b = decltype(B)::value;
+                uint32_t x[8];
+#pragma unroll
+                for (int e = 0; e < 8; e++) {
+                    const int t = 2 * cc + (e >> 2);
+                    x[e] = Fp4<T>::template pair<b>(vc[t][e & 3], scale_of(vs[t], e & 3));
+                }
+                u32x4 lo, hi;
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    lo[e] = __builtin_amdgcn_perm(x[2 * e + 1], x[2 * e], 0x05040100u);
+                    hi[e] = __builtin_amdgcn_perm(x[2 * e + 1], x[2 * e], 0x07060302u);
+                }
+                o[2 * b] = Op<T>::mfma16(__builtin_bit_cast(v8, lo), pf, o[2 * b]);
+                o[2 * b + 1] = Op<T>::mfma16(__builtin_bit_cast(v8, hi), pf, o[2 * b + 1]);
+            };
+            two(std::integral_constant<int, 0>{});
+            two(std::integral_constant<int, 1>{});
+            two(std::integral_constant<int, 2>{});
+            two(std::integral_constant<int, 3>{});
+        }
+    }
+
+    // the four waves' results into one: lane (r, h) holds dims 8 (4 h + i) + db
+    l += __shfl_xor(l, 16, 64);
+    l += __shfl_xor(l, 32, 64);
+    if (h == 0) {
+        sm[w][r] = m;
+        sl[w][r] = l;
+    }
+    if (r < cols)
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            float* d = &so[w][r][8 * (4 * h + i)];
+            *(f32x4*)d = f32x4{o[0][i], o[1][i], o[2][i], o[3][i]};
+            *(f32x4*)(d + 4) = f32x4{o[4][i], o[5][i], o[6][i], o[7][i]};
+        }
+    __syncthreads();
+    const int col = tid >> 4, d0 = 8 * (tid & 15);
+    if (col >= cols) return;
+    float M = fmaxf(fmaxf(sm[0][col], sm[1][col]), fmaxf(sm[2][col], sm[3][col]));
+    const float Mz = M == -__builtin_inff() ? 0.f : M;
+    float lt = 0.f, x[8] = {};
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+        const float f = __builtin_amdgcn_exp2f(sm[j][col] - Mz);
+        lt = __builtin_fmaf(sl[j][col], f, lt);
+#pragma unroll
+        for (int e = 0; e < 8; e++) x[e] = __builtin_fmaf(so[j][col][d0 + e], f, x[e]);
+    }
+    const int64_t cc = c0 + col;
+    const int orow = (int)(cc / a.group), ohead = kh * a.group + (int)(cc % a.group);
+    if (kv_runs(np, per) > 1) {
+        const size_t at = ((size_t)blockIdx.x * a.b.kvh + kh) * KV_TILE + col;
+        float* ml = a.part + 2 * at;
+        float* po = a.part + 2 * (size_t)a.items * a.b.kvh * KV_TILE + at * LTX_HD + d0;
+        if (d0 == 0) *(f32x2*)ml = f32x2{M, lt};
+        *(f32x4*)po = f32x4{x[0], x[1], x[2], x[3]};
+        *(f32x4*)(po + 4) = f32x4{x[4], x[5], x[6], x[7]};
+        return;
+    }
+    const int grow = it.s.s0 + orow;
+    const float g = a.glog ? 2.0f * sigmoid_f(a.glog[(size_t)grow * a.heads + ohead]) : 1.0f;
+    const float f = kv_limit(a.causal, it.s, orow) > 0 ? g / lt : 0.f;
+    u32x4 out;
+#pragma unroll
+    for (int e = 0; e < 4; e++) out[e] = Op<T>::cvt2(x[2 * e] * f, x[2 * e + 1] * f);
+    *(u32x4*)((uint16_t*)a.out + (size_t)grow * a.ldo + (size_t)ohead * LTX_HD + d0) = out;
+}
+
+extern "C" __global__ void __launch_bounds__(256) ltx_kv_attn_f16(const LtxKvAttnArgs a) { kv_attn<_Float16>(a); }
+extern "C" __global__ void __launch_bounds__(256) ltx_kv_attn_bf16(const LtxKvAttnArgs a) { kv_attn<__bf16>(a); }
+
+// The runs of a tile into one: a wave takes a row and query head.
+template <typename T>
+__device__ void kv_join(const LtxKvAttnArgs& a) {
+    const int lane = threadIdx.x & 63, row = blockIdx.x, head = 4 * blockIdx.y + (threadIdx.x >> 6);
+    if (head >= a.heads) return;
+    const int b = __builtin_amdgcn_readfirstlane(kv_find(a.b, row, 0));
+    if (b >= a.b.nseq) return;
+    const KvSeq s = kv_seq(a.b, b);
+    const int i = row - s.s0, kh = head / a.group;
+    if (i < 0 || i >= s.n) return;
+    const int per = kv_per(a, KV_TILE, KV_LEAST);
+    uint64_t base = 0;  // items of the sequences before
+    if (b > 0) {
+        for (int j = lane; j < b; j += 64) {
+            const KvSeq q = kv_seq(a.b, j);
+            base += (uint64_t)kv_tiles(q.n, a.group, KV_TILE) * kv_runs(kv_pages(q.L), per);
+        }
+        base = wave_sum(base);
+    }
+    const int64_t c = (int64_t)i * a.group + head % a.group;
+    const int tile = (int)(c / KV_TILE), col = (int)(c % KV_TILE);
+    const int runs = kv_runs(kv_pages(kv_tile_limit(a.causal, s, a.group, tile, KV_TILE)), per);
+    const uint64_t item = base + (uint64_t)tile * kv_runs(kv_pages(s.L), per);
+    if (runs <= 1 || item + runs > (uint64_t)a.items) return;
+    const float* ml = a.part + 2 * ((item * a.b.kvh + kh) * KV_TILE + col);
+    const float* po = a.part + 2 * (size_t)a.items * a.b.kvh * KV_TILE +
+                      ((item * a.b.kvh + kh) * KV_TILE + col) * LTX_HD + 2 * lane;
+    const size_t step = (size_t)a.b.kvh * KV_TILE;
+    float M = -__builtin_inff();
+    for (int j = 0; j < runs; j++) M = fmaxf(M, ml[2 * step * j]);
+    const float Mz = M == -__builtin_inff() ? 0.f : M;
+    float lt = 0.f, x0 = 0.f, x1 = 0.f;
+    for (int j = 0; j < runs; j++) {
+        const f32x2 v = *(const f32x2*)(ml + 2 * step * j), y = *(const f32x2*)(po + LTX_HD * step * j);
+        const float f = __builtin_amdgcn_exp2f(v[0] - Mz);
+        lt = __builtin_fmaf(v[1], f, lt);
+        x0 = __builtin_fmaf(y[0], f, x0);
+        x1 = __builtin_fmaf(y[1], f, x1);
+    }
+    const float g = a.glog ? 2.0f * sigmoid_f(a.glog[(size_t)row * a.heads + head]) : 1.0f;
+    const float f = kv_limit(a.causal, s, i) > 0 ? g / lt : 0.f;
+    *(uint32_t*)((uint16_t*)a.out + (size_t)row * a.ldo + (size_t)head * LTX_HD + 2 * lane) =
+        Op<T>::cvt2(x0 * f, x1 * f);
+}
+
+extern "C" __global__ void __launch_bounds__(256) ltx_kv_join_f16(const LtxKvAttnArgs a) { kv_join<_Float16>(a); }
+extern "C" __global__ void __launch_bounds__(256) ltx_kv_join_bf16(const LtxKvAttnArgs a) { kv_join<__bf16>(a); }

@@ -356,6 +356,65 @@ typedef struct {
     float sigma;
 } LtxTimestepArgs;
 
+// ---- 4-bit key/value cache --------------------------------------------------
+// A page holds 64 tokens of every cached head; a (page, head) block is
+// LTX_KV_BLOCK bytes: K codes, V codes (4096 each), K scales, V scales (256
+// each). Two e2m1 codes a byte (the even dim low), one scale byte e + 127 per 32
+// dims (255: a group that held a non-finite value). With key = 16 t + r:
+//   K code dword of dims 8 o .. + 7:  1024 t + 64 r + 4 o
+//   K scale of dims 32 g .. + 31:     16 r + 4 g + t
+// and with key = 16 t + 4 h + i:
+//   V code dword of dims 8 o .. + 7:  1024 t + 16 (16 h + o) + 4 i
+//   V scale of dims 32 g .. + 31:     64 g + 16 h + 4 t + i
+#define LTX_KV_PAGE 64
+#define LTX_KV_BLOCK 8704
+#define LTX_KV_V 4096
+#define LTX_KV_KS 8192
+#define LTX_KV_VS 8448
+
+typedef struct {
+    uint8_t* data;             // [pool][kvh] blocks
+    uint32_t* flags;           // [pool]: non-zero where a page has held a non-finite value
+    unsigned long long* bad;   // rows and pages left out because a page index is outside the pool
+    const int32_t* row_start;  // [nseq + 1], or NULL: one row a sequence
+    const int32_t* kv_len;     // [nseq] keys, the new rows among them
+    const int32_t* pages;      // [nseq][max_pages]
+    int nseq, rows, max_pages, pool, kvh;
+} LtxKvBatchArgs;
+
+// k and v (or what is read back), rows of kvh * 128 values, ldk and ldv elements apart
+typedef struct {
+    LtxKvBatchArgs b;
+    void* k;
+    void* v;
+    int64_t ldk, ldv;
+} LtxKvRowsArgs;
+
+typedef struct {
+    LtxKvBatchArgs b;
+    const void* q;      // [rows][heads * 128], ldq elements apart
+    void* out;          // the same, ldo elements apart
+    const float* glog;  // [rows][heads] or NULL
+    float* part;        // partial results of `items` items (see kv_plan), or NULL: no split
+    int64_t ldq, ldo;
+    int heads, group;   // group = heads / kvh query heads a cached head
+    int causal;
+    int slots;          // items aimed at for a cached head's keys (0: no split)
+    int items;          // items of the grid
+    float scale_log2;   // log2(e) / sqrt(128)
+} LtxKvAttnArgs;
+
+// y = a . (q s)^T (+ bias), 4-bit weights
+typedef struct {
+    const void* a;       // [M][K] 16-bit or f32
+    const uint8_t* q;    // [N][K / 2]
+    const void* scales;  // [N][K / 128] f32 or f16
+    const float* bias;   // [N] or NULL
+    void* y;             // [M][N] f32 or the 16-bit type
+    int M, N, K;
+    int scale_f16, gelu, out_f32;
+} LtxLinearQ4Args;
+
 #ifdef __cplusplus
 }
 #endif

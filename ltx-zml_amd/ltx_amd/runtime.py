@@ -60,6 +60,15 @@ def lib() -> C.CDLL:
         "ltx_op_linear_q8": (i32, [vp, vp, vp, vp, i32, vp, vp, i32, i32, i32, i32, i32, i32, vp]),
         "ltx_op_linear_q8_noalloc": (i32, [vp, vp, vp, vp, i32, vp, vp, i32, i32, i32, i32, i32, i32, vp]),
         "ltx_op_attention": (i32, [vp, vp, vp, vp, vp, vp, i32, i32, i32, vp]),
+        "ltx_op_linear_q4": (i32, [vp, vp, vp, vp, i32, vp, vp, i32, i32, i32, i32, i32, i32, vp]),
+        "ltx_kv_cache_create": (i32, [vp, i32, i32, i32, C.POINTER(vp)]),
+        "ltx_kv_cache_free": (None, [vp, vp]),
+        "ltx_kv_cache_bytes": (u64, [vp]),
+        "ltx_kv_cache_faults": (i32, [vp, vp, vp, C.POINTER(u64), i32]),
+        "ltx_op_kv_write": (i32, [vp, vp, vp, vp, i64, vp, i64, vp]),
+        "ltx_op_kv_read": (i32, [vp, vp, vp, vp, i64, vp, i64, vp]),
+        "ltx_op_kv_attention_workspace": (i32, [vp, vp, vp, i32, C.POINTER(u64)]),
+        "ltx_op_kv_attention": (i32, [vp, vp, vp, vp, i64, i32, i32, vp, vp, i64, vp, u64, vp]),
         "ltx_op_dequant": (i32, [vp, vp, vp, i32, i32, i32, vp, vp, i32, vp]),
         "ltx_rope_tables": (i32, [vp, i32, vp, vp, i32]),
         "ltx_profile_enable": (i32, [vp, i32]),
@@ -202,6 +211,61 @@ class BlockGraph:
             pass
 
 
+class _KvBatchArgs(C.Structure):  # ltx_kv_batch
+    _fields_ = [("nseq", C.c_int), ("rows", C.c_int), ("row_start", C.c_void_p), ("kv_len", C.c_void_p),
+                ("pages", C.c_void_p), ("max_pages", C.c_int)]
+
+
+class KvBatch:
+    """The sequences of a call on a KvCache (ltx_kv_batch): int32 device tensors
+    kv_len [nseq], pages [nseq, max_pages] and row_start [nseq + 1] (None: one row
+    a sequence), and the rows that the call's tensors have."""
+
+    def __init__(self, kv_len, pages, row_start=None, rows: int | None = None):
+        import torch
+        nseq = kv_len.shape[0]
+        for t, shape in ((kv_len, (nseq,)), (pages, (nseq, pages.shape[-1])), (row_start, (nseq + 1,))):
+            if t is not None and (t.dtype != torch.int32 or tuple(t.shape) != shape or not t.is_contiguous()):
+                raise LtxError(f"KvBatch: an int32 contiguous tensor of shape {shape} is needed")
+        if rows is None and row_start is not None:
+            raise LtxError("KvBatch: row_start needs rows")
+        self.rows = nseq if rows is None else rows
+        self._keep = (kv_len, pages, row_start)
+        self.args = _KvBatchArgs(nseq, self.rows, _ptr(row_start), _ptr(kv_len), _ptr(pages), pages.shape[1])
+        self.ref = C.addressof(self.args)
+
+
+class KvCache:
+    """A key/value cache in 4 bits (ltx_kv_cache)."""
+
+    def __init__(self, ctx: "Context", handle: int, kv_heads: int, pages: int, mode: int):
+        self.ctx, self.handle = ctx, handle
+        self.kv_heads, self.pages, self.mode = kv_heads, pages, mode
+
+    @property
+    def nbytes(self) -> int:
+        return lib().ltx_kv_cache_bytes(self.handle)
+
+    def faults(self, reset: bool = True, stream=None) -> int:
+        """Page indices outside the pool met since the last reset (ltx_kv_cache_faults)."""
+        st = stream.cuda_stream if stream is not None else _current_stream()
+        n = C.c_uint64()
+        self.ctx._check(lib().ltx_kv_cache_faults(self.ctx.handle, self.handle, st, C.byref(n), int(reset)),
+                        "ltx_kv_cache_faults")
+        return n.value
+
+    def free(self):
+        if self.handle:
+            lib().ltx_kv_cache_free(self.ctx.handle, self.handle)
+            self.handle = None
+
+    def __del__(self):
+        try:
+            self.free()
+        except Exception:
+            pass
+
+
 class Context:
     """One device context (ltx_init). Not thread-safe."""
 
@@ -212,6 +276,7 @@ class Context:
         self.handle = h.value
         self.device = device
         self._graphs = weakref.WeakSet()
+        self._caches = weakref.WeakSet()
 
     def _check(self, ok: int, what: str):
         if not ok:
@@ -221,6 +286,8 @@ class Context:
         if self.handle:
             for g in list(self._graphs):  # graphs hold the context's workspace
                 g.free()
+            for k in list(self._caches):
+                k.free()
             lib().ltx_destroy(self.handle)
             self.handle = None
 
@@ -319,6 +386,69 @@ class Context:
                                            m, st), "ltx_op_attention")
         return out
 
+    def linear_q4(self, a, q, s, bias, y, mode=MODE_F16, gelu=False, stream=None):
+        """a [M, K], q uint8 [N, K / 2] (two weights a byte), s [N, K / 128]."""
+        M, K = a.shape
+        N = q.shape[0]
+        import torch
+        _want(K == 2 * q.shape[1] and tuple(s.shape) == (N, K // 128) and tuple(y.shape) == (M, N)
+              and (bias is None or bias.numel() == N), "linear_q4: the shapes do not fit")
+        _want(all(t.is_contiguous() for t in (a, q, s, y)) and (bias is None or bias.is_contiguous()),
+              "linear_q4: contiguous tensors are needed")
+        x = _torch_dtype(mode)
+        _want(a.dtype == x and q.dtype == torch.uint8 and s.dtype in (torch.float16, torch.float32)
+              and y.dtype in (x, torch.float32) and (bias is None or bias.dtype == torch.float32),
+              "linear_q4: the types do not fit the mode")
+        st = stream.cuda_stream if stream is not None else _current_stream()
+        self._check(lib().ltx_op_linear_q4(self.handle, _ptr(a), _ptr(q), _ptr(s), int(s.dtype == torch.float16),
+                                           _ptr(bias), _ptr(y), int(y.dtype == torch.float32), M, N, K, int(gelu),
+                                           mode, st), "ltx_op_linear_q4")
+        return y
+
+    # ---- the 4-bit key/value cache ----
+    def kv_cache(self, kv_heads: int, pages: int, mode: int = MODE_F16) -> KvCache:
+        h = C.c_void_p()
+        self._check(lib().ltx_kv_cache_create(self.handle, mode, kv_heads, pages, C.byref(h)), "ltx_kv_cache_create")
+        c = KvCache(self, h.value, kv_heads, pages, mode)
+        self._caches.add(c)
+        return c
+
+    def kv_write(self, cache: KvCache, batch: KvBatch, k, v, stream=None):
+        """k, v [rows, kv_heads * 128] (rows may be strided) -> the cache (ltx_op_kv_write)."""
+        st = stream.cuda_stream if stream is not None else _current_stream()
+        _rows("kv_write", batch, cache, cache.kv_heads, k, v)
+        self._check(lib().ltx_op_kv_write(self.handle, cache.handle, batch.ref, _ptr(k), k.stride(0), _ptr(v),
+                                          v.stride(0), st), "ltx_op_kv_write")
+
+    def kv_read(self, cache: KvCache, batch: KvBatch, k, v, stream=None):
+        """What the cache holds of the batch's rows -> k, v (ltx_op_kv_read)."""
+        st = stream.cuda_stream if stream is not None else _current_stream()
+        _rows("kv_read", batch, cache, cache.kv_heads, k, v)
+        self._check(lib().ltx_op_kv_read(self.handle, cache.handle, batch.ref, _ptr(k), k.stride(0), _ptr(v),
+                                         v.stride(0), st), "ltx_op_kv_read")
+
+    def kv_attention_workspace(self, cache: KvCache, batch: KvBatch, heads: int) -> int:
+        """Bytes of `work` for kv_attention with this batch's nseq, rows and max_pages."""
+        n = C.c_uint64()
+        self._check(lib().ltx_op_kv_attention_workspace(self.handle, cache.handle, batch.ref, heads, C.byref(n)),
+                    "ltx_op_kv_attention_workspace")
+        return n.value
+
+    def kv_attention(self, cache: KvCache, batch: KvBatch, q, out, heads: int, causal: bool = True, glog=None,
+                     work=None, stream=None):
+        """q, out [rows, heads * 128] (rows may be strided); glog [rows, heads] f32
+        or None; work: a uint8 tensor of kv_attention_workspace bytes, or None
+        (ltx_op_kv_attention)."""
+        st = stream.cuda_stream if stream is not None else _current_stream()
+        _rows("kv_attention", batch, cache, heads, q, out)
+        _want(glog is None or (tuple(glog.shape) == (batch.rows, heads) and glog.is_contiguous()
+                               and glog.element_size() == 4), "kv_attention: glog must be f32 [rows, heads]")
+        self._check(lib().ltx_op_kv_attention(self.handle, cache.handle, batch.ref, _ptr(q), q.stride(0), heads,
+                                              int(causal), _ptr(glog), _ptr(out), out.stride(0), _ptr(work),
+                                              0 if work is None else work.numel() * work.element_size(), st),
+                    "ltx_op_kv_attention")
+        return out
+
     def dequant(self, q, s, out32, out16, mode=MODE_F16, stream=None):
         import torch
         N, K = q.shape
@@ -393,6 +523,24 @@ class Context:
         ms, n = C.c_double(), C.c_int()
         self._check(lib().ltx_profile_read(self.handle, substr.encode(), C.byref(ms), C.byref(n)), "ltx_profile_read")
         return ms.value, n.value
+
+
+def _want(ok: bool, what: str):
+    if not ok:
+        raise LtxError(what)
+
+
+def _torch_dtype(mode: int):
+    import torch
+    return {MODE_F16: torch.float16, MODE_BF16: torch.bfloat16, MODE_F32: torch.float32}.get(mode)
+
+
+def _rows(name: str, batch: KvBatch, cache: KvCache, heads: int, *tensors):
+    """Tensors [rows, heads * 128] of the cache's type, values of a row next to each other."""
+    dt = _torch_dtype(cache.mode)
+    for t in tensors:
+        _want(t.dim() == 2 and t.shape[0] == batch.rows and t.shape[1] == heads * 128 and t.dtype == dt
+              and t.stride(1) == 1, f"{name}: [{batch.rows}, {heads * 128}] tensors of the cache's type are needed")
 
 
 def _current_stream() -> int:

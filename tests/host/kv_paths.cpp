@@ -1,0 +1,246 @@
+// The 4-bit cache and linear on the recording HIP stand-in (refusals, workspaces,
+// routes), and the kernels' index arithmetic compiled for the host. Run by
+// tests/test_kv_host.py.
+#include <algorithm>
+#include <random>
+
+#include "fake_hip.hpp"
+#include "ltx_internal.hpp"
+#include "ltx_kv_index.h"
+
+#define CHECK(cond, ...)                                  \
+    do {                                                  \
+        if (!(cond)) {                                    \
+            std::printf("line %d: %s: ", __LINE__, #cond); \
+            std::printf(__VA_ARGS__);                     \
+            std::printf("\n");                            \
+            std::exit(1);                                 \
+        }                                                 \
+    } while (0)
+
+static char* const X = (char*)(1ull << 36);  // a caller's tensors: aligned addresses
+static char* ptr(int i) { return X + ((size_t)i << 30); }
+
+static int launches(const char* prefix) {
+    int n = 0;
+    for (const fake::Op& o : fake::log) n += o.what == "launch" && o.name.rfind(prefix, 0) == 0;
+    return n;
+}
+
+struct Fixture {
+    ltx_ctx* c = nullptr;
+    ltx_kv_cache* cache = nullptr;
+    ltx_kv_batch b{};
+    Fixture(int heads = 8, int mode = LTX_MODE_F16) {
+        CHECK(ltx_init(0, &c), "%s", ltx_last_error(nullptr));
+        CHECK(ltx_kv_cache_create(c, mode, heads, 100, &cache), "%s", ltx_last_error(c));
+        b = {3, 10, (const int32_t*)ptr(0), (const int32_t*)ptr(1), (const int32_t*)ptr(2), 20};
+    }
+    int write(const void* k = ptr(3), int64_t ldk = 1024, const void* v = ptr(4), int64_t ldv = 1024) {
+        return ltx_op_kv_write(c, cache, &b, k, ldk, v, ldv, nullptr);
+    }
+    int read(void* k = ptr(3), int64_t ldk = 1024, void* v = ptr(4), int64_t ldv = 1024) {
+        return ltx_op_kv_read(c, cache, &b, k, ldk, v, ldv, nullptr);
+    }
+    int attend(const void* q = ptr(5), int64_t ldq = 4096, int heads = 32, void* out = ptr(6), int64_t ldo = 4096,
+               void* work = ptr(7), uint64_t bytes = 1ull << 30, hipStream_t st = nullptr) {
+        return ltx_op_kv_attention(c, cache, &b, q, ldq, heads, 1, nullptr, out, ldo, work, bytes, st);
+    }
+};
+
+#define REFUSED(call, text)                                                                          \
+    do {                                                                                             \
+        fake::log.clear();                                                                           \
+        CHECK(!(call), "taken: %s", #call);                                                          \
+        CHECK(std::strstr(ltx_last_error(f.c), text), "%s: %s", #call, ltx_last_error(f.c));         \
+        CHECK(launches("") == 0, "%s launched", #call);                                              \
+    } while (0)
+
+static void refusals() {
+    Fixture f;
+    ltx_kv_cache* k = nullptr;
+    REFUSED(ltx_kv_cache_create(f.c, LTX_MODE_F32, 8, 10, &k), "16-bit mode");
+    REFUSED(ltx_kv_cache_create(f.c, 7, 8, 10, &k), "16-bit mode");
+    REFUSED(ltx_kv_cache_create(f.c, 0, 0, 10, &k), "bad cache shape");
+    REFUSED(ltx_kv_cache_create(f.c, 0, 8, 0, &k), "bad cache shape");
+    REFUSED(ltx_kv_cache_create(f.c, 0, 8, 1 << 25, &k), "at most");
+    REFUSED(ltx_kv_cache_create(f.c, 0, 8, 10, nullptr), "NULL");
+    CHECK(f.write() && f.read() && f.attend(), "%s", ltx_last_error(f.c));
+    REFUSED(ltx_op_kv_write(f.c, nullptr, &f.b, ptr(3), 1024, ptr(4), 1024, nullptr), "NULL");
+    REFUSED(ltx_op_kv_write(f.c, f.cache, nullptr, ptr(3), 1024, ptr(4), 1024, nullptr), "NULL");
+    CHECK(!ltx_op_kv_write(nullptr, f.cache, &f.b, ptr(3), 1024, ptr(4), 1024, nullptr), "NULL context");
+    CHECK(!ltx_op_kv_attention(nullptr, f.cache, &f.b, ptr(3), 4096, 32, 1, nullptr, ptr(4), 4096, nullptr, 0, nullptr),
+          "NULL context");
+    const ltx_kv_batch good = f.b;
+    auto each = [&](auto set, const char* text) {
+        f.b = good;
+        set(f.b);
+        REFUSED(f.write(), text);
+        REFUSED(f.read(), text);
+        REFUSED(f.attend(), text);
+        uint64_t n;
+        REFUSED(ltx_op_kv_attention_workspace(f.c, f.cache, &f.b, 32, &n), text);
+        f.b = good;
+    };
+    each([](ltx_kv_batch& b) { b.nseq = 0; }, "nseq");
+    each([](ltx_kv_batch& b) { b.rows = -1; }, "rows");
+    each([](ltx_kv_batch& b) { b.max_pages = 0; }, "max_pages");
+    each([](ltx_kv_batch& b) { b.max_pages = (1 << 24) + 1; }, "max_pages");
+    each([](ltx_kv_batch& b) { b.kv_len = nullptr; }, "kv_len");
+    each([](ltx_kv_batch& b) { b.pages = nullptr; }, "pages");
+    each([](ltx_kv_batch& b) { b.row_start = nullptr; }, "row_start");
+    REFUSED(f.write(nullptr), "k is NULL");
+    REFUSED(f.write(ptr(3) + 8), "k:");
+    REFUSED(f.write(ptr(3), 1023), "k:");
+    REFUSED(f.write(ptr(3), 1016), "k:");
+    REFUSED(f.write(ptr(3), 1028), "k:");
+    REFUSED(f.write(ptr(3), 1024, nullptr), "v is NULL");
+    REFUSED(f.write(ptr(3), 1024, ptr(4), 8), "v:");
+    REFUSED(f.read(ptr(3), 1024, ptr(4) + 2), "v:");
+    REFUSED(f.attend(nullptr), "q is NULL");
+    REFUSED(f.attend(ptr(5), 4088), "q:");
+    REFUSED(f.attend(ptr(5), 4096, 32, ptr(6) + 4), "out:");
+    REFUSED(f.attend(ptr(5), 4096, 0), "heads");
+    REFUSED(f.attend(ptr(5), 4096, 12), "heads");
+    REFUSED(f.attend(ptr(5), 4096, 32, ptr(6), 4096, ptr(7) + 8), "work");
+    uint64_t n = 0;
+    CHECK(ltx_op_kv_attention_workspace(f.c, f.cache, &f.b, 32, &n) && n, "%s", ltx_last_error(f.c));
+    REFUSED(f.attend(ptr(5), 4096, 32, ptr(6), 4096, ptr(7), n - 1), "work");
+    CHECK(f.attend(ptr(5), 4096, 32, ptr(6), 4096, ptr(7), n), "%s", ltx_last_error(f.c));
+    // no rows: nothing to do, nothing launched
+    fake::log.clear();
+    f.b.rows = 0;
+    CHECK(f.write() && f.read() && f.attend() && launches("") == 0, "%s", ltx_last_error(f.c));
+    f.b.rows = 1 << 24;
+    REFUSED(f.attend(), "too many rows");
+
+    auto q4 = [&](const void* a, const void* q, const void* s, int s16, const void* bias, void* y, int f32, int M, int N,
+                  int K, int mode) {
+        return ltx_op_linear_q4(f.c, a, (const uint8_t*)q, s, s16, (const float*)bias, y, f32, M, N, K, 0, mode, nullptr);
+    };
+    CHECK(q4(ptr(0), ptr(1), ptr(2), 1, ptr(3), ptr(4), 0, 5, 33, 128, 0), "%s", ltx_last_error(f.c));
+    for (int bad : {0, -1, 64, 129, 130})
+        REFUSED(q4(ptr(0), ptr(1), ptr(2), 1, ptr(3), ptr(4), 0, 5, 32, bad, 0), "bad linear shape");
+    REFUSED(q4(ptr(0), ptr(1), ptr(2), 1, ptr(3), ptr(4), 0, 0, 32, 128, 0), "bad linear shape");
+    REFUSED(q4(ptr(0), ptr(1), ptr(2), 1, ptr(3), ptr(4), 0, 5, -3, 128, 0), "bad linear shape");
+    REFUSED(q4(ptr(0), ptr(1), ptr(2), 1, ptr(3), ptr(4), 0, 5, 32, 128, 3), "unknown mode");
+    REFUSED(q4(ptr(0), ptr(1), ptr(2), 1, ptr(3), ptr(4), 0, 5, 32, 128, 2), "f32 output");
+    REFUSED(q4(ptr(0) + 8, ptr(1), ptr(2), 1, ptr(3), ptr(4), 0, 5, 32, 128, 0), "16 bytes");
+    REFUSED(q4(ptr(0), ptr(1) + 4, ptr(2), 1, ptr(3), ptr(4), 0, 5, 32, 128, 0), "16 bytes");
+    REFUSED(q4(ptr(0), ptr(1), ptr(2) + 2, 0, ptr(3), ptr(4), 0, 5, 32, 128, 0), "scales");
+    REFUSED(q4(ptr(0), ptr(1), ptr(2), 1, ptr(3) + 2, ptr(4), 0, 5, 32, 128, 0), "bias");
+    REFUSED(q4(ptr(0), ptr(1), ptr(2), 1, ptr(3), ptr(4) + 2, 1, 5, 32, 128, 0), "y");
+    REFUSED(q4(nullptr, ptr(1), ptr(2), 1, ptr(3), ptr(4), 1, 5, 32, 128, 0), "NULL");
+    REFUSED(q4(ptr(0), ptr(1), ptr(2), 1, ptr(3), ptr(4), 0, 1 << 21, 32, 128, 0), "too many rows");
+}
+
+// Without `work`: scratch of the context, ordered behind its last use; a captured
+// call, and one without memory, runs unsplit and needs none.
+static void scratch() {
+    Fixture f;
+    hipStream_t s = (hipStream_t)0x77;
+    fake::log.clear();
+    CHECK(f.attend(ptr(5), 4096, 32, ptr(6), 4096, nullptr, 0, s), "%s", ltx_last_error(f.c));
+    CHECK(launches("ltx_kv_attn") == 1 && launches("ltx_kv_join") == 1, "split");
+    CHECK(fake::log.back().what == "record", "the scratch's use is recorded");
+    fake::log.clear();
+    CHECK(f.attend(ptr(5), 4096, 32, ptr(6), 4096, nullptr, 0, s), "%s", ltx_last_error(f.c));
+    CHECK(fake::log.front().what == "wait", "and waited for");
+    fake::log.clear();
+    fake::capturing.insert(s);
+    CHECK(f.attend(ptr(5), 4096, 32, ptr(6), 4096, nullptr, 0, s), "%s", ltx_last_error(f.c));
+    CHECK(fake::log.size() == 1 && launches("ltx_kv_attn") == 1 && !fake::broken_capture, "captured: one launch");
+    fake::log.clear();
+    CHECK(f.attend(ptr(5), 4096, 32, ptr(6), 4096, ptr(7), 1ull << 30, s), "%s", ltx_last_error(f.c));
+    CHECK(launches("ltx_kv_attn") == 1 && launches("ltx_kv_join") == 1 && fake::log.size() == 2, "captured with work");
+    fake::capturing.clear();
+    Fixture g;
+    fake::limit = fake::in_use;
+    fake::log.clear();
+    CHECK(g.attend(ptr(5), 4096, 32, ptr(6), 4096, nullptr, 0, s), "%s", ltx_last_error(g.c));
+    CHECK(launches("ltx_kv_attn") == 1 && launches("ltx_kv_join") == 0, "no memory: not split");
+}
+
+static void memory() {
+    const uint64_t before = fake::in_use;
+    Fixture f;
+    const uint64_t with = fake::in_use;
+    CHECK(ltx_kv_cache_bytes(f.cache) >= 100ull * 64 * 8 * 136, "%llu", (unsigned long long)ltx_kv_cache_bytes(f.cache));
+    ltx_kv_cache_free(f.c, f.cache);
+    CHECK(with - fake::in_use >= 100ull * 64 * 8 * 136 && before <= fake::in_use, "freed");
+    fake::limit = fake::in_use;
+    ltx_kv_cache* k = (ltx_kv_cache*)1;
+    CHECK(!ltx_kv_cache_create(f.c, 0, 8, 100, &k) && !k, "no memory: refused, no handle");
+    ltx_kv_cache_free(f.c, nullptr);
+}
+
+// The index arithmetic on arrays of any contents: what a kernel would read and
+// write stays inside what the call names, and the items fit the grid.
+static void index_bounds(unsigned seed) {
+    std::mt19937 rng(seed);
+    auto pick = [&](int lo, int hi) { return std::uniform_int_distribution<int>(lo, hi)(rng); };
+    const int wild[] = {0, 1, -1, 63, 64, 65, 0x7fffffff, (int)0x80000000, 100, 1 << 24};
+    for (int trial = 0; trial < 2000; trial++) {
+        const bool sane = trial % 2 == 0;
+        const int nseq = pick(1, 9), max_pages = pick(1, 12), pool = pick(1, 30), group = pick(1, 9);
+        const int tile = 16 << pick(0, 4), slots = pick(0, 40), least = pick(1, 8);
+        int rows = pick(0, 90);
+        std::vector<int32_t> start(nseq + 1), len(nseq), pages(nseq * max_pages);
+        for (auto& p : pages) p = pick(0, 3) ? pick(0, pool - 1) : wild[pick(0, 9)];
+        for (int b = 0; b < nseq; b++) len[b] = sane ? pick(0, 64 * max_pages) : wild[pick(0, 9)];
+        if (sane) {
+            for (auto& s : start) s = pick(0, rows);
+            std::sort(start.begin(), start.end());
+            start[0] = 0;
+        } else
+            for (auto& s : start) s = pick(0, 1) ? pick(-5, rows + 5) : wild[pick(0, 9)];
+        LtxKvBatchArgs a{nullptr, nullptr, nullptr, start.data(), len.data(), pages.data(), nseq, rows, max_pages, pool, 3};
+        uint64_t work = 0;
+        for (int b = 0; b < nseq; b++) {
+            const KvSeq s = kv_seq(a, b);
+            CHECK(s.s0 >= 0 && s.n >= 0 && s.s0 + s.n <= rows && s.L >= 0 && s.L <= 64 * max_pages, "%d %d %d", s.s0, s.n, s.L);
+            for (int row = -1; row <= rows; row++) {
+                const int pos = kv_position(s, row);
+                CHECK(pos == -1 || (pos >= 0 && pos / 64 < max_pages && row >= s.s0 && row < s.s0 + s.n), "%d", pos);
+                if (pos < 0) continue;
+                const int page = kv_page(a, b, pos / 64);
+                CHECK(kv_in_pool(a, page) == (page >= 0 && page < pool), "%d", page);
+                CHECK(kv_limit(1, s, row - s.s0) == pos + 1, "%d", pos);
+            }
+            work += (uint64_t)kv_tiles(s.n, group, tile) * kv_pages(s.L);
+        }
+        const int per = slots ? kv_per_of(work, slots, least) : KV_NO_SPLIT;
+        const int grid = (int)((int64_t)rows * group / tile + nseq + slots);
+        int64_t items = 0;
+        for (int b = 0; b < nseq; b++) {
+            const KvSeq s = kv_seq(a, b);
+            const int tiles = kv_tiles(s.n, group, tile), runs = kv_runs(kv_pages(s.L), per);
+            items += (int64_t)tiles * runs;
+            for (int t = 0; t < tiles; t++)
+                for (int causal = 0; causal < 2; causal++) {
+                    const int limit = kv_tile_limit(causal, s, group, t, tile);
+                    CHECK(limit >= 0 && limit <= s.L && kv_runs(kv_pages(limit), per) <= runs, "%d of %d", limit, s.L);
+                }
+        }
+        if (sane) CHECK(items <= grid, "%lld items, a grid of %d", (long long)items, grid);
+    }
+    LtxKvBatchArgs big{nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, 1, 1, 1, 1 << 25, 32};
+    CHECK(kv_block(big, (1 << 25) - 1, 31) == ((1ull << 30) - 1) * LTX_KV_BLOCK, "places pass 32 bits");
+}
+
+int main(int argc, char** argv) {
+    const std::string cmd = argc > 1 ? argv[1] : "";
+    if (cmd == "refusals")
+        refusals();
+    else if (cmd == "scratch")
+        scratch();
+    else if (cmd == "memory")
+        memory();
+    else if (cmd == "index")
+        index_bounds(std::atoi(argv[2]));
+    else
+        CHECK(false, "unknown command %s", cmd.c_str());
+    std::printf("ok\n");
+    std::fflush(stdout);
+    std::_Exit(0);  // (the library's own teardown belongs to the real runtime)
+}

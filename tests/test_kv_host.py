@@ -1,0 +1,66 @@
+"""The 4-bit cache and linear without a GPU: refusals, workspaces and routes on the
+recording stand-in for the HIP runtime (tests/host/fake_hip.hpp), the kernels' index
+arithmetic on arrays of any contents, and the Python entry points' own checks."""
+import pathlib
+import subprocess
+
+import pytest
+
+ROOT = pathlib.Path(__file__).resolve().parent.parent
+PKG = ROOT / "ltx-zml_amd"
+
+
+@pytest.fixture(scope="session")
+def kv_paths(tmp_path_factory):
+    exe = tmp_path_factory.mktemp("kv") / "kv_paths"
+    subprocess.run(["g++", "-O1", "-std=c++17", "-D__HIP_PLATFORM_AMD__", "-Wno-unused-result", "-rdynamic",
+                    "-I/opt/rocm/include", f"-I{ROOT / 'include'}", f"-I{PKG / 'csrc'}", f"-I{PKG / 'csrc' / 'host'}",
+                    str(ROOT / "tests" / "host" / "kv_paths.cpp"), "-o", str(exe), str(PKG / "libltx_amd.so"),
+                    f"-Wl,-rpath,{PKG}", "-Wl,--allow-shlib-undefined", "-pthread"], check=True)
+
+    def run(*args):
+        r = subprocess.run([str(exe), *map(str, args)], capture_output=True, text=True, timeout=120)
+        assert r.returncode == 0 and r.stdout.endswith("ok\n"), r.stdout + r.stderr
+    return run
+
+
+def test_refusals(kv_paths):
+    kv_paths("refusals")
+
+
+def test_attention_scratch(kv_paths):
+    kv_paths("scratch")
+
+
+def test_cache_memory(kv_paths):
+    kv_paths("memory")
+
+
+@pytest.mark.parametrize("seed", [1, 2, 3])
+def test_index_arithmetic_stays_inside(kv_paths, seed):
+    kv_paths("index", seed)
+
+
+def test_python_checks():
+    """What the bindings refuse before a call: shapes, types and strides that the
+    C interface cannot see."""
+    torch = pytest.importorskip("torch")
+    from ltx_amd import runtime as rt
+
+    i32 = dict(dtype=torch.int32)
+    lens, pages = torch.zeros(3, **i32), torch.zeros(3, 4, **i32)
+    b = rt.KvBatch(lens, pages, torch.zeros(4, **i32), 7)
+    assert (b.args.nseq, b.args.rows, b.args.max_pages) == (3, 7, 4)
+    assert rt.KvBatch(lens, pages).rows == 3
+    for bad in [(lens.long(), pages), (lens, pages[:2]), (lens, pages.T.contiguous().T), (lens, pages, lens, 7),
+                (lens, pages, torch.zeros(4, **i32))]:
+        with pytest.raises(rt.LtxError):
+            rt.KvBatch(*bad)
+
+    class Cache:
+        kv_heads, mode, handle = 2, rt.MODE_F16, 0
+    good = torch.zeros(7, 256, dtype=torch.float16)
+    rt._rows("x", b, Cache, 2, good, torch.zeros(7, 768, dtype=torch.float16)[:, 256:512])
+    for bad in [good[:6], good[:, :128], good.bfloat16(), torch.zeros(256, 7, dtype=torch.float16).T, good[0]]:
+        with pytest.raises(rt.LtxError):
+            rt._rows("x", b, Cache, 2, bad)
