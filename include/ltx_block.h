@@ -277,7 +277,8 @@ int ltx_op_dequant(ltx_ctx* ctx, const int8_t* q, const void* scales, int scale_
  * three exact bf16 planes. The weights are exact operands, a group's scale
  * multiplies its f32 sum. No scratch: calls may overlap and be captured. Refused:
  * M, N or K not positive, K no multiple of 128, a or q not on 16 bytes, scales,
- * bias or y not aligned to their types, an unknown mode, more than 1,048,560 rows. */
+ * bias or y not aligned to their types, an unknown mode, M above 1,048,560, N from
+ * 2^27, K above 2^23. */
 int ltx_op_linear_q4(ltx_ctx* ctx, const void* a, const uint8_t* q, const void* scales, int scale_f16,
                      const float* bias, void* y, int out_f32, int M, int N, int K, int gelu, int mode,
                      void* stream);

@@ -1,4 +1,6 @@
 // The linear with 4-bit weights.
+#include <cstdio>
+
 #include "ltx_internal.hpp"
 
 extern "C" int ltx_op_linear_q4(ltx_ctx* c, const void* a, const uint8_t* q, const void* scales, int scale_f16,
@@ -15,12 +17,25 @@ extern "C" int ltx_op_linear_q4(ltx_ctx* c, const void* a, const uint8_t* q, con
         if ((uintptr_t)bias & 3 || (uintptr_t)y & (out_f32 || mode == LTX_MODE_F32 ? 3 : 1))
             throw ltx::Error("bias and y must be aligned to their types");
         if (mode == LTX_MODE_F32 && !out_f32) throw ltx::Error("mode F32 has an f32 output");
-        if (((int64_t)N + 15) / 16 >= 1 << 24 || ((int64_t)M + 15) / 16 > 65535) throw ltx::Error("too many rows");
+        // the grid's limits, 2^32 threads along x and 65,535 workgroups along y, and
+        // 32-bit offsets of a tile's 64 rows of q and 32 of a
+        if (N >= 1 << 27 || M > 65535 * 16 || K > 1 << 23) throw ltx::Error("too many rows or columns");
         HIPC(hipSetDevice(c->device));
         LtxLinearQ4Args g{a, q, scales, bias, y, M, N, K, scale_f16 != 0, gelu != 0, out_f32 != 0};
-        c->launch(mode == LTX_MODE_F16    ? "ltx_linear_q4_f16"
-                  : mode == LTX_MODE_BF16 ? "ltx_linear_q4_bf16"
-                                          : "ltx_linear_q4_f32",
-                  (N + 15) / 16, (M + 15) / 16, 1, 256, &g, (hipStream_t)stream);
+        // Tiles of 32 rows of a where there are more than 16 (mode F32: 16, its three
+        // planes fill the LDS), and the fewest columns of 16, 32 or 64 whose workgroups
+        // are at most one a CU: more columns a workgroup read a fewer times, fewer
+        // leave no CU idle. us, 16 / 32 / 64 columns: one row of 4,096 x 4,096 5.7 / 6.8 /
+        // 9.2, of 8,192 8.7 / 7.0 / 10.1, of 12,288 12.0 / 11.8 / 10.1, of 16,384 16.1 /
+        // 12.4 / 10.4; 64 rows of 4,096 x 4,096 13.6 / 9.2 / 12.1, of 8,192 24.9 / 17.2 /
+        // 13.4; mode F32, 32 rows of 4,096 x 4,096 20.8 / 11.9 / 14.9.
+        const bool f32 = mode == LTX_MODE_F32;
+        const int mt = f32 || M <= 16 ? 1 : 2, gy = (M + 16 * mt - 1) / (16 * mt);
+        int nt = 1;
+        while (nt < 4 && ((int64_t)N + 16 * nt - 1) / (16 * nt) * gy > c->num_cu) nt *= 2;
+        char name[48];
+        std::snprintf(name, sizeof(name), "ltx_linear_q4_%s_s%d_%d_%d",
+                      f32 ? "f32" : mode == LTX_MODE_F16 ? "f16" : "bf16", scale_f16 ? 16 : 32, mt, nt);
+        c->launch(name, (unsigned)(((int64_t)N + 16 * nt - 1) / (16 * nt)), gy, 1, 512, &g, (hipStream_t)stream);
     })
 }

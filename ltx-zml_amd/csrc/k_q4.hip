@@ -3,85 +3,71 @@
 #include "ltx_device.h"
 
 // Eight weights of a dword (two's complement nibbles, the lowest first) as 16-bit
-// operands of value q / 16: v_cvt_off_f32_i4 is exact, and so is the rounding.
+// operands of value q / 16: v_cvt_off_f32_i4 (of the low four bits, exact) takes any
+// byte of its operand, so that a shift serves the four odd nibbles; the rounding is
+// exact too. 13 instructions.
 template <typename T>
 __device__ __forceinline__ u32x4 q4_operand(uint32_t w) {
+    uint32_t o = w >> 4;
+    asm("" : "+v"(o));  // one shift, not one an odd nibble
     u32x4 r;
 #pragma unroll
     for (int e = 0; e < 4; e++)
-        r[e] = Op<T>::cvt2(__builtin_amdgcn_cvt_off_f32_i4(w >> (8 * e)),
-                           __builtin_amdgcn_cvt_off_f32_i4(w >> (8 * e + 4)));
+        r[e] = Op<T>::cvt2(__builtin_amdgcn_cvt_off_f32_i4((w >> (8 * e)) & 0xffu),
+                           __builtin_amdgcn_cvt_off_f32_i4((o >> (8 * e)) & 0xffu));
     return r;
 }
 
-// Activations of mode M: the operand type and the exact planes that make a value.
-struct Q4F16 {
-    typedef _Float16 T;
-    static constexpr int planes = 1, bytes = 2;
-};
-struct Q4BF16 {
-    typedef __bf16 T;
-    static constexpr int planes = 1, bytes = 2;
-};
-struct Q4F32 {
-    typedef __bf16 T;
-    static constexpr int planes = 3, bytes = 4;
-};
+#define Q4_WAVES 8
 
-// A workgroup takes 16 rows of a and 16 of q; its four waves share the groups of
-// 128. Lane (r, h) = (l % 16, l / 16) holds weights 32 h .. + 31 of a group of row
-// r, one 16-byte load; step j of the group sums k = 32 h + 8 j .. + 7. The scale
-// multiplies the group's f32 sum: one a lane, as D's column is the weight row.
-template <typename P>
-__device__ void linear_q4(const LtxLinearQ4Args& a) {
-    typedef typename P::T T;
-    typedef typename Op<T>::v8 v8;
-    __shared__ f32x4 part[4][64];
-    const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, r = lane & 15, h = lane >> 4;
-    const int n = blockIdx.x * 16 + r, m = blockIdx.y * 16 + r;
-    const int G = a.K / LTX_GROUP;
-    const uint8_t* q = a.q + (size_t)min(n, a.N - 1) * (a.K / 2) + 16 * h;
-    const char* x = (const char*)a.a + ((size_t)min(m, a.M - 1) * a.K + 32 * h) * P::bytes;
-    const size_t s0 = (size_t)min(n, a.N - 1) * G;
-    f32x4 acc = {0, 0, 0, 0};
-    for (int g = w; g < G; g += 4) {
-        const u32x4 wq = *(const u32x4*)(q + 64 * (size_t)g);
-        const float s = a.scale_f16 ? f16_bits_to_f32(((const uint16_t*)a.scales)[s0 + g])
-                                    : ((const float*)a.scales)[s0 + g];
-        f32x4 d = {0, 0, 0, 0};
-#pragma unroll
-        for (int j = 0; j < 4; j++) {
-            const char* xp = x + ((size_t)LTX_GROUP * g + 8 * j) * P::bytes;
-            const v8 wv = __builtin_bit_cast(v8, q4_operand<T>(wq[j]));
-            if (P::planes == 1) {
-                d = Op<T>::mfma16(__builtin_bit_cast(v8, *(const u32x4*)xp), wv, d);
-            } else {
-                float f[8];
-                u32x4 p[3];
-                *(f32x4*)f = *(const f32x4*)xp;
-                *(f32x4*)(f + 4) = *(const f32x4*)(xp + 16);
-                split3(f, p);
-#pragma unroll
-                for (int i = 0; i < 3; i++) d = Op<T>::mfma16(__builtin_bit_cast(v8, p[i]), wv, d);
-            }
-        }
-        const float s16 = 16.0f * s;
-#pragma unroll
-        for (int i = 0; i < 4; i++) acc[i] = __builtin_fmaf(d[i], s16, acc[i]);
+// Operands come through buffer resources that begin at the workgroup's first row:
+// rows past the last read as zeros without an access. The group goes into the scalar
+// offset, which takes no part in that check; for a group that is not there the
+// resource is empty instead. So the loads need no branch and no vector arithmetic.
+typedef __amdgpu_buffer_rsrc_t q4_rsrc;
+struct Q4Buffer {
+    const void* base;
+    int bytes;
+    __device__ __forceinline__ q4_rsrc rsrc(bool there) const {
+        return __builtin_amdgcn_make_buffer_rsrc((void*)base, 0, there ? bytes : 0, 0x00020000);
     }
-    part[w][lane] = acc;
-    __syncthreads();
-    if (w) return;
-    acc = (part[0][lane] + part[1][lane]) + (part[2][lane] + part[3][lane]);
-    if (n >= a.N) return;
-    const float bias = a.bias ? a.bias[n] : 0.0f;
+};
+__device__ __forceinline__ u32x4 q4_load16(q4_rsrc b, uint32_t lane, uint32_t all) {
+    return __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(b, lane, all, 0));
+}
+template <bool S16>
+__device__ __forceinline__ uint32_t q4_load_scale(q4_rsrc b, uint32_t lane, uint32_t all) {
+    return S16 ? (uint32_t)__builtin_amdgcn_raw_buffer_load_b16(b, 2 * lane, 2 * all, 0)
+               : (uint32_t)__builtin_amdgcn_raw_buffer_load_b32(b, 4 * lane, 4 * all, 0);
+}
+template <bool S16>
+__device__ __forceinline__ float q4_scale(uint32_t bits) {
+    return S16 ? f16_bits_to_f32((uint16_t)bits) : __builtin_bit_cast(float, bits);
+}
+
+// The waves' sums into one, in the waves' order, and y. my: the wave's slot of SLOT
+// bytes in lds.
+template <typename T, int MT, int NT, int SLOT>
+__device__ __forceinline__ void q4_finish(const LtxLinearQ4Args& a, uint8_t* lds, int w, int lane,
+                                          const f32x4 (&acc)[MT][NT], int m0, int n0, int rows) {
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
-        const int row = blockIdx.y * 16 + 4 * h + i;
-        if (row >= a.M) break;
-        float y = acc[i] + bias;
+    for (int m = 0; m < MT; m++)
+#pragma unroll
+        for (int t = 0; t < NT; t++) *(f32x4*)(lds + SLOT * w + 1024 * (m * NT + t) + 16 * lane) = acc[m][t];
+    __syncthreads();
+    for (int e = threadIdx.x; e < MT * NT * 256; e += 64 * Q4_WAVES) {
+        // element e: column of the tile fastest, so that rows of y are written whole
+        const int t = (e >> 4) % NT, row = (e >> 4) / NT, col = e & 15, m = row >> 4;
+        const int n = n0 + 16 * t + col;
+        if (row >= rows || n >= a.N) continue;
+        const uint8_t* p = lds + 1024 * (m * NT + t) + 16 * (16 * ((row & 15) >> 2) + col) + 4 * (row & 3);
+        float y = 0.f;
+#pragma unroll
+        for (int j = 0; j < Q4_WAVES; j++) y += *(const float*)(p + SLOT * j);
+        y *= 16.0f;  // of the operands
+        if (a.bias) y += a.bias[n];
         if (a.gelu) y = gelu_tanh(y);
-        const size_t at = (size_t)row * a.N + n;
+        const size_t at = (size_t)(m0 + row) * a.N + n;
         if (a.out_f32)
             ((float*)a.y)[at] = y;
         else
@@ -89,6 +75,206 @@ __device__ void linear_q4(const LtxLinearQ4Args& a) {
     }
 }
 
-extern "C" __global__ void __launch_bounds__(256) ltx_linear_q4_f16(const LtxLinearQ4Args a) { linear_q4<Q4F16>(a); }
-extern "C" __global__ void __launch_bounds__(256) ltx_linear_q4_bf16(const LtxLinearQ4Args a) { linear_q4<Q4BF16>(a); }
-extern "C" __global__ void __launch_bounds__(256) ltx_linear_q4_f32(const LtxLinearQ4Args a) { linear_q4<Q4F32>(a); }
+// The scales of four groups, group h's in lanes 16 h .. + 15, to all lanes each.
+__device__ __forceinline__ void q4_spread(uint32_t x, uint32_t (&s)[4]) {
+    auto a = __builtin_amdgcn_permlane32_swap(x, x, false, false);  // groups 0 1 0 1 and 2 3 2 3
+    auto b = __builtin_amdgcn_permlane16_swap(a[0], a[0], false, false);
+    s[0] = b[0], s[1] = b[1];
+    b = __builtin_amdgcn_permlane16_swap(a[1], a[1], false, false);
+    s[2] = b[0], s[3] = b[1];
+}
+
+// Four values as three bf16 planes, x = p0 + p1 + p2 exactly (split3 of the f32 GEMM,
+// four at a time).
+__device__ __forceinline__ void q4_split(f32x4 x, u32x2 (&p)[3]) {
+    uint32_t h[4], m[4], l[4];
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+        const float v = x[e];  // (a bit cast of a vector's element itself takes element 0)
+        h[e] = __builtin_bit_cast(uint32_t, v) & 0xffff0000u;
+        const float d = __builtin_isinf(v) ? 0.0f : v - __builtin_bit_cast(float, h[e]);
+        m[e] = __builtin_bit_cast(uint32_t, d) & 0xffff0000u;
+        l[e] = __builtin_bit_cast(uint32_t, d - __builtin_bit_cast(float, m[e]));
+    }
+#pragma unroll
+    for (int e = 0; e < 2; e++) {
+        p[0][e] = __builtin_amdgcn_perm(h[2 * e + 1], h[2 * e], 0x07060302u);
+        p[1][e] = __builtin_amdgcn_perm(m[2 * e + 1], m[2 * e], 0x07060302u);
+        p[2][e] = __builtin_amdgcn_perm(l[2 * e + 1], l[2 * e], 0x07060302u);
+    }
+}
+
+// A workgroup takes 16 MT rows of a and 16 NT of q, each of its eight waves an
+// eighth of the groups of 128. PL: the exact planes that make a value of a, three in
+// mode F32. D's column is the weight row, so a lane needs one scale of a group, which
+// multiplies the group's f32 sum.
+//
+// Bound: the weights, read once, 4,096 x 4,096 in 2 us at the rate of a large copy
+// (4.9 TB/s). MFMA operands want neighbouring lanes in different rows; loaded that
+// way every lane is an access of its own, 64 an instruction where 16 would do, and
+// the texture unit bounds the kernel (16 rows of 16,384 x 4,096: 12.6 million
+// accesses, 30 us; with scalar offsets in place of a third of the vector
+// instructions no faster). So both operands are loaded along their rows and change
+// lanes in LDS of the wave's own (no barrier, and the order of a wave's LDS
+// operations lets one buffer do): chunk c (16 bytes) of row r of a at c ^ r, of q at
+// c ^ r / 2, free of conflicts. AW groups of q and AA of a are in flight.
+// Measured back to back in a graph, where an empty launch takes 3.8 us: one row 5.7
+// us (4,096 x 4,096), 10.4 (16,384 x 4,096), 10.4 (4,096 x 16,384); 32 rows of
+// 16,384 x 4,096 13.9 us (17.5 with NT = 2, 21.1 with MT = 1); mode F32, five rows
+// of 4,096 x 16,384, 19.5 us (forming the planes bounds it).
+template <typename T, int PL, bool S16, int MT, int NT, int AW, int AA, int EARLY>
+__device__ __forceinline__ void linear_q4(const LtxLinearQ4Args& a) {
+    typedef typename Op<T>::v8 v8;
+    constexpr bool F32 = PL == 3;
+    constexpr int XT = MT * PL * 4096, TILE = XT + NT * 1024, PART = MT * NT * 1024;
+    constexpr int SLOT = TILE > PART ? TILE : PART;
+    __shared__ __attribute__((aligned(16))) uint8_t lds[Q4_WAVES * SLOT];
+    const int tid = threadIdx.x, lane = tid & 63, r = lane & 15, h = lane >> 4;
+    const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int n0 = blockIdx.x * 16 * NT, m0 = blockIdx.y * 16 * MT;
+    const int rows = min(16 * MT, a.M - m0), cols = min(16 * NT, a.N - n0);
+    const int G = a.K / LTX_GROUP, each = (G + Q4_WAVES - 1) / Q4_WAVES;
+    const int g0 = w * each, g1 = min(G, g0 + each);
+    uint8_t* my = lds + w * SLOT;
+    const Q4Buffer bq{a.q + (size_t)n0 * (a.K / 2), cols * (a.K / 2)};
+    const Q4Buffer bs{(const char*)a.scales + (size_t)n0 * G * (S16 ? 2 : 4), cols * G * (S16 ? 2 : 4)};
+    const Q4Buffer bx{(const char*)a.a + (size_t)m0 * a.K * (F32 ? 4 : 2), rows * a.K * (F32 ? 4 : 2)};
+    // loads: q chunk l % 4 of row l / 4; a chunk l % 16 (8 values) of rows 4 i + l / 16
+    const uint32_t oq = (lane >> 2) * (a.K / 2) + 16 * (lane & 3), os = r * G + h;
+    const uint32_t ox = F32 ? (lane >> 5) * 4 * a.K + 16 * (lane & 31) : h * 2 * a.K + 16 * r;
+    uint8_t* wq_st = my + XT + 64 * (lane >> 2) + 16 * ((lane & 3) ^ ((lane >> 3) & 3));
+    const uint8_t* wq_ld = my + XT + 64 * r + 16 * (h ^ ((r >> 1) & 3));
+
+    constexpr int NX = F32 ? 8 * MT : 4 * MT, RX = F32 ? 2 : 4;  // loads of a group of a, rows of a load
+    u32x4 wq[AW][NT], xa[AA][NX];
+    uint32_t sc[NT];
+    auto load_w = [&](int u, int g) {
+        const q4_rsrc rq = bq.rsrc(g < g1);
+#pragma unroll
+        for (int t = 0; t < NT; t++) wq[u][t] = q4_load16(rq, oq + 16 * t * (a.K / 2), 64 * g);
+    };
+    auto load_s = [&](int g) {  // groups g .. g + 3, zero past the wave's last one
+#pragma unroll
+        for (int t = 0; t < NT; t++)
+            sc[t] = q4_load_scale<S16>(bs.rsrc(g < g1), g + h < g1 ? os + 16 * t * G : 0x20000000u, g);
+    };
+    auto load_a = [&](int u, int g) {
+        const q4_rsrc rx = bx.rsrc(g < g1);
+#pragma unroll
+        for (int i = 0; i < NX; i++) xa[u][i] = q4_load16(rx, ox + 8 * i * a.K, (F32 ? 512 : 256) * g);
+    };
+    struct Frags {
+        u32x4 w[NT];
+        v8 x[MT][PL][4];
+    };
+    auto exchange = [&](int u, Frags& f) {
+#pragma unroll
+        for (int t = 0; t < NT; t++) *(u32x4*)(wq_st + 1024 * t) = wq[u % AW][t];
+#pragma unroll
+        for (int i = 0; i < NX; i++) {
+            if (RX * i >= rows) continue;
+            if (F32) {
+                const int row = 2 * i + (lane >> 5), c = lane & 31;
+                uint8_t* d = my + 256 * row + 16 * ((c >> 1) ^ (row & 15)) + 8 * (c & 1);
+                u32x2 p[3];
+                q4_split(__builtin_bit_cast(f32x4, xa[u % AA][i]), p);
+#pragma unroll
+                for (int j = 0; j < 3; j++) *(u32x2*)(d + 4096 * MT * j) = p[j];
+            } else {
+                const int row = 4 * i + h;
+                *(u32x4*)(my + 256 * row + 16 * (r ^ (row & 15))) = xa[u % AA][i];
+            }
+        }
+#pragma unroll
+        for (int t = 0; t < NT; t++) f.w[t] = *(const u32x4*)(wq_ld + 1024 * t);
+#pragma unroll
+        for (int m = 0; m < MT; m++)
+#pragma unroll
+            for (int p = 0; p < PL; p++)
+#pragma unroll
+                for (int j = 0; j < 4; j++)
+                    f.x[m][p][j] = __builtin_bit_cast(
+                        v8, *(const u32x4*)(my + 4096 * (MT * p + m) + 256 * r + 16 * ((4 * h + j) ^ r)));
+    };
+    f32x4 acc[MT][NT];
+#pragma unroll
+    for (int m = 0; m < MT; m++)
+#pragma unroll
+        for (int t = 0; t < NT; t++) acc[m][t] = f32x4{0, 0, 0, 0};
+
+    load_s(g0);
+#pragma unroll
+    for (int u = 0; u < AW; u++) {
+        load_w(u, g0 + u);
+        if (u < AA) load_a(u, g0 + u);
+        __builtin_amdgcn_sched_barrier(0);
+    }
+    // EARLY 1: a group's exchange runs before the products of the one before it
+    Frags f[1 + EARLY];
+    if (EARLY) {
+        exchange(0, f[0]);
+        load_w(0, g0 + AW);
+        load_a(0, g0 + AA);
+    }
+    for (int g = g0; g < g1; g += AW) {
+        uint32_t sg[NT][4];
+#pragma unroll
+        for (int t = 0; t < NT; t++) q4_spread(sc[t], sg[t]);
+        load_s(g + AW);
+#pragma unroll
+        for (int u = 0; u < AW; u++) {
+            exchange(u + EARLY, f[(u + EARLY) & EARLY]);
+            // the loads stay here: gathered behind all of the step's products they
+            // would be waited for all at once
+            load_w((u + EARLY) % AW, g + u + EARLY + AW);
+            load_a((u + EARLY) % AA, g + u + EARLY + AA);
+            f32x4 d[MT][NT];
+#pragma unroll
+            for (int m = 0; m < MT; m++)
+#pragma unroll
+                for (int t = 0; t < NT; t++) d[m][t] = f32x4{0, 0, 0, 0};
+#pragma unroll
+            for (int j = 0; j < 4; j++)
+#pragma unroll
+                for (int t = 0; t < NT; t++) {
+                    const v8 wv = __builtin_bit_cast(v8, q4_operand<T>(f[u & EARLY].w[t][j]));
+#pragma unroll
+                    for (int m = 0; m < MT; m++)
+#pragma unroll
+                        for (int p = 0; p < PL; p++) d[m][t] = Op<T>::mfma16(f[u & EARLY].x[m][p][j], wv, d[m][t]);
+                }
+#pragma unroll
+            for (int t = 0; t < NT; t++) {
+                const float s = q4_scale<S16>(sg[t][u]);
+#pragma unroll
+                for (int m = 0; m < MT; m++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++) acc[m][t][i] = __builtin_fmaf(d[m][t][i], s, acc[m][t][i]);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    }
+    q4_finish<T, MT, NT, SLOT>(a, lds, w, lane, acc, m0, n0, rows);
+}
+
+#define Q4_KERNEL(NAME, ...)                                                                        \
+    extern "C" __global__ void __launch_bounds__(64 * Q4_WAVES) NAME(const LtxLinearQ4Args a) {    \
+        linear_q4<__VA_ARGS__>(a);                                                                  \
+    }
+#define Q4_KERNELS(MT, NT, ...)                                                           \
+    Q4_KERNEL(ltx_linear_q4_f16_s32_##MT##_##NT, _Float16, 1, false, MT, NT, __VA_ARGS__) \
+    Q4_KERNEL(ltx_linear_q4_f16_s16_##MT##_##NT, _Float16, 1, true, MT, NT, __VA_ARGS__)  \
+    Q4_KERNEL(ltx_linear_q4_bf16_s32_##MT##_##NT, __bf16, 1, false, MT, NT, __VA_ARGS__)  \
+    Q4_KERNEL(ltx_linear_q4_bf16_s16_##MT##_##NT, __bf16, 1, true, MT, NT, __VA_ARGS__)
+#define Q4_PLANES(NT, ...)                                                                \
+    Q4_KERNEL(ltx_linear_q4_f32_s32_1_##NT, __bf16, 3, false, 1, NT, __VA_ARGS__)         \
+    Q4_KERNEL(ltx_linear_q4_f32_s16_1_##NT, __bf16, 3, true, 1, NT, __VA_ARGS__)
+Q4_KERNELS(1, 1, 4, 4, 1)
+Q4_KERNELS(1, 2, 4, 4, 1)
+Q4_KERNELS(1, 4, 4, 2, 0)
+Q4_KERNELS(2, 1, 4, 2, 1)
+Q4_KERNELS(2, 2, 4, 2, 0)
+Q4_KERNELS(2, 4, 2, 1, 0)
+Q4_PLANES(1, 4, 2, 1)
+Q4_PLANES(2, 4, 2, 0)
+Q4_PLANES(4, 4, 1, 0)

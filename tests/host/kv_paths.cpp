@@ -132,6 +132,8 @@ static void refusals() {
     REFUSED(q4(ptr(0), ptr(1), ptr(2), 1, ptr(3), ptr(4) + 2, 1, 5, 32, 128, 0), "y");
     REFUSED(q4(nullptr, ptr(1), ptr(2), 1, ptr(3), ptr(4), 1, 5, 32, 128, 0), "NULL");
     REFUSED(q4(ptr(0), ptr(1), ptr(2), 1, ptr(3), ptr(4), 0, 1 << 21, 32, 128, 0), "too many rows");
+    REFUSED(q4(ptr(0), ptr(1), ptr(2), 1, ptr(3), ptr(4), 0, 1, 1 << 27, 128, 0), "too many rows");
+    REFUSED(q4(ptr(0), ptr(1), ptr(2), 1, ptr(3), ptr(4), 0, 1, 32, (1 << 23) + 128, 0), "too many rows");
 }
 
 // Without `work`: scratch of the context, ordered behind its last use; a captured
