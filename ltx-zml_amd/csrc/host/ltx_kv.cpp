@@ -1,4 +1,5 @@
 // The 4-bit key/value cache: its handle, rows written and read back, attention.
+#include <cstdlib>
 #include <cstring>
 
 #include "ltx_internal.hpp"
@@ -16,9 +17,6 @@ struct ltx_kv_cache {
 namespace ltx {
 namespace {
 
-constexpr int kTile = 16;          // columns of an item (k_kv.hip)
-constexpr int kLeastPages = 4;     // pages of a run, at least
-constexpr int kTargetItems = 1024; // items of all cached heads that a call aims at: four workgroups a CU
 constexpr int kMaxPages = 1 << 24; // of a table: positions stay in 31 bits
 
 // Checks of a batch that need no device value; rows == 0 is an empty call.
@@ -55,19 +53,31 @@ void kv_rows(ltx_ctx* c, const ltx_kv_cache* k, const ltx_kv_batch* b, void* kp,
 }
 
 struct AttnPlan {
-    int slots = 0, items = 0;
+    int nq = 0;  // 0: the kernel of few columns (16 a tile), else 128 nq a tile
+    int tile = 16, least = 4, slots = 0, items = 0;
     size_t bytes = 0;  // of partial results
 };
 
-AttnPlan attn_plan(const ltx_kv_cache* k, const ltx_kv_batch* b, int heads, bool split) {
-    const int64_t group = heads / k->kv_heads;
-    const int64_t tiles = (int64_t)b->rows * group / kTile + b->nseq;
+AttnPlan attn_plan(const ltx_ctx* c, const ltx_kv_cache* k, const ltx_kv_batch* b, int heads, bool split) {
+    const int64_t group = heads / k->kv_heads, columns = (int64_t)b->rows * group;
     AttnPlan p;
-    if (split && b->max_pages > kLeastPages) p.slots = (kTargetItems + k->kv_heads - 1) / k->kv_heads;
-    // the grids' limit, 2^32 threads along x
-    if (tiles + p.slots >= 1 << 24 || b->rows >= 1 << 24) throw Error("too many rows for one call");
+    int forced = -1;
+    if (const char* e = std::getenv("KVNQ")) forced = std::atoi(e);
+    int target = 4;
+    if (const char* e = std::getenv("KVTARGET")) target = std::atoi(e);
+    p.nq = forced >= 0 ? forced : columns <= 32 * (int64_t)b->nseq ? 0 : columns * k->kv_heads <= 128ll * c->num_cu ? 1 : 2;
+    if (p.nq) {
+        p.tile = 128 * p.nq;
+        p.least = 8;
+        target = 1;
+    }
+    if (const char* e = std::getenv("KVLEAST")) p.least = std::atoi(e);
+    const int64_t tiles = columns / p.tile + b->nseq;
+    if (split && b->max_pages > p.least) p.slots = (target * c->num_cu + k->kv_heads - 1) / k->kv_heads;
+    // the grids' limits: 2^32 threads along x, 2^31 items in all
+    if (tiles + p.slots >= (1 << 23) / k->kv_heads || b->rows >= 1 << 24) throw Error("too many rows for one call");
     p.items = (int)(tiles + p.slots);
-    if (p.slots) p.bytes = (size_t)p.items * k->kv_heads * kTile * (LTX_HD + 2) * sizeof(float);
+    if (p.slots) p.bytes = (size_t)p.items * k->kv_heads * p.tile * (LTX_HD + 2) * sizeof(float);
     return p;
 }
 
@@ -155,7 +165,7 @@ int ltx_op_kv_attention_workspace(ltx_ctx* c, const ltx_kv_cache* cache, const l
         if (!c || !bytes) throw ltx::Error("NULL argument");
         ltx::batch_args(c, cache, batch);
         ltx::check_heads(cache, heads);
-        *bytes = ltx::attn_plan(cache, batch, heads, true).bytes;
+        *bytes = ltx::attn_plan(c, cache, batch, heads, true).bytes;
     })
 }
 
@@ -170,13 +180,13 @@ int ltx_op_kv_attention(ltx_ctx* c, const ltx_kv_cache* cache, const ltx_kv_batc
         ltx::check_rows(q, ldq, heads * LTX_HD, batch->rows, "q");
         ltx::check_rows(out, ldo, heads * LTX_HD, batch->rows, "out");
         if ((uintptr_t)work & 15) throw ltx::Error("work must start on 16 bytes");
-        ltx::AttnPlan p = ltx::attn_plan(cache, batch, heads, true);
+        ltx::AttnPlan p = ltx::attn_plan(c, cache, batch, heads, true);
         if (work && work_bytes < p.bytes) throw ltx::Error("work is smaller than ltx_op_kv_attention_workspace says");
         if (batch->rows == 0) return LTX_OK;
         HIPC(hipSetDevice(c->device));
         hipStream_t st = (hipStream_t)stream;
         ltx::ScratchUse use(c->op_scratch, st);
-        if (p.bytes && !work && !(work = use.take(p.bytes))) p = ltx::attn_plan(cache, batch, heads, false);
+        if (p.bytes && !work && !(work = use.take(p.bytes))) p = ltx::attn_plan(c, cache, batch, heads, false);
         a.q = q;
         a.out = out;
         a.glog = glog;
@@ -186,11 +196,18 @@ int ltx_op_kv_attention(ltx_ctx* c, const ltx_kv_cache* cache, const ltx_kv_batc
         a.heads = heads;
         a.group = heads / cache->kv_heads;
         a.causal = causal != 0;
+        a.tile = p.tile;
+        a.least = p.least;
         a.slots = p.slots;
         a.items = p.items;
         a.scale_log2 = 0.12751743f;  // log2(e) / sqrt(128)
         const bool f16 = cache->mode == LTX_MODE_F16;
-        c->launch(f16 ? "ltx_kv_attn_f16" : "ltx_kv_attn_bf16", p.items, cache->kv_heads, 1, 256, &a, st);
+        if (p.nq == 0)
+            c->launch(f16 ? "ltx_kv_attn_f16" : "ltx_kv_attn_bf16", p.items, cache->kv_heads, 1, 256, &a, st);
+        else
+            c->launch(p.nq == 1 ? (f16 ? "ltx_kv_attn_f16_rows1" : "ltx_kv_attn_bf16_rows1")
+                                : (f16 ? "ltx_kv_attn_f16_rows2" : "ltx_kv_attn_bf16_rows2"),
+                      (unsigned)(((int64_t)p.items * cache->kv_heads + 7) / 8 * 8), 1, 1, 512, &a, st);
         if (p.slots)
             c->launch(f16 ? "ltx_kv_join_f16" : "ltx_kv_join_bf16", batch->rows, (heads + 3) / 4, 1, 256, &a, st);
     })

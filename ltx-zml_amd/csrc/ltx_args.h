@@ -361,8 +361,8 @@ typedef struct {
 // LTX_KV_BLOCK bytes: K codes, V codes (4096 each), K scales, V scales (256
 // each). Two e2m1 codes a byte (the even dim low), one scale byte e + 127 per 32
 // dims (255: a group that held a non-finite value). With key = 16 t + r:
-//   K code dword of dims 8 o .. + 7:  1024 t + 64 r + 4 o
-//   K scale of dims 32 g .. + 31:     16 r + 4 g + t
+//   K code dword of dims 8 o .. + 7:  1024 t + 256 (o / 4) + 16 r + 4 (o % 4)
+//   K scale of dims 32 g .. + 31:     64 g + 4 r + t
 // and with key = 16 t + 4 h + i:
 //   V code dword of dims 8 o .. + 7:  1024 t + 16 (16 h + o) + 4 i
 //   V scale of dims 32 g .. + 31:     64 g + 16 h + 4 t + i
@@ -399,8 +399,10 @@ typedef struct {
     int64_t ldq, ldo;
     int heads, group;   // group = heads / kvh query heads a cached head
     int causal;
+    int tile;           // columns of an item
+    int least;          // pages of a run, at least
     int slots;          // items aimed at for a cached head's keys (0: no split)
-    int items;          // items of the grid
+    int items;          // items of a cached head in the grid
     float scale_log2;   // log2(e) / sqrt(128)
 } LtxKvAttnArgs;
 
