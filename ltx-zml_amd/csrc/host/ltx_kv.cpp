@@ -73,9 +73,10 @@ AttnPlan attn_plan(const ltx_ctx* c, const ltx_kv_cache* k, const ltx_kv_batch* 
     }
     if (const char* e = std::getenv("KVLEAST")) p.least = std::atoi(e);
     const int64_t tiles = columns / p.tile + b->nseq;
-    if (split && b->max_pages > p.least) p.slots = (target * c->num_cu + k->kv_heads - 1) / k->kv_heads;
-    // the grids' limits: 2^32 threads along x, 2^31 items in all
-    if (tiles + p.slots >= (1 << 23) / k->kv_heads || b->rows >= 1 << 24) throw Error("too many rows for one call");
+    // (as many workgroups without a split: none pays)
+    if (split && b->max_pages > p.least && (p.nq == 0 || columns / p.tile * k->kv_heads < c->num_cu)) p.slots = (target * c->num_cu + k->kv_heads - 1) / k->kv_heads;
+    // the grids' limit, 2^32 threads along x; columns stay in 31 bits
+    if (tiles + p.slots >= (1 << 23) / k->kv_heads || columns >= 1 << 30 || b->rows >= 1 << 24) throw Error("too many rows for one call");
     p.items = (int)(tiles + p.slots);
     if (p.slots) p.bytes = (size_t)p.items * k->kv_heads * p.tile * (LTX_HD + 2) * sizeof(float);
     return p;

@@ -43,6 +43,15 @@ __device__ __forceinline__ float scale_of(uint32_t w, int i) {
 }
 
 // ---- the batch ----------------------------------------------------------------
+// A sequence that is the same for all lanes, in scalar registers
+__device__ __forceinline__ KvSeq kv_seq_all(const LtxKvBatchArgs& a, int b) {
+    KvSeq s = kv_seq(a, b);
+    s.s0 = __builtin_amdgcn_readfirstlane(s.s0);
+    s.n = __builtin_amdgcn_readfirstlane(s.n);
+    s.L = __builtin_amdgcn_readfirstlane(s.L);
+    return s;
+}
+
 // The sequences of rows row0 .. row0 + 3, each lane that of row0 + sub (nseq or
 // more: of none). All 64 lanes call it with one row0.
 __device__ __forceinline__ int kv_find(const LtxKvBatchArgs& a, int row0, int sub) {
@@ -183,7 +192,7 @@ __device__ __forceinline__ int kv_per(const LtxKvAttnArgs& a) {
     const int lane = threadIdx.x & 63;
     uint64_t w = 0;
     if (a.b.nseq == 1) {
-        const KvSeq s = kv_seq(a.b, 0);
+        const KvSeq s = kv_seq_all(a.b, 0);
         w = (uint64_t)kv_tiles(s.n, a.group, a.tile) * kv_pages(s.L);
     } else {
         for (int b = lane; b < a.b.nseq; b += 64) {
@@ -192,7 +201,7 @@ __device__ __forceinline__ int kv_per(const LtxKvAttnArgs& a) {
         }
         w = wave_sum(w);
     }
-    return kv_per_of(w, a.slots, a.least);
+    return __builtin_amdgcn_readfirstlane(kv_per_of(w, a.slots, a.least));
 }
 
 // The item's sequence, tile and run; false: there is none. A sequence's last tile,
@@ -227,7 +236,7 @@ __device__ __forceinline__ bool kv_item(const LtxKvAttnArgs& a, int per, int ite
         item = __builtin_amdgcn_readfirstlane(item);
         if (it.b < 0) return false;
     }
-    it.s = kv_seq(a.b, it.b);
+    it.s = kv_seq_all(a.b, it.b);
     const int runs = kv_runs(kv_pages(it.s.L), per);
     it.tile = kv_tiles(it.s.n, a.group, a.tile) - 1 - item / runs;
     it.run = item % runs;
@@ -243,6 +252,12 @@ __device__ __forceinline__ float kv_quad_max(float x) {  // over lanes l, l ^ 16
     return fmaxf(__builtin_bit_cast(float, (uint32_t)q[0]), __builtin_bit_cast(float, (uint32_t)q[1]));
 }
 
+// x where m is 0, y where it is ~0 (bit operations: as compares and selects, the
+// rare paths below took more scalar registers than there are, and spilled)
+__device__ __forceinline__ float kv_select(int m, float x, uint32_t y) {
+    return __builtin_bit_cast(float, (__builtin_bit_cast(uint32_t, x) & ~(uint32_t)m) | (y & (uint32_t)m));
+}
+
 // The scores of page p's keys that column limits leave out: -inf. s[t][i] is key 16 t
 // + 4 h + i; a column sees the keys below `mine`.
 __device__ __forceinline__ void kv_mask(f32x4 (&s)[4], int p, int mine, int h) {
@@ -250,8 +265,7 @@ __device__ __forceinline__ void kv_mask(f32x4 (&s)[4], int p, int mine, int h) {
 #pragma unroll
     for (int t = 0; t < 4; t++)
 #pragma unroll
-        for (int i = 0; i < 4; i++)
-            if (16 * t + i >= left) s[t][i] = -__builtin_inff();
+        for (int i = 0; i < 4; i++) s[t][i] = kv_select((left - (16 * t + i + 1)) >> 31, s[t][i], 0xff800000u);
 }
 
 // Online softmax of a page for a column: its scores -> weights (16-bit pairs), moved
@@ -294,13 +308,12 @@ __device__ __forceinline__ bool kv_softmax(const f32x4 (&s)[4], float C, float& 
 __device__ __forceinline__ uint32_t kv_drop_nan(u32x4& vs) {
     uint32_t bits = 0;
 #pragma unroll
-    for (int t = 0; t < 4; t++)
-#pragma unroll
-        for (int i = 0; i < 4; i++)
-            if (((vs[t] >> (8 * i)) & 255u) == 255u) {
-                bits |= 1u << (4 * t + i);
-                vs[t] &= ~(255u << (8 * i));
-            }
+    for (int t = 0; t < 4; t++) {
+        const uint32_t y = ~vs[t];
+        const uint32_t z = ~(((y & 0x7f7f7f7fu) + 0x7f7f7f7fu) | y | 0x7f7f7f7fu);  // 128 in the bytes that were 255
+        vs[t] &= ~((z >> 7) * 255u);
+        bits |= ((z >> 7 & 1u) | (z >> 14 & 2u) | (z >> 21 & 4u) | (z >> 28 & 8u)) << (4 * t);
+    }
     bits |= __shfl_xor(bits, 4, 64);
     return bits | __shfl_xor(bits, 8, 64);
 }
@@ -310,8 +323,7 @@ __device__ __forceinline__ void kv_set_nan(f32x4 (&s)[4], uint32_t bits) {
 #pragma unroll
     for (int t = 0; t < 4; t++)
 #pragma unroll
-        for (int i = 0; i < 4; i++)
-            if (bits & (1u << (4 * t + i))) s[t][i] = __builtin_nanf("");
+        for (int i = 0; i < 4; i++) s[t][i] = kv_select((int)(bits << (31 - 4 * t - i)) >> 31, s[t][i], 0x7fc00000u);
 }
 
 // Byte B of the codes of eight keys (x[e] of key e) with their scales -> the MFMA
@@ -355,13 +367,11 @@ __device__ void kv_attn(const LtxKvAttnArgs& a) {
     if (it.run > 0 && p0 >= np) return;
 
     // this lane's column: row, query head, keys it sees
-    const int64_t ncol = (int64_t)it.s.n * a.group;
-    const int64_t c0 = (int64_t)it.tile * KV_TILE;
-    const int cols = (int)min((int64_t)KV_TILE, ncol - c0);
-    const int64_t c = min(c0 + r, ncol - 1);
-    const int row = (int)(c / a.group), head = kh * a.group + (int)(c % a.group);
+    const int ncol = it.s.n * a.group, c0 = it.tile * KV_TILE;
+    const int cols = min(KV_TILE, ncol - c0), c = min(c0 + r, ncol - 1);
+    const int row = c / a.group, head = kh * a.group + c % a.group;
     const int mine = kv_limit(a.causal, it.s, row);
-    const int all = kv_limit(a.causal, it.s, (int)(c0 / a.group));  // keys that every column sees
+    const int all = kv_limit(a.causal, it.s, c0 / a.group);  // keys that every column sees
     v8 qf[4];
     const uint16_t* Q = (const uint16_t*)a.q + (size_t)(it.s.s0 + row) * a.ldq + (size_t)head * LTX_HD + 32 * h;
 #pragma unroll
@@ -458,8 +468,7 @@ __device__ void kv_attn(const LtxKvAttnArgs& a) {
 #pragma unroll
         for (int e = 0; e < 8; e++) x[e] = __builtin_fmaf(so[j][col][d0 + e], f, x[e]);
     }
-    const int64_t cc = c0 + col;
-    const int orow = (int)(cc / a.group), ohead = kh * a.group + (int)(cc % a.group);
+    const int cc = c0 + col, orow = cc / a.group, ohead = kh * a.group + cc % a.group;
     if (kv_runs(np, per) > 1) {
         const size_t at = ((size_t)blockIdx.x * a.b.kvh + kh) * KV_TILE + col;
         float* ml = a.part + 2 * at;
@@ -492,8 +501,10 @@ __device__ __forceinline__ void kv_attn_rows(const LtxKvAttnArgs& a) {
     __shared__ __attribute__((aligned(1024))) uint8_t sk[2][16384];
     __shared__ __attribute__((aligned(1024))) uint8_t sv[2][16384];
     __shared__ uint32_t snan[2][2][4];
-    const int tid = threadIdx.x, lane = tid & 63, r = lane & 15, h = lane >> 4;
-    const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+    // (the lane is taken anew where it is needed: what would be derived from it once
+    // and kept through the loop cost more registers than there are)
+    const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    auto my_lane = []() { return opaque_tid() & 63; };
     // the items of a cached head follow each other on one XCD
     const int total = a.items * a.b.kvh, id = (blockIdx.x & 7) * (gridDim.x >> 3) + (blockIdx.x >> 3);
     if (id >= total) return;
@@ -505,60 +516,53 @@ __device__ __forceinline__ void kv_attn_rows(const LtxKvAttnArgs& a) {
     const int p0 = it.run * per, p1 = min(np, p0 + min(per, np));
     if (it.run > 0 && p0 >= np) return;
 
-    const int64_t ncol = (int64_t)it.s.n * a.group;
-    const int64_t c0 = (int64_t)it.tile * a.tile + 16 * NQ * w;  // the wave's first column
+    const int ncol = it.s.n * a.group, c0 = it.tile * a.tile + 16 * NQ * w;  // the wave's first column
     const bool idle = c0 >= ncol;
-    int row[NQ], head[NQ], mine[NQ];
+    // keys that the lane's column of block q sees
+    auto limit_of = [&](int q) {
+        return kv_limit(a.causal, it.s, min(c0 + 16 * q + (my_lane() & 15), ncol - 1) / a.group);
+    };
     v8 qf[NQ][4];
 #pragma unroll
     for (int q = 0; q < NQ; q++) {
-        const int64_t c = min(c0 + 16 * q + r, ncol - 1);
-        row[q] = (int)(c / a.group);
-        head[q] = kh * a.group + (int)(c % a.group);
-        mine[q] = kv_limit(a.causal, it.s, row[q]);
-        const uint16_t* Q =
-            (const uint16_t*)a.q + (size_t)(it.s.s0 + row[q]) * a.ldq + (size_t)head[q] * LTX_HD + 32 * h;
+        const int lane = my_lane(), r = lane & 15, h = lane >> 4;
+        const int c = min(c0 + 16 * q + r, ncol - 1), row = c / a.group;
+        const uint16_t* Q = (const uint16_t*)a.q + (size_t)(it.s.s0 + row) * a.ldq +
+                            (size_t)(kh * a.group + c % a.group) * LTX_HD + 32 * h;
 #pragma unroll
         for (int j = 0; j < 4; j++) qf[q][j] = __builtin_bit_cast(v8, *(const u32x4*)(Q + 8 * j));
     }
-    const int all = kv_limit(a.causal, it.s, (int)(min(c0, ncol - 1) / a.group));  // keys that every column sees
-    const int most = kv_limit(a.causal, it.s, (int)((min(c0 + 16 * NQ, ncol) - 1) / a.group));  // or any does
+    const int all = kv_limit(a.causal, it.s, min(c0, ncol - 1) / a.group);  // keys that every column sees
 
-    // staging: a page's index and flag, 64 pages a lane each
-    int ids = 0;
-    uint32_t flags = 0;
-    auto look_up = [&](int p) {
-        const int at = p + lane;
-        ids = at < p1 ? kv_page(a.b, it.b, at) : 0;
-        const bool none = !kv_in_pool(a.b, ids);
-        if (none) {
-            if (w == 0 && kh == 0) atomicAdd(a.b.bad, 1ull);
-            ids = 0;
-        }
-        flags = a.b.flags[ids] ? 1u : 0u;
-        if (none) flags |= 2u;
-    };
-    u32x4 x0, x1;
-    uint32_t y0, y1, fl[2];  // codes and scales in flight; the flags of their page, and of the page in LDS
-    const int vt = 2 * ((w - 4) >> 1);  // V: first 16-key block of the wave's 32 keys
+    // Staging. A page's index is read two pages before its codes are used, its flag
+    // beside them, by scalar loads (the constant address space: nothing writes them
+    // while the kernel runs); K's waves use x0 and y0. One set of loads for both kinds
+    // of wave: a branch's own would be waited for where the branches meet.
+    typedef const __attribute__((address_space(4))) uint32_t* scalar_ptr;
+    const scalar_ptr table = (scalar_ptr)(uintptr_t)(a.b.pages + (size_t)it.b * a.b.max_pages);
+    const scalar_ptr flags = (scalar_ptr)(uintptr_t)a.b.flags;
+    uint32_t next = p0 < p1 ? table[p0] : 0u;  // index of the page whose codes come next
+    u32x4 x0, x1;                              // its codes and scales
+    uint32_t y0, y1, flag = 0, none = 0;       // its flag, or that it is outside the pool
+    uint32_t flag_s = 0, none_s = 0;           // those of the page in LDS
+    const int vt = 2 * ((w - 4) >> 1);         // V: first 16-key block of the wave's 32 keys
+    const uint32_t ox = w < 4 ? 1024 * w : LTX_KV_V + 1024 * vt, dx = w < 4 ? 0 : 1024;
+    const uint32_t oy = w < 4 ? LTX_KV_KS : LTX_KV_VS + 4 * vt, is_k = w < 4 ? ~0u : 0u;
     auto load = [&](int p) {
-        if (((p - p0) & 63) == 0) look_up(p);
-        const int l = (p - p0) & 63;
-        const int page = __builtin_amdgcn_readlane(ids, l);
-        fl[0] = __builtin_amdgcn_readlane(flags, l);
+        none = next < (uint32_t)a.b.pool ? 0u : 1u;
+        const uint32_t page = none ? 0u : next, lane = my_lane();
+        if (none && w == 0 && kh == 0 && lane == 0) atomicAdd(a.b.bad, 1ull);
         const uint8_t* blk = a.b.data + kv_block(a.b, page, kh);
-        if (w < 4) {
-            x0 = *(const u32x4*)(blk + 1024 * w + 16 * lane);
-            y0 = *(const uint32_t*)(blk + LTX_KV_KS + 4 * lane);
-        } else {
-            x0 = *(const u32x4*)(blk + LTX_KV_V + 1024 * vt + 16 * lane);
-            x1 = *(const u32x4*)(blk + LTX_KV_V + 1024 * vt + 1024 + 16 * lane);
-            const u32x2 y = *(const u32x2*)(blk + LTX_KV_VS + 64 * (r >> 2) + 16 * h + 4 * vt);
-            y0 = y[0];
-            y1 = y[1];
-        }
+        x0 = *(const u32x4*)(blk + ox + 16 * lane);
+        x1 = *(const u32x4*)(blk + ox + dx + 16 * lane);
+        const uint32_t at = oy + (((4 * lane) & is_k) | (((lane & 12) << 4 | (lane & 48)) & ~is_k));
+        y0 = *(const uint32_t*)(blk + at);
+        y1 = *(const uint32_t*)(blk + at + 4);
+        flag = flags[page];
+        next = p + 1 < p1 ? table[p + 1] : 0u;
     };
     auto stage = [&](int buf) {
+        const int lane = my_lane();
         if (w < 4) {
             const float f = __builtin_bit_cast(float, ((y0 >> (8 * w)) & 255u) << 23);
 #pragma unroll
@@ -567,12 +571,12 @@ __device__ __forceinline__ void kv_attn_rows(const LtxKvAttnArgs& a) {
                     u32x4{Fp4<T>::template pair<0>(x0[j], f), Fp4<T>::template pair<1>(x0[j], f),
                           Fp4<T>::template pair<2>(x0[j], f), Fp4<T>::template pair<3>(x0[j], f)};
         } else {
-            if (fl[0] & 1u) {
+            if (flag) {
                 u32x4 vs = {y0, y1, 0, 0};
                 const uint32_t bits = kv_drop_nan(vs);
                 y0 = vs[0];
                 y1 = vs[1];
-                if ((w & 1) == 0 && r == 0) snan[buf][vt >> 1][h] = bits;
+                if ((w & 1) == 0 && (lane & 15) == 0) snan[buf][vt >> 1][lane >> 4] = bits;
             }
             const uint32_t x[8] = {x0[0], x0[1], x0[2], x0[3], x1[0], x1[1], x1[2], x1[3]}, f[2] = {y0, y1};
             uint8_t* d = sv[buf] + 1024 * (4 * vt) + 16 * lane;
@@ -595,8 +599,9 @@ __device__ __forceinline__ void kv_attn_rows(const LtxKvAttnArgs& a) {
         }
     };
 
-    f32x4 o[8][NQ];
-    float m[NQ], l[NQ];
+    f32x4 o[8][NQ], s[NQ][4];  // O^T, S^T
+    v8 pf[NQ][2];
+    float m[NQ], l[NQ];  // running maximum (times C) and sum
 #pragma unroll
     for (int q = 0; q < NQ; q++) {
 #pragma unroll
@@ -605,81 +610,147 @@ __device__ __forceinline__ void kv_attn_rows(const LtxKvAttnArgs& a) {
         l[q] = 0.f;
     }
     const float C = a.scale_log2;
-    if (p0 < p1) {
+    const int nt = max(p1 - p0, 0);
+
+    auto sync = [&]() {
+        __builtin_amdgcn_sched_barrier(0);
+        asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    auto pv = [&](int t) {
+        const uint8_t* b = sv[t & 1] + 16 * my_lane();
+#pragma unroll
+        for (int c = 0; c < 2; c++)
+#pragma unroll
+            for (int db = 0; db < 8; db++) {
+                const v8 vf = __builtin_bit_cast(v8, *(const u32x4*)(b + 1024 * (8 * c + db)));
+#pragma unroll
+                for (int q = 0; q < NQ; q++) o[db][q] = Op<T>::mfma16(vf, pf[q][c], o[db][q]);
+            }
+    };
+    auto scores = [&](int t) {
+        const uint8_t* b = sk[t & 1] + 16 * my_lane();
+#pragma unroll
+        for (int j = 0; j < 4; j++)
+#pragma unroll
+            for (int x = 0; x < 4; x++) {
+                const v8 kf = __builtin_bit_cast(v8, *(const u32x4*)(b + 1024 * (4 * x + j)));
+#pragma unroll
+                for (int q = 0; q < NQ; q++) s[q][x] = Op<T>::mfma16(kf, qf[q][j], j == 0 ? f32x4{0} : s[q][x]);
+            }
+    };
+    // PV(t - 1), then S(t); the operands' reads run four ahead of their products
+    // (masks: 0x100 DS read, 0x008 MFMA)
+    auto products = [&](int t) {
+        if (idle) return;
+        __builtin_amdgcn_s_setprio(1);
+        pv(t - 1);
+        scores(t);
+        __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
+#pragma unroll
+        for (int i = 0; i < 32; i++) {
+            __builtin_amdgcn_sched_group_barrier(0x008, NQ, 0);
+            if (i < 28) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+        }
+        __builtin_amdgcn_s_setprio(0);
+    };
+    // scores -> weights with maximum mc, and their sum
+    auto weights = [&](int q, float mc) {
+        float sum = 0.f;
+#pragma unroll
+        for (int c = 0; c < 2; c++) {
+            u32x4 pw;
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const f32x4& x = s[q][2 * c + (e >> 1)];
+                const int i = 2 * (e & 1);
+                pw[e] = Op<T>::cvt2(__builtin_amdgcn_exp2f(__builtin_fmaf(x[i], C, -mc)),
+                                    __builtin_amdgcn_exp2f(__builtin_fmaf(x[i + 1], C, -mc)));
+                sum = Op<T>::sum2(pw[e], sum);
+            }
+            pf[q][c] = __builtin_bit_cast(v8, pw);
+        }
+        return sum;
+    };
+    auto softmax = [&](int t) {
+        const int p = p0 + t;
+        if (idle) return;
+        if (flag_s) {
+            const int h = my_lane() >> 4;
+            const uint32_t bits = snan[t & 1][0][h] | snan[t & 1][1][h] << 8;
+#pragma unroll
+            for (int q = 0; q < NQ; q++) kv_set_nan(s[q], bits);
+        }
+        if (none_s || (p + 1) * LTX_KV_PAGE > all)
+#pragma unroll
+            for (int q = 0; q < NQ; q++) kv_mask(s[q], p, none_s ? 0 : limit_of(q), my_lane() >> 4);
+#pragma unroll
+        for (int q = 0; q < NQ; q++) {
+            // weights with the maximum so far; only where a column's sum of them is
+            // beyond 2^8 (as it is before it has had a score: m is -inf) the page's
+            // maximum is taken, m moved, and the weights formed again
+            float sum = weights(q, m[q]);
+            if (__builtin_amdgcn_ballot_w64(!(sum <= 256.f)) != 0) {
+                float mx = s[q][0][0];
+#pragma unroll
+                for (int x = 0; x < 4; x++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++) mx = fmaxf(mx, s[q][x][i]);
+                const float mn = fmaxf(m[q], kv_quad_max(mx) * C), mz = mn == -__builtin_inff() ? 0.f : mn;
+                const float corr = __builtin_amdgcn_exp2f(m[q] - mz);
+                m[q] = mn;
+                l[q] *= corr;
+#pragma unroll
+                for (int db = 0; db < 8; db++) o[db][q] *= corr;
+                sum = weights(q, mz);
+            }
+            l[q] += sum;
+        }
+    };
+
+    // Two groups of waves a phase apart: while one runs its products, the other runs
+    // its softmax and stages (group 0 the next page's K, group 1 the next page's V),
+    // so that each SIMD's matrix and vector units both have work. Phase 2 t + group:
+    // products(t), phase 2 t + 1 + group: softmax(t).
+    //   K(t + 1) written in phase 2 t + 1, read in 2 t + 2 and 2 t + 3; V(t + 1)
+    //   written in 2 t + 2, read in 2 t + 4 and 2 t + 5; and K(t - 1)'s and V(t -
+    //   1)'s buffers, which they take, were last read in 2 t - 1 and 2 t + 1.
+    if (nt > 0) {
+        const int group = w >> 2;
         load(p0);
         stage(0);
-        fl[1] = fl[0];
-        if (p0 + 1 < p1) load(p0 + 1);
-    }
-    __syncthreads();
-    for (int p = p0; p < p1; p++) {
-        const int buf = (p - p0) & 1;
-        const uint32_t flag = fl[1];
-        const bool busy = !idle && p * LTX_KV_PAGE < most;
-        f32x4 s[NQ][4];
-        if (busy) {
-#pragma unroll
-            for (int q = 0; q < NQ; q++)
-#pragma unroll
-                for (int t = 0; t < 4; t++) s[q][t] = f32x4{0};
-#pragma unroll
-            for (int j = 0; j < 4; j++)
-#pragma unroll
-                for (int t = 0; t < 4; t++) {
-                    const v8 kf = __builtin_bit_cast(v8, *(const u32x4*)(sk[buf] + 1024 * (4 * t + j) + 16 * lane));
-#pragma unroll
-                    for (int q = 0; q < NQ; q++) s[q][t] = Op<T>::mfma16(kf, qf[q][j], s[q][t]);
-                }
+        flag_s = flag, none_s = none;
+        if (nt > 1) load(p0 + 1);
+        sync();
+        if (group) sync();
+        if (!idle) scores(0);
+        sync();
+#pragma nounroll
+        for (int t = 0; t + 1 < nt; t++) {
+            softmax(t);
+            stage((t + 1) & 1);
+            flag_s = flag, none_s = none;
+            if (t + 2 < nt) load(p0 + t + 2);
+            sync();
+            products(t + 1);
+            sync();
         }
-        // the next page into the other buffer, the one after it on its way
-        if (p + 1 < p1) {
-            stage(buf ^ 1);
-            fl[1] = fl[0];
-            if (p + 2 < p1) load(p + 2);
-        }
-        if (busy) {
-            if (flag & 1u) {
-                const uint32_t bits = snan[buf][0][h] | snan[buf][1][h] << 8;
-#pragma unroll
-                for (int q = 0; q < NQ; q++) kv_set_nan(s[q], bits);
-            }
-            if ((flag & 2u) || (p + 1) * LTX_KV_PAGE > all)
-#pragma unroll
-                for (int q = 0; q < NQ; q++) kv_mask(s[q], p, flag & 2u ? 0 : mine[q], h);
-            v8 pf[NQ][2];
-#pragma unroll
-            for (int q = 0; q < NQ; q++) {
-                uint32_t pw[4][2];
-                float corr;
-                if (kv_softmax<T>(s[q], C, m[q], l[q], pw, corr))
-#pragma unroll
-                    for (int db = 0; db < 8; db++) o[db][q] *= corr;
-#pragma unroll
-                for (int c = 0; c < 2; c++)
-                    pf[q][c] = __builtin_bit_cast(v8, (u32x4){pw[2 * c][0], pw[2 * c][1], pw[2 * c + 1][0],
-                                                              pw[2 * c + 1][1]});
-            }
-#pragma unroll
-            for (int c = 0; c < 2; c++)
-#pragma unroll
-                for (int db = 0; db < 8; db++) {
-                    const v8 vf = __builtin_bit_cast(v8, *(const u32x4*)(sv[buf] + 1024 * (8 * c + db) + 16 * lane));
-#pragma unroll
-                    for (int q = 0; q < NQ; q++) o[db][q] = Op<T>::mfma16(vf, pf[q][c], o[db][q]);
-                }
-        }
-        __syncthreads();
+        softmax(nt - 1);
+        sync();
+        if (!idle) pv(nt - 1);
+        if (!group) sync();
     }
 
     if (idle) return;
     const bool whole = kv_runs(np, per) == 1;
 #pragma unroll
     for (int q = 0; q < NQ; q++) {
-        if (c0 + 16 * q + r >= ncol) continue;
+        const int lane = my_lane(), h = lane >> 4, c = c0 + 16 * q + (lane & 15);
+        if (c >= ncol) continue;
         float lt = l[q] + __shfl_xor(l[q], 16, 64);
         lt += __shfl_xor(lt, 32, 64);
         if (!whole) {
-            const size_t at = ((size_t)item * a.b.kvh + kh) * a.tile + 16 * (NQ * w + q) + r;
+            const size_t at = ((size_t)item * a.b.kvh + kh) * a.tile + (c - it.tile * a.tile);
             float* po = a.part + 2 * (size_t)a.items * a.b.kvh * a.tile + at * LTX_HD + 32 * h;
             if (h == 0) *(f32x2*)(a.part + 2 * at) = f32x2{m[q], lt};
 #pragma unroll
@@ -689,10 +760,10 @@ __device__ __forceinline__ void kv_attn_rows(const LtxKvAttnArgs& a) {
             }
             continue;
         }
-        const int grow = it.s.s0 + row[q];
-        const float g = a.glog ? 2.0f * sigmoid_f(a.glog[(size_t)grow * a.heads + head[q]]) : 1.0f;
-        const float f = mine[q] > 0 ? g / lt : 0.f;
-        uint16_t* out = (uint16_t*)a.out + (size_t)grow * a.ldo + (size_t)head[q] * LTX_HD + 32 * h;
+        const int row = it.s.s0 + c / a.group, head = kh * a.group + c % a.group;
+        const float g = a.glog ? 2.0f * sigmoid_f(a.glog[(size_t)row * a.heads + head]) : 1.0f;
+        const float f = limit_of(q) > 0 ? g / lt : 0.f;
+        uint16_t* out = (uint16_t*)a.out + (size_t)row * a.ldo + (size_t)head * LTX_HD + 32 * h;
 #pragma unroll
         for (int i = 0; i < 4; i++) {
             u32x4 v;
