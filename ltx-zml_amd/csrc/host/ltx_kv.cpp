@@ -1,4 +1,5 @@
 // The 4-bit key/value cache: its handle, rows written and read back, attention.
+#include <algorithm>
 #include <cstdlib>
 #include <cstring>
 
@@ -54,7 +55,7 @@ void kv_rows(ltx_ctx* c, const ltx_kv_cache* k, const ltx_kv_batch* b, void* kp,
 
 struct AttnPlan {
     int nq = 0;  // 0: the kernel of few columns (16 a tile), else 128 nq a tile
-    int tile = 16, least = 4, slots = 0, items = 0;
+    int tile = 16, least = 4, slots = 0, items = 0, parts = 0;
     size_t bytes = 0;  // of partial results
 };
 
@@ -63,22 +64,33 @@ AttnPlan attn_plan(const ltx_ctx* c, const ltx_kv_cache* k, const ltx_kv_batch* 
     AttnPlan p;
     int forced = -1;
     if (const char* e = std::getenv("KVNQ")) forced = std::atoi(e);
-    int target = 4;
-    if (const char* e = std::getenv("KVTARGET")) target = std::atoi(e);
+    int target = 2;
     p.nq = forced >= 0 ? forced : columns <= 32 * (int64_t)b->nseq ? 0 : columns * k->kv_heads <= 128ll * c->num_cu ? 1 : 2;
     if (p.nq) {
         p.tile = 128 * p.nq;
         p.least = 8;
         target = 1;
     }
+    if (const char* e = std::getenv("KVTARGET")) target = std::atoi(e);
     if (const char* e = std::getenv("KVLEAST")) p.least = std::atoi(e);
-    const int64_t tiles = columns / p.tile + b->nseq;
-    // (as many workgroups without a split: none pays)
-    if (split && b->max_pages > p.least && (p.nq == 0 || columns / p.tile * k->kv_heads < c->num_cu)) p.slots = (target * c->num_cu + k->kv_heads - 1) / k->kv_heads;
+    // tiles of the batch, at most
+    const int64_t tiles = !b->row_start || b->nseq == 1
+                              ? (int64_t)b->nseq * ((columns / b->nseq + p.tile - 1) / p.tile)
+                              : columns / p.tile + b->nseq;
     // the grids' limit, 2^32 threads along x; columns stay in 31 bits
-    if (tiles + p.slots >= (1 << 23) / k->kv_heads || columns >= 1 << 30 || b->rows >= 1 << 24) throw Error("too many rows for one call");
-    p.items = (int)(tiles + p.slots);
-    if (p.slots) p.bytes = (size_t)p.items * k->kv_heads * p.tile * (LTX_HD + 2) * sizeof(float);
+    if (tiles >= (1 << 22) / k->kv_heads || columns >= 1 << 30 || b->rows >= 1 << 24)
+        throw Error("too many rows for one call");
+    // A split where the tiles are fewer than the CUs take in a round and their pages
+    // (units, which are counted in 32 bits) are more than a least item each
+    const int64_t round = ((int64_t)target * c->num_cu + k->kv_heads - 1) / k->kv_heads, units = tiles * b->max_pages;
+    const bool few = p.nq == 0 || columns / p.tile * k->kv_heads < c->num_cu;
+    if (split && few && b->max_pages > p.least && units < 1ll << 31)
+        p.slots = (int)std::min(round, (units + p.least - 1) / p.least);
+    p.items = p.slots ? p.slots : (int)tiles;
+    if (p.slots) {
+        p.parts = (int)(p.slots + tiles);
+        p.bytes = (size_t)p.parts * k->kv_heads * p.tile * (LTX_HD + 2) * sizeof(float);
+    }
     return p;
 }
 
@@ -201,16 +213,18 @@ int ltx_op_kv_attention(ltx_ctx* c, const ltx_kv_cache* cache, const ltx_kv_batc
         a.least = p.least;
         a.slots = p.slots;
         a.items = p.items;
+        a.parts = p.parts;
         a.scale_log2 = 0.12751743f;  // log2(e) / sqrt(128)
         const bool f16 = cache->mode == LTX_MODE_F16;
-        if (p.nq == 0)
+        if (p.nq == 0) {
             c->launch(f16 ? "ltx_kv_attn_f16" : "ltx_kv_attn_bf16", p.items, cache->kv_heads, 1, 256, &a, st);
-        else
-            c->launch(p.nq == 1 ? (f16 ? "ltx_kv_attn_f16_rows1" : "ltx_kv_attn_bf16_rows1")
-                                : (f16 ? "ltx_kv_attn_f16_rows2" : "ltx_kv_attn_bf16_rows2"),
-                      (unsigned)(((int64_t)p.items * cache->kv_heads + 7) / 8 * 8), 1, 1, 512, &a, st);
+        } else {
+            const std::string name = std::string(f16 ? "ltx_kv_attn_f16_rows" : "ltx_kv_attn_bf16_rows") +
+                                     (p.nq == 1 ? "1" : "2") + (p.slots ? "_split" : "");
+            c->launch(name.c_str(), (unsigned)(((int64_t)p.items * cache->kv_heads + 7) / 8 * 8), 1, 1, 512, &a, st);
+        }
         if (p.slots)
-            c->launch(f16 ? "ltx_kv_join_f16" : "ltx_kv_join_bf16", batch->rows, (heads + 3) / 4, 1, 256, &a, st);
+            c->launch(f16 ? "ltx_kv_join_f16" : "ltx_kv_join_bf16", batch->rows, heads, 1, 256, &a, st);
     })
 }
 

@@ -170,77 +170,105 @@ KV_ROWS(ltx_kv_read_f16, _Float16, false)
 KV_ROWS(ltx_kv_read_bf16, __bf16, false)
 
 // ---- attention ------------------------------------------------------------------
-// Items. The rows of a sequence times the query heads of a cached head are its
-// columns c = i * group + g; a tile is `tile` of them. Its keys are split into runs
-// of `per` pages, the same for all sequences: as many as make about `slots` items of
-// a cached head in all. Every wave works the split out from the batch's lengths, so
-// lengths may change behind one launch (a graph's), and a table may be wider than
-// what is in use. Items: sequence by sequence, tile by tile, run by run.
-struct KvItem {
-    int b, tile, run;
+// The rows of a sequence times the query heads of a cached head are its columns c =
+// i * group + g; a tile is a.tile of them. Where there are few tiles, `slots` items of
+// a cached head share all pages of all tiles, in order and `per` each: the k-th item
+// takes units k per .. + per - 1 of them, parts of one tile or of several (a span
+// each). So every item has the same work, whatever the lengths, and one round of
+// workgroups does it. Each wave works the split out from the batch's arrays: lengths
+// may change behind one launch (a graph's), and a table may be wider than what is in
+// use. A tile that one item does whole is written by it; the partial result of item k
+// for the e-th tile lies at k + e, and kv_join puts them together.
+struct KvSpan {
+    int b, tile, tiles;  // the tile, of the sequence's
+    int page, pages;     // first unit of the span and units of the tile
+    int entity;          // the tile's number in the batch
+    int left;            // units left to the item
     KvSeq s;
 };
 
-__device__ __forceinline__ uint64_t wave_sum(uint64_t v) {
-    for (int o = 32; o > 0; o >>= 1) v += __shfl_xor((unsigned long long)v, o, 64);
-    return v;
+__device__ __forceinline__ uint32_t wave_scan(uint32_t x) {  // inclusive sums over the lanes
+    x += __builtin_amdgcn_update_dpp(0, (int)x, 0x111, 0xf, 0xf, false);
+    x += __builtin_amdgcn_update_dpp(0, (int)x, 0x112, 0xf, 0xf, false);
+    x += __builtin_amdgcn_update_dpp(0, (int)x, 0x114, 0xf, 0xf, false);
+    x += __builtin_amdgcn_update_dpp(0, (int)x, 0x118, 0xf, 0xf, false);
+    x += __builtin_amdgcn_update_dpp(0, (int)x, 0x142, 0xa, 0xf, false);  // lane 15's to 16 .. 31, 47's to 48 .. 63
+    x += __builtin_amdgcn_update_dpp(0, (int)x, 0x143, 0xc, 0xf, false);  // lane 31's to 32 .. 63
+    return x;
 }
 
-// pages a run
-__device__ __forceinline__ int kv_per(const LtxKvAttnArgs& a) {
-    if (a.slots == 0) return KV_NO_SPLIT;
-    const int lane = threadIdx.x & 63;
-    uint64_t w = 0;
-    if (a.b.nseq == 1) {
-        const KvSeq s = kv_seq_all(a.b, 0);
-        w = (uint64_t)kv_tiles(s.n, a.group, a.tile) * kv_pages(s.L);
-    } else {
-        for (int b = lane; b < a.b.nseq; b += 64) {
-            const KvSeq s = kv_seq(a.b, b);
-            w += (uint64_t)kv_tiles(s.n, a.group, a.tile) * kv_pages(s.L);
-        }
-        w = wave_sum(w);
-    }
-    return __builtin_amdgcn_readfirstlane(kv_per_of(w, a.slots, a.least));
+// Sequence base + lane, and what it adds to the tiles and units before the next one
+struct KvLane {
+    KvSeq s;
+    uint32_t tiles, units, tiles_to, units_to;  // its own, and inclusive sums from `base` on
+};
+__device__ __forceinline__ KvLane kv_lane(const LtxKvAttnArgs& a, int base) {
+    const int b = base + (threadIdx.x & 63);
+    KvLane k;
+    k.s = KvSeq{0, 0, 0};
+    if (b < a.b.nseq) k.s = kv_seq(a.b, b);
+    k.tiles = kv_tiles(k.s.n, a.group, a.tile);
+    k.units = a.slots ? k.tiles * (uint32_t)kv_units(k.s.L) : k.tiles;
+    k.tiles_to = wave_scan(k.tiles);
+    k.units_to = wave_scan(k.units);
+    return k;
+}
+__device__ __forceinline__ uint32_t lane_of(uint32_t x, int l) { return __builtin_amdgcn_readlane(x, l); }
+
+// units an item: `first` is kv_lane(a, 0)
+__device__ __forceinline__ int kv_per(const LtxKvAttnArgs& a, const KvLane& first) {
+    if (!a.slots) return 1;
+    uint32_t units = lane_of(first.units_to, 63);
+    for (int base = 64; base < a.b.nseq; base += 64) units += lane_of(kv_lane(a, base).units_to, 63);
+    return kv_per_of(units, a.slots, a.least);
 }
 
-// The item's sequence, tile and run; false: there is none. A sequence's last tile,
-// which sees the most keys where the mask is causal, comes first.
-__device__ __forceinline__ bool kv_item(const LtxKvAttnArgs& a, int per, int item, KvItem& it) {
-    if (a.b.nseq == 1) {
-        it.b = 0;
-    } else {
-        const int lane = threadIdx.x & 63;
-        it.b = -1;
-        for (int base = 0; base < a.b.nseq; base += 64) {
-            int c = 0;
-            if (base + lane < a.b.nseq) {
-                const KvSeq s = kv_seq(a.b, base + lane);
-                c = kv_tiles(s.n, a.group, a.tile) * kv_runs(kv_pages(s.L), per);
-            }
-            int sum = c;
-            for (int o = 1; o < 64; o <<= 1) {
-                const int up = __shfl_up(sum, o, 64);
-                if (lane >= o) sum += up;
-            }
-            const uint64_t here = __builtin_amdgcn_ballot_w64(item < sum && item >= sum - c);
-            if (here) {
-                const int l = __builtin_ctzll(here);
-                it.b = base + l;
-                item -= __shfl(sum - c, l, 64);
-                break;
-            }
-            item -= __shfl(sum, 63, 64);
+// The item's first span; false: there is none. Without a split an item is a tile, a
+// sequence's last one, which sees the most keys where the mask is causal, first.
+__device__ __forceinline__ bool kv_begin(const LtxKvAttnArgs& a, int item, KvSpan& it) {
+    KvLane k = kv_lane(a, 0);
+    it.left = kv_per(a, k);
+    const uint64_t first = (uint64_t)item * it.left;
+    if (first >> 32) return false;
+    uint32_t u = (uint32_t)first, entities = 0;
+    for (int base = 0; base < a.b.nseq; base += 64) {
+        if (base) k = kv_lane(a, base);
+        const uint64_t here = __builtin_amdgcn_ballot_w64(u < k.units_to && u >= k.units_to - k.units);
+        if (here) {
+            const int l = __builtin_ctzll(here);
+            u -= lane_of(k.units_to - k.units, l);
+            it.b = base + l;
+            it.s = KvSeq{(int)lane_of(k.s.s0, l), (int)lane_of(k.s.n, l), (int)lane_of(k.s.L, l)};
+            it.tiles = lane_of(k.tiles, l);
+            it.pages = kv_units(it.s.L);
+            it.tile = a.slots ? (int)(u / (uint32_t)it.pages) : it.tiles - 1 - (int)u;
+            it.page = a.slots ? (int)(u % (uint32_t)it.pages) : 0;
+            it.entity = (int)(entities + lane_of(k.tiles_to - k.tiles, l)) + it.tile;
+            if (!a.slots) it.left = it.pages;
+            return true;
         }
-        it.b = __builtin_amdgcn_readfirstlane(it.b);
-        item = __builtin_amdgcn_readfirstlane(item);
-        if (it.b < 0) return false;
+        u -= lane_of(k.units_to, 63);
+        entities += lane_of(k.tiles_to, 63);
     }
-    it.s = kv_seq_all(a.b, it.b);
-    const int runs = kv_runs(kv_pages(it.s.L), per);
-    it.tile = kv_tiles(it.s.n, a.group, a.tile) - 1 - item / runs;
-    it.run = item % runs;
-    return it.tile >= 0;
+    return false;
+}
+// units of the span
+__device__ __forceinline__ int kv_span(const KvSpan& it) { return min(it.left, it.pages - it.page); }
+// the next one
+__device__ __forceinline__ bool kv_next(const LtxKvAttnArgs& a, KvSpan& it) {
+    it.left -= kv_span(it);
+    if (it.left <= 0 || !a.slots) return false;
+    it.page = 0;
+    it.entity++;
+    if (++it.tile < it.tiles) return true;
+    it.tile = 0;
+    while (++it.b < a.b.nseq) {
+        it.s = kv_seq_all(a.b, it.b);
+        it.tiles = kv_tiles(it.s.n, a.group, a.tile);
+        it.pages = kv_units(it.s.L);
+        if (it.tiles > 0) return true;
+    }
+    return false;
 }
 
 __device__ __forceinline__ float kv_quad_max(float x) {  // over lanes l, l ^ 16, l ^ 32, l ^ 48
@@ -351,151 +379,178 @@ __device__ __forceinline__ void kv_v_pair(const uint32_t (&x)[8], const uint32_t
 // 8 r .. + 7 of the keys 16 t + 4 h + i that its scores belong to, 16 scales in one
 // load. MFMA db of O^T has dim 8 r + db in row r. All loads are contiguous over the
 // lanes.
+// A wave's next page is on its way while it computes on one, its index read a page
+// earlier still.
 template <typename T>
-__device__ void kv_attn(const LtxKvAttnArgs& a) {
+__device__ __forceinline__ void kv_attn(const LtxKvAttnArgs& a) {
     typedef typename Op<T>::v8 v8;
     __shared__ __attribute__((aligned(16))) float so[4][KV_TILE][LTX_HD + 4];
     __shared__ float sm[4][KV_TILE], sl[4][KV_TILE];
     const int tid = threadIdx.x, lane = tid & 63, r = lane & 15, h = lane >> 4;
     const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int kh = blockIdx.y;
-    const int per = kv_per(a);
-    KvItem it;
-    if (!kv_item(a, per, blockIdx.x, it)) return;
-    const int limit = kv_tile_limit(a.causal, it.s, a.group, it.tile, KV_TILE), np = kv_pages(limit);
-    const int p0 = it.run * per, p1 = min(np, p0 + min(per, np));
-    if (it.run > 0 && p0 >= np) return;
-
-    // this lane's column: row, query head, keys it sees
-    const int ncol = it.s.n * a.group, c0 = it.tile * KV_TILE;
-    const int cols = min(KV_TILE, ncol - c0), c = min(c0 + r, ncol - 1);
-    const int row = c / a.group, head = kh * a.group + c % a.group;
-    const int mine = kv_limit(a.causal, it.s, row);
-    const int all = kv_limit(a.causal, it.s, c0 / a.group);  // keys that every column sees
-    v8 qf[4];
-    const uint16_t* Q = (const uint16_t*)a.q + (size_t)(it.s.s0 + row) * a.ldq + (size_t)head * LTX_HD + 32 * h;
-#pragma unroll
-    for (int j = 0; j < 4; j++) qf[j] = __builtin_bit_cast(v8, *(const u32x4*)(Q + 8 * j));
-
-    f32x4 o[8];
-#pragma unroll
-    for (int db = 0; db < 8; db++) o[db] = f32x4{0};
-    float m = -__builtin_inff(), l = 0.f;
     const float C = a.scale_log2;
-    for (int p = p0 + w; p < p1; p += 4) {
-        int page = __builtin_amdgcn_readfirstlane(kv_page(a.b, it.b, p));
-        const bool none = !kv_in_pool(a.b, page);
-        if (none) {  // a page outside the pool: its keys are left out
-            if (lane == 0 && kh == 0) atomicAdd(a.b.bad, 1ull);
-            page = 0;
-        }
-        const uint8_t* blk = a.b.data + kv_block(a.b, page, kh);
-        const uint32_t flag = a.b.flags[page];
-        u32x4 kc[4], vc[4];
-#pragma unroll
-        for (int t = 0; t < 4; t++) {
-            kc[t] = *(const u32x4*)(blk + 1024 * t + 16 * lane);
-            vc[t] = *(const u32x4*)(blk + LTX_KV_V + 1024 * t + 16 * lane);
-        }
-        const uint32_t ks = *(const uint32_t*)(blk + LTX_KV_KS + 4 * lane);
-        u32x4 vs = *(const u32x4*)(blk + LTX_KV_VS + 64 * (r >> 2) + 16 * h);
+    // (the constant address space: scalar loads; nothing writes them while this runs)
+    typedef const __attribute__((address_space(4))) uint32_t* scalar_ptr;
+    const scalar_ptr flags = (scalar_ptr)(uintptr_t)a.b.flags;
+    KvSpan it;
+    if (!kv_begin(a, blockIdx.x, it)) return;
+    do {
+        const int limit = kv_tile_limit(a.causal, it.s, a.group, it.tile, KV_TILE), np = kv_pages(limit);
+        const int p0 = it.page, units = kv_span(it), p1 = min(np, p0 + units);
+        const scalar_ptr table = (scalar_ptr)(uintptr_t)(a.b.pages + (size_t)it.b * a.b.max_pages);
+        uint32_t next = p0 + w < p1 ? table[p0 + w] : 0u;
 
-        f32x4 s[4];
+        // this lane's column: row, query head, keys it sees
+        const int ncol = it.s.n * a.group, c0 = it.tile * KV_TILE;
+        const int cols = min(KV_TILE, ncol - c0), c = min(c0 + r, ncol - 1);
+        const int row = c / a.group, head = kh * a.group + c % a.group;
+        const int mine = kv_limit(a.causal, it.s, row);
+        const int all = kv_limit(a.causal, it.s, c0 / a.group);  // keys that every column sees
+        v8 qf[4];
+        const uint16_t* Q = (const uint16_t*)a.q + (size_t)(it.s.s0 + row) * a.ldq + (size_t)head * LTX_HD + 32 * h;
 #pragma unroll
-        for (int t = 0; t < 4; t++) {
-            const float f = scale_of(ks, t);
-            s[t] = f32x4{0};
+        for (int j = 0; j < 4; j++) qf[j] = __builtin_bit_cast(v8, *(const u32x4*)(Q + 8 * j));
+
+        f32x4 o[8];
+#pragma unroll
+        for (int db = 0; db < 8; db++) o[db] = f32x4{0};
+        float m = -__builtin_inff(), l = 0.f;
+        struct Page {
+            u32x4 k[4], v[4], vs;
+            uint32_t ks, flag;
+            bool none;
+        };
+        auto load = [&](Page& x, int p) {
+            if (p >= p1) return;
+            x.none = next >= (uint32_t)a.b.pool;
+            const uint32_t page = x.none ? 0u : next;
+            // a page outside the pool: its keys are left out
+            if (x.none && lane == 0 && kh == 0) atomicAdd(a.b.bad, 1ull);
+            const uint8_t* blk = a.b.data + kv_block(a.b, page, kh);
+            x.flag = flags[page];
+#pragma unroll
+            for (int t = 0; t < 4; t++) x.k[t] = *(const u32x4*)(blk + 1024 * t + 16 * lane);
+            x.ks = *(const uint32_t*)(blk + LTX_KV_KS + 4 * lane);
+#pragma unroll
+            for (int t = 0; t < 4; t++) x.v[t] = *(const u32x4*)(blk + LTX_KV_V + 1024 * t + 16 * lane);
+            x.vs = *(const u32x4*)(blk + LTX_KV_VS + 64 * (r >> 2) + 16 * h);
+            next = p + 4 < p1 ? table[p + 4] : 0u;
+            __builtin_amdgcn_sched_barrier(0);
+        };
+        auto compute = [&](Page& x, int p) {
+            f32x4 s[4];
+#pragma unroll
+            for (int t = 0; t < 4; t++) {
+                const float f = scale_of(x.ks, t);
+                s[t] = f32x4{0};
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    const uint32_t y = x.k[t][j];
+                    const u32x4 d = {Fp4<T>::template pair<0>(y, f), Fp4<T>::template pair<1>(y, f),
+                                     Fp4<T>::template pair<2>(y, f), Fp4<T>::template pair<3>(y, f)};
+                    s[t] = Op<T>::mfma16(__builtin_bit_cast(v8, d), qf[j], s[t]);
+                }
+            }
+            __builtin_amdgcn_sched_barrier(0);
+            if (x.flag) kv_set_nan(s, kv_drop_nan(x.vs));
+            if (x.none || (p + 1) * LTX_KV_PAGE > all) kv_mask(s, p, x.none ? 0 : mine, h);
+            uint32_t pw[4][2];
+            float corr;
+            if (kv_softmax<T>(s, C, m, l, pw, corr))
+#pragma unroll
+                for (int db = 0; db < 8; db++) o[db] *= corr;
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int cc = 0; cc < 2; cc++) {
+                const v8 pf = __builtin_bit_cast(v8, (u32x4){pw[2 * cc][0], pw[2 * cc][1], pw[2 * cc + 1][0],
+                                                             pw[2 * cc + 1][1]});
+                uint32_t y[8], f[2] = {x.vs[2 * cc], x.vs[2 * cc + 1]};
+#pragma unroll
+                for (int e = 0; e < 8; e++) y[e] = x.v[2 * cc + (e >> 2)][e & 3];
+                auto two = [&](auto B) {  // dims 8 r + 2 B and + 1: eight keys each
+                    constexpr int b = decltype(B)::value;
+                    u32x4 lo, hi;
+                    kv_v_pair<T, b>(y, f, lo, hi);
+                    o[2 * b] = Op<T>::mfma16(__builtin_bit_cast(v8, lo), pf, o[2 * b]);
+                    o[2 * b + 1] = Op<T>::mfma16(__builtin_bit_cast(v8, hi), pf, o[2 * b + 1]);
+                };
+                two(std::integral_constant<int, 0>{});
+                two(std::integral_constant<int, 1>{});
+                two(std::integral_constant<int, 2>{});
+                two(std::integral_constant<int, 3>{});
+            }
+        };
+        Page x[2];
+        load(x[0], p0 + w);
+#pragma nounroll
+        for (int p = p0 + w; p < p1; p += 8) {
+            load(x[1], p + 4);
+            compute(x[0], p);
+            if (p + 4 >= p1) break;
+            load(x[0], p + 8);
+            compute(x[1], p + 4);
+        }
+
+        // the four waves' results into one: lane (r, h) holds dims 8 (4 h + i) + db
+        l += __shfl_xor(l, 16, 64);
+        l += __shfl_xor(l, 32, 64);
+        if (h == 0) {
+            sm[w][r] = m;
+            sl[w][r] = l;
+        }
+        if (r < cols)
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                float* d = &so[w][r][8 * (4 * h + i)];
+                *(f32x4*)d = f32x4{o[0][i], o[1][i], o[2][i], o[3][i]};
+                *(f32x4*)(d + 4) = f32x4{o[4][i], o[5][i], o[6][i], o[7][i]};
+            }
+        __syncthreads();
+        const int col = tid >> 4, d0 = 8 * (tid & 15);
+        if (col < cols) {
+            const float M = fmaxf(fmaxf(sm[0][col], sm[1][col]), fmaxf(sm[2][col], sm[3][col]));
+            const float Mz = M == -__builtin_inff() ? 0.f : M;
+            float lt = 0.f, y[8] = {};
 #pragma unroll
             for (int j = 0; j < 4; j++) {
-                const uint32_t x = kc[t][j];
-                const u32x4 d = {Fp4<T>::template pair<0>(x, f), Fp4<T>::template pair<1>(x, f),
-                                 Fp4<T>::template pair<2>(x, f), Fp4<T>::template pair<3>(x, f)};
-                s[t] = Op<T>::mfma16(__builtin_bit_cast(v8, d), qf[j], s[t]);
+                const float f = __builtin_amdgcn_exp2f(sm[j][col] - Mz);
+                lt = __builtin_fmaf(sl[j][col], f, lt);
+#pragma unroll
+                for (int e = 0; e < 8; e++) y[e] = __builtin_fmaf(so[j][col][d0 + e], f, y[e]);
+            }
+            const int cc = c0 + col, orow = cc / a.group, ohead = kh * a.group + cc % a.group;
+            if (units < it.pages) {
+                const size_t part = (size_t)blockIdx.x + it.entity, at = (part * a.b.kvh + kh) * KV_TILE + col;
+                if (part < (size_t)a.parts) {
+                    float* po = a.part + 2 * (size_t)a.parts * a.b.kvh * KV_TILE + at * LTX_HD + d0;
+                    if (d0 == 0) *(f32x2*)(a.part + 2 * at) = f32x2{M, lt};
+                    *(f32x4*)po = f32x4{y[0], y[1], y[2], y[3]};
+                    *(f32x4*)(po + 4) = f32x4{y[4], y[5], y[6], y[7]};
+                }
+            } else {
+                const int grow = it.s.s0 + orow;
+                const float g = a.glog ? 2.0f * sigmoid_f(a.glog[(size_t)grow * a.heads + ohead]) : 1.0f;
+                const float f = kv_limit(a.causal, it.s, orow) > 0 ? g / lt : 0.f;
+                u32x4 out;
+#pragma unroll
+                for (int e = 0; e < 4; e++) out[e] = Op<T>::cvt2(y[2 * e] * f, y[2 * e + 1] * f);
+                *(u32x4*)((uint16_t*)a.out + (size_t)grow * a.ldo + (size_t)ohead * LTX_HD + d0) = out;
             }
         }
-        if (flag) kv_set_nan(s, kv_drop_nan(vs));
-        if (none || (p + 1) * LTX_KV_PAGE > all) kv_mask(s, p, none ? 0 : mine, h);
-        uint32_t pw[4][2];
-        float corr;
-        if (kv_softmax<T>(s, C, m, l, pw, corr))
-#pragma unroll
-            for (int db = 0; db < 8; db++) o[db] *= corr;
-#pragma unroll
-        for (int cc = 0; cc < 2; cc++) {
-            const v8 pf = __builtin_bit_cast(v8, (u32x4){pw[2 * cc][0], pw[2 * cc][1], pw[2 * cc + 1][0],
-                                                         pw[2 * cc + 1][1]});
-            uint32_t x[8], f[2] = {vs[2 * cc], vs[2 * cc + 1]};
-#pragma unroll
-            for (int e = 0; e < 8; e++) x[e] = vc[2 * cc + (e >> 2)][e & 3];
-            auto two = [&](auto B) {  // dims 8 r + 2 B and + 1: eight keys each
-                constexpr int b = decltype(B)::value;
-                u32x4 lo, hi;
-                kv_v_pair<T, b>(x, f, lo, hi);
-                o[2 * b] = Op<T>::mfma16(__builtin_bit_cast(v8, lo), pf, o[2 * b]);
-                o[2 * b + 1] = Op<T>::mfma16(__builtin_bit_cast(v8, hi), pf, o[2 * b + 1]);
-            };
-            two(std::integral_constant<int, 0>{});
-            two(std::integral_constant<int, 1>{});
-            two(std::integral_constant<int, 2>{});
-            two(std::integral_constant<int, 3>{});
-        }
-    }
-
-    // the four waves' results into one: lane (r, h) holds dims 8 (4 h + i) + db
-    l += __shfl_xor(l, 16, 64);
-    l += __shfl_xor(l, 32, 64);
-    if (h == 0) {
-        sm[w][r] = m;
-        sl[w][r] = l;
-    }
-    if (r < cols)
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            float* d = &so[w][r][8 * (4 * h + i)];
-            *(f32x4*)d = f32x4{o[0][i], o[1][i], o[2][i], o[3][i]};
-            *(f32x4*)(d + 4) = f32x4{o[4][i], o[5][i], o[6][i], o[7][i]};
-        }
-    __syncthreads();
-    const int col = tid >> 4, d0 = 8 * (tid & 15);
-    if (col >= cols) return;
-    float M = fmaxf(fmaxf(sm[0][col], sm[1][col]), fmaxf(sm[2][col], sm[3][col]));
-    const float Mz = M == -__builtin_inff() ? 0.f : M;
-    float lt = 0.f, x[8] = {};
-#pragma unroll
-    for (int j = 0; j < 4; j++) {
-        const float f = __builtin_amdgcn_exp2f(sm[j][col] - Mz);
-        lt = __builtin_fmaf(sl[j][col], f, lt);
-#pragma unroll
-        for (int e = 0; e < 8; e++) x[e] = __builtin_fmaf(so[j][col][d0 + e], f, x[e]);
-    }
-    const int cc = c0 + col, orow = cc / a.group, ohead = kh * a.group + cc % a.group;
-    if (kv_runs(np, per) > 1) {
-        const size_t at = ((size_t)blockIdx.x * a.b.kvh + kh) * KV_TILE + col;
-        float* ml = a.part + 2 * at;
-        float* po = a.part + 2 * (size_t)a.items * a.b.kvh * KV_TILE + at * LTX_HD + d0;
-        if (d0 == 0) *(f32x2*)ml = f32x2{M, lt};
-        *(f32x4*)po = f32x4{x[0], x[1], x[2], x[3]};
-        *(f32x4*)(po + 4) = f32x4{x[4], x[5], x[6], x[7]};
-        return;
-    }
-    const int grow = it.s.s0 + orow;
-    const float g = a.glog ? 2.0f * sigmoid_f(a.glog[(size_t)grow * a.heads + ohead]) : 1.0f;
-    const float f = kv_limit(a.causal, it.s, orow) > 0 ? g / lt : 0.f;
-    u32x4 out;
-#pragma unroll
-    for (int e = 0; e < 4; e++) out[e] = Op<T>::cvt2(x[2 * e] * f, x[2 * e + 1] * f);
-    *(u32x4*)((uint16_t*)a.out + (size_t)grow * a.ldo + (size_t)ohead * LTX_HD + d0) = out;
+        __syncthreads();
+    } while (kv_next(a, it));
 }
 
-extern "C" __global__ void __launch_bounds__(256) ltx_kv_attn_f16(const LtxKvAttnArgs a) { kv_attn<_Float16>(a); }
-extern "C" __global__ void __launch_bounds__(256) ltx_kv_attn_bf16(const LtxKvAttnArgs a) { kv_attn<__bf16>(a); }
+extern "C" __global__ void __launch_bounds__(256, 2) ltx_kv_attn_f16(const LtxKvAttnArgs a) { kv_attn<_Float16>(a); }
+extern "C" __global__ void __launch_bounds__(256, 2) ltx_kv_attn_bf16(const LtxKvAttnArgs a) { kv_attn<__bf16>(a); }
 
 // Many columns: a workgroup takes 128 NQ columns, its eight waves 16 NQ each, and a
 // run of pages. A page's codes become MFMA operands once for all eight waves, in LDS,
 // in the order the operands are read (16 bytes a lane, no conflicts): waves 0 .. 3 a
 // 16-key block of K each, waves 4 .. 7 half the dims of 32 keys of V each, one page
 // ahead, from codes loaded two pages ahead. One barrier a page.
-template <typename T, int NQ>
+template <typename T, int NQ, bool SPLIT>
 __device__ __forceinline__ void kv_attn_rows(const LtxKvAttnArgs& a) {
     typedef typename Op<T>::v8 v8;
     __shared__ __attribute__((aligned(1024))) uint8_t sk[2][16384];
@@ -509,12 +564,11 @@ __device__ __forceinline__ void kv_attn_rows(const LtxKvAttnArgs& a) {
     const int total = a.items * a.b.kvh, id = (blockIdx.x & 7) * (gridDim.x >> 3) + (blockIdx.x >> 3);
     if (id >= total) return;
     const int kh = id / a.items, item = id - kh * a.items;
-    const int per = kv_per(a);
-    KvItem it;
-    if (!kv_item(a, per, item, it)) return;
+    KvSpan it;
+    if (!kv_begin(a, item, it)) return;
+    do {
     const int limit = kv_tile_limit(a.causal, it.s, a.group, it.tile, a.tile), np = kv_pages(limit);
-    const int p0 = it.run * per, p1 = min(np, p0 + min(per, np));
-    if (it.run > 0 && p0 >= np) return;
+    const int p0 = SPLIT ? it.page : 0, units = SPLIT ? kv_span(it) : np, p1 = min(np, p0 + units);
 
     const int ncol = it.s.n * a.group, c0 = it.tile * a.tile + 16 * NQ * w;  // the wave's first column
     const bool idle = c0 >= ncol;
@@ -727,10 +781,12 @@ __device__ __forceinline__ void kv_attn_rows(const LtxKvAttnArgs& a) {
         sync();
 #pragma nounroll
         for (int t = 0; t + 1 < nt; t++) {
-            softmax(t);
             stage((t + 1) & 1);
-            flag_s = flag, none_s = none;
+            const uint32_t flag_n = flag, none_n = none;
             if (t + 2 < nt) load(p0 + t + 2);
+            __builtin_amdgcn_sched_barrier(0);
+            softmax(t);
+            flag_s = flag_n, none_s = none_n;
             sync();
             products(t + 1);
             sync();
@@ -741,17 +797,17 @@ __device__ __forceinline__ void kv_attn_rows(const LtxKvAttnArgs& a) {
         if (!group) sync();
     }
 
-    if (idle) return;
-    const bool whole = kv_runs(np, per) == 1;
+    const bool whole = !SPLIT || units == it.pages;
+    const size_t part = (size_t)item + it.entity;
 #pragma unroll
     for (int q = 0; q < NQ; q++) {
         const int lane = my_lane(), h = lane >> 4, c = c0 + 16 * q + (lane & 15);
-        if (c >= ncol) continue;
+        if (c >= ncol || (!whole && part >= (size_t)a.parts)) continue;
         float lt = l[q] + __shfl_xor(l[q], 16, 64);
         lt += __shfl_xor(lt, 32, 64);
         if (!whole) {
-            const size_t at = ((size_t)item * a.b.kvh + kh) * a.tile + (c - it.tile * a.tile);
-            float* po = a.part + 2 * (size_t)a.items * a.b.kvh * a.tile + at * LTX_HD + 32 * h;
+            const size_t at = (part * a.b.kvh + kh) * a.tile + (c - it.tile * a.tile);
+            float* po = a.part + 2 * (size_t)a.parts * a.b.kvh * a.tile + at * LTX_HD + 32 * h;
             if (h == 0) *(f32x2*)(a.part + 2 * at) = f32x2{m[q], lt};
 #pragma unroll
             for (int i = 0; i < 4; i++) {
@@ -771,54 +827,106 @@ __device__ __forceinline__ void kv_attn_rows(const LtxKvAttnArgs& a) {
             for (int e = 0; e < 4; e++) v[e] = Op<T>::cvt2(o[2 * e][q][i] * f, o[2 * e + 1][q][i] * f);
             *(u32x4*)(out + 8 * i) = v;
         }
-    }
+    }    if (SPLIT) __syncthreads();
+    } while (SPLIT && kv_next(a, it));
 }
 
-#define KV_ATTN_ROWS(NAME, T, NQ) \
-    extern "C" __global__ void __launch_bounds__(512) NAME(const LtxKvAttnArgs a) { kv_attn_rows<T, NQ>(a); }
+// (the span loop costs the kernel without a split 10 %: a kernel each)
+#define KV_ATTN_ROWS(NAME, T, NQ)                                                         \
+    extern "C" __global__ void __launch_bounds__(512) NAME(const LtxKvAttnArgs a) {       \
+        kv_attn_rows<T, NQ, false>(a);                                                    \
+    }                                                                                     \
+    extern "C" __global__ void __launch_bounds__(512) NAME##_split(const LtxKvAttnArgs a) { \
+        kv_attn_rows<T, NQ, true>(a);                                                     \
+    }
 KV_ATTN_ROWS(ltx_kv_attn_f16_rows1, _Float16, 1)
 KV_ATTN_ROWS(ltx_kv_attn_bf16_rows1, __bf16, 1)
 KV_ATTN_ROWS(ltx_kv_attn_f16_rows2, _Float16, 2)
 KV_ATTN_ROWS(ltx_kv_attn_bf16_rows2, __bf16, 2)
 
-// The runs of a tile into one: a wave takes a row and query head.
+// The runs of a tile into one: a workgroup takes a row and query head, a wave every
+// fourth run, a lane two dims. In the runs' order: the same bits every time.
 template <typename T>
-__device__ void kv_join(const LtxKvAttnArgs& a) {
-    const int lane = threadIdx.x & 63, row = blockIdx.x, head = 4 * blockIdx.y + (threadIdx.x >> 6);
-    if (head >= a.heads) return;
-    const int b = __builtin_amdgcn_readfirstlane(kv_find(a.b, row, 0));
-    if (b >= a.b.nseq) return;
-    const KvSeq s = kv_seq(a.b, b);
-    const int i = row - s.s0, kh = head / a.group;
-    if (i < 0 || i >= s.n) return;
-    const int per = kv_per(a);
-    uint64_t base = 0;  // items of the sequences before
-    if (b > 0) {
-        for (int j = lane; j < b; j += 64) {
-            const KvSeq q = kv_seq(a.b, j);
-            base += (uint64_t)kv_tiles(q.n, a.group, a.tile) * kv_runs(kv_pages(q.L), per);
+__device__ __forceinline__ void kv_join(const LtxKvAttnArgs& a) {
+    __shared__ float sx[4][LTX_HD], sml[4][2];
+    const int lane = threadIdx.x & 63, row = blockIdx.x, head = blockIdx.y;
+    const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    // the row's sequence, and the tiles and units of those before it
+    KvLane k = kv_lane(a, 0);
+    const int per = kv_per(a, k);
+    uint32_t unit = 0, entity = 0;
+    KvSeq s = {0, 0, 0};
+    bool found = false;
+    for (int base = 0; base < a.b.nseq; base += 64) {
+        if (base) k = kv_lane(a, base);
+        const uint64_t here = __builtin_amdgcn_ballot_w64(row >= k.s.s0 && row < k.s.s0 + k.s.n);
+        if (here) {
+            const int l = __builtin_ctzll(here);
+            unit += lane_of(k.units_to - k.units, l);
+            entity += lane_of(k.tiles_to - k.tiles, l);
+            s = KvSeq{(int)lane_of(k.s.s0, l), (int)lane_of(k.s.n, l), (int)lane_of(k.s.L, l)};
+            found = true;
+            break;
         }
-        base = wave_sum(base);
+        unit += lane_of(k.units_to, 63);
+        entity += lane_of(k.tiles_to, 63);
     }
-    const int64_t c = (int64_t)i * a.group + head % a.group;
-    const int tile = (int)(c / a.tile), col = (int)(c % a.tile);
-    const int runs = kv_runs(kv_pages(kv_tile_limit(a.causal, s, a.group, tile, a.tile)), per);
-    const uint64_t item = base + (uint64_t)(kv_tiles(s.n, a.group, a.tile) - 1 - tile) * kv_runs(kv_pages(s.L), per);
-    if (runs <= 1 || item + runs > (uint64_t)a.items) return;
-    const float* ml = a.part + 2 * ((item * a.b.kvh + kh) * a.tile + col);
-    const float* po = a.part + 2 * (size_t)a.items * a.b.kvh * a.tile +
-                      ((item * a.b.kvh + kh) * a.tile + col) * LTX_HD + 2 * lane;
-    const size_t step = (size_t)a.b.kvh * a.tile;
-    float M = -__builtin_inff();
-    for (int j = 0; j < runs; j++) M = fmaxf(M, ml[2 * step * j]);
+    if (!found) return;
+    const int i = row - s.s0, kh = head / a.group;
+    const int c = i * a.group + head % a.group, tile = c / a.tile, col = c % a.tile, pages = kv_units(s.L);
+    unit += (uint32_t)tile * pages;
+    entity += tile;
+    const uint32_t i0 = unit / (uint32_t)per;
+    const int runs = (int)((unit + pages - 1) / (uint32_t)per - i0) + 1;
+    if (runs <= 1 || (uint64_t)i0 + entity + runs > (uint64_t)a.parts) return;
+    const size_t step = (size_t)a.b.kvh * a.tile, at = (((size_t)i0 + entity) * a.b.kvh + kh) * a.tile + col;
+    const float* ml = a.part + 2 * at;
+    const float* po = a.part + 2 * (size_t)a.parts * step + at * LTX_HD + 2 * lane;
+    float M = -__builtin_inff(), lt = 0.f, x0 = 0.f, x1 = 0.f;
+    for (int j0 = w; j0 < runs; j0 += 16) {  // four runs of the wave's at a time
+        f32x2 v[4], y[4];
+        float mn = M;
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            const int j = min(j0 + 4 * e, runs - 1);
+            v[e] = *(const f32x2*)(ml + 2 * step * j);
+            y[e] = *(const f32x2*)(po + LTX_HD * step * j);
+        }
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            if (j0 + 4 * e >= runs) v[e] = f32x2{-__builtin_inff(), 0.f};
+            mn = fmaxf(mn, v[e][0]);
+        }
+        const float mz = mn == -__builtin_inff() ? 0.f : mn, f0 = __builtin_amdgcn_exp2f(M - mz);
+        M = mn;
+        lt *= f0;
+        x0 *= f0;
+        x1 *= f0;
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            const bool there = j0 + 4 * e < runs;
+            const float f = __builtin_amdgcn_exp2f(v[e][0] - mz);
+            lt = there ? __builtin_fmaf(v[e][1], f, lt) : lt;
+            x0 = there ? __builtin_fmaf(y[e][0], f, x0) : x0;
+            x1 = there ? __builtin_fmaf(y[e][1], f, x1) : x1;
+        }
+    }
+    *(f32x2*)&sx[w][2 * lane] = f32x2{x0, x1};
+    if (lane == 0) {
+        sml[w][0] = M;
+        sml[w][1] = lt;
+    }
+    __syncthreads();
+    if (w) return;
+    M = fmaxf(fmaxf(sml[0][0], sml[1][0]), fmaxf(sml[2][0], sml[3][0]));
     const float Mz = M == -__builtin_inff() ? 0.f : M;
-    float lt = 0.f, x0 = 0.f, x1 = 0.f;
-    for (int j = 0; j < runs; j++) {
-        const f32x2 v = *(const f32x2*)(ml + 2 * step * j), y = *(const f32x2*)(po + LTX_HD * step * j);
-        const float f = __builtin_amdgcn_exp2f(v[0] - Mz);
-        lt = __builtin_fmaf(v[1], f, lt);
-        x0 = __builtin_fmaf(y[0], f, x0);
-        x1 = __builtin_fmaf(y[1], f, x1);
+    lt = x0 = x1 = 0.f;
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+        const float f = __builtin_amdgcn_exp2f(sml[j][0] - Mz);
+        lt = __builtin_fmaf(sml[j][1], f, lt);
+        x0 = __builtin_fmaf(sx[j][2 * lane], f, x0);
+        x1 = __builtin_fmaf(sx[j][2 * lane + 1], f, x1);
     }
     const float g = a.glog ? 2.0f * sigmoid_f(a.glog[(size_t)row * a.heads + head]) : 1.0f;
     const float f = kv_limit(a.causal, s, i) > 0 ? g / lt : 0.f;

@@ -395,14 +395,15 @@ typedef struct {
     const void* q;      // [rows][heads * 128], ldq elements apart
     void* out;          // the same, ldo elements apart
     const float* glog;  // [rows][heads] or NULL
-    float* part;        // partial results of `items` items (see kv_plan), or NULL: no split
+    float* part;        // `parts` partial results of a tile each (see k_kv.hip), or NULL: no split
     int64_t ldq, ldo;
     int heads, group;   // group = heads / kvh query heads a cached head
     int causal;
     int tile;           // columns of an item
-    int least;          // pages of a run, at least
-    int slots;          // items aimed at for a cached head's keys (0: no split)
+    int least;          // pages of an item, at least
+    int slots;          // items that share a cached head's pages (0: an item a tile)
     int items;          // items of a cached head in the grid
+    int parts;
     float scale_log2;   // log2(e) / sqrt(128)
 } LtxKvAttnArgs;
 

@@ -48,14 +48,12 @@ KV_FN size_t kv_block(const LtxKvBatchArgs& a, int page, int head) {
 
 KV_FN int kv_pages(int keys) { return (int)(((int64_t)keys + LTX_KV_PAGE - 1) / LTX_KV_PAGE); }
 KV_FN int kv_tiles(int n, int group, int tile) { return (int)(((int64_t)n * group + tile - 1) / tile); }
-// runs of `per` pages that `pages` make, one at least (it writes the zeros of rows
-// that see no key)
-KV_FN int kv_runs(int pages, int per) { return (int)kv_max(1, ((int64_t)pages + per - 1) / per); }
-// pages a run: `work` (tiles times pages, over all sequences) in about `slots` items
-#define KV_NO_SPLIT 0x40000000
-KV_FN int kv_per_of(uint64_t work, int slots, int least) {
-    const uint64_t per = (work + slots - 1) / slots;
-    return per >= KV_NO_SPLIT ? KV_NO_SPLIT : (int)kv_max(least, (int64_t)per);
+// Work of a split attention call: a tile's pages, one at least (a tile without keys
+// still writes its zeros); and the pages that each of about `slots` items takes of
+// all of them.
+KV_FN int kv_units(int keys) { return (int)kv_max(1, kv_pages(keys)); }
+KV_FN int kv_per_of(uint32_t units, int slots, int least) {
+    return (int)kv_max(least, ((int64_t)units + slots - 1) / slots);
 }
 
 // keys that row i of the sequence sees

@@ -185,7 +185,7 @@ static void index_bounds(unsigned seed) {
     for (int trial = 0; trial < 2000; trial++) {
         const bool sane = trial % 2 == 0;
         const int nseq = pick(1, 9), max_pages = pick(1, 12), pool = pick(1, 30), group = pick(1, 9);
-        const int tile = 16 << pick(0, 4), slots = pick(0, 40), least = pick(1, 8);
+        const int tile = 16 << pick(0, 4), slots = pick(1, 40), least = pick(1, 8);
         int rows = pick(0, 90);
         std::vector<int32_t> start(nseq + 1), len(nseq), pages(nseq * max_pages);
         for (auto& p : pages) p = pick(0, 3) ? pick(0, pool - 1) : wild[pick(0, 9)];
@@ -197,7 +197,6 @@ static void index_bounds(unsigned seed) {
         } else
             for (auto& s : start) s = pick(0, 1) ? pick(-5, rows + 5) : wild[pick(0, 9)];
         LtxKvBatchArgs a{nullptr, nullptr, nullptr, start.data(), len.data(), pages.data(), nseq, rows, max_pages, pool, 3};
-        uint64_t work = 0;
         for (int b = 0; b < nseq; b++) {
             const KvSeq s = kv_seq(a, b);
             CHECK(s.s0 >= 0 && s.n >= 0 && s.s0 + s.n <= rows && s.L >= 0 && s.L <= 64 * max_pages, "%d %d %d", s.s0, s.n, s.L);
@@ -209,22 +208,36 @@ static void index_bounds(unsigned seed) {
                 CHECK(kv_in_pool(a, page) == (page >= 0 && page < pool), "%d", page);
                 CHECK(kv_limit(1, s, row - s.s0) == pos + 1, "%d", pos);
             }
-            work += (uint64_t)kv_tiles(s.n, group, tile) * kv_pages(s.L);
         }
-        const int per = slots ? kv_per_of(work, slots, least) : KV_NO_SPLIT;
-        const int grid = (int)((int64_t)rows * group / tile + nseq + slots);
-        int64_t items = 0;
+        // the split: items of `per` units over the tiles in order; every unit once, every
+        // partial result at a place of its own below the count that the host sizes
+        const int64_t bound = (int64_t)rows * group / tile + nseq;
+        std::vector<int> pages_of;
+        uint32_t units = 0;
         for (int b = 0; b < nseq; b++) {
             const KvSeq s = kv_seq(a, b);
-            const int tiles = kv_tiles(s.n, group, tile), runs = kv_runs(kv_pages(s.L), per);
-            items += (int64_t)tiles * runs;
-            for (int t = 0; t < tiles; t++)
+            const int tiles = kv_tiles(s.n, group, tile);
+            for (int t = 0; t < tiles; t++) {
                 for (int causal = 0; causal < 2; causal++) {
                     const int limit = kv_tile_limit(causal, s, group, t, tile);
-                    CHECK(limit >= 0 && limit <= s.L && kv_runs(kv_pages(limit), per) <= runs, "%d of %d", limit, s.L);
+                    CHECK(limit >= 0 && limit <= s.L && kv_pages(limit) <= kv_units(s.L), "%d of %d", limit, s.L);
                 }
+                pages_of.push_back(kv_units(s.L));
+                units += kv_units(s.L);
+            }
         }
-        if (sane) CHECK(items <= grid, "%lld items, a grid of %d", (long long)items, grid);
+        if (sane) CHECK((int64_t)pages_of.size() <= bound, "%zu tiles", pages_of.size());
+        const int per = kv_per_of(units, slots, least);
+        CHECK(per >= least && (int64_t)per * slots >= units, "%d", per);
+        int last = -1;
+        uint32_t at = 0;
+        for (int e = 0; e < (int)pages_of.size(); e++) {
+            const uint32_t i0 = at / per, i1 = (at + pages_of[e] - 1) / per;
+            CHECK(i1 < (uint32_t)slots && (int)(i0 + e) > last, "item %u for tile %d", i0, e);
+            last = (int)(i1 + e);
+            if (sane) CHECK(last < slots + bound, "part %d", last);
+            at += pages_of[e];
+        }
     }
     LtxKvBatchArgs big{nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, 1, 1, 1, 1 << 25, 32};
     CHECK(kv_block(big, (1 << 25) - 1, 31) == ((1ull << 30) - 1) * LTX_KV_BLOCK, "places pass 32 bits");
