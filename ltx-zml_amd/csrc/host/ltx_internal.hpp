@@ -169,6 +169,7 @@ struct ltx_ctx {
     bool gemm_persistent = true;  // LDS-DMA GEMM: at most one workgroup per CU, looping over tiles
     bool attn_pp = true;
     bool attn_kv = true;
+    int kv_tile = 0;  // columns of a tile of the 4-bit cache's attention: 0 by the rule, or 16, 128 or 256 (tests)
     // side stream of a forward: work off the main chain (gate logits, the
     // cross-attention K/V) overlaps it, ordered by the events
     hipStream_t side = nullptr;

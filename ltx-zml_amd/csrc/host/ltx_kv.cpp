@@ -1,6 +1,5 @@
 // The 4-bit key/value cache: its handle, rows written and read back, attention.
 #include <algorithm>
-#include <cstdlib>
 #include <cstring>
 
 #include "ltx_internal.hpp"
@@ -54,25 +53,41 @@ void kv_rows(ltx_ctx* c, const ltx_kv_cache* k, const ltx_kv_batch* b, void* kp,
 }
 
 struct AttnPlan {
-    int nq = 0;  // 0: the kernel of few columns (16 a tile), else 128 nq a tile
-    int tile = 16, least = 4, slots = 0, items = 0, parts = 0;
+    int tile = 16;  // columns (rows times query heads of a cached head) of a tile: 16, 128 or 256
+    int least = 4, slots = 0, items = 0, parts = 0;
     size_t bytes = 0;  // of partial results
 };
+
+// Tiles of 16 columns (four waves that share a tile's pages), or of 128 or 256 (eight
+// waves that share a page's operands). Wide tiles pay where they fill the CUs without
+// a split, 256 columns before 128; a split into wide tiles only where its partial
+// results (256 columns each) are spread over many pages. us on 16 / 128 / 256
+// columns, `columns` a sequence:
+//   one sequence of 8,192 keys, 8 cached heads: 128 columns 22 / 29 / 33, 1,024 76 /
+//   82 / 77, 2,048 142 / 136 / 126, 4,096 274 / 197 / 213; of 28,672 keys: 64 columns
+//   27 / 31 / 42, 256 67 / 62 / 61, 1,024 214 / 192 / 160, 4,096 808 / 674 / 565
+//   32 cached heads, 2,048 keys: 512 columns 62 / 69 / 74, 1,024 114 / 56 / 112, 2,048
+//   219 / 79 / 73
+//   16 sequences of 2,048 keys, 8 cached heads: 64 columns 41 / 45 / 57, 128 70 / 67 /
+//   75, 256 131 / 59 / 113, 512 245 / 82 / 76
+//   8 sequences of 1,000 keys, 32 cached heads: 32 columns 31 / 36 / 49, 64 51 / 48 /
+//   60, 128 94 / 45 / 82
+// The table's width stands for the lengths, which the host does not know.
+int tile_columns(const ltx_ctx* c, const ltx_kv_cache* k, const ltx_kv_batch* b, int64_t columns) {
+    if (c->kv_tile) return c->kv_tile;
+    const int64_t each = columns / b->nseq, wide = columns * k->kv_heads / 256;  // workgroups of 256 columns
+    const int64_t pages = wide * b->max_pages / c->num_cu;                       // of each, if split
+    if (each >= 192 && wide >= c->num_cu) return 256;
+    if (each >= 256 && pages >= 128) return 256;
+    if (each >= 64 && (each + 127) / 128 * b->nseq * k->kv_heads >= c->num_cu) return 128;
+    if (each >= 256 && pages >= 24) return 256;
+    return 16;
+}
 
 AttnPlan attn_plan(const ltx_ctx* c, const ltx_kv_cache* k, const ltx_kv_batch* b, int heads, bool split) {
     const int64_t group = heads / k->kv_heads, columns = (int64_t)b->rows * group;
     AttnPlan p;
-    int forced = -1;
-    if (const char* e = std::getenv("KVNQ")) forced = std::atoi(e);
-    int target = 2;
-    p.nq = forced >= 0 ? forced : columns <= 32 * (int64_t)b->nseq ? 0 : columns * k->kv_heads <= 128ll * c->num_cu ? 1 : 2;
-    if (p.nq) {
-        p.tile = 128 * p.nq;
-        p.least = 8;
-        target = 1;
-    }
-    if (const char* e = std::getenv("KVTARGET")) target = std::atoi(e);
-    if (const char* e = std::getenv("KVLEAST")) p.least = std::atoi(e);
+    p.tile = tile_columns(c, k, b, columns);
     // tiles of the batch, at most
     const int64_t tiles = !b->row_start || b->nseq == 1
                               ? (int64_t)b->nseq * ((columns / b->nseq + p.tile - 1) / p.tile)
@@ -80,10 +95,13 @@ AttnPlan attn_plan(const ltx_ctx* c, const ltx_kv_cache* k, const ltx_kv_batch* 
     // the grids' limit, 2^32 threads along x; columns stay in 31 bits
     if (tiles >= (1 << 22) / k->kv_heads || columns >= 1 << 30 || b->rows >= 1 << 24)
         throw Error("too many rows for one call");
-    // A split where the tiles are fewer than the CUs take in a round and their pages
-    // (units, which are counted in 32 bits) are more than a least item each
-    const int64_t round = ((int64_t)target * c->num_cu + k->kv_heads - 1) / k->kv_heads, units = tiles * b->max_pages;
-    const bool few = p.nq == 0 || columns / p.tile * k->kv_heads < c->num_cu;
+    // A split shares the pages (units, counted in 32 bits) of all tiles among the
+    // workgroups of one round, two a CU of the narrow kernel, one of the wide: a step of
+    // four sequences of 28,672 tokens 98 us, in half as many 133, in twice as many 111.
+    p.least = p.tile == 16 ? 4 : 8;
+    const int64_t round = ((p.tile == 16 ? 2ll : 1ll) * c->num_cu + k->kv_heads - 1) / k->kv_heads;
+    const int64_t units = tiles * b->max_pages;
+    const bool few = p.tile == 16 || (p.tile == 256 && columns / 256 * k->kv_heads < c->num_cu);
     if (split && few && b->max_pages > p.least && units < 1ll << 31)
         p.slots = (int)std::min(round, (units + p.least - 1) / p.least);
     p.items = p.slots ? p.slots : (int)tiles;
@@ -216,13 +234,13 @@ int ltx_op_kv_attention(ltx_ctx* c, const ltx_kv_cache* cache, const ltx_kv_batc
         a.parts = p.parts;
         a.scale_log2 = 0.12751743f;  // log2(e) / sqrt(128)
         const bool f16 = cache->mode == LTX_MODE_F16;
-        if (p.nq == 0) {
+        if (p.tile == 16)
             c->launch(f16 ? "ltx_kv_attn_f16" : "ltx_kv_attn_bf16", p.items, cache->kv_heads, 1, 256, &a, st);
-        } else {
-            const std::string name = std::string(f16 ? "ltx_kv_attn_f16_rows" : "ltx_kv_attn_bf16_rows") +
-                                     (p.nq == 1 ? "1" : "2") + (p.slots ? "_split" : "");
-            c->launch(name.c_str(), (unsigned)(((int64_t)p.items * cache->kv_heads + 7) / 8 * 8), 1, 1, 512, &a, st);
-        }
+        else
+            c->launch(p.tile == 128 ? (f16 ? "ltx_kv_attn_f16_rows1" : "ltx_kv_attn_bf16_rows1")
+                      : p.slots     ? (f16 ? "ltx_kv_attn_f16_rows2_split" : "ltx_kv_attn_bf16_rows2_split")
+                                    : (f16 ? "ltx_kv_attn_f16_rows2" : "ltx_kv_attn_bf16_rows2"),
+                      (unsigned)(((int64_t)p.items * cache->kv_heads + 7) / 8 * 8), 1, 1, 512, &a, st);
         if (p.slots)
             c->launch(f16 ? "ltx_kv_join_f16" : "ltx_kv_join_bf16", batch->rows, heads, 1, 256, &a, st);
     })

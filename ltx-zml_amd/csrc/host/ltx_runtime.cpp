@@ -238,6 +238,8 @@ int ltx_init(int device, ltx_ctx** out) {
         if (const char* e = std::getenv("LTX_GEMM_F3")) c->gemm_f3 = std::strcmp(e, "off") != 0;
         if (const char* e = std::getenv("LTX_SIDE_EARLY"))
             c->side_early = std::strcmp(e, "off") == 0 ? 0 : std::strcmp(e, "all") == 0 ? 2 : 1;
+        if (const char* e = std::getenv("LTX_KV_TILE"))  // 16, 128 or 256 columns of the 4-bit cache's attention
+            c->kv_tile = std::strcmp(e, "16") == 0 ? 16 : std::strcmp(e, "128") == 0 ? 128 : std::strcmp(e, "256") == 0 ? 256 : 0;
         if (const char* e = std::getenv("LTX_ATTN_VARIANT")) {
             c->attn_pp = std::strcmp(e, "w8") != 0;
             c->attn_kv = c->attn_pp && std::strcmp(e, "pp") != 0;

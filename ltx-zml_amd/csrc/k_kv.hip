@@ -831,18 +831,17 @@ __device__ __forceinline__ void kv_attn_rows(const LtxKvAttnArgs& a) {
     } while (SPLIT && kv_next(a, it));
 }
 
-// (the span loop costs the kernel without a split 10 %: a kernel each)
-#define KV_ATTN_ROWS(NAME, T, NQ)                                                         \
-    extern "C" __global__ void __launch_bounds__(512) NAME(const LtxKvAttnArgs a) {       \
-        kv_attn_rows<T, NQ, false>(a);                                                    \
-    }                                                                                     \
-    extern "C" __global__ void __launch_bounds__(512) NAME##_split(const LtxKvAttnArgs a) { \
-        kv_attn_rows<T, NQ, true>(a);                                                     \
+// (the span loop costs the kernel that needs none 10 %: a kernel of its own)
+#define KV_ATTN_ROWS(NAME, T, NQ, SPLIT)                                            \
+    extern "C" __global__ void __launch_bounds__(512) NAME(const LtxKvAttnArgs a) { \
+        kv_attn_rows<T, NQ, SPLIT>(a);                                              \
     }
-KV_ATTN_ROWS(ltx_kv_attn_f16_rows1, _Float16, 1)
-KV_ATTN_ROWS(ltx_kv_attn_bf16_rows1, __bf16, 1)
-KV_ATTN_ROWS(ltx_kv_attn_f16_rows2, _Float16, 2)
-KV_ATTN_ROWS(ltx_kv_attn_bf16_rows2, __bf16, 2)
+KV_ATTN_ROWS(ltx_kv_attn_f16_rows1, _Float16, 1, false)
+KV_ATTN_ROWS(ltx_kv_attn_bf16_rows1, __bf16, 1, false)
+KV_ATTN_ROWS(ltx_kv_attn_f16_rows2, _Float16, 2, false)
+KV_ATTN_ROWS(ltx_kv_attn_bf16_rows2, __bf16, 2, false)
+KV_ATTN_ROWS(ltx_kv_attn_f16_rows2_split, _Float16, 2, true)
+KV_ATTN_ROWS(ltx_kv_attn_bf16_rows2_split, __bf16, 2, true)
 
 // The runs of a tile into one: a workgroup takes a row and query head, a wave every
 // fourth run, a lane two dims. In the runs' order: the same bits every time.

@@ -51,6 +51,19 @@ def held(x, mode):
     return out.reshape(x.shape)
 
 
+@pytest.fixture(params=["rule", "16", "128", "256"])
+def any_tile(request, monkeypatch, ctx):
+    """The context, and one for each kernel of the attention (columns of a tile)
+    whatever the rule would take."""
+    if request.param == "rule":
+        yield ctx
+        return
+    monkeypatch.setenv("LTX_KV_TILE", request.param)
+    c = rt.Context(0)
+    yield c
+    c.close()
+
+
 def ints(a):
     return torch.tensor(np.asarray(a), dtype=torch.int32, device="cuda")
 
@@ -234,9 +247,10 @@ def test_rows_before_the_first_position_and_bad_pages(ctx):
 
 
 @pytest.mark.parametrize("mode", ["f16", "bf16"])
-def test_values_that_are_not_finite(ctx, mode):
+def test_values_that_are_not_finite(any_tile, mode):
     """Read back as NaN of their group; NaN for the rows that see them, and no trace
     for those that do not (causal rows before them, keys past the end, other heads)."""
+    ctx = any_tile
     say(f"kv not finite {mode}")
     g = torch.Generator().manual_seed(3)
     keys, rows = [150, 40, 70], [140, 3, 70]
@@ -293,7 +307,8 @@ SHAPES = [
 @pytest.mark.parametrize("causal", [True, False])
 @pytest.mark.parametrize("mode", ["f16", "bf16"])
 @pytest.mark.parametrize("heads,kvh,rows,keys", SHAPES)
-def test_attention(ctx, mode, heads, kvh, rows, keys, causal):
+def test_attention(any_tile, mode, heads, kvh, rows, keys, causal):
+    ctx = any_tile
     say(f"kv attention {mode} heads={heads}/{kvh} rows={rows[:4]} keys={keys[:4]} causal={causal}")
     s = Setup(ctx, mode, kvh, rows, keys, seed=sum(keys) + heads)
     gate = torch.randn(s.total, heads, generator=s.g) if heads != 32 else None
@@ -310,8 +325,9 @@ def test_attention(ctx, mode, heads, kvh, rows, keys, causal):
 
 @pytest.mark.parametrize("mode", ["f16", "bf16"])
 @pytest.mark.parametrize("scale", [30.0, 0.01])
-def test_attention_peaked_and_flat(ctx, mode, scale):
+def test_attention_peaked_and_flat(any_tile, mode, scale):
     """Scores of hundreds, whose maximum moves from page to page, and near zero."""
+    ctx = any_tile
     say(f"kv attention {mode} q scale {scale}")
     s = Setup(ctx, mode, 2, [1, 33, 150], [700, 333, 300], seed=8)
     q = s.queries(4, scale)
@@ -319,9 +335,10 @@ def test_attention_peaked_and_flat(ctx, mode, scale):
     check(s.attend(q, 4, True), want, tol)
 
 
-def test_attention_rows_without_keys(ctx):
+def test_attention_rows_without_keys(any_tile):
     """Empty sequences and rows before the first position give zeros; rows behind
     the last sequence stay."""
+    ctx = any_tile
     say("kv attention rows without keys")
     s = Setup(ctx, "f16", 2, [1, 5, 0, 80, 2], [0, 3, 10, 70, 0], seed=9)
     q = s.queries(4)
@@ -336,7 +353,8 @@ def test_attention_rows_without_keys(ctx):
     assert (out[s.total:] == 7).all()
 
 
-def test_attention_leaves_bad_pages_out(ctx):
+def test_attention_leaves_bad_pages_out(any_tile):
+    ctx = any_tile
     say("kv attention bad pages")
     for rows, keys in (([1, 2], [300, 900]), ([200, 70], [300, 900])):
         s = Setup(ctx, "bf16", 2, rows, keys, seed=10)
@@ -394,10 +412,11 @@ def test_places_behind_32_bits(ctx):
     cache.free()
 
 
-def test_captured_steps_follow_the_lengths(ctx):
+def test_captured_steps_follow_the_lengths(any_tile):
     """A step (write, attention) of two contexts' worth of graphs, captured with their
     own workspaces and replayed together while the lengths grow: each replay equals
     the eager result."""
+    ctx = any_tile
     say("kv graphs")
     runs = []
     for i, mode in enumerate(("f16", "bf16")):
