@@ -49,7 +49,7 @@ void kv_rows(ltx_ctx* c, const ltx_kv_cache* k, const ltx_kv_batch* b, void* kp,
     HIPC(hipSetDevice(c->device));
     const bool f16 = k->mode == LTX_MODE_F16;
     c->launch(write ? (f16 ? "ltx_kv_write_f16" : "ltx_kv_write_bf16") : (f16 ? "ltx_kv_read_f16" : "ltx_kv_read_bf16"),
-              (unsigned)(((size_t)b->rows + 15) / 16), k->kv_heads, 1, 256, &a, st);
+              (unsigned)(((size_t)b->rows + 15) / 16), (k->kv_heads + 3) / 4, 1, 256, &a, st);
 }
 
 struct AttnPlan {

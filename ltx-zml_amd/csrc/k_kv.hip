@@ -69,19 +69,24 @@ __device__ __forceinline__ int kv_find(const LtxKvBatchArgs& a, int row0, int su
     return b;
 }
 
-// The block of (row's position, head), and its key within the page; NULL where the
-// row is in no sequence, before the first position, or on no page of the pool.
-__device__ __forceinline__ uint8_t* kv_place(const LtxKvBatchArgs& a, int row, int b, int head, int& key) {
+// The first head's block of the row's page, and its key within the page; NULL where
+// the row is in no sequence, before the first position, or on no page of the pool
+// (`counts`: this lane counts it). in: whether it is a row of a sequence.
+__device__ __forceinline__ uint8_t* kv_place(const LtxKvBatchArgs& a, int row, int b, bool counts, int& key, bool& in) {
+    in = false;
+    key = 0;
     if (row >= a.rows || b >= a.nseq) return nullptr;
-    const int pos = kv_position(kv_seq(a, b), row);
+    const KvSeq s = kv_seq(a, b);
+    in = row >= s.s0 && row < s.s0 + s.n;
+    const int pos = kv_position(s, row);
     if (pos < 0) return nullptr;
     const int page = kv_page(a, b, pos / LTX_KV_PAGE);
     if (!kv_in_pool(a, page)) {
-        if (head == 0 && (threadIdx.x & 15) == 0) atomicAdd(a.bad, 1ull);
+        if (counts) atomicAdd(a.bad, 1ull);
         return nullptr;
     }
     key = pos % LTX_KV_PAGE;
-    return a.data + kv_block(a, page, head);
+    return a.data + kv_block(a, page, 0);
 }
 
 __device__ __forceinline__ uint32_t quad_max(uint32_t x) {  // over lanes 4 j .. 4 j + 3
@@ -103,8 +108,7 @@ __device__ __forceinline__ uint32_t kv_encode(u32x4 w, uint32_t& code) {
     top = quad_max(top);
     const int e = (int)(top >> 23) - 2 + ((top & 0x7fffffu) > 0x600000u ? 1 : 0);
     code = top >= 0x7f800000u ? 255u : (uint32_t)min(max(e, Fp4<T>::lo), Fp4<T>::hi);
-    if (code == 255u) return 0u;
-    const float s = __builtin_bit_cast(float, code << 23);
+    const float s = __builtin_bit_cast(float, code << 23);  // (255: codes of any value)
     uint32_t q = 0;
     q = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(q, x[0], x[1], s, 0);
     q = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(q, x[2], x[3], s, 1);
@@ -113,52 +117,152 @@ __device__ __forceinline__ uint32_t kv_encode(u32x4 w, uint32_t& code) {
     return q;
 }
 
-// Rows into the cache and out of it: a wave takes four rows of a head, 16 lanes of
-// eight dims each. Four positions of a quad are 256 consecutive bytes of V codes.
+// Dword j of lane i and dword i of lane j change places, over the lanes 4 q + 0 .. 3;
+__device__ __forceinline__ void quad_transpose(u32x4& x) {
+    const bool odd = threadIdx.x & 1, high = threadIdx.x & 2;
+    auto cross = [](bool upper, uint32_t& a, uint32_t& b, auto dpp) {
+        const uint32_t fa = dpp(a), fb = dpp(b);
+        a = upper ? fb : a;
+        b = upper ? b : fa;
+    };
+    uint32_t x0 = x[0], x1 = x[1], x2 = x[2], x3 = x[3];
+    auto one = [](uint32_t v) { return (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0xB1, 0xf, 0xf, true); };
+    auto two = [](uint32_t v) { return (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0x4E, 0xf, 0xf, true); };
+    cross(odd, x0, x1, one);
+    cross(odd, x2, x3, one);
+    cross(high, x0, x2, two);
+    cross(high, x1, x3, two);
+    x = u32x4{x0, x1, x2, x3};
+}
+// and over the lanes l, l + 16, l + 32, l + 48.
+__device__ __forceinline__ void row_transpose(u32x4& x) {
+    auto p = __builtin_amdgcn_permlane32_swap(x[0], x[2], false, false);
+    const uint32_t a0 = p[0], a2 = p[1];
+    p = __builtin_amdgcn_permlane32_swap(x[1], x[3], false, false);
+    const uint32_t a1 = p[0], a3 = p[1];
+    p = __builtin_amdgcn_permlane16_swap(a0, a1, false, false);
+    const uint32_t b0 = p[0], b1 = p[1];
+    p = __builtin_amdgcn_permlane16_swap(a2, a3, false, false);
+    x = u32x4{b0, b1, p[0], p[1]};
+}
+// x of the lane's place in its quad
+__device__ __forceinline__ uint32_t quad_pick(u32x4 x) {
+    const bool odd = threadIdx.x & 1, high = threadIdx.x & 2;
+    const uint32_t low = odd ? x[1] : x[0], up = odd ? x[3] : x[2];
+    return high ? up : low;
+}
+
+// Rows into the cache and out of it: a wave takes four rows of four heads, 16 lanes of
+// eight dims each. Memory bounds it, and before that the count of accesses: a dword of
+// codes a lane and head would be an access each. So the lanes of a quad exchange their
+// K codes of four heads, and each has one head's 16 bytes; with four rows on one quad
+// of positions (the rule but for a first few rows) V's codes go the same way over the
+// rows, 16 bytes of four keys a lane. All of a wave's loads are on their way at once.
+#define KV_HB 4
 template <typename T, bool WRITE>
-__device__ void kv_rows(const LtxKvRowsArgs& a) {
+__device__ __forceinline__ void kv_rows(const LtxKvRowsArgs& a) {
     const int lane = threadIdx.x & 63, o = lane & 15, sub = lane >> 4;
-    const int row0 = 4 * (4 * blockIdx.x + (threadIdx.x >> 6)), row = row0 + sub, head = blockIdx.y;
+    // consecutive rows on one XCD: a page's scales are bytes of the same lines for
+    // every four workgroups, and lines written in parts by several L2s are merged in
+    // memory
+    const uint32_t each = gridDim.x >> 3, x = blockIdx.x;
+    const uint32_t group = x < 8 * each ? (x & 7) * each + (x >> 3) : x;
+    const int row0 = 4 * (4 * group + (threadIdx.x >> 6)), row = row0 + sub, head0 = KV_HB * blockIdx.y;
+    const int heads = min(KV_HB, a.b.kvh - head0);
+    uint16_t* k = (uint16_t*)a.k + (size_t)row * a.ldk + head0 * LTX_HD + 8 * o;
+    uint16_t* v = (uint16_t*)a.v + (size_t)row * a.ldv + head0 * LTX_HD + 8 * o;
+    u32x4 wk[KV_HB], wv[KV_HB];
+    if (WRITE)
+#pragma unroll
+        for (int e = 0; e < KV_HB; e++) {
+            wk[e] = wv[e] = u32x4{0, 0, 0, 0};
+            if (row < a.b.rows && e < heads) {
+                wk[e] = *(const u32x4*)(k + LTX_HD * e);
+                wv[e] = *(const u32x4*)(v + LTX_HD * e);
+            }
+        }
     const int b = kv_find(a.b, row0, sub);
-    int key = 0;
-    uint8_t* blk = kv_place(a.b, row, b, head, key);
+    int key;
+    bool in;
+    uint8_t* blk = kv_place(a.b, row, b, head0 == 0 && o == 0, key, in);
     const int t = key >> 4, r = key & 15;
-    uint16_t* k = (uint16_t*)a.k + (size_t)row * a.ldk + head * LTX_HD + 8 * o;
-    uint16_t* v = (uint16_t*)a.v + (size_t)row * a.ldv + head * LTX_HD + 8 * o;
-    const uint32_t ck = 1024 * t + 256 * (o >> 2) + 16 * r + 4 * (o & 3), sk = LTX_KV_KS + 64 * (o >> 2) + 4 * r + t;
-    const uint32_t cv = LTX_KV_V + 1024 * t + 16 * (16 * (r >> 2) + o) + 4 * (r & 3);
+    // the four rows on one quad of positions
+    const uint32_t place = (uint32_t)((uintptr_t)blk >> 8);  // (blocks are multiples of 256 bytes; of one pool)
+    const bool together = __builtin_amdgcn_ballot_w64(
+                              blk && place == (uint32_t)__builtin_amdgcn_readfirstlane((int)place) &&
+                              key == (__builtin_amdgcn_readfirstlane(key) & ~3) + sub) == ~0ull;
+    // what the lane holds in memory: K codes and the scales of head o % 4, V codes of
+    // four keys of head sub
+    const bool mine = blk && (o & 3) < heads, mine_v = sub < heads;
+    uint8_t* d = blk + (size_t)(head0 + (o & 3)) * LTX_KV_BLOCK;
+    uint8_t* dv = blk + (size_t)(head0 + sub) * LTX_KV_BLOCK + LTX_KV_V + 1024 * t + 16 * (16 * (r >> 2) + o);
+    const uint32_t ck = 1024 * t + 256 * (o >> 2) + 16 * r;
+    const uint32_t cv = LTX_KV_V + 1024 * t + 16 * (16 * (r >> 2) + o) + 4 * (r & 3);  // one key's
+    const uint32_t sk = LTX_KV_KS + 64 * (o >> 2) + 4 * r + t;
     const uint32_t sv = LTX_KV_VS + 64 * (o >> 2) + 16 * (r >> 2) + 4 * t + (r & 3);
     if (WRITE) {
-        const u32x4 zero = {0, 0, 0, 0};
-        const u32x4 wk = blk ? *(const u32x4*)k : zero, wv = blk ? *(const u32x4*)v : zero;
-        uint32_t ek, ev;
-        const uint32_t qk = kv_encode<T>(wk, ek), qv = kv_encode<T>(wv, ev);
-        if (!blk) return;
-        *(uint32_t*)(blk + ck) = qk;
-        *(uint32_t*)(blk + cv) = qv;
-        if ((o & 3) == 0) {
-            blk[sk] = (uint8_t)ek;
-            blk[sv] = (uint8_t)ev;
-            if (ek == 255u || ev == 255u)
-                a.b.flags[(size_t)(blk - a.b.data) / LTX_KV_BLOCK / a.b.kvh] = 1u;
+        u32x4 qk, qv, ek, ev;
+#pragma unroll
+        for (int e = 0; e < KV_HB; e++) {
+            uint32_t c0, c1;
+            qk[e] = kv_encode<T>(wk[e], c0);
+            qv[e] = kv_encode<T>(wv[e], c1);
+            ek[e] = c0;
+            ev[e] = c1;
+        }
+        const u32x4 qv1 = qv;
+        quad_transpose(qk);
+        row_transpose(qv);
+        const uint32_t fk = quad_pick(ek), fv = quad_pick(ev);
+        if (mine) {
+            *(u32x4*)(d + ck) = qk;
+            d[sk] = (uint8_t)fk;
+            d[sv] = (uint8_t)fv;
+            if (fk == 255u || fv == 255u) a.b.flags[(size_t)(blk - a.b.data) / LTX_KV_BLOCK / a.b.kvh] = 1u;
+        }
+        if (together) {
+            if (mine_v) *(u32x4*)dv = qv;
+        } else if (blk) {
+#pragma unroll
+            for (int e = 0; e < KV_HB; e++)
+                if (e < heads) *(uint32_t*)(blk + (size_t)(head0 + e) * LTX_KV_BLOCK + cv) = qv1[e];
         }
     } else {
         // rows of a sequence that are on no page read as zeros; rows of none stay
-        if (row >= a.b.rows || b >= a.b.nseq) return;
-        const KvSeq s = kv_seq(a.b, b);
-        if (row < s.s0 || row >= s.s0 + s.n) return;
-        u32x4 wk = {0, 0, 0, 0}, wv = {0, 0, 0, 0};
-        if (blk) {
-            const uint32_t qk = *(const uint32_t*)(blk + ck), qv = *(const uint32_t*)(blk + cv);
-            const float fk = __builtin_bit_cast(float, (uint32_t)blk[sk] << 23);
-            const float fv = __builtin_bit_cast(float, (uint32_t)blk[sv] << 23);
-            wk = u32x4{Fp4<T>::template pair<0>(qk, fk), Fp4<T>::template pair<1>(qk, fk),
-                       Fp4<T>::template pair<2>(qk, fk), Fp4<T>::template pair<3>(qk, fk)};
-            wv = u32x4{Fp4<T>::template pair<0>(qv, fv), Fp4<T>::template pair<1>(qv, fv),
-                       Fp4<T>::template pair<2>(qv, fv), Fp4<T>::template pair<3>(qv, fv)};
+        u32x4 qk = {0, 0, 0, 0}, qv = {0, 0, 0, 0};
+        uint32_t fk = 0, fv = 0;
+        if (mine) {
+            qk = *(const u32x4*)(d + ck);
+            fk = d[sk];
+            fv = d[sv];
         }
-        *(u32x4*)k = wk;
-        *(u32x4*)v = wv;
+        if (together) {
+            if (mine_v) qv = *(const u32x4*)dv;
+        } else if (blk) {
+#pragma unroll
+            for (int e = 0; e < KV_HB; e++)
+                if (e < heads) qv[e] = *(const uint32_t*)(blk + (size_t)(head0 + e) * LTX_KV_BLOCK + cv);
+        }
+        quad_transpose(qk);
+        if (together) row_transpose(qv);
+        const uint32_t sks[4] = {(uint32_t)__builtin_amdgcn_mov_dpp((int)fk, 0x00, 0xf, 0xf, true),
+                                 (uint32_t)__builtin_amdgcn_mov_dpp((int)fk, 0x55, 0xf, 0xf, true),
+                                 (uint32_t)__builtin_amdgcn_mov_dpp((int)fk, 0xAA, 0xf, 0xf, true),
+                                 (uint32_t)__builtin_amdgcn_mov_dpp((int)fk, 0xFF, 0xf, 0xf, true)};
+        const uint32_t svs[4] = {(uint32_t)__builtin_amdgcn_mov_dpp((int)fv, 0x00, 0xf, 0xf, true),
+                                 (uint32_t)__builtin_amdgcn_mov_dpp((int)fv, 0x55, 0xf, 0xf, true),
+                                 (uint32_t)__builtin_amdgcn_mov_dpp((int)fv, 0xAA, 0xf, 0xf, true),
+                                 (uint32_t)__builtin_amdgcn_mov_dpp((int)fv, 0xFF, 0xf, 0xf, true)};
+#pragma unroll
+        for (int e = 0; e < KV_HB; e++) {
+            if (!in || e >= heads) continue;
+            const float sk1 = scale_of(sks[e], 0), sv1 = scale_of(svs[e], 0);
+            const uint32_t q0 = qk[e], q1 = qv[e];
+            *(u32x4*)(k + LTX_HD * e) = u32x4{Fp4<T>::template pair<0>(q0, sk1), Fp4<T>::template pair<1>(q0, sk1),
+                                              Fp4<T>::template pair<2>(q0, sk1), Fp4<T>::template pair<3>(q0, sk1)};
+            *(u32x4*)(v + LTX_HD * e) = u32x4{Fp4<T>::template pair<0>(q1, sv1), Fp4<T>::template pair<1>(q1, sv1),
+                                              Fp4<T>::template pair<2>(q1, sv1), Fp4<T>::template pair<3>(q1, sv1)};
+        }
     }
 }
 
