@@ -388,17 +388,18 @@ class Context:
 
     def linear_q4(self, a, q, s, bias, y, mode=MODE_F16, gelu=False, stream=None):
         """a [M, K], q uint8 [N, K / 2] (two weights a byte), s [N, K / 128]."""
-        M, K = a.shape
-        N = q.shape[0]
         import torch
-        _want(K == 2 * q.shape[1] and tuple(s.shape) == (N, K // 128) and tuple(y.shape) == (M, N)
-              and (bias is None or bias.numel() == N), "linear_q4: the shapes do not fit")
-        _want(all(t.is_contiguous() for t in (a, q, s, y)) and (bias is None or bias.is_contiguous()),
-              "linear_q4: contiguous tensors are needed")
-        x = _torch_dtype(mode)
-        _want(a.dtype == x and q.dtype == torch.uint8 and s.dtype in (torch.float16, torch.float32)
-              and y.dtype in (x, torch.float32) and (bias is None or bias.dtype == torch.float32),
-              "linear_q4: the types do not fit the mode")
+        (M, K), N = a.shape, q.shape[0]
+        if not (q.shape == (N, K // 2) and K % 128 == 0 and s.shape == (N, K // 128) and y.shape == (M, N)
+                and (bias is None or bias.shape == (N,))):
+            raise LtxError("linear_q4: the shapes do not fit")
+        if not (a.is_contiguous() and q.is_contiguous() and s.is_contiguous() and y.is_contiguous()
+                and (bias is None or bias.is_contiguous())):
+            raise LtxError("linear_q4: contiguous tensors are needed")
+        x, f32, half = _torch_dtype(mode), torch.float32, torch.float16
+        if not (a.dtype == x and q.dtype == torch.uint8 and (s.dtype == half or s.dtype == f32)
+                and (y.dtype == x or y.dtype == f32) and (bias is None or bias.dtype == f32)):
+            raise LtxError("linear_q4: the types do not fit the mode")
         st = stream.cuda_stream if stream is not None else _current_stream()
         self._check(lib().ltx_op_linear_q4(self.handle, _ptr(a), _ptr(q), _ptr(s), int(s.dtype == torch.float16),
                                            _ptr(bias), _ptr(y), int(y.dtype == torch.float32), M, N, K, int(gelu),
@@ -441,8 +442,9 @@ class Context:
         (ltx_op_kv_attention)."""
         st = stream.cuda_stream if stream is not None else _current_stream()
         _rows("kv_attention", batch, cache, heads, q, out)
-        _want(glog is None or (tuple(glog.shape) == (batch.rows, heads) and glog.is_contiguous()
-                               and glog.element_size() == 4), "kv_attention: glog must be f32 [rows, heads]")
+        if glog is not None and not (glog.shape == (batch.rows, heads) and glog.is_contiguous()
+                                     and glog.dtype == _torch_dtype(MODE_F32)):
+            raise LtxError("kv_attention: glog must be f32 [rows, heads]")
         self._check(lib().ltx_op_kv_attention(self.handle, cache.handle, batch.ref, _ptr(q), q.stride(0), heads,
                                               int(causal), _ptr(glog), _ptr(out), out.stride(0), _ptr(work),
                                               0 if work is None else work.numel() * work.element_size(), st),
@@ -525,27 +527,29 @@ class Context:
         return ms.value, n.value
 
 
-def _want(ok: bool, what: str):
-    if not ok:
-        raise LtxError(what)
+_DTYPES: dict = {}
 
 
 def _torch_dtype(mode: int):
-    import torch
-    return {MODE_F16: torch.float16, MODE_BF16: torch.bfloat16, MODE_F32: torch.float32}.get(mode)
+    if not _DTYPES:
+        import torch
+        _DTYPES.update({MODE_F16: torch.float16, MODE_BF16: torch.bfloat16, MODE_F32: torch.float32})
+    return _DTYPES.get(mode)
 
 
 def _rows(name: str, batch: KvBatch, cache: KvCache, heads: int, *tensors):
     """Tensors [rows, heads * 128] of the cache's type, values of a row next to each other."""
-    dt = _torch_dtype(cache.mode)
+    shape, dt = (batch.rows, heads * 128), _torch_dtype(cache.mode)
     for t in tensors:
-        _want(t.dim() == 2 and t.shape[0] == batch.rows and t.shape[1] == heads * 128 and t.dtype == dt
-              and t.stride(1) == 1, f"{name}: [{batch.rows}, {heads * 128}] tensors of the cache's type are needed")
+        if t.shape != shape or t.dtype != dt or t.stride(1) != 1:
+            raise LtxError(f"{name}: {list(shape)} tensors of the cache's type are needed")
 
 
 def _current_stream() -> int:
     import torch
-    return torch.cuda.current_stream().cuda_stream
+    # the raw handle of the current device's current stream: 0.2 us, against 3 us
+    # of a Stream object's making
+    return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
 
 
 def _memcpy_dtod(dst: int, src: int, n: int):
