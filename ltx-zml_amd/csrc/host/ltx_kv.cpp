@@ -58,7 +58,7 @@ struct AttnPlan {
     size_t bytes = 0;  // of partial results
 };
 
-// Tiles of 16 columns (four waves that share a tile's pages), or of 128 or 256 (eight
+// Tiles of 16 columns (eight waves that share a tile's pages), or of 128 or 256 (eight
 // waves that share a page's operands). Wide tiles pay where they fill the CUs without
 // a split, 256 columns before 128; a split into wide tiles only where its partial
 // results (256 columns each) are spread over many pages. us on 16 / 128 / 256
@@ -95,15 +95,19 @@ AttnPlan attn_plan(const ltx_ctx* c, const ltx_kv_cache* k, const ltx_kv_batch* 
     // the grids' limit, 2^32 threads along x; columns stay in 31 bits
     if (tiles >= (1 << 22) / k->kv_heads || columns >= 1 << 30 || b->rows >= 1 << 24)
         throw Error("too many rows for one call");
-    // A split shares the pages (units, counted in 32 bits) of all tiles among the
-    // workgroups of one round, two a CU of the narrow kernel, one of the wide: a step of
-    // four sequences of 28,672 tokens 98 us, in half as many 133, in twice as many 111.
-    p.least = p.tile == 16 ? 4 : 8;
-    const int64_t round = ((p.tile == 16 ? 2ll : 1ll) * c->num_cu + k->kv_heads - 1) / k->kv_heads;
+    // A split shares the pages (units, counted in 32 bits) of all tiles among one round
+    // of workgroups, one a CU, and costs a launch that joins the parts: where the tiles
+    // alone do not fill the CUs and are longer than 16 pages. us split / not: one row
+    // of 32 cached heads, 1,000 keys 11.5 / 9.7, 2,000 11.7 / 13.0, 16,000 23 / 61; 8
+    // sequences of 8 cached heads (64 workgroups), 1,000 keys 11.8 / 9.8, 4,000 20 / 21,
+    // 16,000 36 / 62; of 32 (256 workgroups), 4,000 keys 32 / 29, 16,000 111 / 108;
+    // ragged, 32 x 8 cached heads up to 8,192 keys 40 / 37, 8 x 32 up to 16,000 65 / 74.
+    p.least = 8;
+    const int64_t round = ((int64_t)c->num_cu + k->kv_heads - 1) / k->kv_heads;
     const int64_t units = tiles * b->max_pages;
-    const bool few = p.tile == 16 || (p.tile == 256 && columns / 256 * k->kv_heads < c->num_cu);
-    if (split && few && b->max_pages > p.least && units < 1ll << 31)
-        p.slots = (int)std::min(round, (units + p.least - 1) / p.least);
+    const bool few = p.tile == 16 ? tiles * k->kv_heads < c->num_cu && b->max_pages > 16
+                                  : p.tile == 256 && columns / 256 * k->kv_heads < c->num_cu && b->max_pages > p.least;
+    if (split && few && units < 1ll << 31) p.slots = (int)std::min(round, (units + p.least - 1) / p.least);
     p.items = p.slots ? p.slots : (int)tiles;
     if (p.slots) {
         p.parts = (int)(p.slots + tiles);
@@ -235,7 +239,7 @@ int ltx_op_kv_attention(ltx_ctx* c, const ltx_kv_cache* cache, const ltx_kv_batc
         a.scale_log2 = 0.12751743f;  // log2(e) / sqrt(128)
         const bool f16 = cache->mode == LTX_MODE_F16;
         if (p.tile == 16)
-            c->launch(f16 ? "ltx_kv_attn_f16" : "ltx_kv_attn_bf16", p.items, cache->kv_heads, 1, 256, &a, st);
+            c->launch(f16 ? "ltx_kv_attn_f16" : "ltx_kv_attn_bf16", p.items, cache->kv_heads, 1, 512, &a, st);
         else
             c->launch(p.tile == 128 ? (f16 ? "ltx_kv_attn_f16_rows1" : "ltx_kv_attn_bf16_rows1")
                       : p.slots     ? (f16 ? "ltx_kv_attn_f16_rows2_split" : "ltx_kv_attn_bf16_rows2_split")

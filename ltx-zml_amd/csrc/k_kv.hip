@@ -473,6 +473,7 @@ __device__ __forceinline__ void kv_v_pair(const uint32_t (&x)[8], const uint32_t
 }
 
 #define KV_TILE 16
+#define KV_WAVES 8  // (the lines below that take the waves' sums apart count on 512 threads)
 
 // Few columns: a workgroup takes 16 columns and a run of pages, a page a wave in
 // turn, everything in registers. Scores transposed, S^T = K . Q^T, and O^T = V^T .
@@ -488,8 +489,8 @@ __device__ __forceinline__ void kv_v_pair(const uint32_t (&x)[8], const uint32_t
 template <typename T>
 __device__ __forceinline__ void kv_attn(const LtxKvAttnArgs& a) {
     typedef typename Op<T>::v8 v8;
-    __shared__ __attribute__((aligned(16))) float so[4][KV_TILE][LTX_HD + 4];
-    __shared__ float sm[4][KV_TILE], sl[4][KV_TILE];
+    __shared__ __attribute__((aligned(16))) float so[KV_WAVES][KV_TILE][LTX_HD + 4];
+    __shared__ float sm[KV_WAVES][KV_TILE], sl[KV_WAVES][KV_TILE];
     const int tid = threadIdx.x, lane = tid & 63, r = lane & 15, h = lane >> 4;
     const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int kh = blockIdx.y;
@@ -539,7 +540,7 @@ __device__ __forceinline__ void kv_attn(const LtxKvAttnArgs& a) {
 #pragma unroll
             for (int t = 0; t < 4; t++) x.v[t] = *(const u32x4*)(blk + LTX_KV_V + 1024 * t + 16 * lane);
             x.vs = *(const u32x4*)(blk + LTX_KV_VS + 64 * (r >> 2) + 16 * h);
-            next = p + 4 < p1 ? table[p + 4] : 0u;
+            next = p + KV_WAVES < p1 ? table[p + KV_WAVES] : 0u;
             __builtin_amdgcn_sched_barrier(0);
         };
         auto compute = [&](Page& x, int p) {
@@ -588,15 +589,15 @@ __device__ __forceinline__ void kv_attn(const LtxKvAttnArgs& a) {
         Page x[2];
         load(x[0], p0 + w);
 #pragma nounroll
-        for (int p = p0 + w; p < p1; p += 8) {
-            load(x[1], p + 4);
+        for (int p = p0 + w; p < p1; p += 2 * KV_WAVES) {
+            load(x[1], p + KV_WAVES);
             compute(x[0], p);
-            if (p + 4 >= p1) break;
-            load(x[0], p + 8);
-            compute(x[1], p + 4);
+            if (p + KV_WAVES >= p1) break;
+            load(x[0], p + 2 * KV_WAVES);
+            compute(x[1], p + KV_WAVES);
         }
 
-        // the four waves' results into one: lane (r, h) holds dims 8 (4 h + i) + db
+        // the waves' results into one: lane (r, h) holds dims 8 (4 h + i) + db
         l += __shfl_xor(l, 16, 64);
         l += __shfl_xor(l, 32, 64);
         if (h == 0) {
@@ -611,17 +612,19 @@ __device__ __forceinline__ void kv_attn(const LtxKvAttnArgs& a) {
                 *(f32x4*)(d + 4) = f32x4{o[4][i], o[5][i], o[6][i], o[7][i]};
             }
         __syncthreads();
-        const int col = tid >> 4, d0 = 8 * (tid & 15);
+        const int col = tid >> 5, d0 = 4 * (tid & 31);
         if (col < cols) {
-            const float M = fmaxf(fmaxf(sm[0][col], sm[1][col]), fmaxf(sm[2][col], sm[3][col]));
-            const float Mz = M == -__builtin_inff() ? 0.f : M;
-            float lt = 0.f, y[8] = {};
+            float M = sm[0][col];
 #pragma unroll
-            for (int j = 0; j < 4; j++) {
+            for (int j = 1; j < KV_WAVES; j++) M = fmaxf(M, sm[j][col]);
+            const float Mz = M == -__builtin_inff() ? 0.f : M;
+            float lt = 0.f, y[4] = {};
+#pragma unroll
+            for (int j = 0; j < KV_WAVES; j++) {
                 const float f = __builtin_amdgcn_exp2f(sm[j][col] - Mz);
                 lt = __builtin_fmaf(sl[j][col], f, lt);
 #pragma unroll
-                for (int e = 0; e < 8; e++) y[e] = __builtin_fmaf(so[j][col][d0 + e], f, y[e]);
+                for (int e = 0; e < 4; e++) y[e] = __builtin_fmaf(so[j][col][d0 + e], f, y[e]);
             }
             const int cc = c0 + col, orow = cc / a.group, ohead = kh * a.group + cc % a.group;
             if (units < it.pages) {
@@ -630,24 +633,21 @@ __device__ __forceinline__ void kv_attn(const LtxKvAttnArgs& a) {
                     float* po = a.part + 2 * (size_t)a.parts * a.b.kvh * KV_TILE + at * LTX_HD + d0;
                     if (d0 == 0) *(f32x2*)(a.part + 2 * at) = f32x2{M, lt};
                     *(f32x4*)po = f32x4{y[0], y[1], y[2], y[3]};
-                    *(f32x4*)(po + 4) = f32x4{y[4], y[5], y[6], y[7]};
                 }
             } else {
                 const int grow = it.s.s0 + orow;
                 const float g = a.glog ? 2.0f * sigmoid_f(a.glog[(size_t)grow * a.heads + ohead]) : 1.0f;
                 const float f = kv_limit(a.causal, it.s, orow) > 0 ? g / lt : 0.f;
-                u32x4 out;
-#pragma unroll
-                for (int e = 0; e < 4; e++) out[e] = Op<T>::cvt2(y[2 * e] * f, y[2 * e + 1] * f);
-                *(u32x4*)((uint16_t*)a.out + (size_t)grow * a.ldo + (size_t)ohead * LTX_HD + d0) = out;
+                *(u32x2*)((uint16_t*)a.out + (size_t)grow * a.ldo + (size_t)ohead * LTX_HD + d0) =
+                    u32x2{Op<T>::cvt2(y[0] * f, y[1] * f), Op<T>::cvt2(y[2] * f, y[3] * f)};
             }
         }
         __syncthreads();
     } while (kv_next(a, it));
 }
 
-extern "C" __global__ void __launch_bounds__(256, 2) ltx_kv_attn_f16(const LtxKvAttnArgs a) { kv_attn<_Float16>(a); }
-extern "C" __global__ void __launch_bounds__(256, 2) ltx_kv_attn_bf16(const LtxKvAttnArgs a) { kv_attn<__bf16>(a); }
+extern "C" __global__ void __launch_bounds__(64 * KV_WAVES) ltx_kv_attn_f16(const LtxKvAttnArgs a) { kv_attn<_Float16>(a); }
+extern "C" __global__ void __launch_bounds__(64 * KV_WAVES) ltx_kv_attn_bf16(const LtxKvAttnArgs a) { kv_attn<__bf16>(a); }
 
 // Many columns: a workgroup takes 128 NQ columns, its eight waves 16 NQ each, and a
 // run of pages. A page's codes become MFMA operands once for all eight waves, in LDS,
