@@ -303,7 +303,7 @@ int ltx_op_linear_q4(ltx_ctx* ctx, const void* a, const uint8_t* q, const void* 
 #define LTX_KV_PAGE_TOKENS 64
 typedef struct ltx_kv_cache ltx_kv_cache;
 int ltx_kv_cache_create(ltx_ctx* ctx, int mode, int kv_heads, int pages, ltx_kv_cache** out);
-/* Waits for the device; before the context is destroyed. */
+/* Waits for the device's work; call it before ltx_destroy of the context. */
 void ltx_kv_cache_free(ltx_ctx* ctx, ltx_kv_cache* cache);
 /* Device bytes held by the cache. */
 uint64_t ltx_kv_cache_bytes(const ltx_kv_cache* cache);
@@ -319,7 +319,7 @@ uint64_t ltx_kv_cache_bytes(const ltx_kv_cache* cache);
  * pool is not followed: the row is not written, or read as zeros, or the page's
  * keys take no part in the attention, and it is counted (ltx_kv_cache_faults).
  * The host checks what it can see: nseq and max_pages (at most 2^24) positive,
- * rows not negative (0: nothing to do), pointers, heads, and that rows of k, v, q
+ * rows not negative (0: nothing to do; below 2^24 for the attention, 2^28 else), pointers, heads, and that rows of k, v, q
  * and out start on 16 bytes with strides (in elements) that are multiples of 8 and
  * not shorter than a row. */
 typedef struct ltx_kv_batch {
@@ -350,13 +350,14 @@ int ltx_op_kv_read(ltx_ctx* ctx, const ltx_kv_cache* cache, const ltx_kv_batch* 
  * the rows' own k and v first): q and out [rows][heads * 128], query head j on the
  * cached head j / (heads / kv_heads); scores q . k / sqrt(128); causal: a row sees
  * the keys up to its own position, else all kv_len; glog [rows][heads] f32 or NULL,
- * the gate of ltx_op_attention. A row that sees no key gives zeros; a row that
+ * the gate of ltx_op_attention; out may not overlap q. A row that sees no key gives zeros; a row that
  * sees a token with a value of v (or k) that is not finite in that head gives NaN,
  * and one that does not is untouched by it. f32 statistics and sums, weights
  * rounded to 16 bits. Results do not depend on other calls' timing.
- * Keys are split over workgroups, whose partial results lie in `work`: device
- * memory of ltx_op_kv_attention_workspace bytes (for the batch's nseq, rows and
- * max_pages), not used by two calls at once; for calls that are captured. NULL:
+ * With few rows the keys are split over workgroups, whose partial results lie in
+ * `work`: device memory of ltx_op_kv_attention_workspace bytes (for the batch's nseq,
+ * rows and max_pages, with or without row_start), not used by two calls at once; for
+ * calls that are captured. NULL:
  * scratch of the context, as in ltx_op_attention (a call being captured, or one
  * that finds no memory, does not split). */
 int ltx_op_kv_attention_workspace(ltx_ctx* ctx, const ltx_kv_cache* cache, const ltx_kv_batch* batch, int heads,

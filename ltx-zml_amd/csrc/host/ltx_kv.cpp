@@ -45,6 +45,7 @@ void kv_rows(ltx_ctx* c, const ltx_kv_cache* k, const ltx_kv_batch* b, void* kp,
     const int width = k->kv_heads * LTX_HD;
     check_rows(kp, ldk, width, b->rows, "k");
     check_rows(vp, ldv, width, b->rows, "v");
+    if (b->rows >= 1 << 28) throw Error("too many rows for one call");  // 2^32 threads along x
     if (b->rows == 0) return;
     HIPC(hipSetDevice(c->device));
     const bool f16 = k->mode == LTX_MODE_F16;
@@ -135,6 +136,7 @@ int ltx_kv_cache_create(ltx_ctx* c, int mode, int kv_heads, int pages, ltx_kv_ca
         if (kv_heads <= 0 || kv_heads > 65535 || pages <= 0) throw ltx::Error("bad cache shape");
         if ((int64_t)pages * LTX_KV_PAGE > 0x7fffffff) throw ltx::Error("a cache holds at most 2^25 - 1 pages");
         HIPC(hipSetDevice(c->device));
+        ltx::RelaxedCapture relaxed;
         ltx_kv_cache* k = new ltx_kv_cache();
         try {
             k->device = c->device;
@@ -143,8 +145,10 @@ int ltx_kv_cache_create(ltx_ctx* c, int mode, int kv_heads, int pages, ltx_kv_ca
             k->pages = pages;
             k->blocks = (size_t)pages * kv_heads * LTX_KV_BLOCK;
             k->buf.alloc(k->blocks + 256 + (size_t)pages * 4);
-            // zeros: no page holds a code of a non-finite value before it is written
-            HIPC(hipMemset(k->buf.p, 0, k->buf.bytes));
+            // zeros: no page holds a code of a non-finite value before it is written (on
+            // the context's own stream, which a capture elsewhere does not see)
+            HIPC(hipMemsetAsync(k->buf.p, 0, k->buf.bytes, c->side));
+            HIPC(hipStreamSynchronize(c->side));
         } catch (...) {
             delete k;
             throw;
@@ -155,10 +159,10 @@ int ltx_kv_cache_create(ltx_ctx* c, int mode, int kv_heads, int pages, ltx_kv_ca
 
 void ltx_kv_cache_free(ltx_ctx* c, ltx_kv_cache* k) {
     if (!k) return;
-    (void)hipSetDevice(k->device);
-    (void)hipDeviceSynchronize();
     (void)c;
-    delete k;
+    (void)hipSetDevice(k->device);
+    ltx::RelaxedCapture relaxed;
+    delete k;  // hipFree waits for the device
 }
 
 uint64_t ltx_kv_cache_bytes(const ltx_kv_cache* k) { return k ? k->buf.bytes : 0; }

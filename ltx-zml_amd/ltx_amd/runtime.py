@@ -230,6 +230,9 @@ class KvBatch:
         if rows is None and row_start is not None:
             raise LtxError("KvBatch: row_start needs rows")
         self.rows = nseq if rows is None else rows
+        self.device = kv_len.get_device()
+        if any(t is not None and t.get_device() != self.device for t in (pages, row_start)):
+            raise LtxError("KvBatch: the tensors are on different devices")
         self._keep = (kv_len, pages, row_start)
         self.args = _KvBatchArgs(nseq, self.rows, _ptr(row_start), _ptr(kv_len), _ptr(pages), pages.shape[1])
         self.ref = C.addressof(self.args)
@@ -393,6 +396,9 @@ class Context:
         if not (q.shape == (N, K // 2) and K % 128 == 0 and s.shape == (N, K // 128) and y.shape == (M, N)
                 and (bias is None or bias.shape == (N,))):
             raise LtxError("linear_q4: the shapes do not fit")
+        if not (a.get_device() == q.get_device() == s.get_device() == y.get_device() == self.device
+                and (bias is None or bias.get_device() == self.device)):
+            raise LtxError("linear_q4: tensors on the context's device are needed")
         if not (a.is_contiguous() and q.is_contiguous() and s.is_contiguous() and y.is_contiguous()
                 and (bias is None or bias.is_contiguous())):
             raise LtxError("linear_q4: contiguous tensors are needed")
@@ -443,8 +449,11 @@ class Context:
         st = stream.cuda_stream if stream is not None else _current_stream()
         _rows("kv_attention", batch, cache, heads, q, out)
         if glog is not None and not (glog.shape == (batch.rows, heads) and glog.is_contiguous()
-                                     and glog.dtype == _torch_dtype(MODE_F32)):
-            raise LtxError("kv_attention: glog must be f32 [rows, heads]")
+                                     and glog.dtype == _torch_dtype(MODE_F32)
+                                     and glog.get_device() == self.device):
+            raise LtxError("kv_attention: glog must be f32 [rows, heads] on the context's device")
+        if work is not None and not (work.is_contiguous() and work.get_device() == self.device):
+            raise LtxError("kv_attention: work must be contiguous, on the context's device")
         self._check(lib().ltx_op_kv_attention(self.handle, cache.handle, batch.ref, _ptr(q), q.stride(0), heads,
                                               int(causal), _ptr(glog), _ptr(out), out.stride(0), _ptr(work),
                                               0 if work is None else work.numel() * work.element_size(), st),
@@ -539,8 +548,12 @@ def _torch_dtype(mode: int):
 
 def _rows(name: str, batch: KvBatch, cache: KvCache, heads: int, *tensors):
     """Tensors [rows, heads * 128] of the cache's type, values of a row next to each other."""
-    shape, dt = (batch.rows, heads * 128), _torch_dtype(cache.mode)
+    shape, dt, device = (batch.rows, heads * 128), _torch_dtype(cache.mode), cache.ctx.device
+    if batch.device != device:
+        raise LtxError(f"{name}: a batch on the context's device is needed")
     for t in tensors:
+        if t.get_device() != device:
+            raise LtxError(f"{name}: tensors on the context's device are needed")
         if t.shape != shape or t.dtype != dt or t.stride(1) != 1:
             raise LtxError(f"{name}: {list(shape)} tensors of the cache's type are needed")
 

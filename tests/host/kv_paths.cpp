@@ -8,6 +8,11 @@
 #include "ltx_internal.hpp"
 #include "ltx_kv_index.h"
 
+// what fake_hip.hpp leaves out
+extern "C" hipError_t hipMemsetAsync(void*, int, size_t, hipStream_t s) {
+    return fake::capturing.count(s) ? hipErrorStreamCaptureUnsupported : hipSuccess;
+}
+
 #define CHECK(cond, ...)                                  \
     do {                                                  \
         if (!(cond)) {                                    \
@@ -113,6 +118,9 @@ static void refusals() {
     CHECK(f.write() && f.read() && f.attend() && launches("") == 0, "%s", ltx_last_error(f.c));
     f.b.rows = 1 << 24;
     REFUSED(f.attend(), "too many rows");
+    f.b.rows = 1 << 28;
+    REFUSED(f.write(), "too many rows");
+    REFUSED(f.read(), "too many rows");
 
     auto q4 = [&](const void* a, const void* q, const void* s, int s16, const void* bias, void* y, int f32, int M, int N,
                   int K, int mode) {
@@ -170,6 +178,13 @@ static void memory() {
     CHECK(ltx_kv_cache_bytes(f.cache) >= 100ull * 64 * 8 * 136, "%llu", (unsigned long long)ltx_kv_cache_bytes(f.cache));
     ltx_kv_cache_free(f.c, f.cache);
     CHECK(with - fake::in_use >= 100ull * 64 * 8 * 136 && before <= fake::in_use, "freed");
+    // made and freed beside a capture of another stream, in the global mode
+    fake::capturing.insert((hipStream_t)0x77);
+    ltx_kv_cache* beside = nullptr;
+    CHECK(ltx_kv_cache_create(f.c, 0, 8, 100, &beside), "%s", ltx_last_error(f.c));
+    ltx_kv_cache_free(f.c, beside);
+    CHECK(!fake::broken_capture, "the capture is broken");
+    fake::capturing.clear();
     fake::limit = fake::in_use;
     ltx_kv_cache* k = (ltx_kv_cache*)1;
     CHECK(!ltx_kv_cache_create(f.c, 0, 8, 100, &k) && !k, "no memory: refused, no handle");

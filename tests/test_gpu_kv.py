@@ -454,6 +454,79 @@ def test_captured_steps_follow_the_lengths(any_tile):
             assert torch.equal(eager, x["out"]) and torch.isfinite(eager).all()
 
 
+def test_captured_without_a_workspace(any_tile):
+    """A captured call that is given no workspace does not split: within the same
+    bounds, at every replay."""
+    ctx = any_tile
+    say("kv graph without workspace")
+    s = Setup(ctx, "f16", 2, [1, 3, 130], [1500, 64, 2000], seed=25)
+    q = s.queries(4)
+    want, tol = s.want(q, 4, True)
+    dev, out = q.cuda(), torch.zeros(s.total, 4 * HD, dtype=s.dt, device="cuda")
+    ctx.kv_attention(s.cache, s.batch, dev, out, 4)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        ctx.kv_attention(s.cache, s.batch, dev, out, 4)
+    for _ in range(3):
+        out.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        check(out, want, tol)
+        eager = torch.zeros_like(out)
+        ctx.kv_attention(s.cache, s.batch, dev, eager, 4)
+        check(eager, want, tol)
+
+
+def test_two_calls_at_once(any_tile):
+    """Two eager calls on two streams, each with its own workspace, and two that share
+    the context's scratch: the bits of the calls one by one."""
+    ctx = any_tile
+    say("kv two streams")
+    a = Setup(ctx, "f16", 2, [1, 1], [3000, 1200], seed=26)
+    b = Setup(ctx, "bf16", 4, [40], [2500], seed=27)
+    torch.cuda.synchronize()
+    cases = [(s, s.queries(8).cuda()) for s in (a, b)]
+    alone = [s.attend(q, 8, True) for s, q in cases]
+    works = [torch.empty(max(16, ctx.kv_attention_workspace(s.cache, s.batch, 8)), dtype=torch.uint8, device="cuda")
+             for s, _ in cases]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for shared in (False, True):
+        for _ in range(5):
+            outs = [torch.zeros_like(o) for o in alone]
+            torch.cuda.synchronize()
+            for (s, q), out, work, st in zip(cases, outs, works, streams):
+                ctx.kv_attention(s.cache, s.batch, q, out, 8, work=None if shared else work, stream=st)
+            torch.cuda.synchronize()
+            for out, ref in zip(outs, alone):
+                assert torch.equal(out, ref)
+
+
+def test_rows_of_no_sequence(any_tile):
+    """Rows before the first sequence's and between row_start's ends are of none: out
+    and what is read back stay as they were, the cache too."""
+    ctx = any_tile
+    say("kv rows of no sequence")
+    s = Setup(ctx, "bf16", 2, [2, 70], [100, 300], seed=28)
+    q = s.queries(4)
+    want, tol = s.want(q, 4, True)
+    shift = 5
+    wide = torch.full((s.total + shift + 2, 4 * HD), math.nan, dtype=s.dt, device="cuda")
+    wide[shift:shift + s.total] = q.cuda()
+    out = torch.full_like(wide, 7.0)
+    b = rt.KvBatch(s.lens, s.pages, ints(s.row_start + shift), wide.shape[0])
+    ctx.kv_attention(s.cache, b, wide, out, 4)
+    check(out[shift:shift + s.total], want, tol)
+    assert (out[:shift] == 7).all() and (out[shift + s.total:] == 7).all()
+    k = torch.full((2, wide.shape[0], 2 * HD), 9.0, dtype=s.dt, device="cuda")
+    ctx.kv_read(s.cache, b, k[0], k[1])
+    assert (k[:, :shift] == 9).all() and (k[:, shift + s.total:] == 9).all() and (k[:, shift:shift + s.total] != 9).all()
+    k[:, :shift] = math.nan
+    k[:, shift + s.total:] = math.nan
+    ctx.kv_write(s.cache, b, k[0], k[1])  # what is held already, and NaN in rows of none
+    check(s.attend(q, 4, True), want, tol)
+
+
 @pytest.mark.parametrize("mode", ["f16", "bf16"])
 def test_a_decoder_step(ctx, mode):
     """The operators as one layer's step uses them: the 4-bit q|k|v projection, its k

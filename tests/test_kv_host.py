@@ -57,10 +57,16 @@ def test_python_checks():
         with pytest.raises(rt.LtxError):
             rt.KvBatch(*bad)
 
+    class Ctx:
+        device = -1  # the tensors' here: the CPU
+
     class Cache:
-        kv_heads, mode, handle = 2, rt.MODE_F16, 0
+        kv_heads, mode, handle, ctx = 2, rt.MODE_F16, 0, Ctx
     good = torch.zeros(7, 256, dtype=torch.float16)
     rt._rows("x", b, Cache, 2, good, torch.zeros(7, 768, dtype=torch.float16)[:, 256:512])
     for bad in [good[:6], good[:, :128], good.bfloat16(), torch.zeros(256, 7, dtype=torch.float16).T, good[0]]:
         with pytest.raises(rt.LtxError):
             rt._rows("x", b, Cache, 2, bad)
+    Ctx.device = 0
+    with pytest.raises(rt.LtxError, match="device"):
+        rt._rows("x", b, Cache, 2, good)
