@@ -177,8 +177,8 @@ __device__ __forceinline__ void kv_rows(const LtxKvRowsArgs& a) {
         for (int e = 0; e < KV_HB; e++) {
             wk[e] = wv[e] = u32x4{0, 0, 0, 0};
             if (row < a.b.rows && e < heads) {
-                wk[e] = *(const u32x4*)(k + LTX_HD * e);
-                wv[e] = *(const u32x4*)(v + LTX_HD * e);
+                wk[e] = __builtin_nontemporal_load((const u32x4*)(k + LTX_HD * e));
+                wv[e] = __builtin_nontemporal_load((const u32x4*)(v + LTX_HD * e));
             }
         }
     const int b = kv_find(a.b, row0, sub);
@@ -258,10 +258,12 @@ __device__ __forceinline__ void kv_rows(const LtxKvRowsArgs& a) {
             if (!in || e >= heads) continue;
             const float sk1 = scale_of(sks[e], 0), sv1 = scale_of(svs[e], 0);
             const uint32_t q0 = qk[e], q1 = qv[e];
-            *(u32x4*)(k + LTX_HD * e) = u32x4{Fp4<T>::template pair<0>(q0, sk1), Fp4<T>::template pair<1>(q0, sk1),
-                                              Fp4<T>::template pair<2>(q0, sk1), Fp4<T>::template pair<3>(q0, sk1)};
-            *(u32x4*)(v + LTX_HD * e) = u32x4{Fp4<T>::template pair<0>(q1, sv1), Fp4<T>::template pair<1>(q1, sv1),
-                                              Fp4<T>::template pair<2>(q1, sv1), Fp4<T>::template pair<3>(q1, sv1)};
+            const u32x4 xk = {Fp4<T>::template pair<0>(q0, sk1), Fp4<T>::template pair<1>(q0, sk1),
+                              Fp4<T>::template pair<2>(q0, sk1), Fp4<T>::template pair<3>(q0, sk1)};
+            const u32x4 xv = {Fp4<T>::template pair<0>(q1, sv1), Fp4<T>::template pair<1>(q1, sv1),
+                              Fp4<T>::template pair<2>(q1, sv1), Fp4<T>::template pair<3>(q1, sv1)};
+            __builtin_nontemporal_store(xk, (u32x4*)(k + LTX_HD * e));
+            __builtin_nontemporal_store(xv, (u32x4*)(v + LTX_HD * e));
         }
     }
 }
@@ -486,7 +488,8 @@ __device__ __forceinline__ void kv_v_pair(const uint32_t (&x)[8], const uint32_t
 // lanes.
 // A wave's next page is on its way while it computes on one, its index read a page
 // earlier still.
-template <typename T>
+// NT: the codes as streaming loads, for caches beyond what the memory-side cache holds.
+template <typename T, bool NT>
 __device__ __forceinline__ void kv_attn(const LtxKvAttnArgs& a) {
     typedef typename Op<T>::v8 v8;
     __shared__ __attribute__((aligned(16))) float so[KV_WAVES][KV_TILE][LTX_HD + 4];
@@ -526,6 +529,9 @@ __device__ __forceinline__ void kv_attn(const LtxKvAttnArgs& a) {
             uint32_t ks, flag;
             bool none;
         };
+        auto codes = [](const uint8_t* at) {
+            return NT ? __builtin_nontemporal_load((const u32x4*)at) : *(const u32x4*)at;
+        };
         auto load = [&](Page& x, int p) {
             if (p >= p1) return;
             x.none = next >= (uint32_t)a.b.pool;
@@ -535,10 +541,11 @@ __device__ __forceinline__ void kv_attn(const LtxKvAttnArgs& a) {
             const uint8_t* blk = a.b.data + kv_block(a.b, page, kh);
             x.flag = flags[page];
 #pragma unroll
-            for (int t = 0; t < 4; t++) x.k[t] = *(const u32x4*)(blk + 1024 * t + 16 * lane);
+            for (int t = 0; t < 4; t++) x.k[t] = codes(blk + 1024 * t + 16 * lane);
             x.ks = *(const uint32_t*)(blk + LTX_KV_KS + 4 * lane);
 #pragma unroll
-            for (int t = 0; t < 4; t++) x.v[t] = *(const u32x4*)(blk + LTX_KV_V + 1024 * t + 16 * lane);
+            for (int t = 0; t < 4; t++)
+                x.v[t] = codes(blk + LTX_KV_V + 1024 * t + 16 * lane);
             x.vs = *(const u32x4*)(blk + LTX_KV_VS + 64 * (r >> 2) + 16 * h);
             next = p + KV_WAVES < p1 ? table[p + KV_WAVES] : 0u;
             __builtin_amdgcn_sched_barrier(0);
@@ -646,8 +653,14 @@ __device__ __forceinline__ void kv_attn(const LtxKvAttnArgs& a) {
     } while (kv_next(a, it));
 }
 
-extern "C" __global__ void __launch_bounds__(64 * KV_WAVES) ltx_kv_attn_f16(const LtxKvAttnArgs a) { kv_attn<_Float16>(a); }
-extern "C" __global__ void __launch_bounds__(64 * KV_WAVES) ltx_kv_attn_bf16(const LtxKvAttnArgs a) { kv_attn<__bf16>(a); }
+#define KV_ATTN(NAME, T, NT)                                                                  \
+    extern "C" __global__ void __launch_bounds__(64 * KV_WAVES) NAME(const LtxKvAttnArgs a) { \
+        kv_attn<T, NT>(a);                                                                    \
+    }
+KV_ATTN(ltx_kv_attn_f16, _Float16, false)
+KV_ATTN(ltx_kv_attn_bf16, __bf16, false)
+KV_ATTN(ltx_kv_attn_f16_nt, _Float16, true)
+KV_ATTN(ltx_kv_attn_bf16_nt, __bf16, true)
 
 // Many columns: a workgroup takes 128 NQ columns, its eight waves 16 NQ each, and a
 // run of pages. A page's codes become MFMA operands once for all eight waves, in LDS,

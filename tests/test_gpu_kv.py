@@ -368,6 +368,26 @@ def test_attention_leaves_bad_pages_out(any_tile):
         assert s.cache.faults() > 0
 
 
+@pytest.mark.parametrize("mode", ["f16", "bf16"])
+def test_tables_wider_than_what_is_in_use(any_tile, mode):
+    """A table of 10,000 pages a sequence, nothing behind the first few looked at: the
+    kernel of large caches, and splits over few real pages."""
+    ctx = any_tile
+    say(f"kv wide table {mode}")
+    s = Setup(ctx, mode, 2, [1, 1, 40], [700, 0, 1300], seed=29)
+    wide = torch.full((3, 10000), 0x7ffffff0, dtype=torch.int32, device="cuda")
+    wide[:, :s.pages.shape[1]] = s.pages
+    wide[1] = -1
+    s.pages = wide
+    s.batch = rt.KvBatch(s.lens, wide, ints(s.row_start), s.total)
+    assert 3 * 10000 * 2 * 8704 > 384 << 20
+    for causal in (True, False):
+        q = s.queries(4)
+        want, tol = s.want(q, 4, causal)
+        check(s.attend(q, 4, causal), want, tol)
+    assert s.cache.faults() == 0
+
+
 def test_strides_streams_and_repeats(ctx):
     """q and out as slices of wider rows, on another stream; equal bits every time."""
     say("kv attention strides and streams")
