@@ -28,14 +28,15 @@ extern "C" int ltx_op_linear_q4(ltx_ctx* c, const void* a, const uint8_t* q, con
         // leave no CU idle. us, 16 / 32 / 64 columns: one row of 4,096 x 4,096 5.7 / 6.8 /
         // 9.2, of 8,192 8.7 / 7.0 / 10.1, of 12,288 12.0 / 11.8 / 10.1, of 16,384 16.1 /
         // 12.4 / 10.4; 64 rows of 4,096 x 4,096 13.6 / 9.2 / 12.1, of 8,192 24.9 / 17.2 /
-        // 13.4; mode F32, 32 rows of 4,096 x 4,096 20.8 / 11.9 / 14.9.
+        // 13.4; mode F32, one row of 4,096 x 4,096 6.0 / 7.4 / 9.7, of 16,384 17.3 / 13.6 /
+        // 10.9, 32 rows of 4,096 x 4,096 20.8 / 11.9 / 14.9.
         const bool f32 = mode == LTX_MODE_F32;
         const int mt = f32 || M <= 16 ? 1 : 2, gy = (M + 16 * mt - 1) / (16 * mt);
         int nt = 1;
         while (nt < 4 && ((int64_t)N + 16 * nt - 1) / (16 * nt) * gy > c->num_cu) nt *= 2;
         char name[48];
         std::snprintf(name, sizeof(name), "ltx_linear_q4_%s_s%d_%d_%d",
-                      f32 ? "f32" : mode == LTX_MODE_F16 ? "f16" : "bf16", scale_f16 ? 16 : 32, mt, nt);
+                      f32 ? M <= LTX_Q4_PACKED ? "f32p" : "f32" : mode == LTX_MODE_F16 ? "f16" : "bf16", scale_f16 ? 16 : 32, mt, nt);
         c->launch(name, (unsigned)(((int64_t)N + 16 * nt - 1) / (16 * nt)), gy, 1, 512, &g, (hipStream_t)stream);
     })
 }

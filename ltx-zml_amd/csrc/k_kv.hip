@@ -157,7 +157,11 @@ __device__ __forceinline__ uint32_t quad_pick(u32x4 x) {
 // codes a lane and head would be an access each. So the lanes of a quad exchange their
 // K codes of four heads, and each has one head's 16 bytes; with four rows on one quad
 // of positions (the rule but for a first few rows) V's codes go the same way over the
-// rows, 16 bytes of four keys a lane. All of a wave's loads are on their way at once.
+// rows, 16 bytes of four keys a lane. All of a wave's loads are on their way at once,
+// and nothing here is read twice: streaming loads and stores. Measured: 26,624 rows of
+// 32 heads written in 138 us and read in 80, 28,672 read in 89 (594 MB, 6.7 TB/s); with
+// loads and stores that stay in the caches 164, 94 and 119 .. 152, with a dword of codes
+// a lane besides 175, 185 and 213 .. 230.
 #define KV_HB 4
 template <typename T, bool WRITE>
 __device__ __forceinline__ void kv_rows(const LtxKvRowsArgs& a) {
@@ -488,6 +492,10 @@ __device__ __forceinline__ void kv_v_pair(const uint32_t (&x)[8], const uint32_t
 // lanes.
 // A wave's next page is on its way while it computes on one, its index read a page
 // earlier still.
+// Bound: the cache's bytes. Four sequences of 28,672 keys and 32 heads (499 MB) in 87
+// us, 5.7 TB/s; 32 ragged ones of up to 8,192 keys and 8 heads (146 MB, of which the
+// memory-side cache holds much between calls) in 36. One short sequence is latency: a
+// page's index, its codes, two rounds of products and the waves' join, 8 us.
 // NT: the codes as streaming loads, for caches beyond what the memory-side cache holds.
 template <typename T, bool NT>
 __device__ __forceinline__ void kv_attn(const LtxKvAttnArgs& a) {
@@ -666,7 +674,15 @@ KV_ATTN(ltx_kv_attn_bf16_nt, __bf16, true)
 // run of pages. A page's codes become MFMA operands once for all eight waves, in LDS,
 // in the order the operands are read (16 bytes a lane, no conflicts): waves 0 .. 3 a
 // 16-key block of K each, waves 4 .. 7 half the dims of 32 keys of V each, one page
-// ahead, from codes loaded two pages ahead. One barrier a page.
+// ahead, from codes loaded two pages ahead. Two barriers a page, see below.
+// Bound: a page is 1,024 cycles of MFMAs a SIMD and takes about 2,000, the rest
+// being the exponentials, the conversions and the operands' reads from LDS, which the
+// other group's products hide in part. 2,048 columns of 32 heads over 28,672 keys (962
+// GFLOP) take 825 us, 1.17 PFLOP/s, causal runs of three sequences of up to 2,970
+// tokens (154 GFLOP) 190. On the way there, the same call: every wave forming its own
+// operands 1,675 us, operands in LDS 1,176, two groups a phase apart 1,137, loads
+// without branches 1,100, one straight block of products without spills 900, staging
+// before the softmax 840.
 template <typename T, int NQ, bool SPLIT>
 __device__ __forceinline__ void kv_attn_rows(const LtxKvAttnArgs& a) {
     typedef typename Op<T>::v8 v8;
@@ -684,267 +700,268 @@ __device__ __forceinline__ void kv_attn_rows(const LtxKvAttnArgs& a) {
     KvSpan it;
     if (!kv_begin(a, item, it)) return;
     do {
-    const int limit = kv_tile_limit(a.causal, it.s, a.group, it.tile, a.tile), np = kv_pages(limit);
-    const int p0 = SPLIT ? it.page : 0, units = SPLIT ? kv_span(it) : np, p1 = min(np, p0 + units);
+        const int limit = kv_tile_limit(a.causal, it.s, a.group, it.tile, a.tile), np = kv_pages(limit);
+        const int p0 = SPLIT ? it.page : 0, units = SPLIT ? kv_span(it) : np, p1 = min(np, p0 + units);
 
-    const int ncol = it.s.n * a.group, c0 = it.tile * a.tile + 16 * NQ * w;  // the wave's first column
-    const bool idle = c0 >= ncol;
-    // keys that the lane's column of block q sees
-    auto limit_of = [&](int q) {
-        return kv_limit(a.causal, it.s, min(c0 + 16 * q + (my_lane() & 15), ncol - 1) / a.group);
-    };
-    v8 qf[NQ][4];
-#pragma unroll
-    for (int q = 0; q < NQ; q++) {
-        const int lane = my_lane(), r = lane & 15, h = lane >> 4;
-        const int c = min(c0 + 16 * q + r, ncol - 1), row = c / a.group;
-        const uint16_t* Q = (const uint16_t*)a.q + (size_t)(it.s.s0 + row) * a.ldq +
-                            (size_t)(kh * a.group + c % a.group) * LTX_HD + 32 * h;
-#pragma unroll
-        for (int j = 0; j < 4; j++) qf[q][j] = __builtin_bit_cast(v8, *(const u32x4*)(Q + 8 * j));
-    }
-    const int all = kv_limit(a.causal, it.s, min(c0, ncol - 1) / a.group);  // keys that every column sees
-
-    // Staging. A page's index is read two pages before its codes are used, its flag
-    // beside them, by scalar loads (the constant address space: nothing writes them
-    // while the kernel runs); K's waves use x0 and y0. One set of loads for both kinds
-    // of wave: a branch's own would be waited for where the branches meet.
-    typedef const __attribute__((address_space(4))) uint32_t* scalar_ptr;
-    const scalar_ptr table = (scalar_ptr)(uintptr_t)(a.b.pages + (size_t)it.b * a.b.max_pages);
-    const scalar_ptr flags = (scalar_ptr)(uintptr_t)a.b.flags;
-    uint32_t next = p0 < p1 ? table[p0] : 0u;  // index of the page whose codes come next
-    u32x4 x0, x1;                              // its codes and scales
-    uint32_t y0, y1, flag = 0, none = 0;       // its flag, or that it is outside the pool
-    uint32_t flag_s = 0, none_s = 0;           // those of the page in LDS
-    const int vt = 2 * ((w - 4) >> 1);         // V: first 16-key block of the wave's 32 keys
-    const uint32_t ox = w < 4 ? 1024 * w : LTX_KV_V + 1024 * vt, dx = w < 4 ? 0 : 1024;
-    const uint32_t oy = w < 4 ? LTX_KV_KS : LTX_KV_VS + 4 * vt, is_k = w < 4 ? ~0u : 0u;
-    auto load = [&](int p) {
-        none = next < (uint32_t)a.b.pool ? 0u : 1u;
-        const uint32_t page = none ? 0u : next, lane = my_lane();
-        if (none && w == 0 && kh == 0 && lane == 0) atomicAdd(a.b.bad, 1ull);
-        const uint8_t* blk = a.b.data + kv_block(a.b, page, kh);
-        x0 = *(const u32x4*)(blk + ox + 16 * lane);
-        x1 = *(const u32x4*)(blk + ox + dx + 16 * lane);
-        const uint32_t at = oy + (((4 * lane) & is_k) | (((lane & 12) << 4 | (lane & 48)) & ~is_k));
-        y0 = *(const uint32_t*)(blk + at);
-        y1 = *(const uint32_t*)(blk + at + 4);
-        flag = flags[page];
-        next = p + 1 < p1 ? table[p + 1] : 0u;
-    };
-    auto stage = [&](int buf) {
-        const int lane = my_lane();
-        if (w < 4) {
-            const float f = __builtin_bit_cast(float, ((y0 >> (8 * w)) & 255u) << 23);
-#pragma unroll
-            for (int j = 0; j < 4; j++)
-                *(u32x4*)(sk[buf] + 1024 * (4 * w + j) + 16 * lane) =
-                    u32x4{Fp4<T>::template pair<0>(x0[j], f), Fp4<T>::template pair<1>(x0[j], f),
-                          Fp4<T>::template pair<2>(x0[j], f), Fp4<T>::template pair<3>(x0[j], f)};
-        } else {
-            if (flag) {
-                u32x4 vs = {y0, y1, 0, 0};
-                const uint32_t bits = kv_drop_nan(vs);
-                y0 = vs[0];
-                y1 = vs[1];
-                if ((w & 1) == 0 && (lane & 15) == 0) snan[buf][vt >> 1][lane >> 4] = bits;
-            }
-            const uint32_t x[8] = {x0[0], x0[1], x0[2], x0[3], x1[0], x1[1], x1[2], x1[3]}, f[2] = {y0, y1};
-            uint8_t* d = sv[buf] + 1024 * (4 * vt) + 16 * lane;
-            u32x4 lo, hi;
-            if ((w & 1) == 0) {
-                kv_v_pair<T, 0>(x, f, lo, hi);
-                *(u32x4*)d = lo;
-                *(u32x4*)(d + 1024) = hi;
-                kv_v_pair<T, 1>(x, f, lo, hi);
-                *(u32x4*)(d + 2048) = lo;
-                *(u32x4*)(d + 3072) = hi;
-            } else {
-                kv_v_pair<T, 2>(x, f, lo, hi);
-                *(u32x4*)(d + 4096) = lo;
-                *(u32x4*)(d + 5120) = hi;
-                kv_v_pair<T, 3>(x, f, lo, hi);
-                *(u32x4*)(d + 6144) = lo;
-                *(u32x4*)(d + 7168) = hi;
-            }
-        }
-    };
-
-    f32x4 o[8][NQ], s[NQ][4];  // O^T, S^T
-    v8 pf[NQ][2];
-    float m[NQ], l[NQ];  // running maximum (times C) and sum
-#pragma unroll
-    for (int q = 0; q < NQ; q++) {
-#pragma unroll
-        for (int db = 0; db < 8; db++) o[db][q] = f32x4{0};
-        m[q] = -__builtin_inff();
-        l[q] = 0.f;
-    }
-    const float C = a.scale_log2;
-    const int nt = max(p1 - p0, 0);
-
-    auto sync = [&]() {
-        __builtin_amdgcn_sched_barrier(0);
-        asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-        __builtin_amdgcn_sched_barrier(0);
-    };
-    auto pv = [&](int t) {
-        const uint8_t* b = sv[t & 1] + 16 * my_lane();
-#pragma unroll
-        for (int c = 0; c < 2; c++)
-#pragma unroll
-            for (int db = 0; db < 8; db++) {
-                const v8 vf = __builtin_bit_cast(v8, *(const u32x4*)(b + 1024 * (8 * c + db)));
-#pragma unroll
-                for (int q = 0; q < NQ; q++) o[db][q] = Op<T>::mfma16(vf, pf[q][c], o[db][q]);
-            }
-    };
-    auto scores = [&](int t) {
-        const uint8_t* b = sk[t & 1] + 16 * my_lane();
-#pragma unroll
-        for (int j = 0; j < 4; j++)
-#pragma unroll
-            for (int x = 0; x < 4; x++) {
-                const v8 kf = __builtin_bit_cast(v8, *(const u32x4*)(b + 1024 * (4 * x + j)));
-#pragma unroll
-                for (int q = 0; q < NQ; q++) s[q][x] = Op<T>::mfma16(kf, qf[q][j], j == 0 ? f32x4{0} : s[q][x]);
-            }
-    };
-    // PV(t - 1), then S(t); the operands' reads run four ahead of their products
-    // (masks: 0x100 DS read, 0x008 MFMA)
-    auto products = [&](int t) {
-        if (idle) return;
-        __builtin_amdgcn_s_setprio(1);
-        pv(t - 1);
-        scores(t);
-        __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
-#pragma unroll
-        for (int i = 0; i < 32; i++) {
-            __builtin_amdgcn_sched_group_barrier(0x008, NQ, 0);
-            if (i < 28) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
-        }
-        __builtin_amdgcn_s_setprio(0);
-    };
-    // scores -> weights with maximum mc, and their sum
-    auto weights = [&](int q, float mc) {
-        float sum = 0.f;
-#pragma unroll
-        for (int c = 0; c < 2; c++) {
-            u32x4 pw;
-#pragma unroll
-            for (int e = 0; e < 4; e++) {
-                const f32x4& x = s[q][2 * c + (e >> 1)];
-                const int i = 2 * (e & 1);
-                pw[e] = Op<T>::cvt2(__builtin_amdgcn_exp2f(__builtin_fmaf(x[i], C, -mc)),
-                                    __builtin_amdgcn_exp2f(__builtin_fmaf(x[i + 1], C, -mc)));
-                sum = Op<T>::sum2(pw[e], sum);
-            }
-            pf[q][c] = __builtin_bit_cast(v8, pw);
-        }
-        return sum;
-    };
-    auto softmax = [&](int t) {
-        const int p = p0 + t;
-        if (idle) return;
-        if (flag_s) {
-            const int h = my_lane() >> 4;
-            const uint32_t bits = snan[t & 1][0][h] | snan[t & 1][1][h] << 8;
-#pragma unroll
-            for (int q = 0; q < NQ; q++) kv_set_nan(s[q], bits);
-        }
-        if (none_s || (p + 1) * LTX_KV_PAGE > all)
-#pragma unroll
-            for (int q = 0; q < NQ; q++) kv_mask(s[q], p, none_s ? 0 : limit_of(q), my_lane() >> 4);
+        const int ncol = it.s.n * a.group, c0 = it.tile * a.tile + 16 * NQ * w;  // the wave's first column
+        const bool idle = c0 >= ncol;
+        // keys that the lane's column of block q sees
+        auto limit_of = [&](int q) {
+            return kv_limit(a.causal, it.s, min(c0 + 16 * q + (my_lane() & 15), ncol - 1) / a.group);
+        };
+        v8 qf[NQ][4];
 #pragma unroll
         for (int q = 0; q < NQ; q++) {
-            // weights with the maximum so far; only where a column's sum of them is
-            // beyond 2^8 (as it is before it has had a score: m is -inf) the page's
-            // maximum is taken, m moved, and the weights formed again
-            float sum = weights(q, m[q]);
-            if (__builtin_amdgcn_ballot_w64(!(sum <= 256.f)) != 0) {
-                float mx = s[q][0][0];
+            const int lane = my_lane(), r = lane & 15, h = lane >> 4;
+            const int c = min(c0 + 16 * q + r, ncol - 1), row = c / a.group;
+            const uint16_t* Q = (const uint16_t*)a.q + (size_t)(it.s.s0 + row) * a.ldq +
+                                (size_t)(kh * a.group + c % a.group) * LTX_HD + 32 * h;
 #pragma unroll
-                for (int x = 0; x < 4; x++)
+            for (int j = 0; j < 4; j++) qf[q][j] = __builtin_bit_cast(v8, *(const u32x4*)(Q + 8 * j));
+        }
+        const int all = kv_limit(a.causal, it.s, min(c0, ncol - 1) / a.group);  // keys that every column sees
+
+        // Staging. A page's index is read two pages before its codes are used, its flag
+        // beside them, by scalar loads (the constant address space: nothing writes them
+        // while the kernel runs); K's waves use x0 and y0. One set of loads for both kinds
+        // of wave: a branch's own would be waited for where the branches meet.
+        typedef const __attribute__((address_space(4))) uint32_t* scalar_ptr;
+        const scalar_ptr table = (scalar_ptr)(uintptr_t)(a.b.pages + (size_t)it.b * a.b.max_pages);
+        const scalar_ptr flags = (scalar_ptr)(uintptr_t)a.b.flags;
+        uint32_t next = p0 < p1 ? table[p0] : 0u;  // index of the page whose codes come next
+        u32x4 x0, x1;                              // its codes and scales
+        uint32_t y0, y1, flag = 0, none = 0;       // its flag, or that it is outside the pool
+        uint32_t flag_s = 0, none_s = 0;           // those of the page in LDS
+        const int vt = 2 * ((w - 4) >> 1);         // V: first 16-key block of the wave's 32 keys
+        const uint32_t ox = w < 4 ? 1024 * w : LTX_KV_V + 1024 * vt, dx = w < 4 ? 0 : 1024;
+        const uint32_t oy = w < 4 ? LTX_KV_KS : LTX_KV_VS + 4 * vt, is_k = w < 4 ? ~0u : 0u;
+        auto load = [&](int p) {
+            none = next < (uint32_t)a.b.pool ? 0u : 1u;
+            const uint32_t page = none ? 0u : next, lane = my_lane();
+            if (none && w == 0 && kh == 0 && lane == 0) atomicAdd(a.b.bad, 1ull);
+            const uint8_t* blk = a.b.data + kv_block(a.b, page, kh);
+            x0 = *(const u32x4*)(blk + ox + 16 * lane);
+            x1 = *(const u32x4*)(blk + ox + dx + 16 * lane);
+            const uint32_t at = oy + (((4 * lane) & is_k) | (((lane & 12) << 4 | (lane & 48)) & ~is_k));
+            y0 = *(const uint32_t*)(blk + at);
+            y1 = *(const uint32_t*)(blk + at + 4);
+            flag = flags[page];
+            next = p + 1 < p1 ? table[p + 1] : 0u;
+        };
+        auto stage = [&](int buf) {
+            const int lane = my_lane();
+            if (w < 4) {
+                const float f = __builtin_bit_cast(float, ((y0 >> (8 * w)) & 255u) << 23);
 #pragma unroll
-                    for (int i = 0; i < 4; i++) mx = fmaxf(mx, s[q][x][i]);
-                const float mn = fmaxf(m[q], kv_quad_max(mx) * C), mz = mn == -__builtin_inff() ? 0.f : mn;
-                const float corr = __builtin_amdgcn_exp2f(m[q] - mz);
-                m[q] = mn;
-                l[q] *= corr;
-#pragma unroll
-                for (int db = 0; db < 8; db++) o[db][q] *= corr;
-                sum = weights(q, mz);
+                for (int j = 0; j < 4; j++)
+                    *(u32x4*)(sk[buf] + 1024 * (4 * w + j) + 16 * lane) =
+                        u32x4{Fp4<T>::template pair<0>(x0[j], f), Fp4<T>::template pair<1>(x0[j], f),
+                              Fp4<T>::template pair<2>(x0[j], f), Fp4<T>::template pair<3>(x0[j], f)};
+            } else {
+                if (flag) {
+                    u32x4 vs = {y0, y1, 0, 0};
+                    const uint32_t bits = kv_drop_nan(vs);
+                    y0 = vs[0];
+                    y1 = vs[1];
+                    if ((w & 1) == 0 && (lane & 15) == 0) snan[buf][vt >> 1][lane >> 4] = bits;
+                }
+                const uint32_t x[8] = {x0[0], x0[1], x0[2], x0[3], x1[0], x1[1], x1[2], x1[3]}, f[2] = {y0, y1};
+                uint8_t* d = sv[buf] + 1024 * (4 * vt) + 16 * lane;
+                u32x4 lo, hi;
+                if ((w & 1) == 0) {
+                    kv_v_pair<T, 0>(x, f, lo, hi);
+                    *(u32x4*)d = lo;
+                    *(u32x4*)(d + 1024) = hi;
+                    kv_v_pair<T, 1>(x, f, lo, hi);
+                    *(u32x4*)(d + 2048) = lo;
+                    *(u32x4*)(d + 3072) = hi;
+                } else {
+                    kv_v_pair<T, 2>(x, f, lo, hi);
+                    *(u32x4*)(d + 4096) = lo;
+                    *(u32x4*)(d + 5120) = hi;
+                    kv_v_pair<T, 3>(x, f, lo, hi);
+                    *(u32x4*)(d + 6144) = lo;
+                    *(u32x4*)(d + 7168) = hi;
+                }
             }
-            l[q] += sum;
-        }
-    };
+        };
 
-    // Two groups of waves a phase apart: while one runs its products, the other runs
-    // its softmax and stages (group 0 the next page's K, group 1 the next page's V),
-    // so that each SIMD's matrix and vector units both have work. Phase 2 t + group:
-    // products(t), phase 2 t + 1 + group: softmax(t).
-    //   K(t + 1) written in phase 2 t + 1, read in 2 t + 2 and 2 t + 3; V(t + 1)
-    //   written in 2 t + 2, read in 2 t + 4 and 2 t + 5; and K(t - 1)'s and V(t -
-    //   1)'s buffers, which they take, were last read in 2 t - 1 and 2 t + 1.
-    if (nt > 0) {
-        const int group = w >> 2;
-        load(p0);
-        stage(0);
-        flag_s = flag, none_s = none;
-        if (nt > 1) load(p0 + 1);
-        sync();
-        if (group) sync();
-        if (!idle) scores(0);
-        sync();
-#pragma nounroll
-        for (int t = 0; t + 1 < nt; t++) {
-            stage((t + 1) & 1);
-            const uint32_t flag_n = flag, none_n = none;
-            if (t + 2 < nt) load(p0 + t + 2);
-            __builtin_amdgcn_sched_barrier(0);
-            softmax(t);
-            flag_s = flag_n, none_s = none_n;
-            sync();
-            products(t + 1);
-            sync();
-        }
-        softmax(nt - 1);
-        sync();
-        if (!idle) pv(nt - 1);
-        if (!group) sync();
-    }
-
-    const bool whole = !SPLIT || units == it.pages;
-    const size_t part = (size_t)item + it.entity;
+        f32x4 o[8][NQ], s[NQ][4];  // O^T, S^T
+        v8 pf[NQ][2];
+        float m[NQ], l[NQ];  // running maximum (times C) and sum
 #pragma unroll
-    for (int q = 0; q < NQ; q++) {
-        const int lane = my_lane(), h = lane >> 4, c = c0 + 16 * q + (lane & 15);
-        if (c >= ncol || (!whole && part >= (size_t)a.parts)) continue;
-        float lt = l[q] + __shfl_xor(l[q], 16, 64);
-        lt += __shfl_xor(lt, 32, 64);
-        if (!whole) {
-            const size_t at = (part * a.b.kvh + kh) * a.tile + (c - it.tile * a.tile);
-            float* po = a.part + 2 * (size_t)a.parts * a.b.kvh * a.tile + at * LTX_HD + 32 * h;
-            if (h == 0) *(f32x2*)(a.part + 2 * at) = f32x2{m[q], lt};
+        for (int q = 0; q < NQ; q++) {
+#pragma unroll
+            for (int db = 0; db < 8; db++) o[db][q] = f32x4{0};
+            m[q] = -__builtin_inff();
+            l[q] = 0.f;
+        }
+        const float C = a.scale_log2;
+        const int nt = max(p1 - p0, 0);
+
+        auto sync = [&]() {
+            __builtin_amdgcn_sched_barrier(0);
+            asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+            __builtin_amdgcn_sched_barrier(0);
+        };
+        auto pv = [&](int t) {
+            const uint8_t* b = sv[t & 1] + 16 * my_lane();
+#pragma unroll
+            for (int c = 0; c < 2; c++)
+#pragma unroll
+                for (int db = 0; db < 8; db++) {
+                    const v8 vf = __builtin_bit_cast(v8, *(const u32x4*)(b + 1024 * (8 * c + db)));
+#pragma unroll
+                    for (int q = 0; q < NQ; q++) o[db][q] = Op<T>::mfma16(vf, pf[q][c], o[db][q]);
+                }
+        };
+        auto scores = [&](int t) {
+            const uint8_t* b = sk[t & 1] + 16 * my_lane();
+#pragma unroll
+            for (int j = 0; j < 4; j++)
+#pragma unroll
+                for (int x = 0; x < 4; x++) {
+                    const v8 kf = __builtin_bit_cast(v8, *(const u32x4*)(b + 1024 * (4 * x + j)));
+#pragma unroll
+                    for (int q = 0; q < NQ; q++) s[q][x] = Op<T>::mfma16(kf, qf[q][j], j == 0 ? f32x4{0} : s[q][x]);
+                }
+        };
+        // PV(t - 1), then S(t); the operands' reads run four ahead of their products
+        // (masks: 0x100 DS read, 0x008 MFMA)
+        auto products = [&](int t) {
+            if (idle) return;
+            __builtin_amdgcn_s_setprio(1);
+            pv(t - 1);
+            scores(t);
+            __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
+#pragma unroll
+            for (int i = 0; i < 32; i++) {
+                __builtin_amdgcn_sched_group_barrier(0x008, NQ, 0);
+                if (i < 28) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+            }
+            __builtin_amdgcn_s_setprio(0);
+        };
+        // scores -> weights with maximum mc, and their sum
+        auto weights = [&](int q, float mc) {
+            float sum = 0.f;
+#pragma unroll
+            for (int c = 0; c < 2; c++) {
+                u32x4 pw;
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const f32x4& x = s[q][2 * c + (e >> 1)];
+                    const int i = 2 * (e & 1);
+                    pw[e] = Op<T>::cvt2(__builtin_amdgcn_exp2f(__builtin_fmaf(x[i], C, -mc)),
+                                        __builtin_amdgcn_exp2f(__builtin_fmaf(x[i + 1], C, -mc)));
+                    sum = Op<T>::sum2(pw[e], sum);
+                }
+                pf[q][c] = __builtin_bit_cast(v8, pw);
+            }
+            return sum;
+        };
+        auto softmax = [&](int t) {
+            const int p = p0 + t;
+            if (idle) return;
+            if (flag_s) {
+                const int h = my_lane() >> 4;
+                const uint32_t bits = snan[t & 1][0][h] | snan[t & 1][1][h] << 8;
+#pragma unroll
+                for (int q = 0; q < NQ; q++) kv_set_nan(s[q], bits);
+            }
+            if (none_s || (p + 1) * LTX_KV_PAGE > all)
+#pragma unroll
+                for (int q = 0; q < NQ; q++) kv_mask(s[q], p, none_s ? 0 : limit_of(q), my_lane() >> 4);
+#pragma unroll
+            for (int q = 0; q < NQ; q++) {
+                // weights with the maximum so far; only where a column's sum of them is
+                // beyond 2^8 (as it is before it has had a score: m is -inf) the page's
+                // maximum is taken, m moved, and the weights formed again
+                float sum = weights(q, m[q]);
+                if (__builtin_amdgcn_ballot_w64(!(sum <= 256.f)) != 0) {
+                    float mx = s[q][0][0];
+#pragma unroll
+                    for (int x = 0; x < 4; x++)
+#pragma unroll
+                        for (int i = 0; i < 4; i++) mx = fmaxf(mx, s[q][x][i]);
+                    const float mn = fmaxf(m[q], kv_quad_max(mx) * C), mz = mn == -__builtin_inff() ? 0.f : mn;
+                    const float corr = __builtin_amdgcn_exp2f(m[q] - mz);
+                    m[q] = mn;
+                    l[q] *= corr;
+#pragma unroll
+                    for (int db = 0; db < 8; db++) o[db][q] *= corr;
+                    sum = weights(q, mz);
+                }
+                l[q] += sum;
+            }
+        };
+
+        // Two groups of waves a phase apart: while one runs its products, the other runs
+        // its softmax and stages (group 0 the next page's K, group 1 the next page's V),
+        // so that each SIMD's matrix and vector units both have work. Phase 2 t + group:
+        // products(t), phase 2 t + 1 + group: softmax(t).
+        //   K(t + 1) written in phase 2 t + 1, read in 2 t + 2 and 2 t + 3; V(t + 1)
+        //   written in 2 t + 2, read in 2 t + 4 and 2 t + 5; and K(t - 1)'s and V(t -
+        //   1)'s buffers, which they take, were last read in 2 t - 1 and 2 t + 1.
+        if (nt > 0) {
+            const int group = w >> 2;
+            load(p0);
+            stage(0);
+            flag_s = flag, none_s = none;
+            if (nt > 1) load(p0 + 1);
+            sync();
+            if (group) sync();
+            if (!idle) scores(0);
+            sync();
+#pragma nounroll
+            for (int t = 0; t + 1 < nt; t++) {
+                stage((t + 1) & 1);
+                const uint32_t flag_n = flag, none_n = none;
+                if (t + 2 < nt) load(p0 + t + 2);
+                __builtin_amdgcn_sched_barrier(0);
+                softmax(t);
+                flag_s = flag_n, none_s = none_n;
+                sync();
+                products(t + 1);
+                sync();
+            }
+            softmax(nt - 1);
+            sync();
+            if (!idle) pv(nt - 1);
+            if (!group) sync();
+        }
+
+        const bool whole = !SPLIT || units == it.pages;
+        const size_t part = (size_t)item + it.entity;
+#pragma unroll
+        for (int q = 0; q < NQ; q++) {
+            const int lane = my_lane(), h = lane >> 4, c = c0 + 16 * q + (lane & 15);
+            if (c >= ncol || (!whole && part >= (size_t)a.parts)) continue;
+            float lt = l[q] + __shfl_xor(l[q], 16, 64);
+            lt += __shfl_xor(lt, 32, 64);
+            if (!whole) {
+                const size_t at = (part * a.b.kvh + kh) * a.tile + (c - it.tile * a.tile);
+                float* po = a.part + 2 * (size_t)a.parts * a.b.kvh * a.tile + at * LTX_HD + 32 * h;
+                if (h == 0) *(f32x2*)(a.part + 2 * at) = f32x2{m[q], lt};
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    *(f32x4*)(po + 8 * i) = f32x4{o[0][q][i], o[1][q][i], o[2][q][i], o[3][q][i]};
+                    *(f32x4*)(po + 8 * i + 4) = f32x4{o[4][q][i], o[5][q][i], o[6][q][i], o[7][q][i]};
+                }
+                continue;
+            }
+            const int row = it.s.s0 + c / a.group, head = kh * a.group + c % a.group;
+            const float g = a.glog ? 2.0f * sigmoid_f(a.glog[(size_t)row * a.heads + head]) : 1.0f;
+            const float f = limit_of(q) > 0 ? g / lt : 0.f;
+            uint16_t* out = (uint16_t*)a.out + (size_t)row * a.ldo + (size_t)head * LTX_HD + 32 * h;
 #pragma unroll
             for (int i = 0; i < 4; i++) {
-                *(f32x4*)(po + 8 * i) = f32x4{o[0][q][i], o[1][q][i], o[2][q][i], o[3][q][i]};
-                *(f32x4*)(po + 8 * i + 4) = f32x4{o[4][q][i], o[5][q][i], o[6][q][i], o[7][q][i]};
+                u32x4 v;
+#pragma unroll
+                for (int e = 0; e < 4; e++) v[e] = Op<T>::cvt2(o[2 * e][q][i] * f, o[2 * e + 1][q][i] * f);
+                *(u32x4*)(out + 8 * i) = v;
             }
-            continue;
         }
-        const int row = it.s.s0 + c / a.group, head = kh * a.group + c % a.group;
-        const float g = a.glog ? 2.0f * sigmoid_f(a.glog[(size_t)row * a.heads + head]) : 1.0f;
-        const float f = limit_of(q) > 0 ? g / lt : 0.f;
-        uint16_t* out = (uint16_t*)a.out + (size_t)row * a.ldo + (size_t)head * LTX_HD + 32 * h;
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            u32x4 v;
-#pragma unroll
-            for (int e = 0; e < 4; e++) v[e] = Op<T>::cvt2(o[2 * e][q][i] * f, o[2 * e + 1][q][i] * f);
-            *(u32x4*)(out + 8 * i) = v;
-        }
-    }    if (SPLIT) __syncthreads();
+        if (SPLIT) __syncthreads();
     } while (SPLIT && kv_next(a, it));
 }
 
@@ -960,8 +977,9 @@ KV_ATTN_ROWS(ltx_kv_attn_bf16_rows2, __bf16, 2, false)
 KV_ATTN_ROWS(ltx_kv_attn_f16_rows2_split, _Float16, 2, true)
 KV_ATTN_ROWS(ltx_kv_attn_bf16_rows2_split, __bf16, 2, true)
 
-// The runs of a tile into one: a workgroup takes a row and query head, a wave every
-// fourth run, a lane two dims. In the runs' order: the same bits every time.
+// The runs of a tile into one, where items share tiles: a workgroup takes a row and query head, a wave every
+// fourth run, a lane two dims. In the runs' order: the same bits every time. Bound by
+// its launch: 5 us for four rows of 32 heads.
 template <typename T>
 __device__ __forceinline__ void kv_join(const LtxKvAttnArgs& a) {
     __shared__ float sx[4][LTX_HD], sml[4][2];

@@ -46,8 +46,8 @@ __device__ __forceinline__ float q4_scale(uint32_t bits) {
 }
 
 // The waves' sums into one, in the waves' order, and y. my: the wave's slot of SLOT
-// bytes in lds.
-template <typename T, int MT, int NT, int SLOT>
+// bytes in lds. IN: rows of D that make a row of y.
+template <typename T, int MT, int NT, int SLOT, int IN>
 __device__ __forceinline__ void q4_finish(const LtxLinearQ4Args& a, uint8_t* lds, int w, int lane,
                                           const f32x4 (&acc)[MT][NT], int m0, int n0, int rows) {
 #pragma unroll
@@ -60,10 +60,15 @@ __device__ __forceinline__ void q4_finish(const LtxLinearQ4Args& a, uint8_t* lds
         const int t = (e >> 4) % NT, row = (e >> 4) / NT, col = e & 15, m = row >> 4;
         const int n = n0 + 16 * t + col;
         if (row >= rows || n >= a.N) continue;
-        const uint8_t* p = lds + 1024 * (m * NT + t) + 16 * (16 * ((row & 15) >> 2) + col) + 4 * (row & 3);
         float y = 0.f;
 #pragma unroll
-        for (int j = 0; j < Q4_WAVES; j++) y += *(const float*)(p + SLOT * j);
+        for (int j = 0; j < Q4_WAVES; j++)
+#pragma unroll
+            for (int i = 0; i < IN; i++) {
+                const int d = IN * row + i;
+                y += *(const float*)(lds + SLOT * j + 1024 * (m * NT + t) + 16 * (16 * ((d & 15) >> 2) + col) +
+                                     4 * (d & 3));
+            }
         y *= 16.0f;  // of the operands
         if (a.bias) y += a.bias[n];
         if (a.gelu) y = gelu_tanh(y);
@@ -105,9 +110,10 @@ __device__ __forceinline__ void q4_split(f32x4 x, u32x2 (&p)[3]) {
 }
 
 // A workgroup takes 16 MT rows of a and 16 NT of q, each of its eight waves an
-// eighth of the groups of 128. PL: the exact planes that make a value of a, three in
-// mode F32. D's column is the weight row, so a lane needs one scale of a group, which
-// multiplies the group's f32 sum.
+// eighth of the groups of 128. PLANES: the exact planes that make a value of a, three
+// in mode F32. PACK: they are rows of one tile, 3 row + plane, summed with the waves'
+// parts at the end, where up to five rows of a leave it place. D's column is the weight
+// row, so a lane needs one scale of a group, which multiplies the group's f32 sum.
 //
 // Bound: the weights, read once, 4,096 x 4,096 in 2 us at the rate of a large copy
 // (4.9 TB/s). MFMA operands want neighbouring lanes in different rows; loaded that
@@ -120,12 +126,15 @@ __device__ __forceinline__ void q4_split(f32x4 x, u32x2 (&p)[3]) {
 // c ^ r / 2, free of conflicts. AW groups of q and AA of a are in flight.
 // Measured back to back in a graph, where an empty launch takes 3.8 us: one row 5.7
 // us (4,096 x 4,096), 10.4 (16,384 x 4,096), 10.4 (4,096 x 16,384); 32 rows of
-// 16,384 x 4,096 13.9 us (17.5 with NT = 2, 21.1 with MT = 1); mode F32, five rows
-// of 4,096 x 16,384, 19.5 us (forming the planes bounds it).
-template <typename T, int PL, bool S16, int MT, int NT, int AW, int AA, int EARLY>
+// 16,384 x 4,096 13.9 us (17.5 with NT = 2, 21.1 with MT = 1); mode F32, one row of
+// 4,096 x 16,384 11.4 us, five 16.4 (without PACK 15.9 and 20.2: three times the LDS
+// reads and products; what five rows take beyond one is every workgroup's reading and
+// splitting of all of them).
+template <typename T, int PLANES, bool PACK, bool S16, int MT, int NT, int AW, int AA, int EARLY>
 __device__ __forceinline__ void linear_q4(const LtxLinearQ4Args& a) {
     typedef typename Op<T>::v8 v8;
-    constexpr bool F32 = PL == 3;
+    constexpr bool F32 = PLANES == 3;
+    constexpr int PL = PACK ? 1 : PLANES;  // of them in tiles of their own
     constexpr int XT = MT * PL * 4096, TILE = XT + NT * 1024, PART = MT * NT * 1024;
     constexpr int SLOT = TILE > PART ? TILE : PART;
     __shared__ __attribute__((aligned(16))) uint8_t lds[Q4_WAVES * SLOT];
@@ -145,7 +154,7 @@ __device__ __forceinline__ void linear_q4(const LtxLinearQ4Args& a) {
     uint8_t* wq_st = my + XT + 64 * (lane >> 2) + 16 * ((lane & 3) ^ ((lane >> 3) & 3));
     const uint8_t* wq_ld = my + XT + 64 * r + 16 * (h ^ ((r >> 1) & 3));
 
-    constexpr int NX = F32 ? 8 * MT : 4 * MT, RX = F32 ? 2 : 4;  // loads of a group of a, rows of a load
+    constexpr int NX = PACK ? 3 : F32 ? 8 * MT : 4 * MT, RX = F32 ? 2 : 4;  // loads of a group of a, rows of a load
     u32x4 wq[AW][NT], xa[AA][NX];
     uint32_t sc[NT];
     auto load_w = [&](int u, int g) {
@@ -175,11 +184,15 @@ __device__ __forceinline__ void linear_q4(const LtxLinearQ4Args& a) {
             if (RX * i >= rows) continue;
             if (F32) {
                 const int row = 2 * i + (lane >> 5), c = lane & 31;
-                uint8_t* d = my + 256 * row + 16 * ((c >> 1) ^ (row & 15)) + 8 * (c & 1);
                 u32x2 p[3];
                 q4_split(__builtin_bit_cast(f32x4, xa[u % AA][i]), p);
+                if (PACK && row >= LTX_Q4_PACKED) continue;
 #pragma unroll
-                for (int j = 0; j < 3; j++) *(u32x2*)(d + 4096 * MT * j) = p[j];
+                for (int j = 0; j < 3; j++) {
+                    const int at = PACK ? 3 * row + j : row;
+                    *(u32x2*)(my + (PACK ? 0 : 4096 * MT * j) + 256 * at + 16 * ((c >> 1) ^ (at & 15)) +
+                              8 * (c & 1)) = p[j];
+                }
             } else {
                 const int row = 4 * i + h;
                 *(u32x4*)(my + 256 * row + 16 * (r ^ (row & 15))) = xa[u % AA][i];
@@ -254,7 +267,7 @@ __device__ __forceinline__ void linear_q4(const LtxLinearQ4Args& a) {
             __builtin_amdgcn_sched_barrier(0);
         }
     }
-    q4_finish<T, MT, NT, SLOT>(a, lds, w, lane, acc, m0, n0, rows);
+    q4_finish<T, MT, NT, SLOT, PACK ? 3 : 1>(a, lds, w, lane, acc, m0, n0, rows);
 }
 
 #define Q4_KERNEL(NAME, ...)                                                                        \
@@ -262,19 +275,22 @@ __device__ __forceinline__ void linear_q4(const LtxLinearQ4Args& a) {
         linear_q4<__VA_ARGS__>(a);                                                                  \
     }
 #define Q4_KERNELS(MT, NT, ...)                                                           \
-    Q4_KERNEL(ltx_linear_q4_f16_s32_##MT##_##NT, _Float16, 1, false, MT, NT, __VA_ARGS__) \
-    Q4_KERNEL(ltx_linear_q4_f16_s16_##MT##_##NT, _Float16, 1, true, MT, NT, __VA_ARGS__)  \
-    Q4_KERNEL(ltx_linear_q4_bf16_s32_##MT##_##NT, __bf16, 1, false, MT, NT, __VA_ARGS__)  \
-    Q4_KERNEL(ltx_linear_q4_bf16_s16_##MT##_##NT, __bf16, 1, true, MT, NT, __VA_ARGS__)
-#define Q4_PLANES(NT, ...)                                                                \
-    Q4_KERNEL(ltx_linear_q4_f32_s32_1_##NT, __bf16, 3, false, 1, NT, __VA_ARGS__)         \
-    Q4_KERNEL(ltx_linear_q4_f32_s16_1_##NT, __bf16, 3, true, 1, NT, __VA_ARGS__)
+    Q4_KERNEL(ltx_linear_q4_f16_s32_##MT##_##NT, _Float16, 1, false, false, MT, NT, __VA_ARGS__) \
+    Q4_KERNEL(ltx_linear_q4_f16_s16_##MT##_##NT, _Float16, 1, false, true, MT, NT, __VA_ARGS__)  \
+    Q4_KERNEL(ltx_linear_q4_bf16_s32_##MT##_##NT, __bf16, 1, false, false, MT, NT, __VA_ARGS__)  \
+    Q4_KERNEL(ltx_linear_q4_bf16_s16_##MT##_##NT, __bf16, 1, false, true, MT, NT, __VA_ARGS__)
+#define Q4_PLANES(MODE, PACK, NT, ...)                                                             \
+    Q4_KERNEL(ltx_linear_q4_##MODE##_s32_1_##NT, __bf16, 3, PACK, false, 1, NT, __VA_ARGS__)       \
+    Q4_KERNEL(ltx_linear_q4_##MODE##_s16_1_##NT, __bf16, 3, PACK, true, 1, NT, __VA_ARGS__)
 Q4_KERNELS(1, 1, 4, 4, 1)
 Q4_KERNELS(1, 2, 4, 4, 1)
 Q4_KERNELS(1, 4, 4, 2, 0)
 Q4_KERNELS(2, 1, 4, 2, 1)
 Q4_KERNELS(2, 2, 4, 2, 0)
 Q4_KERNELS(2, 4, 2, 1, 0)
-Q4_PLANES(1, 4, 2, 1)
-Q4_PLANES(2, 4, 2, 0)
-Q4_PLANES(4, 4, 1, 0)
+Q4_PLANES(f32, false, 1, 4, 2, 1)
+Q4_PLANES(f32, false, 2, 4, 2, 0)
+Q4_PLANES(f32, false, 4, 4, 1, 0)
+Q4_PLANES(f32p, true, 1, 4, 4, 1)
+Q4_PLANES(f32p, true, 2, 4, 4, 1)
+Q4_PLANES(f32p, true, 4, 4, 2, 0)

@@ -417,6 +417,8 @@ typedef struct {
     int M, N, K;
     int scale_f16, gelu, out_f32;
 } LtxLinearQ4Args;
+// Rows of a (mode F32) whose three planes are 15 of the 16 rows of one tile.
+#define LTX_Q4_PACKED 5
 
 #ifdef __cplusplus
 }

@@ -179,3 +179,20 @@ def test_refusals(ctx):
     with pytest.raises(rt.LtxError, match="unknown mode|types"):
         ctx.linear_q4(a, q, s, b, y, mode=5)
     assert (y == 7).all()
+
+
+@pytest.mark.parametrize("scale", ["f16", "f32"])
+@pytest.mark.parametrize("N", [48, 4112, 8200])
+@pytest.mark.parametrize("M", [1, 2, 3, 4, 5, 6])
+def test_f32_planes_of_few_rows(ctx, M, N, scale):
+    """Up to five rows share a tile with their planes, six do not."""
+    say(f"linear_q4 f32 few rows M={M} N={N} {scale}")
+    a, w, s, b = case("f32", M, N, 640, scale, seed=M)
+    got = run(ctx, "f32", a, w, s, b, False, True).double().cpu().numpy()
+    ws = w.double().numpy() * s.double().repeat_interleave(128, 1).numpy()
+    ax, bx = a.double().numpy(), b.double().numpy()[None]
+    want = ax @ ws.T + bx
+    size = np.abs(ax) @ np.abs(ws).T
+    tol = 2 * 2.0 ** -24 * (3 * 128 + 16 + 5) * size + 2.0 ** -24 * (np.abs(want) + np.abs(bx))
+    off = np.abs(got - want)
+    assert (off <= tol).all(), float((off / tol).max())
