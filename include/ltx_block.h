@@ -318,10 +318,10 @@ uint64_t ltx_kv_cache_bytes(const ltx_kv_cache* cache);
  * left as they were, and so are the cache's other rows. A page index outside the
  * pool is not followed: the row is not written, or read as zeros, or the page's
  * keys take no part in the attention, and it is counted (ltx_kv_cache_faults).
- * The host checks what it can see: nseq and max_pages (at most 2^24) positive,
- * rows not negative (0: nothing to do; below 2^24 for the attention, 2^28 else), pointers, heads, and that rows of k, v, q
- * and out start on 16 bytes with strides (in elements) that are multiples of 8 and
- * not shorter than a row. */
+ * The host checks what it can see: nseq and max_pages (at most 2^24) positive, rows
+ * not negative (0: nothing to do; below 2^24 for the attention, 2^28 else), pointers,
+ * heads, and that rows of k, v, q and out start on 16 bytes with strides (in
+ * elements) that are multiples of 8 and not shorter than a row. */
 typedef struct ltx_kv_batch {
     int nseq, rows;
     const int32_t* row_start;
@@ -350,16 +350,15 @@ int ltx_op_kv_read(ltx_ctx* ctx, const ltx_kv_cache* cache, const ltx_kv_batch* 
  * the rows' own k and v first): q and out [rows][heads * 128], query head j on the
  * cached head j / (heads / kv_heads); scores q . k / sqrt(128); causal: a row sees
  * the keys up to its own position, else all kv_len; glog [rows][heads] f32 or NULL,
- * the gate of ltx_op_attention; out may not overlap q. A row that sees no key gives zeros; a row that
- * sees a token with a value of v (or k) that is not finite in that head gives NaN,
- * and one that does not is untouched by it. f32 statistics and sums, weights
- * rounded to 16 bits. Results do not depend on other calls' timing.
+ * the gate of ltx_op_attention; out may not overlap q. A row that sees no key gives
+ * zeros; a row that sees a token with a value of v (or k) that is not finite in that
+ * head gives NaN, and one that does not is untouched by it. f32 statistics and sums,
+ * weights rounded to 16 bits. Results do not depend on other calls' timing.
  * With few rows the keys are split over workgroups, whose partial results lie in
  * `work`: device memory of ltx_op_kv_attention_workspace bytes (for the batch's nseq,
  * rows and max_pages, with or without row_start), not used by two calls at once; for
- * calls that are captured. NULL:
- * scratch of the context, as in ltx_op_attention (a call being captured, or one
- * that finds no memory, does not split). */
+ * calls that are captured. NULL: scratch of the context, as in ltx_op_attention (a
+ * call being captured, or one that finds no memory, does not split). */
 int ltx_op_kv_attention_workspace(ltx_ctx* ctx, const ltx_kv_cache* cache, const ltx_kv_batch* batch, int heads,
                                   uint64_t* bytes);
 int ltx_op_kv_attention(ltx_ctx* ctx, const ltx_kv_cache* cache, const ltx_kv_batch* batch, const void* q,

@@ -35,8 +35,8 @@ extern "C" int ltx_op_linear_q4(ltx_ctx* c, const void* a, const uint8_t* q, con
         int nt = 1;
         while (nt < 4 && ((int64_t)N + 16 * nt - 1) / (16 * nt) * gy > c->num_cu) nt *= 2;
         char name[48];
-        std::snprintf(name, sizeof(name), "ltx_linear_q4_%s_s%d_%d_%d",
-                      f32 ? M <= LTX_Q4_PACKED ? "f32p" : "f32" : mode == LTX_MODE_F16 ? "f16" : "bf16", scale_f16 ? 16 : 32, mt, nt);
+        const char* form = f32 ? M <= LTX_Q4_PACKED ? "f32p" : "f32" : mode == LTX_MODE_F16 ? "f16" : "bf16";
+        std::snprintf(name, sizeof(name), "ltx_linear_q4_%s_s%d_%d_%d", form, scale_f16 ? 16 : 32, mt, nt);
         c->launch(name, (unsigned)(((int64_t)N + 16 * nt - 1) / (16 * nt)), gy, 1, 512, &g, (hipStream_t)stream);
     })
 }

@@ -158,11 +158,12 @@ __device__ __forceinline__ uint32_t quad_pick(u32x4 x) {
 // K codes of four heads, and each has one head's 16 bytes; with four rows on one quad
 // of positions (the rule but for a first few rows) V's codes go the same way over the
 // rows, 16 bytes of four keys a lane. All of a wave's loads are on their way at once,
-// and nothing here is read twice: streaming loads and stores. Measured: 26,624 rows of
-// 32 heads written in 138 us and read in 80, 28,672 read in 89 (594 MB, 6.7 TB/s); with
-// loads and stores that stay in the caches 164, 94 and 119 .. 152, with a dword of codes
-// a lane besides 175, 185 and 213 .. 230.
-#define KV_HB 4
+// and nothing here is read twice: streaming loads and stores. Measured one by one:
+// 26,624 rows of 32 heads written in 137 us and read in 80 .. 91, 28,672 read in 89;
+// with loads and stores that stay in the caches 164, 94 and 119 .. 152, with a dword of
+// codes a lane besides 175, 185 and 213 .. 230. Back to back, where a launch waits for
+// the last one's stores to reach memory, 229 for the pair and 125: 4.8 TB/s, the rate
+// of a large copy.
 template <typename T, bool WRITE>
 __device__ __forceinline__ void kv_rows(const LtxKvRowsArgs& a) {
     const int lane = threadIdx.x & 63, o = lane & 15, sub = lane >> 4;
@@ -675,9 +676,9 @@ KV_ATTN(ltx_kv_attn_bf16_nt, __bf16, true)
 // in the order the operands are read (16 bytes a lane, no conflicts): waves 0 .. 3 a
 // 16-key block of K each, waves 4 .. 7 half the dims of 32 keys of V each, one page
 // ahead, from codes loaded two pages ahead. Two barriers a page, see below.
-// Bound: a page is 1,024 cycles of MFMAs a SIMD and takes about 2,000, the rest
-// being the exponentials, the conversions and the operands' reads from LDS, which the
-// other group's products hide in part. 2,048 columns of 32 heads over 28,672 keys (962
+// Bound: a group's products of a page are 1,024 cycles of a SIMD's MFMAs and take
+// about 2,200 beside the other group's exponentials and conversions and the operands'
+// reads from LDS. 2,048 columns of 32 heads over 28,672 keys (962
 // GFLOP) take 825 us, 1.17 PFLOP/s, causal runs of three sequences of up to 2,970
 // tokens (154 GFLOP) 190. On the way there, the same call: every wave forming its own
 // operands 1,675 us, operands in LDS 1,176, two groups a phase apart 1,137, loads
