@@ -164,6 +164,7 @@ __device__ __forceinline__ uint32_t quad_pick(u32x4 x) {
 // codes a lane besides 175, 185 and 213 .. 230. Back to back, where a launch waits for
 // the last one's stores to reach memory, 229 for the pair and 125: 4.8 TB/s, the rate
 // of a large copy.
+#define KV_HB 4
 template <typename T, bool WRITE>
 __device__ __forceinline__ void kv_rows(const LtxKvRowsArgs& a) {
     const int lane = threadIdx.x & 63, o = lane & 15, sub = lane >> 4;
