@@ -253,7 +253,7 @@ int ltx_op_kv_attention(ltx_ctx* c, const ltx_kv_cache* cache, const ltx_kv_batc
             c->launch(p.tile == 128 ? (f16 ? "ltx_kv_attn_f16_rows1" : "ltx_kv_attn_bf16_rows1")
                       : p.slots     ? (f16 ? "ltx_kv_attn_f16_rows2_split" : "ltx_kv_attn_bf16_rows2_split")
                                     : (f16 ? "ltx_kv_attn_f16_rows2" : "ltx_kv_attn_bf16_rows2"),
-                      (unsigned)(((int64_t)p.items * cache->kv_heads + 7) / 8 * 8), 1, 1, 512, &a, st);
+                      (unsigned)((int64_t)p.items * cache->kv_heads), 1, 1, 512, &a, st);
         if (p.slots)
             c->launch(f16 ? "ltx_kv_join_f16" : "ltx_kv_join_bf16", batch->rows, heads, 1, 256, &a, st);
     })

@@ -323,6 +323,24 @@ def test_attention(any_tile, mode, heads, kvh, rows, keys, causal):
     assert s.cache.faults() == 0
 
 
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("heads,kvh,rows,keys", [
+    (32, 32, [300, 5, 130, 0, 515, 200, 1], [700, 0, 130, 9, 515, 258, 1]),
+    (48, 12, [9, 260, 33, 128, 200, 64, 7, 96, 17], [90, 260, 1000, 128, 455, 64, 1200, 3, 400]),
+    (64, 32, [5] * 64, [2 * i + 3 for i in range(64)]),
+    (64, 32, [5] * 65, [131 - 2 * i for i in range(65)]),
+])
+def test_attention_of_more_than_a_round(any_tile, heads, kvh, rows, keys, causal):
+    """More tiles than CUs."""
+    ctx = any_tile
+    say(f"kv attention rounds heads={heads}/{kvh} rows={rows[:4]} keys={keys[:4]} causal={causal}")
+    s = Setup(ctx, "bf16", kvh, rows, keys, seed=sum(keys) + heads)
+    q = s.queries(heads)
+    want, tol = s.want(q, heads, causal)
+    check(s.attend(q, heads, causal), want, tol)
+    assert s.cache.faults() == 0
+
+
 @pytest.mark.parametrize("mode", ["f16", "bf16"])
 @pytest.mark.parametrize("scale", [30.0, 0.01])
 def test_attention_peaked_and_flat(any_tile, mode, scale):
