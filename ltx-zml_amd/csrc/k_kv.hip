@@ -392,6 +392,31 @@ __device__ __forceinline__ float kv_quad_max(float x) {  // over lanes l, l ^ 16
     return fmaxf(__builtin_bit_cast(float, (uint32_t)q[0]), __builtin_bit_cast(float, (uint32_t)q[1]));
 }
 
+// What is added to a column's sum of weights: 0, or NaN where q holds a value that is
+// not finite (all of its scores are infinite or NaN then, and might all be -inf as if
+// no key were seen).
+template <typename T>
+__device__ __forceinline__ float kv_bad_query(const typename Op<T>::v8 (&q)[4]) {
+    typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+    u16x2 top = {0, 0};
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+        const u32x4 x = __builtin_bit_cast(u32x4, q[j]);
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            const uint32_t y = x[e] & 0x7fff7fffu;
+            top = __builtin_elementwise_max(top, __builtin_bit_cast(u16x2, y));
+        }
+    }
+    const uint16_t least = __is_same(T, _Float16) ? 0x7c00 : 0x7f80;
+    return top[0] >= least || top[1] >= least ? __builtin_nanf("") : 0.f;
+}
+// What a column's sums are multiplied by: 0 where it has seen no key (the mask, or
+// pages outside the pool).
+__device__ __forceinline__ float kv_factor(int limit, float lt, float g) {
+    return limit <= 0 || lt == 0.f ? 0.f : g / lt;
+}
+
 // x where m is 0, y where it is ~0 (bit operations: as compares and selects, the
 // rare paths below took more scalar registers than there are, and spilled)
 __device__ __forceinline__ float kv_select(int m, float x, uint32_t y) {
@@ -615,6 +640,7 @@ __device__ __forceinline__ void kv_attn(const LtxKvAttnArgs& a) {
         }
 
         // the waves' results into one: lane (r, h) holds dims 8 (4 h + i) + db
+        l += kv_bad_query<T>(qf);
         l += __shfl_xor(l, 16, 64);
         l += __shfl_xor(l, 32, 64);
         if (h == 0) {
@@ -654,7 +680,7 @@ __device__ __forceinline__ void kv_attn(const LtxKvAttnArgs& a) {
             } else {
                 const int grow = it.s.s0 + orow;
                 const float g = a.glog ? 2.0f * sigmoid_f(a.glog[(size_t)grow * a.heads + ohead]) : 1.0f;
-                const float f = kv_limit(a.causal, it.s, orow) > 0 ? g / lt : 0.f;
+                const float f = kv_factor(kv_limit(a.causal, it.s, orow), lt, g);
                 *(u32x2*)((uint16_t*)a.out + (size_t)grow * a.ldo + (size_t)ohead * LTX_HD + d0) =
                     u32x2{Op<T>::cvt2(y[0] * f, y[1] * f), Op<T>::cvt2(y[2] * f, y[3] * f)};
             }
@@ -939,6 +965,7 @@ __device__ __forceinline__ void kv_attn_rows(const LtxKvAttnArgs& a) {
         for (int q = 0; q < NQ; q++) {
             const int lane = my_lane(), h = lane >> 4, c = c0 + 16 * q + (lane & 15);
             if (c >= ncol || (!whole && part >= (size_t)a.parts)) continue;
+            l[q] += kv_bad_query<T>(qf[q]);
             float lt = l[q] + __shfl_xor(l[q], 16, 64);
             lt += __shfl_xor(lt, 32, 64);
             if (!whole) {
@@ -954,7 +981,7 @@ __device__ __forceinline__ void kv_attn_rows(const LtxKvAttnArgs& a) {
             }
             const int row = it.s.s0 + c / a.group, head = kh * a.group + c % a.group;
             const float g = a.glog ? 2.0f * sigmoid_f(a.glog[(size_t)row * a.heads + head]) : 1.0f;
-            const float f = limit_of(q) > 0 ? g / lt : 0.f;
+            const float f = kv_factor(limit_of(q), lt, g);
             uint16_t* out = (uint16_t*)a.out + (size_t)row * a.ldo + (size_t)head * LTX_HD + 32 * h;
 #pragma unroll
             for (int i = 0; i < 4; i++) {
@@ -1066,7 +1093,7 @@ __device__ __forceinline__ void kv_join(const LtxKvAttnArgs& a) {
         x1 = __builtin_fmaf(sx[j][2 * lane + 1], f, x1);
     }
     const float g = a.glog ? 2.0f * sigmoid_f(a.glog[(size_t)row * a.heads + head]) : 1.0f;
-    const float f = kv_limit(a.causal, s, i) > 0 ? g / lt : 0.f;
+    const float f = kv_factor(kv_limit(a.causal, s, i), lt, g);
     *(uint32_t*)((uint16_t*)a.out + (size_t)row * a.ldo + (size_t)head * LTX_HD + 2 * lane) =
         Op<T>::cvt2(x0 * f, x1 * f);
 }

@@ -386,6 +386,50 @@ def test_attention_leaves_bad_pages_out(any_tile):
         assert s.cache.faults() > 0
 
 
+@pytest.mark.parametrize("keys", [[70, 9, 300, 1], [70, 9, 3000, 1]])
+def test_attention_of_rows_whose_pages_are_all_bad(any_tile, keys):
+    """A padded batch: rows that see only pages outside the pool give zeros."""
+    ctx = any_tile
+    say(f"kv attention padded {keys}")
+    for rows in ([1, 1, 1, 1], [70, 3, 200, 1]):
+        s = Setup(ctx, "f16", 2, rows, keys, seed=12)
+        s.pages[1] = -1
+        s.pages[2] = s.cache.pages
+        s.pages[3] = -1
+        q = s.queries(4)
+        for causal in (True, False):
+            want, tol = s.want(q, 4, causal, skip=lambda b, j: b > 0)
+            assert (want[rows[0]:] == 0).all()
+            check(s.attend(q, 4, causal), want, tol)
+            assert s.cache.faults() > 0
+
+
+@pytest.mark.parametrize("mode", ["f16", "bf16"])
+@pytest.mark.parametrize("bad", [math.inf, -math.inf, math.nan])
+def test_queries_that_are_not_finite(any_tile, mode, bad):
+    """NaN for their row and head, also where every score is -inf; zeros where no key
+    is seen; every other row and head within the bounds that it has without (not the
+    same bits: a column's weights are formed with a maximum that is behind by up to 2^8,
+    moved for the columns of a wave together, and the bound holds for any such one)."""
+    ctx = any_tile
+    say(f"kv attention query {bad} {mode}")
+    g = torch.Generator().manual_seed(4)
+    for rows, keys in (([1, 1, 2], [5, 1500, 1]), ([100, 200, 2], [120, 1500, 1])):
+        k, v = torch.randn(2, sum(keys), 2, HD, generator=g)
+        k[:, 0, 3] = 2.0 + k[:, 0, 3].abs()
+        s = Setup(ctx, mode, 2, rows, keys, kv=(k, v))
+        q = s.queries(4)
+        want, tol = s.want(q, 4, True)
+        last = s.total - 2  # before the first position: sees nothing
+        for row, dim in ((0, 3), (rows[0], HD + 127), (last, 3)):
+            q[row, dim] = bad
+        got = s.attend(q, 4, True)
+        for row, head in ((0, 0), (rows[0], 1)):
+            want[row, head * HD:(head + 1) * HD] = math.nan
+        assert (got[last] == 0).all()
+        check(got, want, tol)
+
+
 @pytest.mark.parametrize("mode", ["f16", "bf16"])
 def test_tables_wider_than_what_is_in_use(any_tile, mode):
     """A table of 10,000 pages a sequence, nothing behind the first few looked at: the
