@@ -353,8 +353,9 @@ int ltx_op_kv_read(ltx_ctx* ctx, const ltx_kv_cache* cache, const ltx_kv_batch* 
  * the gate of ltx_op_attention; out may not overlap q. A row that sees no key gives
  * zeros (also where all its pages are outside the pool); a row that sees a token with
  * a value of v (or k) that is not finite in that head gives NaN, and one that does not
- * is untouched by it; a value of q that is not finite makes its row and head NaN. f32 statistics and
- * sums, weights rounded to 16 bits. Results do not depend on other calls' timing.
+ * is untouched by it; a value of q that is not finite makes its row and head NaN. f32
+ * statistics and sums, weights rounded to 16 bits. Results do not depend on other
+ * calls' timing.
  * With few rows the keys are split over workgroups, whose partial results lie in
  * `work`: device memory of ltx_op_kv_attention_workspace bytes (for the batch's nseq,
  * rows and max_pages, with or without row_start), not used by two calls at once; for

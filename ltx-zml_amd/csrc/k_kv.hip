@@ -802,8 +802,8 @@ __device__ __forceinline__ void kv_attn_rows(const LtxKvAttnArgs& a) {
                     *(u32x4*)d = lo;
                     *(u32x4*)(d + 1024) = hi;
                     kv_v_pair<T, 1>(x, f, lo, hi);
-                    *(u32x4*)(d + 2048) = lo;
-                    *(u32x4*)(d + 3072) = hi;
+                    *(u32x4*)(d + 2 * 1024) = lo;
+                    *(u32x4*)(d + 3 * 1024) = hi;
                 } else {
                     kv_v_pair<T, 2>(x, f, lo, hi);
                     *(u32x4*)(d + 4096) = lo;
