@@ -351,10 +351,12 @@ int ltx_op_kv_read(ltx_ctx* ctx, const ltx_kv_cache* cache, const ltx_kv_batch* 
  * cached head j / (heads / kv_heads); scores q . k / sqrt(128); causal: a row sees
  * the keys up to its own position, else all kv_len; glog [rows][heads] f32 or NULL,
  * the gate of ltx_op_attention; out may not overlap q. A row that sees no key gives
- * zeros (also where all its pages are outside the pool); a row that sees a token with
- * a value of v (or k) that is not finite in that head gives NaN, and one that does not
- * is untouched by it; a value of q that is not finite makes its row and head NaN. f32
- * statistics and sums, weights rounded to 16 bits. Results do not depend on other
+ * zeros whatever its q holds (also where all its pages are outside the pool). Of the
+ * others: a row that sees a token with a value of v (or k) that is not finite in that
+ * head gives NaN, and one that does not is untouched by it; a value of q that is not
+ * finite makes its row and head NaN, and so do scores beyond f32: one of +inf, or all of
+ * -inf (a key of -inf among others weighs nothing). f32 statistics and sums, weights
+ * rounded to 16 bits. Results do not depend on other
  * calls' timing.
  * With few rows the keys are split over workgroups, whose partial results lie in
  * `work`: device memory of ltx_op_kv_attention_workspace bytes (for the batch's nseq,

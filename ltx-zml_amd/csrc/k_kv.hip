@@ -393,8 +393,7 @@ __device__ __forceinline__ float kv_quad_max(float x) {  // over lanes l, l ^ 16
 }
 
 // What is added to a column's sum of weights: 0, or NaN where q holds a value that is
-// not finite (all of its scores are infinite or NaN then, and might all be -inf as if
-// no key were seen).
+// not finite (all of its scores are infinite or NaN then, and might all be -inf).
 template <typename T>
 __device__ __forceinline__ float kv_bad_query(const typename Op<T>::v8 (&q)[4]) {
     typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
@@ -411,11 +410,31 @@ __device__ __forceinline__ float kv_bad_query(const typename Op<T>::v8 (&q)[4]) 
     const uint16_t least = __is_same(T, _Float16) ? 0x7c00 : 0x7f80;
     return top[0] >= least || top[1] >= least ? __builtin_nanf("") : 0.f;
 }
-// What a column's sums are multiplied by: 0 where it has seen no key (the mask, or
-// pages outside the pool).
-__device__ __forceinline__ float kv_factor(int limit, float lt, float g) {
-    return limit <= 0 || lt == 0.f ? 0.f : g / lt;
+// The first of sequence b's pages p0 .. p1 - 1 that is in the pool (2^24: none is).
+// All 64 lanes call it.
+__device__ __forceinline__ int kv_first(const LtxKvBatchArgs& a, int b, int p0, int p1) {
+    for (int base = p0; base < p1; base += 64) {
+        const int p = base + (threadIdx.x & 63);
+        const uint64_t there = __builtin_amdgcn_ballot_w64(p < p1 && kv_in_pool(a, kv_page(a, b, p)));
+        if (there) return base + __builtin_ctzll(there);
+    }
+    return 1 << 24;
 }
+// Whether a column has seen a key of pages p0 .. p1 - 1 is what its maximum says from
+// here on: -inf where it has not (the mask, or pages outside the pool; its sum is 0
+// then, whatever q holds), and at least -FLT_MAX where it has, also where all of its
+// scores are -inf or NaN. Only a sum that is 0 or NaN leaves that open, so the table
+// is looked at for such ones alone. sum: over the column's four lanes; `mine`: the keys
+// that the column's mask leaves. All 64 lanes call it.
+__device__ __forceinline__ void kv_seen(const LtxKvBatchArgs& a, int b, int p0, int p1, int mine, float& m, float& sum) {
+    if (__builtin_amdgcn_ballot_w64(!(sum > 0.f)) == 0) return;
+    const bool saw = kv_first(a, b, p0, p1) * LTX_KV_PAGE < mine;
+    m = saw ? fmaxf(m, -__FLT_MAX__) : -__builtin_inff();
+    sum = saw ? sum : 0.f;
+}
+// What a column's sums are multiplied by: 0 where it has seen no key; a sum of 0 where
+// it has gives NaN (0 times infinity).
+__device__ __forceinline__ float kv_factor(float m, float lt, float g) { return m == -__builtin_inff() ? 0.f : g / lt; }
 
 // x where m is 0, y where it is ~0 (bit operations: as compares and selects, the
 // rare paths below took more scalar registers than there are, and spilled)
@@ -640,9 +659,12 @@ __device__ __forceinline__ void kv_attn(const LtxKvAttnArgs& a) {
         }
 
         // the waves' results into one: lane (r, h) holds dims 8 (4 h + i) + db
-        l += kv_bad_query<T>(qf);
-        l += __shfl_xor(l, 16, 64);
-        l += __shfl_xor(l, 32, 64);
+        if (p0 + w < p1) {
+            l += kv_bad_query<T>(qf);
+            l += __shfl_xor(l, 16, 64);
+            l += __shfl_xor(l, 32, 64);
+            kv_seen(a.b, it.b, p0, p1, mine, m, l);
+        }
         if (h == 0) {
             sm[w][r] = m;
             sl[w][r] = l;
@@ -680,7 +702,7 @@ __device__ __forceinline__ void kv_attn(const LtxKvAttnArgs& a) {
             } else {
                 const int grow = it.s.s0 + orow;
                 const float g = a.glog ? 2.0f * sigmoid_f(a.glog[(size_t)grow * a.heads + ohead]) : 1.0f;
-                const float f = kv_factor(kv_limit(a.causal, it.s, orow), lt, g);
+                const float f = kv_factor(M, lt, g);
                 *(u32x2*)((uint16_t*)a.out + (size_t)grow * a.ldo + (size_t)ohead * LTX_HD + d0) =
                     u32x2{Op<T>::cvt2(y[0] * f, y[1] * f), Op<T>::cvt2(y[2] * f, y[3] * f)};
             }
@@ -964,10 +986,11 @@ __device__ __forceinline__ void kv_attn_rows(const LtxKvAttnArgs& a) {
 #pragma unroll
         for (int q = 0; q < NQ; q++) {
             const int lane = my_lane(), h = lane >> 4, c = c0 + 16 * q + (lane & 15);
-            if (c >= ncol || (!whole && part >= (size_t)a.parts)) continue;
             l[q] += kv_bad_query<T>(qf[q]);
             float lt = l[q] + __shfl_xor(l[q], 16, 64);
             lt += __shfl_xor(lt, 32, 64);
+            if (!idle) kv_seen(a.b, it.b, p0, p1, limit_of(q), m[q], lt);
+            if (c >= ncol || (!whole && part >= (size_t)a.parts)) continue;
             if (!whole) {
                 const size_t at = (part * a.b.kvh + kh) * a.tile + (c - it.tile * a.tile);
                 float* po = a.part + 2 * (size_t)a.parts * a.b.kvh * a.tile + at * LTX_HD + 32 * h;
@@ -981,7 +1004,7 @@ __device__ __forceinline__ void kv_attn_rows(const LtxKvAttnArgs& a) {
             }
             const int row = it.s.s0 + c / a.group, head = kh * a.group + c % a.group;
             const float g = a.glog ? 2.0f * sigmoid_f(a.glog[(size_t)row * a.heads + head]) : 1.0f;
-            const float f = kv_factor(limit_of(q), lt, g);
+            const float f = kv_factor(m[q], lt, g);
             uint16_t* out = (uint16_t*)a.out + (size_t)row * a.ldo + (size_t)head * LTX_HD + 32 * h;
 #pragma unroll
             for (int i = 0; i < 4; i++) {
@@ -1093,7 +1116,7 @@ __device__ __forceinline__ void kv_join(const LtxKvAttnArgs& a) {
         x1 = __builtin_fmaf(sx[j][2 * lane + 1], f, x1);
     }
     const float g = a.glog ? 2.0f * sigmoid_f(a.glog[(size_t)row * a.heads + head]) : 1.0f;
-    const float f = kv_factor(kv_limit(a.causal, s, i), lt, g);
+    const float f = kv_factor(M, lt, g);
     *(uint32_t*)((uint16_t*)a.out + (size_t)row * a.ldo + (size_t)head * LTX_HD + 2 * lane) =
         Op<T>::cvt2(x0 * f, x1 * f);
 }

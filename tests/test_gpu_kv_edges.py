@@ -1,0 +1,90 @@
+"""The 4-bit key/value cache where it can go wrong beside the shapes of
+test_gpu_kv.py: rows that see no key, scores beyond f32."""
+import math
+
+import numpy as np
+import pytest
+
+from conftest import say
+
+torch = pytest.importorskip("torch")
+pytestmark = pytest.mark.gpu
+
+from ltx_amd import runtime as rt  # noqa: E402
+from test_gpu_kv import HD, MODES, PAGE, Setup, any_tile, check  # noqa: E402, F401
+
+
+# ---- rows that see no key ---------------------------------------------------------
+
+@pytest.mark.parametrize("mode", ["f16", "bf16"])
+@pytest.mark.parametrize("keys", [[70, 9, 300, 1], [70, 9, 3000, 1]])
+def test_padded_rows_with_stale_queries(any_tile, mode, keys):
+    """Rows that see only pages outside the pool give zeros whatever their q holds, as
+    rows of a sequence without keys do; a row with such a q that sees a key gives NaN."""
+    ctx = any_tile
+    say(f"kv padded, stale q {mode} {keys}")
+    for rows in ([1, 1, 1, 1], [70, 3, 200, 1]):
+        for bad in (math.nan, math.inf, -math.inf):
+            s = Setup(ctx, mode, 2, rows, keys, seed=12)
+            s.pages[1] = -1
+            s.pages[2] = s.cache.pages
+            s.pages[3] = -1
+            q = s.queries(4)
+            for causal in (True, False):
+                want, tol = s.want(q, 4, causal, skip=lambda b, j: b > 0)
+                stale = q.clone()
+                stale[rows[0]:] = bad
+                stale[rows[0] - 1, HD + 5] = bad  # the last row of the sequence that is there
+                want[rows[0] - 1, HD:2 * HD] = math.nan
+                check(s.attend(stale, 4, causal), want, tol)
+
+
+@pytest.mark.parametrize("mode", ["f16", "bf16"])
+def test_rows_before_the_first_page_of_the_pool(any_tile, mode):
+    """Causal rows whose pages are outside the pool up to a later one: zeros, whatever
+    their q holds; the rows behind attend to that page on."""
+    ctx = any_tile
+    say(f"kv first pages bad {mode}")
+    for rows, keys in (([200, 150], [300, 1500]), ([300, 80], [320, 700])):
+        s = Setup(ctx, mode, 2, rows, keys, seed=13)
+        last = [(k - 1) // PAGE for k in keys]
+        for b in range(2):
+            s.pages[b, :last[b]] = -1
+        q = s.queries(4)
+        want, tol = s.want(q, 4, True, skip=lambda b, j: j // PAGE < last[b])
+        for b in range(2):
+            n, r0 = rows[b], s.row_start[b]
+            blind = max(0, last[b] * PAGE - (keys[b] - n))  # rows at positions before the page
+            assert 0 < blind < n
+            assert (want[r0:r0 + blind] == 0).all() and (want[r0 + blind:r0 + n] != 0).any()
+            q[r0:r0 + blind] = math.nan
+        check(s.attend(q, 4, True), want, tol)
+
+
+def test_scores_beyond_f32(any_tile):
+    """bf16 q and k whose products leave f32: a key with a score of -inf among finite
+    ones weighs nothing; a row all of whose scores are -inf, or with one of +inf, is NaN
+    and not taken for one without keys."""
+    ctx = any_tile
+    say("kv scores beyond f32")
+    for rows, keys in (([1, 1, 1, 2], [64, 1500, 900, 3]), ([150, 100, 70, 2], [200, 1500, 900, 3])):
+        g = torch.Generator().manual_seed(6)
+        total = sum(keys)
+        k, v = torch.randn(2, total, 1, HD, generator=g)
+        k[:, :, 0] = 0
+        start = np.concatenate([[0], np.cumsum(keys)])
+        huge = 2.0 ** 30
+        lost = {(1, j) for j in range(0, keys[1], 3)}
+        for b, j in lost:
+            k[start[b] + j, 0] = 0
+            k[start[b] + j, 0, 0] = -huge
+        k[start[2]:start[3], 0, 0] = -huge   # all of the third sequence
+        k[start[3], 0, 0] = huge             # one key of the fourth
+        s = Setup(ctx, "bf16", 1, rows, keys, kv=(k, v))
+        q = s.queries(2)
+        q[:, 0] = q[:, HD] = 0
+        s.kx[..., 0] = 0  # the finite scores: without the first dim (the lost keys are left out)
+        want, tol = s.want(q, 2, False, skip=lambda b, j: (b, j) in lost)
+        want[s.row_start[2]:] = math.nan
+        q[:, 0] = q[:, HD] = 2.0 ** 100
+        check(s.attend(q, 2, False), want, tol)
