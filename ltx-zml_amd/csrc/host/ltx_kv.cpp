@@ -145,10 +145,15 @@ int ltx_kv_cache_create(ltx_ctx* c, int mode, int kv_heads, int pages, ltx_kv_ca
             k->pages = pages;
             k->blocks = (size_t)pages * kv_heads * LTX_KV_BLOCK;
             k->buf.alloc(k->blocks + 256 + (size_t)pages * 4);
-            // zeros: no page holds a code of a non-finite value before it is written (on
-            // the context's own stream, which a capture elsewhere does not see)
-            HIPC(hipMemsetAsync(k->buf.p, 0, k->buf.bytes, c->side));
-            HIPC(hipStreamSynchronize(c->side));
+            // zeros: no page holds a code of a non-finite value before it is written. On a
+            // stream of this call's own: a captured forward of the context has taken the
+            // context's into the capture
+            hipStream_t st = nullptr;
+            HIPC(hipStreamCreateWithFlags(&st, hipStreamNonBlocking));
+            hipError_t e = hipMemsetAsync(k->buf.p, 0, k->buf.bytes, st);
+            if (e == hipSuccess) e = hipStreamSynchronize(st);
+            (void)hipStreamDestroy(st);
+            ltx::hip_check(e, "clearing the cache");
         } catch (...) {
             delete k;
             throw;

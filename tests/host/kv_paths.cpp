@@ -191,6 +191,20 @@ static void memory() {
     ltx_kv_cache_free(f.c, nullptr);
 }
 
+// Made while a forward of the same context is being captured, whose second stream
+// the capture holds.
+static void own_capture() {
+    Fixture f;
+    fake::capturing.insert((hipStream_t)0x77);
+    fake::capturing.insert(f.c->side);
+    ltx_kv_cache* k = nullptr;
+    CHECK(ltx_kv_cache_create(f.c, 0, 8, 100, &k), "%s", ltx_last_error(f.c));
+    ltx_kv_cache_free(f.c, k);
+    CHECK(!fake::broken_capture, "the capture is broken");
+    for (const fake::Op& o : fake::log) CHECK(!o.stream || !fake::capturing.count(o.stream), "%s", o.what.c_str());
+    fake::capturing.clear();
+}
+
 // The index arithmetic on arrays of any contents: what a kernel would read and
 // write stays inside what the call names, and the items fit the grid.
 static void index_bounds(unsigned seed) {
@@ -266,6 +280,8 @@ int main(int argc, char** argv) {
         scratch();
     else if (cmd == "memory")
         memory();
+    else if (cmd == "own_capture")
+        own_capture();
     else if (cmd == "index")
         index_bounds(std::atoi(argv[2]));
     else

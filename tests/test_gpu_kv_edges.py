@@ -1,5 +1,6 @@
 """The 4-bit key/value cache where it can go wrong beside the shapes of
-test_gpu_kv.py: rows that see no key, scores beyond f32."""
+test_gpu_kv.py: rows that see no key, scores beyond f32,
+calls beside others."""
 import math
 
 import numpy as np
@@ -11,7 +12,8 @@ torch = pytest.importorskip("torch")
 pytestmark = pytest.mark.gpu
 
 from ltx_amd import runtime as rt  # noqa: E402
-from test_gpu_kv import HD, MODES, PAGE, Setup, any_tile, check  # noqa: E402, F401
+from ltx_amd import synth  # noqa: E402
+from test_gpu_kv import HD, MODES, PAGE, Setup, any_tile, check, ints  # noqa: E402, F401
 
 
 # ---- rows that see no key ---------------------------------------------------------
@@ -88,3 +90,43 @@ def test_scores_beyond_f32(any_tile):
         want[s.row_start[2]:] = math.nan
         q[:, 0] = q[:, HD] = 2.0 ** 100
         check(s.attend(q, 2, False), want, tol)
+
+
+# ---- calls beside others ------------------------------------------------------------
+
+def test_a_cache_made_inside_a_capture(block0):
+    """A cache made (and another freed) while the same context's forward is being
+    captured: the graph is whole, the cache holds zeros and takes rows."""
+    say("kv cache made inside a capture")
+    T, S = 250, 40
+    inp = synth.make_inputs(T, S, seed=0, sigma=0.7)
+    dev = lambda a: torch.from_numpy(np.ascontiguousarray(a)).cuda()  # noqa: E731
+    x = [dev(inp[n]) for n in ("x", "tstab", "tidx", "ctx", "pts2")] + [dev(t) for t in rt.rope_tables(inp["grid"])]
+    y, want = torch.empty(2, T, 4096, device="cuda")
+    c = rt.Context(0)
+    try:
+        w = c.upload(block0)
+        gone = c.kv_cache(2, 3)
+        c.forward(w, *x, want, mode=rt.MODE_F16)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, capture_error_mode="global"):
+            c.forward(w, *x, y, mode=rt.MODE_F16)
+            cache = c.kv_cache(2, 5)
+            gone.free()
+            y.add_(0)
+        batch = rt.KvBatch(ints([130]), ints([[4, 0, 2]]), ints([0, 130]), 130)
+        k, v = torch.full((2, 130, 2 * HD), 7.0, dtype=torch.float16, device="cuda")
+        c.kv_read(cache, batch, k, v)
+        assert (k == 0).all() and (v == 0).all()
+        for _ in range(3):
+            y.fill_(math.nan)
+            graph.replay()
+            c.kv_write(cache, batch, k + 1.5, v - 3)
+            c.kv_read(cache, batch, k, v)
+            torch.cuda.synchronize()
+            assert torch.equal(y, want) and (k == 1.5).all() and (v == -3).all()
+            k.zero_()
+            v.zero_()
+    finally:
+        c.close()

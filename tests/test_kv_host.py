@@ -36,6 +36,10 @@ def test_cache_memory(kv_paths):
     kv_paths("memory")
 
 
+def test_cache_made_inside_a_capture_of_its_context(kv_paths):
+    kv_paths("own_capture")
+
+
 @pytest.mark.parametrize("seed", [1, 2, 3])
 def test_index_arithmetic_stays_inside(kv_paths, seed):
     kv_paths("index", seed)
