@@ -332,7 +332,7 @@ typedef struct ltx_kv_batch {
 
 /* The count of bad pages (once a row in ltx_op_kv_write and ltx_op_kv_read, once a
  * page and tile of rows in ltx_op_kv_attention) since creation or the last reset.
- * Waits for `stream`. */
+ * Waits for `stream`, which may not be one that is being captured. */
 int ltx_kv_cache_faults(ltx_ctx* ctx, ltx_kv_cache* cache, void* stream, uint64_t* count, int reset);
 
 /* Quantises the batch's rows of k and v [rows][kv_heads * 128] (ldk and ldv

@@ -176,13 +176,18 @@ int ltx_kv_cache_faults(ltx_ctx* c, ltx_kv_cache* k, void* stream, uint64_t* cou
     LTX_GUARD(c, {
         if (!c || !k || !count) throw ltx::Error("NULL argument");
         HIPC(hipSetDevice(c->device));
-        HIPC(hipStreamSynchronize((hipStream_t)stream));
+        hipStream_t st = (hipStream_t)stream;
+        // (waiting for it would end the capture)
+        if (ltx::is_capturing(st)) throw ltx::Error("the stream is being captured, or the legacy stream beside a capture");
+        ltx::RelaxedCapture relaxed;
         unsigned long long v = 0;
-        HIPC(hipMemcpy(&v, k->bad(), sizeof(v), hipMemcpyDeviceToHost));
+        HIPC(hipMemcpyAsync(&v, k->bad(), sizeof(v), hipMemcpyDeviceToHost, st));
+        HIPC(hipStreamSynchronize(st));
         *count = v;
         if (reset) {
             v = 0;
-            HIPC(hipMemcpy(k->bad(), &v, sizeof(v), hipMemcpyHostToDevice));
+            HIPC(hipMemcpyAsync(k->bad(), &v, sizeof(v), hipMemcpyHostToDevice, st));
+            HIPC(hipStreamSynchronize(st));
         }
     })
 }

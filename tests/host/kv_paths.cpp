@@ -12,6 +12,21 @@
 extern "C" hipError_t hipMemsetAsync(void*, int, size_t, hipStream_t s) {
     return fake::capturing.count(s) ? hipErrorStreamCaptureUnsupported : hipSuccess;
 }
+static uint64_t counter;      // the count of bad pages, as the device holds it
+static uint64_t counted_by_others;  // and what kernels on other streams add right after it is read
+extern "C" hipError_t hipMemcpyAsync(void* d, const void* s, size_t n, hipMemcpyKind kind, hipStream_t st) {
+    fake::log.push_back({"copy", "", st});
+    if (fake::capturing.count(st)) {
+        fake::broken_capture = true;
+        return hipErrorStreamCaptureUnsupported;
+    }
+    if (n == 8 && kind == hipMemcpyDeviceToHost) {
+        std::memcpy(d, &counter, 8);
+        counter += counted_by_others;
+    }
+    if (n == 8 && kind == hipMemcpyHostToDevice) std::memcpy(&counter, s, 8);
+    return hipSuccess;
+}
 
 #define CHECK(cond, ...)                                  \
     do {                                                  \
@@ -205,6 +220,23 @@ static void own_capture() {
     fake::capturing.clear();
 }
 
+// The count of bad pages beside a capture: read on the stream that is named, refused
+// on one that is being captured, and the capture is whole.
+static void faults_beside_a_capture() {
+    Fixture f;
+    hipStream_t captured = (hipStream_t)0x77, other = (hipStream_t)0x55;
+    fake::capturing.insert(captured);
+    counter = 5;
+    uint64_t n = 0;
+    CHECK(ltx_kv_cache_faults(f.c, f.cache, other, &n, 0) && n == 5, "%s", ltx_last_error(f.c));
+    CHECK(!fake::broken_capture, "the capture is broken");
+    REFUSED(ltx_kv_cache_faults(f.c, f.cache, captured, &n, 1), "captured");
+    CHECK(fake::log.empty() && !fake::broken_capture && counter == 5, "the capture is broken");
+    fake::capturing.clear();
+    CHECK(ltx_kv_cache_faults(f.c, f.cache, captured, &n, 1) && n == 5, "%s", ltx_last_error(f.c));
+    CHECK(ltx_kv_cache_faults(f.c, f.cache, captured, &n, 1) && n == 0, "%s", ltx_last_error(f.c));
+}
+
 // The index arithmetic on arrays of any contents: what a kernel would read and
 // write stays inside what the call names, and the items fit the grid.
 static void index_bounds(unsigned seed) {
@@ -282,6 +314,8 @@ int main(int argc, char** argv) {
         memory();
     else if (cmd == "own_capture")
         own_capture();
+    else if (cmd == "faults_beside_a_capture")
+        faults_beside_a_capture();
     else if (cmd == "index")
         index_bounds(std::atoi(argv[2]));
     else

@@ -130,3 +130,31 @@ def test_a_cache_made_inside_a_capture(block0):
             v.zero_()
     finally:
         c.close()
+
+
+def test_faults_beside_a_capture(ctx):
+    """Read on another stream while one is captured; refused on the captured one, which
+    goes on."""
+    say("kv faults beside a capture")
+    s = Setup(ctx, "f16", 2, [1, 3], [100, 70], seed=14)
+    s.pages[1, 0] = -1
+    q = s.queries(4).cuda()
+    out, want = torch.zeros(2, s.total, 4 * HD, dtype=s.dt, device="cuda")
+    work = torch.empty(max(16, ctx.kv_attention_workspace(s.cache, s.batch, 4)), dtype=torch.uint8, device="cuda")
+    ctx.kv_attention(s.cache, s.batch, q, want, 4, work=work)
+    once = s.cache.faults(reset=False)
+    assert once > 0
+    other, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph, capture_error_mode="global"):
+        ctx.kv_attention(s.cache, s.batch, q, out, 4, work=work)
+        assert s.cache.faults(stream=other) == once
+        with pytest.raises(rt.LtxError, match="captured"):
+            s.cache.faults()
+        out.mul_(2)
+    for i in range(3):
+        out.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want * 2)
+        assert s.cache.faults() == once

@@ -40,6 +40,10 @@ def test_cache_made_inside_a_capture_of_its_context(kv_paths):
     kv_paths("own_capture")
 
 
+def test_faults_beside_a_capture(kv_paths):
+    kv_paths("faults_beside_a_capture")
+
+
 @pytest.mark.parametrize("seed", [1, 2, 3])
 def test_index_arithmetic_stays_inside(kv_paths, seed):
     kv_paths("index", seed)
