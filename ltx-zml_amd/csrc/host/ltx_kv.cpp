@@ -9,6 +9,9 @@ struct ltx_kv_cache {
     // blocks [pages][kv_heads], then the count of bad pages, then a flag a page
     ltx::DevBuf buf;
     size_t blocks = 0;
+    // the count at the last reset: the device's is never written from here, which
+    // could lose what kernels of other streams add
+    unsigned long long bad_before = 0;
     uint8_t* data() const { return (uint8_t*)buf.p; }
     unsigned long long* bad() const { return (unsigned long long*)((char*)buf.p + blocks); }
     uint32_t* flags() const { return (uint32_t*)((char*)buf.p + blocks + 256); }
@@ -183,12 +186,8 @@ int ltx_kv_cache_faults(ltx_ctx* c, ltx_kv_cache* k, void* stream, uint64_t* cou
         unsigned long long v = 0;
         HIPC(hipMemcpyAsync(&v, k->bad(), sizeof(v), hipMemcpyDeviceToHost, st));
         HIPC(hipStreamSynchronize(st));
-        *count = v;
-        if (reset) {
-            v = 0;
-            HIPC(hipMemcpyAsync(k->bad(), &v, sizeof(v), hipMemcpyHostToDevice, st));
-            HIPC(hipStreamSynchronize(st));
-        }
+        *count = v - k->bad_before;
+        if (reset) k->bad_before = v;
     })
 }
 

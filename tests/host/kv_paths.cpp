@@ -237,6 +237,23 @@ static void faults_beside_a_capture() {
     CHECK(ltx_kv_cache_faults(f.c, f.cache, captured, &n, 1) && n == 0, "%s", ltx_last_error(f.c));
 }
 
+// Nothing is lost between a reading and its reset, nor to other streams' kernels that
+// count meanwhile.
+static void faults_are_not_lost() {
+    Fixture f;
+    uint64_t n = 0, all = 0;
+    counter = 7;
+    counted_by_others = 3;
+    for (int i = 0; i < 4; i++) {
+        CHECK(ltx_kv_cache_faults(f.c, f.cache, nullptr, &n, 1) && n == (i ? 3u : 7u), "%llu", (unsigned long long)n);
+        all += n;
+    }
+    counted_by_others = 0;
+    for (int reset = 0; reset < 2; reset++)
+        CHECK(ltx_kv_cache_faults(f.c, f.cache, nullptr, &n, reset) && n == 3, "%llu", (unsigned long long)n);
+    CHECK(all + n == counter && ltx_kv_cache_faults(f.c, f.cache, nullptr, &n, 1) && n == 0, "%llu", (unsigned long long)n);
+}
+
 // The index arithmetic on arrays of any contents: what a kernel would read and
 // write stays inside what the call names, and the items fit the grid.
 static void index_bounds(unsigned seed) {
@@ -316,6 +333,8 @@ int main(int argc, char** argv) {
         own_capture();
     else if (cmd == "faults_beside_a_capture")
         faults_beside_a_capture();
+    else if (cmd == "faults_are_not_lost")
+        faults_are_not_lost();
     else if (cmd == "index")
         index_bounds(std::atoi(argv[2]));
     else

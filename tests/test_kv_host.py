@@ -44,6 +44,10 @@ def test_faults_beside_a_capture(kv_paths):
     kv_paths("faults_beside_a_capture")
 
 
+def test_faults_are_not_lost(kv_paths):
+    kv_paths("faults_are_not_lost")
+
+
 @pytest.mark.parametrize("seed", [1, 2, 3])
 def test_index_arithmetic_stays_inside(kv_paths, seed):
     kv_paths("index", seed)
