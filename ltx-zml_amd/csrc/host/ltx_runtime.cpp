@@ -34,6 +34,7 @@ void hip_check(hipError_t e, const char* what) {
     long n = ++g_hip_calls;
     if (g_fail_after > 0 && n >= g_fail_after && e == hipSuccess) e = hipErrorUnknown;  // injected
     if (e != hipSuccess) {
+        (void)hipGetLastError();  // reported by what is thrown here: not once more by a later call
         char buf[512];
         std::snprintf(buf, sizeof(buf), "%s failed: %s (%d)%s", what, hipGetErrorString(e), (int)e,
                       (g_fail_after > 0 && n >= g_fail_after) ? " [LTX_FAIL_AFTER]" : "");

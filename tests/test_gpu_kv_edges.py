@@ -158,3 +158,16 @@ def test_faults_beside_a_capture(ctx):
         torch.cuda.synchronize()
         assert torch.equal(out, want * 2)
         assert s.cache.faults() == once
+
+
+def test_a_pool_that_does_not_fit(ctx):
+    """Refused, and the next calls of this library and of torch know nothing of it."""
+    say("kv pool beyond memory")
+    before = torch.cuda.mem_get_info()[0]
+    with pytest.raises(rt.LtxError):
+        ctx.kv_cache(32, (1 << 25) - 1, rt.MODE_F16)  # 9.3 TB
+    assert (torch.ones(1000, device="cuda") + 1).sum().item() == 2000
+    c = ctx.kv_cache(32, 10, rt.MODE_F16)
+    assert c.faults() == 0
+    c.free()
+    assert abs(torch.cuda.mem_get_info()[0] - before) < 64 << 20
