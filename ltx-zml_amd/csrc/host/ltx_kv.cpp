@@ -214,6 +214,14 @@ int ltx_op_kv_attention_workspace(ltx_ctx* c, const ltx_kv_cache* cache, const l
         ltx::batch_args(c, cache, batch);
         ltx::check_heads(cache, heads);
         *bytes = ltx::attn_plan(c, cache, batch, heads, true).bytes;
+        if (batch->rows == batch->nseq) {  // enough for the other form too: with row_start, or without
+            ltx_kv_batch other = *batch;
+            other.row_start = batch->row_start ? nullptr : batch->kv_len;  // (only whether there is one counts)
+            try {
+                *bytes = std::max<uint64_t>(*bytes, ltx::attn_plan(c, cache, &other, heads, true).bytes);
+            } catch (const ltx::Error&) {  // too many rows in that form: its calls are refused
+            }
+        }
     })
 }
 

@@ -254,6 +254,34 @@ static void faults_are_not_lost() {
     CHECK(all + n == counter && ltx_kv_cache_faults(f.c, f.cache, nullptr, &n, 1) && n == 0, "%llu", (unsigned long long)n);
 }
 
+// A workspace's size serves calls with row_start and without.
+static void workspace_forms() {
+    int split = 0;
+    for (int heads : {32, 8, 4, 3})
+        for (int group : {1, 4, 20}) {
+            Fixture f(heads);
+            for (int n : {1, 3, 16, 31, 70, 200})
+                for (int width : {1, 20, 128, 448}) {
+                    f.b = {n, n, (const int32_t*)ptr(0), (const int32_t*)ptr(1), (const int32_t*)ptr(2), width};
+                    ltx_kv_batch one = f.b;
+                    one.row_start = nullptr;
+                    uint64_t with = 0, without = 0;
+                    CHECK(ltx_op_kv_attention_workspace(f.c, f.cache, &f.b, heads * group, &with), "%s", ltx_last_error(f.c));
+                    CHECK(ltx_op_kv_attention_workspace(f.c, f.cache, &one, heads * group, &without), "%s", ltx_last_error(f.c));
+                    split += with > 0;
+                    const int64_t ld = heads * group * 128;
+                    auto taken = [&](uint64_t bytes) {
+                        return f.attend(ptr(5), ld, heads * group, ptr(6), ld, bytes ? ptr(7) : nullptr, bytes);
+                    };
+                    CHECK(with == without && taken(without), "%d of %d, %d heads x %d, %d pages: %s", n, n, heads, group,
+                          width, ltx_last_error(f.c));
+                    f.b = one;
+                    CHECK(taken(with), "%s", ltx_last_error(f.c));
+                }
+        }
+    CHECK(split > 50, "%d", split);
+}
+
 // The index arithmetic on arrays of any contents: what a kernel would read and
 // write stays inside what the call names, and the items fit the grid.
 static void index_bounds(unsigned seed) {
@@ -335,6 +363,8 @@ int main(int argc, char** argv) {
         faults_beside_a_capture();
     else if (cmd == "faults_are_not_lost")
         faults_are_not_lost();
+    else if (cmd == "workspace_forms")
+        workspace_forms();
     else if (cmd == "index")
         index_bounds(std::atoi(argv[2]));
     else

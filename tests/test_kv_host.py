@@ -48,6 +48,10 @@ def test_faults_are_not_lost(kv_paths):
     kv_paths("faults_are_not_lost")
 
 
+def test_one_workspace_for_both_forms(kv_paths):
+    kv_paths("workspace_forms")
+
+
 @pytest.mark.parametrize("seed", [1, 2, 3])
 def test_index_arithmetic_stays_inside(kv_paths, seed):
     kv_paths("index", seed)
