@@ -76,22 +76,24 @@ struct AttnPlan {
 //   75, 256 131 / 59 / 113, 512 245 / 82 / 76
 //   8 sequences of 1,000 keys, 32 cached heads: 32 columns 31 / 36 / 49, 64 51 / 48 /
 //   60, 128 94 / 45 / 82
-// The table's width stands for the lengths, which the host does not know.
-int tile_columns(const ltx_ctx* c, const ltx_kv_cache* k, const ltx_kv_batch* b, int64_t columns) {
+// The table's width stands for the lengths, which the host does not know. A call that
+// cannot split (captured, without a workspace) takes 256 columns only where they fill
+// the CUs: 256 rows of 32 heads on 8 over 28,672 keys 235 us on 16 columns, 815 on 256.
+int tile_columns(const ltx_ctx* c, const ltx_kv_cache* k, const ltx_kv_batch* b, int64_t columns, bool split) {
     if (c->kv_tile) return c->kv_tile;
     const int64_t each = columns / b->nseq, wide = columns * k->kv_heads / 256;  // workgroups of 256 columns
     const int64_t pages = wide * b->max_pages / c->num_cu;                       // of each, if split
     if (each >= 192 && wide >= c->num_cu) return 256;
-    if (each >= 256 && pages >= 128) return 256;
+    if (split && each >= 256 && pages >= 128) return 256;
     if (each >= 64 && (each + 127) / 128 * b->nseq * k->kv_heads >= c->num_cu) return 128;
-    if (each >= 256 && pages >= 24) return 256;
+    if (split && each >= 256 && pages >= 24) return 256;
     return 16;
 }
 
 AttnPlan attn_plan(const ltx_ctx* c, const ltx_kv_cache* k, const ltx_kv_batch* b, int heads, bool split) {
     const int64_t group = heads / k->kv_heads, columns = (int64_t)b->rows * group;
     AttnPlan p;
-    p.tile = tile_columns(c, k, b, columns);
+    p.tile = tile_columns(c, k, b, columns, split);
     // tiles of the batch, at most
     const int64_t tiles = !b->row_start || b->nseq == 1
                               ? (int64_t)b->nseq * ((columns / b->nseq + p.tile - 1) / p.tile)

@@ -282,6 +282,30 @@ static void workspace_forms() {
     CHECK(split > 50, "%d", split);
 }
 
+// A call that cannot split (captured, no workspace) does not take the 256-column tiles
+// that only a split makes worth while: few workgroups would walk all pages. Where such
+// tiles fill the CUs by themselves, it does.
+static void unsplit_tiles() {
+    Fixture f;
+    hipStream_t s = (hipStream_t)0x77;
+    auto kernel = [&](bool captured, int rows, int pages) {
+        f.b = {1, rows, (const int32_t*)ptr(0), (const int32_t*)ptr(1), (const int32_t*)ptr(2), pages};
+        if (captured) fake::capturing.insert(s);
+        fake::log.clear();
+        CHECK(f.attend(ptr(5), 4096, 32, ptr(6), 4096, nullptr, 0, s), "%s", ltx_last_error(f.c));
+        fake::capturing.clear();
+        for (const fake::Op& o : fake::log)
+            if (o.what == "launch") return o.name;
+        return std::string();
+    };
+    CHECK(kernel(false, 256, 448) == "ltx_kv_attn_f16_rows2_split", "%s", kernel(false, 256, 448).c_str());
+    CHECK(kernel(true, 256, 448) == "ltx_kv_attn_f16", "%s", kernel(true, 256, 448).c_str());
+    CHECK(kernel(false, 1024, 448) == "ltx_kv_attn_f16_rows2_split", "%s", kernel(false, 1024, 448).c_str());
+    CHECK(kernel(true, 1024, 448) == "ltx_kv_attn_f16_rows1", "%s", kernel(true, 1024, 448).c_str());
+    for (bool captured : {false, true})
+        CHECK(kernel(captured, 4096, 448) == "ltx_kv_attn_f16_rows2", "%s", kernel(captured, 4096, 448).c_str());
+}
+
 // The index arithmetic on arrays of any contents: what a kernel would read and
 // write stays inside what the call names, and the items fit the grid.
 static void index_bounds(unsigned seed) {
@@ -365,6 +389,8 @@ int main(int argc, char** argv) {
         faults_are_not_lost();
     else if (cmd == "workspace_forms")
         workspace_forms();
+    else if (cmd == "unsplit_tiles")
+        unsplit_tiles();
     else if (cmd == "index")
         index_bounds(std::atoi(argv[2]));
     else

@@ -52,6 +52,10 @@ def test_one_workspace_for_both_forms(kv_paths):
     kv_paths("workspace_forms")
 
 
+def test_tiles_of_calls_that_cannot_split(kv_paths):
+    kv_paths("unsplit_tiles")
+
+
 @pytest.mark.parametrize("seed", [1, 2, 3])
 def test_index_arithmetic_stays_inside(kv_paths, seed):
     kv_paths("index", seed)
