@@ -48,7 +48,7 @@ void kv_rows(ltx_ctx* c, const ltx_kv_cache* k, const ltx_kv_batch* b, void* kp,
     const int width = k->kv_heads * LTX_HD;
     check_rows(kp, ldk, width, b->rows, "k");
     check_rows(vp, ldv, width, b->rows, "v");
-    if (b->rows >= 1 << 28) throw Error("too many rows for one call");  // 2^32 threads along x
+    if (b->rows > (1 << 28) - 16) throw Error("too many rows for one call");  // 2^32 threads along x: one too many
     if (b->rows == 0) return;
     HIPC(hipSetDevice(c->device));
     const bool f16 = k->mode == LTX_MODE_F16;

@@ -306,6 +306,19 @@ static void unsplit_tiles() {
         CHECK(kernel(captured, 4096, 448) == "ltx_kv_attn_f16_rows2", "%s", kernel(captured, 4096, 448).c_str());
 }
 
+// The largest count of rows written or read: 16 a workgroup of 256 threads, fewer than
+// 2^32 threads.
+static void row_limit() {
+    Fixture f;
+    for (int rows : {0x0fffffff, (1 << 28) - 15}) {
+        f.b.rows = rows;
+        REFUSED(f.write(), "too many rows");
+        REFUSED(f.read(), "too many rows");
+    }
+    f.b.rows = (1 << 28) - 16;
+    CHECK(f.write() && f.read(), "%s", ltx_last_error(f.c));
+}
+
 // The index arithmetic on arrays of any contents: what a kernel would read and
 // write stays inside what the call names, and the items fit the grid.
 static void index_bounds(unsigned seed) {
@@ -391,6 +404,8 @@ int main(int argc, char** argv) {
         workspace_forms();
     else if (cmd == "unsplit_tiles")
         unsplit_tiles();
+    else if (cmd == "row_limit")
+        row_limit();
     else if (cmd == "index")
         index_bounds(std::atoi(argv[2]));
     else

@@ -56,6 +56,10 @@ def test_tiles_of_calls_that_cannot_split(kv_paths):
     kv_paths("unsplit_tiles")
 
 
+def test_row_limit(kv_paths):
+    kv_paths("row_limit")
+
+
 @pytest.mark.parametrize("seed", [1, 2, 3])
 def test_index_arithmetic_stays_inside(kv_paths, seed):
     kv_paths("index", seed)
