@@ -319,9 +319,9 @@ uint64_t ltx_kv_cache_bytes(const ltx_kv_cache* cache);
  * pool is not followed: the row is not written, or read as zeros, or the page's
  * keys take no part in the attention, and it is counted (ltx_kv_cache_faults).
  * The host checks what it can see: nseq and max_pages (at most 2^24) positive, rows
- * not negative (0: nothing to do; below 2^24 for the attention, at most 2^28 - 16 else), pointers,
- * heads, and that rows of k, v, q and out start on 16 bytes with strides (in
- * elements) that are multiples of 8 and not shorter than a row. */
+ * not negative (0: nothing to do; below 2^24 for the attention, at most 2^28 - 16 else), pointers
+ * (the arrays and glog on 4 bytes), heads, and that rows of k, v, q and out start on 16
+ * bytes with strides (in elements) that are multiples of 8 and not shorter than a row. */
 typedef struct ltx_kv_batch {
     int nseq, rows;
     const int32_t* row_start;

@@ -29,6 +29,8 @@ LtxKvBatchArgs batch_args(const ltx_ctx* c, const ltx_kv_cache* k, const ltx_kv_
     if (b->nseq <= 0 || b->rows < 0) throw Error("bad batch: nseq must be positive, rows not negative");
     if (b->max_pages <= 0 || b->max_pages > kMaxPages) throw Error("bad batch: max_pages must be 1 .. 2^24");
     if (!b->kv_len || !b->pages) throw Error("bad batch: kv_len and pages are needed");
+    if (((uintptr_t)b->kv_len | (uintptr_t)b->pages | (uintptr_t)b->row_start) & 3)
+        throw Error("bad batch: row_start, kv_len and pages must start on 4 bytes");
     if (!b->row_start && b->rows != b->nseq) throw Error("bad batch: without row_start, rows must equal nseq");
     return LtxKvBatchArgs{k->data(), k->flags(), k->bad(),     b->row_start, b->kv_len,
                           b->pages,  b->nseq,    b->rows, b->max_pages, k->pages, k->kv_heads};
@@ -237,6 +239,7 @@ int ltx_op_kv_attention(ltx_ctx* c, const ltx_kv_cache* cache, const ltx_kv_batc
         ltx::check_heads(cache, heads);
         ltx::check_rows(q, ldq, heads * LTX_HD, batch->rows, "q");
         ltx::check_rows(out, ldo, heads * LTX_HD, batch->rows, "out");
+        if ((uintptr_t)glog & 3) throw ltx::Error("glog must start on 4 bytes");
         if ((uintptr_t)work & 15) throw ltx::Error("work must start on 16 bytes");
         ltx::AttnPlan p = ltx::attn_plan(c, cache, batch, heads, true);
         if (work && work_bytes < p.bytes) throw ltx::Error("work is smaller than ltx_op_kv_attention_workspace says");

@@ -319,6 +319,35 @@ static void row_limit() {
     CHECK(f.write() && f.read(), "%s", ltx_last_error(f.c));
 }
 
+// Arrays that do not start on their type are refused: the kernels' scalar loads take the
+// address without its last two bits.
+static void alignment() {
+    Fixture f;
+    const ltx_kv_batch good = f.b;
+    uint64_t n;
+    for (int i = 0; i < 3; i++)
+        for (int off = 1; off < 4; off++) {
+            f.b = good;
+            const int32_t*& p = i == 0 ? f.b.row_start : i == 1 ? f.b.kv_len : f.b.pages;
+            p = (const int32_t*)((char*)p + off);
+            REFUSED(f.write(), "4 bytes");
+            REFUSED(f.read(), "4 bytes");
+            REFUSED(f.attend(), "4 bytes");
+            REFUSED(ltx_op_kv_attention_workspace(f.c, f.cache, &f.b, 32, &n), "4 bytes");
+        }
+    f.b = good;
+    for (int off = 0; off < 4; off++) {
+        auto call = [&]() {
+            return ltx_op_kv_attention(f.c, f.cache, &f.b, ptr(5), 4096, 32, 1, (const float*)(ptr(8) + off), ptr(6), 4096,
+                                       ptr(7), 1ull << 30, nullptr);
+        };
+        if (off)
+            REFUSED(call(), "4 bytes");
+        else
+            CHECK(call(), "%s", ltx_last_error(f.c));
+    }
+}
+
 // The index arithmetic on arrays of any contents: what a kernel would read and
 // write stays inside what the call names, and the items fit the grid.
 static void index_bounds(unsigned seed) {
@@ -406,6 +435,8 @@ int main(int argc, char** argv) {
         unsplit_tiles();
     else if (cmd == "row_limit")
         row_limit();
+    else if (cmd == "alignment")
+        alignment();
     else if (cmd == "index")
         index_bounds(std::atoi(argv[2]));
     else

@@ -60,6 +60,10 @@ def test_row_limit(kv_paths):
     kv_paths("row_limit")
 
 
+def test_alignment_of_the_batch(kv_paths):
+    kv_paths("alignment")
+
+
 @pytest.mark.parametrize("seed", [1, 2, 3])
 def test_index_arithmetic_stays_inside(kv_paths, seed):
     kv_paths("index", seed)
