@@ -195,7 +195,7 @@ class BlockGraph:
         self._keep = keep  # the bound tensors stay alive with the graph
 
     def launch(self, stream=None):
-        st = stream.cuda_stream if stream is not None else _current_stream()
+        st = stream.cuda_stream if stream is not None else _current_stream(self.ctx.device)
         self.ctx._check(lib().ltx_block_graph_launch(self.handle, st), "ltx_block_graph_launch")
 
     def free(self):
@@ -251,7 +251,7 @@ class KvCache:
 
     def faults(self, reset: bool = True, stream=None) -> int:
         """Page indices outside the pool met since the last reset (ltx_kv_cache_faults)."""
-        st = stream.cuda_stream if stream is not None else _current_stream()
+        st = stream.cuda_stream if stream is not None else _current_stream(self.ctx.device)
         n = C.c_uint64()
         self.ctx._check(lib().ltx_kv_cache_faults(self.ctx.handle, self.handle, st, C.byref(n), int(reset)),
                         "ltx_kv_cache_faults")
@@ -323,7 +323,7 @@ class Context:
         """Streaming upload from `mem_ptr` (pinned host memory, e.g. a ring
         slot) on `stream`; returns at once. Keep the memory unchanged until
         the stream passes this call."""
-        st = stream.cuda_stream if stream is not None else _current_stream()
+        st = stream.cuda_stream if stream is not None else _current_stream(self.device)
         h = C.c_void_p()
         self._check(lib().ltx_block_weights_from_blob_async(self.handle, mem_ptr, nbytes, manifest_json.encode(),
                                                             block, reuse.handle if reuse else None, st, C.byref(h)),
@@ -333,7 +333,7 @@ class Context:
     # ---- forward ----
     def forward(self, w: Weights, x, tstab, tidx, ctx, pts2, cos, sin, y, mode: int = MODE_F16, stream=None):
         T, S, K = x.shape[0], ctx.shape[0], tstab.shape[0]
-        st = stream.cuda_stream if stream is not None else _current_stream()
+        st = stream.cuda_stream if stream is not None else _current_stream(self.device)
         self._check(lib().ltx_block_forward(self.handle, w.handle, _ptr(x), _ptr(tstab), K, _ptr(tidx), _ptr(ctx), S,
                                             _ptr(pts2), _ptr(cos), _ptr(sin), T, _ptr(y), mode, st),
                     "ltx_block_forward")
@@ -353,7 +353,7 @@ class Context:
 
     def range_count(self, reset: bool = True, stream=None) -> int:
         """16-bit stores out of range since the last reset (ltx_range_count)."""
-        st = stream.cuda_stream if stream is not None else _current_stream()
+        st = stream.cuda_stream if stream is not None else _current_stream(self.device)
         n = C.c_uint64()
         self._check(lib().ltx_range_count(self.handle, st, C.byref(n), int(reset)), "ltx_range_count")
         return n.value
@@ -374,7 +374,7 @@ class Context:
         M, K = a.shape
         N = q.shape[0]
         import torch
-        st = stream.cuda_stream if stream is not None else _current_stream()
+        st = stream.cuda_stream if stream is not None else _current_stream(self.device)
         name = "ltx_op_linear_q8_noalloc" if noalloc else "ltx_op_linear_q8"
         self._check(getattr(lib(), name)(self.handle, _ptr(a), _ptr(q), _ptr(s), int(s.dtype == torch.float16),
                                          _ptr(bias), _ptr(y), int(y.dtype == torch.float32), M, N, K, int(gelu),
@@ -383,7 +383,7 @@ class Context:
 
     def attention(self, q, k, v, glog, out, lq, lkv, mode=MODE_F16, stream=None, q_scaled=False):
         """q_scaled: q already holds q * log2(e) / sqrt(128) (LTX_ATTN_Q_SCALED)."""
-        st = stream.cuda_stream if stream is not None else _current_stream()
+        st = stream.cuda_stream if stream is not None else _current_stream(self.device)
         m = mode | (ATTN_Q_SCALED if q_scaled else 0)
         self._check(lib().ltx_op_attention(self.handle, _ptr(q), _ptr(k), _ptr(v), _ptr(glog), _ptr(out), lq, lkv,
                                            m, st), "ltx_op_attention")
@@ -406,7 +406,7 @@ class Context:
         if not (a.dtype == x and q.dtype == torch.uint8 and (s.dtype == half or s.dtype == f32)
                 and (y.dtype == x or y.dtype == f32) and (bias is None or bias.dtype == f32)):
             raise LtxError("linear_q4: the types do not fit the mode")
-        st = stream.cuda_stream if stream is not None else _current_stream()
+        st = stream.cuda_stream if stream is not None else _current_stream(self.device)
         self._check(lib().ltx_op_linear_q4(self.handle, _ptr(a), _ptr(q), _ptr(s), int(s.dtype == torch.float16),
                                            _ptr(bias), _ptr(y), int(y.dtype == torch.float32), M, N, K, int(gelu),
                                            mode, st), "ltx_op_linear_q4")
@@ -422,14 +422,14 @@ class Context:
 
     def kv_write(self, cache: KvCache, batch: KvBatch, k, v, stream=None):
         """k, v [rows, kv_heads * 128] (rows may be strided) -> the cache (ltx_op_kv_write)."""
-        st = stream.cuda_stream if stream is not None else _current_stream()
+        st = stream.cuda_stream if stream is not None else _current_stream(self.device)
         _rows("kv_write", batch, cache, cache.kv_heads, k, v)
         self._check(lib().ltx_op_kv_write(self.handle, cache.handle, batch.ref, _ptr(k), k.stride(0), _ptr(v),
                                           v.stride(0), st), "ltx_op_kv_write")
 
     def kv_read(self, cache: KvCache, batch: KvBatch, k, v, stream=None):
         """What the cache holds of the batch's rows -> k, v (ltx_op_kv_read)."""
-        st = stream.cuda_stream if stream is not None else _current_stream()
+        st = stream.cuda_stream if stream is not None else _current_stream(self.device)
         _rows("kv_read", batch, cache, cache.kv_heads, k, v)
         self._check(lib().ltx_op_kv_read(self.handle, cache.handle, batch.ref, _ptr(k), k.stride(0), _ptr(v),
                                          v.stride(0), st), "ltx_op_kv_read")
@@ -446,7 +446,7 @@ class Context:
         """q, out [rows, heads * 128] (rows may be strided); glog [rows, heads] f32
         or None; work: a uint8 tensor of kv_attention_workspace bytes, or None
         (ltx_op_kv_attention)."""
-        st = stream.cuda_stream if stream is not None else _current_stream()
+        st = stream.cuda_stream if stream is not None else _current_stream(self.device)
         _rows("kv_attention", batch, cache, heads, q, out)
         if glog is not None and not (glog.shape == (batch.rows, heads) and glog.is_contiguous()
                                      and glog.dtype == _torch_dtype(MODE_F32)
@@ -463,7 +463,7 @@ class Context:
     def dequant(self, q, s, out32, out16, mode=MODE_F16, stream=None):
         import torch
         N, K = q.shape
-        st = stream.cuda_stream if stream is not None else _current_stream()
+        st = stream.cuda_stream if stream is not None else _current_stream(self.device)
         self._check(lib().ltx_op_dequant(self.handle, _ptr(q), _ptr(s), int(s.dtype == torch.float16), N, K,
                                          _ptr(out32), _ptr(out16), mode, st), "ltx_op_dequant")
 
@@ -480,32 +480,32 @@ class Context:
 
     def conditioning(self, cw: CoreWeights, t, sigma, tstab, emb, pts2, stream=None):
         """t [K] f32, sigma [1] f32 (device) -> tstab [K, 9, D], emb [K, D], pts2 [2, D]."""
-        st = stream.cuda_stream if stream is not None else _current_stream()
+        st = stream.cuda_stream if stream is not None else _current_stream(self.device)
         self._check(lib().ltx_core_conditioning(self.handle, cw.handle, _ptr(t), t.shape[0], _ptr(sigma), _ptr(tstab),
                                                 _ptr(emb), _ptr(pts2), st), "ltx_core_conditioning")
 
     def patchify(self, cw: CoreWeights, latent, x, stream=None):
-        st = stream.cuda_stream if stream is not None else _current_stream()
+        st = stream.cuda_stream if stream is not None else _current_stream(self.device)
         self._check(lib().ltx_core_patchify(self.handle, cw.handle, _ptr(latent), latent.shape[0], _ptr(x), st),
                     "ltx_core_patchify")
         return x
 
     def tail(self, cw: CoreWeights, x, emb, tidx, vel, stream=None):
-        st = stream.cuda_stream if stream is not None else _current_stream()
+        st = stream.cuda_stream if stream is not None else _current_stream(self.device)
         self._check(lib().ltx_core_tail(self.handle, cw.handle, _ptr(x), _ptr(emb), _ptr(tidx), x.shape[0], _ptr(vel),
                                         st), "ltx_core_tail")
         return vel
 
     def noise_init(self, clean, noise, maskk, tidx, noise_scale: float, out, stream=None):
         T, Cc = clean.shape
-        st = stream.cuda_stream if stream is not None else _current_stream()
+        st = stream.cuda_stream if stream is not None else _current_stream(self.device)
         self._check(lib().ltx_sched_noise_init(self.handle, _ptr(clean), _ptr(noise), _ptr(maskk), _ptr(tidx), T, Cc,
                                                float(noise_scale), _ptr(out), st), "ltx_sched_noise_init")
         return out
 
     def sched_step(self, x, vel, tk, maskk, tidx, clean, sigma: float, sigma_next: float, out, stream=None):
         T, Cc = x.shape
-        st = stream.cuda_stream if stream is not None else _current_stream()
+        st = stream.cuda_stream if stream is not None else _current_stream(self.device)
         self._check(lib().ltx_sched_step(self.handle, _ptr(x), _ptr(vel), _ptr(tk), _ptr(maskk), _ptr(tidx),
                                          _ptr(clean), T, Cc, float(sigma), float(sigma_next), _ptr(out), st),
                     "ltx_sched_step")
@@ -517,7 +517,7 @@ class Context:
         is updated in place."""
         sig = np.ascontiguousarray(sigmas, np.float32)
         hs = (C.c_void_p * len(blocks))(*[b.handle for b in blocks])
-        st = stream.cuda_stream if stream is not None else _current_stream()
+        st = stream.cuda_stream if stream is not None else _current_stream(self.device)
         self._check(lib().ltx_denoise(self.handle, hs, len(blocks), cw.handle, _ptr(latent), _ptr(clean), _ptr(maskk),
                                       _ptr(tidx), maskk.shape[0], _ptr(ctx), ctx.shape[0], _ptr(cos), _ptr(sin),
                                       latent.shape[0], sig.ctypes.data, len(sig) - 1, mode, st), "ltx_denoise")
@@ -558,11 +558,13 @@ def _rows(name: str, batch: KvBatch, cache: KvCache, heads: int, *tensors):
             raise LtxError(f"{name}: {list(shape)} tensors of the cache's type are needed")
 
 
-def _current_stream() -> int:
+def _current_stream(device: int) -> int:
+    """The handle of a device's current stream."""
     import torch
-    # the raw handle of the current device's current stream: 0.2 us, against 3 us
-    # of a Stream object's making
-    return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
+    try:  # without a Stream object: 0.2 us, against 3 us
+        return torch._C._cuda_getCurrentRawStream(device)
+    except AttributeError:  # not part of torch's public interface
+        return torch.cuda.current_stream(device).cuda_stream
 
 
 def _memcpy_dtod(dst: int, src: int, n: int):

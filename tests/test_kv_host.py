@@ -98,3 +98,35 @@ def test_python_checks():
     Ctx.device = 0
     with pytest.raises(rt.LtxError, match="device"):
         rt._rows("x", b, Cache, 2, good)
+
+
+def test_stream_of_the_contexts_device(monkeypatch):
+    """Without a stream a call takes the current stream of the context's device, which
+    need not be the current one; also on a torch without the raw handle's call."""
+    torch = pytest.importorskip("torch")
+    import types
+
+    from ltx_amd import runtime as rt
+
+    seen = []
+
+    def faults(ctx, cache, st, n, reset):
+        seen.append(st)
+        return 1
+    monkeypatch.setattr(rt, "_lib", types.SimpleNamespace(ltx_kv_cache_faults=faults, ltx_kv_cache_free=lambda *a: None,
+                                                          ltx_block_graph_launch=lambda h, st: seen.append(st) or 1,
+                                                          ltx_block_graph_destroy=lambda h: None))
+    ctx = rt.Context.__new__(rt.Context)
+    ctx.handle, ctx.device = 1, 3
+    cache, graph = rt.KvCache(ctx, 2, 1, 1, rt.MODE_F16), rt.BlockGraph(ctx, 2, ())
+    monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda device: 1000 + device, raising=False)
+    assert cache.faults() == 0
+    graph.launch()
+    assert seen == [1003, 1003]
+    monkeypatch.delattr(torch._C, "_cuda_getCurrentRawStream")
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda device=None: types.SimpleNamespace(cuda_stream=2000 + device))
+    cache.faults()
+    graph.launch()
+    assert seen[2:] == [2003, 2003]
+    cache.faults(stream=types.SimpleNamespace(cuda_stream=5))
+    assert seen[4:] == [5]
