@@ -274,8 +274,9 @@ int ltx_op_dequant(ltx_ctx* ctx, const int8_t* q, const void* scales, int scale_
  * with optional GELU-tanh. q [N][K / 2]: two weights a byte, the even k in the
  * low nibble, two's complement (-8 .. 7); scales [N][K / 128] f32 or f16. Modes
  * F16 and BF16: a 16-bit, y f32 (out_f32) or 16-bit; F32: a and y f32, a taken as
- * three exact bf16 planes. The weights are exact operands, a group's scale
- * multiplies its f32 sum. No scratch: calls may overlap and be captured. Refused:
+ * three bf16 planes (exact from 2^-110 on; of smaller values the bits above 2^-133).
+ * The weights are exact operands, a group's scale multiplies its f32 sum; values of a
+ * up to the type's largest give y wherever y is finite. No scratch: calls may overlap and be captured. Refused:
  * M, N or K not positive, K no multiple of 128, a or q not on 16 bytes, scales,
  * bias or y not aligned to their types, an unknown mode, M above 1,048,560, N from
  * 2^27, K above 2^23. */

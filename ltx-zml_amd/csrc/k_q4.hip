@@ -1,12 +1,15 @@
 // y = a . (q s)^T (+ bias, GELU) with 4-bit weights, two a byte, and a scale per
 // 128 along k: the linear of few rows.
+#include <type_traits>
+
 #include "ltx_device.h"
 
 // Eight weights of a dword (two's complement nibbles, the lowest first) as 16-bit
 // operands of value q / 16: v_cvt_off_f32_i4 (of the low four bits, exact) takes any
 // byte of its operand, so that a shift serves the four odd nibbles; the rounding is
-// exact too. 13 instructions.
-template <typename T>
+// exact too. 13 instructions. X: q / 1,024, six off the exponents of a pair (a zero's
+// stays zero: the subtraction saturates).
+template <typename T, bool X>
 __device__ __forceinline__ u32x4 q4_operand(uint32_t w) {
     uint32_t o = w >> 4;
     asm("" : "+v"(o));  // one shift, not one an odd nibble
@@ -15,6 +18,14 @@ __device__ __forceinline__ u32x4 q4_operand(uint32_t w) {
     for (int e = 0; e < 4; e++)
         r[e] = Op<T>::cvt2(__builtin_amdgcn_cvt_off_f32_i4((w >> (8 * e)) & 0xffu),
                            __builtin_amdgcn_cvt_off_f32_i4((o >> (8 * e)) & 0xffu));
+    if (X) {
+        typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            const uint32_t x = r[e];
+            r[e] = __builtin_bit_cast(uint32_t, __builtin_elementwise_sub_sat(__builtin_bit_cast(u16x2, x), (u16x2)(6 << 7)));
+        }
+    }
     return r;
 }
 
@@ -89,8 +100,8 @@ __device__ __forceinline__ void q4_spread(uint32_t x, uint32_t (&s)[4]) {
     s[2] = b[0], s[3] = b[1];
 }
 
-// Four values as three bf16 planes, x = p0 + p1 + p2 exactly (split3 of the f32 GEMM,
-// four at a time).
+// Four values as three bf16 planes, x = p0 + p1 + p2 exactly from 2^-110 on (the lowest
+// plane ends at bf16's smallest subnormal; split3 of the f32 GEMM, four at a time).
 __device__ __forceinline__ void q4_split(f32x4 x, u32x2 (&p)[3]) {
     uint32_t h[4], m[4], l[4];
 #pragma unroll
@@ -209,63 +220,84 @@ __device__ __forceinline__ void linear_q4(const LtxLinearQ4Args& a) {
                     f.x[m][p][j] = __builtin_bit_cast(
                         v8, *(const u32x4*)(my + 4096 * (MT * p + m) + 256 * r + 16 * ((4 * h + j) ^ r)));
     };
-    f32x4 acc[MT][NT];
+    // acc = the wave's groups; X: with weights times 2^-6 and scales times 2^6
+    auto sums = [&](auto x, f32x4 (&acc)[MT][NT]) {
+        constexpr bool X = decltype(x)::value;
 #pragma unroll
-    for (int m = 0; m < MT; m++)
+        for (int m = 0; m < MT; m++)
 #pragma unroll
-        for (int t = 0; t < NT; t++) acc[m][t] = f32x4{0, 0, 0, 0};
+            for (int t = 0; t < NT; t++) acc[m][t] = f32x4{0, 0, 0, 0};
 
-    load_s(g0);
-#pragma unroll
-    for (int u = 0; u < AW; u++) {
-        load_w(u, g0 + u);
-        if (u < AA) load_a(u, g0 + u);
-        __builtin_amdgcn_sched_barrier(0);
-    }
-    // EARLY 1: a group's exchange runs before the products of the one before it
-    Frags f[1 + EARLY];
-    if (EARLY) {
-        exchange(0, f[0]);
-        load_w(0, g0 + AW);
-        load_a(0, g0 + AA);
-    }
-    for (int g = g0; g < g1; g += AW) {
-        uint32_t sg[NT][4];
-#pragma unroll
-        for (int t = 0; t < NT; t++) q4_spread(sc[t], sg[t]);
-        load_s(g + AW);
+        load_s(g0);
 #pragma unroll
         for (int u = 0; u < AW; u++) {
-            exchange(u + EARLY, f[(u + EARLY) & EARLY]);
-            // the loads stay here: gathered behind all of the step's products they
-            // would be waited for all at once
-            load_w((u + EARLY) % AW, g + u + EARLY + AW);
-            load_a((u + EARLY) % AA, g + u + EARLY + AA);
-            f32x4 d[MT][NT];
+            load_w(u, g0 + u);
+            if (u < AA) load_a(u, g0 + u);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        // EARLY 1: a group's exchange runs before the products of the one before it
+        Frags f[1 + EARLY];
+        if (EARLY) {
+            exchange(0, f[0]);
+            load_w(0, g0 + AW);
+            load_a(0, g0 + AA);
+        }
+        for (int g = g0; g < g1; g += AW) {
+            uint32_t sg[NT][4];
 #pragma unroll
-            for (int m = 0; m < MT; m++)
+            for (int t = 0; t < NT; t++) q4_spread(sc[t], sg[t]);
+            load_s(g + AW);
 #pragma unroll
-                for (int t = 0; t < NT; t++) d[m][t] = f32x4{0, 0, 0, 0};
-#pragma unroll
-            for (int j = 0; j < 4; j++)
-#pragma unroll
-                for (int t = 0; t < NT; t++) {
-                    const v8 wv = __builtin_bit_cast(v8, q4_operand<T>(f[u & EARLY].w[t][j]));
-#pragma unroll
-                    for (int m = 0; m < MT; m++)
-#pragma unroll
-                        for (int p = 0; p < PL; p++) d[m][t] = Op<T>::mfma16(f[u & EARLY].x[m][p][j], wv, d[m][t]);
-                }
-#pragma unroll
-            for (int t = 0; t < NT; t++) {
-                const float s = q4_scale<S16>(sg[t][u]);
+            for (int u = 0; u < AW; u++) {
+                exchange(u + EARLY, f[(u + EARLY) & EARLY]);
+                // the loads stay here: gathered behind all of the step's products they
+                // would be waited for all at once
+                load_w((u + EARLY) % AW, g + u + EARLY + AW);
+                load_a((u + EARLY) % AA, g + u + EARLY + AA);
+                f32x4 d[MT][NT];
 #pragma unroll
                 for (int m = 0; m < MT; m++)
 #pragma unroll
-                    for (int i = 0; i < 4; i++) acc[m][t][i] = __builtin_fmaf(d[m][t][i], s, acc[m][t][i]);
+                    for (int t = 0; t < NT; t++) d[m][t] = f32x4{0, 0, 0, 0};
+#pragma unroll
+                for (int j = 0; j < 4; j++)
+#pragma unroll
+                    for (int t = 0; t < NT; t++) {
+                        const v8 wv = __builtin_bit_cast(v8, q4_operand<T, X>(f[u & EARLY].w[t][j]));
+#pragma unroll
+                        for (int m = 0; m < MT; m++)
+#pragma unroll
+                            for (int p = 0; p < PL; p++) d[m][t] = Op<T>::mfma16(f[u & EARLY].x[m][p][j], wv, d[m][t]);
+                    }
+#pragma unroll
+                for (int t = 0; t < NT; t++) {
+                    const float s = X ? 64.0f * q4_scale<S16>(sg[t][u]) : q4_scale<S16>(sg[t][u]);
+#pragma unroll
+                    for (int m = 0; m < MT; m++)
+#pragma unroll
+                        for (int i = 0; i < 4; i++) acc[m][t][i] = __builtin_fmaf(d[m][t][i], s, acc[m][t][i]);
+                }
+                __builtin_amdgcn_sched_barrier(0);
             }
-            __builtin_amdgcn_sched_barrier(0);
         }
+    };
+    f32x4 acc[MT][NT];
+    sums(std::false_type{}, acc);
+    // A group's sum of a q / 16 may leave f32's range, from |a| = 2^122 on, where y does
+    // not. A wave with a sum that is not finite forms its sums once more with the weights
+    // times 2^-6, whose products are no larger than a, and the scales times 2^6 (exact below 2^122): the
+    // range is that of a and y, and an infinity or NaN in a stays one. (f16 values are
+    // too small for that.)
+    if constexpr (__is_same(T, __bf16)) {
+        float worst = 0.f;  // 0, or NaN
+#pragma unroll
+        for (int m = 0; m < MT; m++)
+#pragma unroll
+            for (int t = 0; t < NT; t++)
+#pragma unroll
+                for (int i = 0; i < 4; i++)  // (rows of D past the last may hold anything)
+                    if (16 * m + 4 * h + i < (PACK ? 3 * rows : rows)) worst = __builtin_fmaf(acc[m][t][i], 0.f, worst);
+        if (__builtin_amdgcn_ballot_w64(worst != 0.f)) sums(std::true_type{}, acc);
     }
     q4_finish<T, MT, NT, SLOT, PACK ? 3 : 1>(a, lds, w, lane, acc, m0, n0, rows);
 }
