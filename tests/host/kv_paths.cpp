@@ -348,6 +348,34 @@ static void alignment() {
     }
 }
 
+// Every tile form of the linear is one that sizes select: rows and columns of
+// test_gpu_q4_forms.py's sweep.
+static void linear_forms() {
+    Fixture f;
+    std::set<std::string> names;
+    for (int mode : {LTX_MODE_F16, LTX_MODE_BF16, LTX_MODE_F32})
+        for (int s16 : {0, 1})
+            for (int N : {48, 4112, 8200, 16400})
+                for (int M : {1, 3, 5, 16, 17, 32, 33, 64}) {
+                    fake::log.clear();
+                    CHECK(ltx_op_linear_q4(f.c, ptr(0), (const uint8_t*)ptr(1), ptr(2), s16, nullptr, ptr(4), 1, M, N, 4736, 0,
+                                           mode, nullptr),
+                          "%s", ltx_last_error(f.c));
+                    CHECK(fake::log.size() == 1, "%zu", fake::log.size());
+                    names.insert(fake::log[0].name);
+                }
+    for (const char* form : {"f16", "bf16", "f32", "f32p"})
+        for (const char* scale : {"s16", "s32"})
+            for (int mt : {1, 2})
+                for (int nt : {1, 2, 4}) {
+                    if (mt == 2 && form[0] == 'f' && form[1] == '3') continue;  // mode F32: 16 rows
+                    const std::string name = std::string("ltx_linear_q4_") + form + "_" + scale + "_" + std::to_string(mt) +
+                                             "_" + std::to_string(nt);
+                    CHECK(names.erase(name) == 1, "%s", name.c_str());
+                }
+    CHECK(names.empty(), "%s", names.begin()->c_str());
+}
+
 // The index arithmetic on arrays of any contents: what a kernel would read and
 // write stays inside what the call names, and the items fit the grid.
 static void index_bounds(unsigned seed) {
@@ -437,6 +465,8 @@ int main(int argc, char** argv) {
         row_limit();
     else if (cmd == "alignment")
         alignment();
+    else if (cmd == "linear_forms")
+        linear_forms();
     else if (cmd == "index")
         index_bounds(std::atoi(argv[2]));
     else

@@ -64,6 +64,10 @@ def test_alignment_of_the_batch(kv_paths):
     kv_paths("alignment")
 
 
+def test_linear_forms(kv_paths):
+    kv_paths("linear_forms")
+
+
 @pytest.mark.parametrize("seed", [1, 2, 3])
 def test_index_arithmetic_stays_inside(kv_paths, seed):
     kv_paths("index", seed)
