@@ -1,6 +1,6 @@
 """The 4-bit key/value cache where it can go wrong beside the shapes of
-test_gpu_kv.py: rows that see no key, scores beyond f32,
-calls beside others."""
+test_gpu_kv.py: rows that see no key, scores beyond f32, subnormal values, long
+sequences whose answer depends on every page, and calls beside others."""
 import math
 
 import numpy as np
@@ -90,6 +90,109 @@ def test_scores_beyond_f32(any_tile):
         want[s.row_start[2]:] = math.nan
         q[:, 0] = q[:, HD] = 2.0 ** 100
         check(s.attend(q, 2, False), want, tol)
+
+
+# ---- the form ---------------------------------------------------------------------
+
+@pytest.mark.parametrize("mode", ["f16", "bf16"])
+def test_subnormal_values(ctx, mode):
+    """Groups of values below the type's smallest normal number, rounded as any other."""
+    say(f"kv subnormal {mode}")
+    dt = MODES[mode][1]
+    step = 2.0 ** -24 if mode == "f16" else 2.0 ** -133
+    per = 1024 if mode == "f16" else 128  # subnormals are 0 .. per - 1 times step
+    g = torch.Generator().manual_seed(2)
+    rows = []
+    for top in (1, 2, 3, 5, per // 4, per // 2, per - 1, 2 * per, 8 * per):
+        x = torch.randint(-top, top + 1, (HD,), generator=g).double()
+        x[::32] = top
+        rows.append(x * step)
+    rows.append(torch.arange(HD).double() * (per // HD) * step)
+    x = torch.stack(rows).to(dt)  # exact
+    assert torch.equal(x[:8].double(), torch.stack(rows[:8]))
+    n = x.shape[0]
+    s = Setup(ctx, mode, 1, [n], [n], kv=(x[:, None], x.flip(0)[:, None]))
+    k, v = torch.empty(2, n, HD, dtype=s.dt, device="cuda")
+    ctx.kv_read(s.cache, s.batch, k, v)
+    assert np.array_equal(k.double().cpu().numpy(), s.kx.reshape(n, HD))
+    assert np.array_equal(v.double().cpu().numpy(), s.vx.reshape(n, HD))
+    assert (s.kx != 0).any()
+
+
+# ---- long sequences: every page counts ----------------------------------------------
+
+def _unsplit(s, q, heads, causal):
+    """A captured call without a workspace: no split."""
+    dev, out = q.cuda(), torch.full((s.total, heads * HD), 7.0, dtype=s.dt, device="cuda")
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        s.ctx.kv_attention(s.cache, s.batch, dev, out, heads, causal=causal)
+    for _ in range(2):
+        out.fill_(7)
+        graph.replay()
+        torch.cuda.synchronize()
+    return out
+
+
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("mode,rows,keys", [
+    ("f16", [1], [9000]), ("bf16", [1], [28672]), ("f16", [1, 2], [28671, 500]), ("f16", [70], [9001]),
+    ("bf16", [300], [28600]), ("f16", [1, 1, 90], [17, 28672, 12345]),
+])
+def test_every_page_of_equal_scores(any_tile, mode, rows, keys, causal):
+    """q = 0: every weight is 1. The keys of page p have one value, 2^(p / 128) in dim p %
+    128, so a page that is left out, taken twice or in the wrong place changes a dim of the
+    output by a fifteenth at least. All sums are whole numbers below 2^24, exact in f32; a
+    division, a product (2^-24 and 2^-23) and the output's rounding remain."""
+    ctx = any_tile
+    say(f"kv every page {mode} {rows} {keys} causal={causal}")
+    total = sum(keys)
+    v = torch.zeros(total, 1, HD)
+    at = np.concatenate([np.arange(k) for k in keys])
+    page = at // PAGE
+    assert page.max() < 512
+    v[np.arange(total), 0, page % HD] = torch.tensor(2.0 ** (page // HD)).float()
+    k = torch.randn(total, 1, HD, generator=torch.Generator().manual_seed(1))
+    s = Setup(ctx, mode, 1, rows, keys, kv=(k, v))
+    assert np.array_equal(s.vx.reshape(total, HD), v.reshape(total, HD).double().numpy())
+    want = []
+    for b, (n, L) in enumerate(zip(rows, keys)):
+        sums = np.cumsum(s.vx[s.start[b]:s.start[b + 1], 0], 0)
+        seen = L - n + 1 + np.arange(n) if causal else np.full(n, L)
+        want.append(sums[seen - 1] / seen[:, None])
+    want = np.repeat(np.concatenate(want)[:, None], 2, 1).reshape(s.total, -1)
+    tol = (torch.finfo(s.dt).eps / 2 + 2.0 ** -21) * want + (2.0 ** -25 if mode == "f16" else 0)
+    q = torch.zeros(s.total, 2 * HD, dtype=s.dt)
+    check(s.attend(q, 2, causal), want, tol)
+    check(_unsplit(s, q, 2, causal), want, tol)
+
+
+@pytest.mark.parametrize("mode", ["f16", "bf16"])
+@pytest.mark.parametrize("keys", [9000, 28672])
+def test_every_page_by_its_own_query(any_tile, mode, keys):
+    """A row a page, whose q is 16 times the signs of one key there: its score is 181 and
+    every other one at least 80 below it (checked), so all but that key have weight 0 and
+    the output is that key's v, exactly: a code of the page's number."""
+    ctx = any_tile
+    say(f"kv page by query {mode} {keys}")
+    n = -(-keys // PAGE)
+    g = torch.Generator().manual_seed(keys)
+    sign = torch.randint(0, 2, (n, HD), generator=g).float() * 2 - 1
+    cross = (sign @ sign.T).fill_diagonal_(0).abs().max().item()
+    assert 16 * (HD - cross) / math.sqrt(HD) > 80
+    key = torch.arange(n) * PAGE + torch.randint(0, PAGE, (n,), generator=g)
+    key = key.clamp_max(keys - 1)
+    k, v = torch.zeros(2, keys, 1, HD)
+    k[key, 0] = sign
+    v[:, 0] = 1.5
+    code = ((torch.arange(n)[:, None] >> (torch.arange(HD) % 9)) & 1).float() * 2 + 1
+    v[key, 0] = code * torch.where(torch.arange(HD) % 2 == 0, 1.0, -1.0)
+    s = Setup(ctx, mode, 1, [n], [keys], kv=(k, v))
+    q = (16 * sign).to(s.dt)
+    want = v[key, 0].double().numpy()
+    check(s.attend(q, 1, False), want, np.zeros_like(want))
+    check(_unsplit(s, q, 1, False), want, np.zeros_like(want))
 
 
 # ---- calls beside others ------------------------------------------------------------
