@@ -452,6 +452,13 @@ __device__ __forceinline__ void kv_mask(f32x4 (&s)[4], int p, int mine, int h) {
         for (int i = 0; i < 4; i++) s[t][i] = kv_select((left - (16 * t + i + 1)) >> 31, s[t][i], 0xff800000u);
 }
 
+// Weights are formed and summed times 2^this (a factor that the division by their sum
+// takes out again): f16's smallest number is then 2^-31 of the weight of a column's
+// maximum, not 2^-24, and a maximum that is behind by 2^8 still leaves them below its
+// largest. At 200,000 keys of weight 2^-25 nothing of them was left without.
+template <typename T>
+constexpr float kv_up = __is_same(T, _Float16) ? 7.f : 0.f;
+
 // Online softmax of a page for a column: its scores -> weights (16-bit pairs), moved
 // maximum, sum of the rounded weights. True: some column's maximum moved, and its
 // sums are to be multiplied by corr.
@@ -472,7 +479,7 @@ __device__ __forceinline__ bool kv_softmax(const f32x4 (&s)[4], float C, float& 
         m = mn;
         l *= corr;
     }
-    const float mz = m == -__builtin_inff() ? 0.f : m;
+    const float mz = (m == -__builtin_inff() ? 0.f : m) - kv_up<T>;
 #pragma unroll
     for (int t = 0; t < 4; t++) {
         float e[4];
@@ -894,6 +901,7 @@ __device__ __forceinline__ void kv_attn_rows(const LtxKvAttnArgs& a) {
         };
         // scores -> weights with maximum mc, and their sum
         auto weights = [&](int q, float mc) {
+            mc -= kv_up<T>;
             float sum = 0.f;
 #pragma unroll
             for (int c = 0; c < 2; c++) {
@@ -925,10 +933,10 @@ __device__ __forceinline__ void kv_attn_rows(const LtxKvAttnArgs& a) {
 #pragma unroll
             for (int q = 0; q < NQ; q++) {
                 // weights with the maximum so far; only where a column's sum of them is
-                // beyond 2^8 (as it is before it has had a score: m is -inf) the page's
+                // beyond 2^8 of it (as before it has had a score: m is -inf) the page's
                 // maximum is taken, m moved, and the weights formed again
                 float sum = weights(q, m[q]);
-                if (__builtin_amdgcn_ballot_w64(!(sum <= 256.f)) != 0) {
+                if (__builtin_amdgcn_ballot_w64(!(sum <= (kv_up<T> ? 32768.f : 256.f))) != 0) {
                     float mx = s[q][0][0];
 #pragma unroll
                     for (int x = 0; x < 4; x++)

@@ -195,6 +195,35 @@ def test_every_page_by_its_own_query(any_tile, mode, keys):
     check(_unsplit(s, q, 1, False), want, np.zeros_like(want))
 
 
+@pytest.mark.parametrize("mode,rows,keys", [("f16", 1, 200000), ("f16", 150, 60000), ("bf16", 1, 200000)])
+def test_many_small_weights(any_tile, mode, rows, keys):
+    """One key whose score is 25.25 (in powers of two) above all others, which share the
+    rest: in f16 their weights are below its smallest number where that key's is 1, and
+    together they are 6.7e-3 of the result. f16 weights are held times 2^7: their rounding is
+    off by 2^-25 / 2^7 at most. bf16's range has room."""
+    ctx = any_tile
+    say(f"kv small weights {mode} {keys}")
+    k, v = torch.zeros(2, keys, 1, HD)
+    at = keys // 3
+    k[at, 0, 0] = 1.0
+    v[:, 0] = 1.0
+    v[at] = 0
+    s = Setup(ctx, mode, 1, [rows], [keys], kv=(k, v))
+    gap = 25.25
+    q = torch.zeros(rows, HD, dtype=s.dt)
+    q[:, 0] = gap * math.sqrt(HD) / 1.4426950408889634
+    score = q[0, 0].item() / math.sqrt(HD) * 1.4426950408889634  # as rounded
+    rest = (keys - 1) * 2.0 ** -score
+    want = np.full((rows, HD), rest / (1 + rest))
+    u = torch.finfo(s.dt).eps / 2
+    # exponents and sums in f32: 2^-22 of the exponent, 2^-24 a key
+    tol = (2 * u + 2.0 ** -22 * (score + 2) + 2 * keys * 2.0 ** -24) * want
+    if mode == "f16":
+        tol = tol + 2 * keys * 2.0 ** -32
+        assert (tol < 0.06 * want).all()
+    check(s.attend(q, 1, False), want, tol)
+
+
 # ---- calls beside others ------------------------------------------------------------
 
 def test_a_cache_made_inside_a_capture(block0):
