@@ -13,7 +13,7 @@ pytestmark = pytest.mark.gpu
 
 from ltx_amd import runtime as rt  # noqa: E402
 from ltx_amd import synth  # noqa: E402
-from test_gpu_kv import HD, MODES, PAGE, Setup, any_tile, check, ints  # noqa: E402, F401
+from test_gpu_kv import HD, MODES, PAGE, Setup, any_tile, check, held, ints  # noqa: E402, F401
 
 
 # ---- rows that see no key ---------------------------------------------------------
@@ -303,3 +303,73 @@ def test_a_pool_that_does_not_fit(ctx):
     assert c.faults() == 0
     c.free()
     assert abs(torch.cuda.mem_get_info()[0] - before) < 64 << 20
+
+
+@pytest.mark.parametrize("mode", ["f16", "bf16"])
+def test_captured_step_with_values_that_are_not_finite(any_tile, mode):
+    """A captured write and attention: rows that hold a NaN make the rows that see them
+    NaN in that replay, and not in the next, which holds others in their place; the page's
+    flag, set by the write, is seen by the attention behind it."""
+    ctx = any_tile
+    say(f"kv captured not finite {mode}")
+    rows, keys = [3, 100], [200, 130]
+    s = Setup(ctx, mode, 2, rows, keys, seed=15)
+    g = s.g
+    q = s.queries(4).cuda()
+    k, v, out = (torch.zeros(s.total, w, dtype=s.dt, device="cuda") for w in (2 * HD, 2 * HD, 4 * HD))
+    work = torch.empty(max(16, ctx.kv_attention_workspace(s.cache, s.batch, 4)), dtype=torch.uint8, device="cuda")
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        ctx.kv_write(s.cache, s.batch, k, v)
+        ctx.kv_attention(s.cache, s.batch, q, out, 4, work=work)
+    for bad in (None, (1, HD + 3), (50, 7), None, (102, 0)):
+        new = [torch.randn(s.total, 2 * HD, generator=g).to(s.dt) for _ in range(2)]
+        if bad:
+            new[1][bad] = math.nan
+        k.copy_(new[0])
+        v.copy_(new[1])
+        for x, t in ((s.kx, new[0]), (s.vx, new[1])):
+            h = held(t.reshape(s.total, 2, HD), mode)
+            for b, (n, L) in enumerate(zip(rows, keys)):
+                x[s.start[b] + L - n:s.start[b] + L] = h[s.row_start[b]:s.row_start[b] + n]
+        out.fill_(5)
+        graph.replay()
+        torch.cuda.synchronize()
+        want, tol = s.want(q.cpu(), 4, True)
+        assert np.isnan(want).any() == (bad is not None)
+        check(out, want, tol)
+
+
+def test_sequences_that_share_pages(any_tile):
+    """A common beginning held once: two sequences whose tables name the same pages."""
+    ctx = any_tile
+    say("kv shared pages")
+    s = Setup(ctx, "f16", 2, [2, 70, 1], [300, 330, 64], seed=16)
+    s.pages[1, :4] = s.pages[0, :4]
+    s.pages[2, 0] = s.pages[0, 2]
+    for x in (s.kx, s.vx):
+        x[s.start[1]:s.start[1] + 256] = x[:256]
+        x[s.start[2]:s.start[2] + 64] = x[128:192]
+    for causal in (True, False):
+        q = s.queries(4)
+        want, tol = s.want(q, 4, causal)
+        check(s.attend(q, 4, causal), want, tol)
+
+
+def test_a_workspace_of_the_other_form(ctx):
+    """Sized without row_start and used with it, and the other way round."""
+    say("kv workspace forms")
+    n = 16
+    s = Setup(ctx, "bf16", 8, [1] * n, [100 * i + 1 for i in range(n)], seed=17)
+    q = s.queries(32)
+    want, tol = s.want(q, 32, True)
+    wide = torch.full((n, 128), -1, dtype=torch.int32, device="cuda")
+    wide[:, :s.pages.shape[1]] = s.pages
+    forms = [rt.KvBatch(s.lens, wide), rt.KvBatch(s.lens, wide, ints(range(n + 1)), n)]
+    for a, b in (forms, forms[::-1]):
+        size = ctx.kv_attention_workspace(s.cache, a, 32)
+        assert size > 0
+        work = torch.full((size,), 255, dtype=torch.uint8, device="cuda")
+        s.batch = b
+        check(s.attend(q, 32, True, work=work), want, tol)
