@@ -297,7 +297,9 @@ int ltx_op_linear_q4(ltx_ctx* ctx, const void* a, const uint8_t* q, const void* 
  * ties to the even code, beyond 6 to 6. With A the group's largest magnitude, e =
  * floor(log2 A) - 2, one more where A > 7 2^e, limited to -23 .. 13 (mode F16) or
  * -125 .. 125 (BF16), so that what a code stands for is a number of the mode's
- * type. A group with a value that is not finite reads back as NaN.
+ * type. A group with a value that is not finite reads back as NaN. (A page that has held
+ * one takes a longer way through the attention from then on, with the same results: 5 to
+ * 30 %. Only a new cache forgets it.)
  *
  * `mode` (LTX_MODE_F16 or LTX_MODE_BF16) is the type of k, v, q and the outputs of
  * every call on the cache. Pages start as zeros. */
@@ -320,7 +322,9 @@ uint64_t ltx_kv_cache_bytes(const ltx_kv_cache* cache);
  * pool is not followed: the row is not written, or read as zeros, or the page's
  * keys take no part in the attention, and it is counted (ltx_kv_cache_faults).
  * The host checks what it can see: nseq and max_pages (at most 2^24) positive, rows
- * not negative (0: nothing to do; below 2^24 for the attention, at most 2^28 - 16 else), pointers
+ * not negative (0: nothing to do; below 2^24 for the attention, at most 2^28 - 16 else; the attention also refuses
+ * 2^22 / kv_heads tiles and more, a tile being 16 columns or more of a sequence's rows
+ * times the query heads of a cached head), pointers
  * (the arrays and glog on 4 bytes), heads, and that rows of k, v, q and out start on 16
  * bytes with strides (in elements) that are multiples of 8 and not shorter than a row. */
 typedef struct ltx_kv_batch {

@@ -437,7 +437,7 @@ __device__ __forceinline__ void kv_seen(const LtxKvBatchArgs& a, int b, int p0, 
 __device__ __forceinline__ float kv_factor(float m, float lt, float g) { return m == -__builtin_inff() ? 0.f : g / lt; }
 
 // x where m is 0, y where it is ~0 (bit operations: as compares and selects, the
-// rare paths below took more scalar registers than there are, and spilled)
+// rare paths below took more scalar registers than there are, in the page loop)
 __device__ __forceinline__ float kv_select(int m, float x, uint32_t y) {
     return __builtin_bit_cast(float, (__builtin_bit_cast(uint32_t, x) & ~(uint32_t)m) | (y & (uint32_t)m));
 }
@@ -460,7 +460,11 @@ template <typename T>
 constexpr float kv_up = __is_same(T, _Float16) ? 7.f : 0.f;
 
 // Online softmax of a page for a column: its scores -> weights (16-bit pairs), moved
-// maximum, sum of the rounded weights. True: some column's maximum moved, and its
+// maximum, sum of the rounded weights. The weights are rounded to the cache's 16-bit type
+// because the matrix instructions take them so; with f32 weights, as two planes, V's half
+// of the products would be done twice. It costs 1.9e-4 of the result in f16 and 1.3e-3 in
+// bf16 (relative RMS), beside 2.1e-4 and 1.6e-3 of the output's own rounding; the sum is of
+// the rounded ones, so that equal values of V come back as they are. True: some column's maximum moved, and its
 // sums are to be multiplied by corr.
 template <typename T>
 __device__ __forceinline__ bool kv_softmax(const f32x4 (&s)[4], float C, float& m, float& l, uint32_t (&pw)[4][2],
@@ -535,7 +539,8 @@ __device__ __forceinline__ void kv_v_pair(const uint32_t (&x)[8], const uint32_t
 #define KV_WAVES 8  // (the lines below that take the waves' sums apart count on 512 threads)
 
 // Few columns: a workgroup takes 16 columns and a run of pages, a page a wave in
-// turn, everything in registers. Scores transposed, S^T = K . Q^T, and O^T = V^T .
+// turn, everything in registers (in f16 all 256; three more values a lane wait in scratch
+// while the page loop runs, which does not touch them). Scores transposed, S^T = K . Q^T, and O^T = V^T .
 // P^T (v_mfma_f32_16x16x32), so that a column's statistics lie in the four lanes
 // l % 16 + 16 j and P^T comes straight from the S^T accumulators. The orders in
 // which dims and keys are summed are free: lane (r, h) = (l % 16, l / 16) holds

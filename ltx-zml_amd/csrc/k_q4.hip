@@ -137,8 +137,8 @@ __device__ __forceinline__ void q4_split(f32x4 x, u32x2 (&p)[3]) {
 // c ^ r / 2, free of conflicts. AW groups of q and AA of a are in flight.
 // Measured back to back in a graph, where an empty launch takes 3.8 us: one row 5.7
 // us (4,096 x 4,096), 10.4 (16,384 x 4,096), 10.4 (4,096 x 16,384); 32 rows of
-// 16,384 x 4,096 13.9 us (17.5 with NT = 2, 21.1 with MT = 1); mode F32, one row of
-// 4,096 x 16,384 11.4 us, five 16.4 (without PACK 15.9 and 20.2: three times the LDS
+// 16,384 x 4,096 14.3 us (bf16; 17.5 with NT = 2, 21.1 with MT = 1); mode F32, one row of
+// 4,096 x 16,384 11.4 us, five 15.7 (without PACK 15.9 and 20.2: three times the LDS
 // reads and products; what five rows take beyond one is every workgroup's reading and
 // splitting of all of them).
 template <typename T, int PLANES, bool PACK, bool S16, int MT, int NT, int AW, int AA, int EARLY>
