@@ -284,6 +284,39 @@ int ltx_op_linear_q4(ltx_ctx* ctx, const void* a, const uint8_t* q, const void* 
                      const float* bias, void* y, int out_f32, int M, int N, int K, int gelu, int mode,
                      void* stream);
 
+/* No counterpart in the reference. Microscaled 4-bit operands: rows [rows][K], K a
+ * multiple of 128, in the form of the 4-bit cache below (groups of 32 along k share a
+ * power of two 2^e, values are e2m1 numbers, the same rule for e; mode F32 has the limits
+ * of BF16). q [rows][K / 2]: two codes a byte, the even k in the low nibble. scales
+ * [K / 128][rows][4]: for each 128 of k, of all rows in turn, the four scale codes e + 127
+ * (255: a group that held a value that is not finite; it is NaN in every use). Files with
+ * [rows][K / 32] scales come into this order by a transposition of 4-byte words.
+ *
+ * ltx_op_mx4_quantise: x [rows][K] of the mode's type (F16, BF16 or F32), rows ldx elements
+ * apart, into the form. ltx_op_mx4_values: what the form stands for, rounded to the mode's
+ * type (exact in the mode that it came from, and in F32; beyond f16's largest: infinity).
+ * rows may be 0. Refused: K not a positive multiple of 128 or above 2^23, x or q not on 16
+ * bytes, scales not on 4, rows of x not on 16 bytes or shorter than K, an unknown mode,
+ * rows (K / 128 + 8) from 2^29 on. */
+int ltx_op_mx4_quantise(ltx_ctx* ctx, const void* x, int64_t ldx, uint8_t* q, uint8_t* scales, int rows, int K,
+                        int mode, void* stream);
+int ltx_op_mx4_values(ltx_ctx* ctx, const uint8_t* q, const uint8_t* scales, void* y, int64_t ldy, int rows, int K,
+                      int mode, void* stream);
+
+/* No counterpart in the reference. The linear of two operands in that form: y[M][N] =
+ * a[M][K] . w[N][K]^T (+ bias) with optional GELU-tanh; f32 sums of exact products. a and
+ * a_scales: M rows in the form, q and scales: N rows (any scale codes; they need not come
+ * from ltx_op_mx4_quantise). a_scales NULL: a holds at most 64 rows of 16-bit values of the
+ * mode, [M][K], which the call quantises on its way, with the bits of
+ * ltx_op_mx4_quantise. y f32 (out_f32, and always in mode F32) or 16-bit. A group that is
+ * NaN makes its row of y, or column, NaN. No scratch: calls may overlap and be captured.
+ * Refused: M, N or K not positive, K no multiple of 128 or above 2^23, a or q not on 16
+ * bytes, scales not on 4, bias or y not aligned to their types, an unknown mode, mode F32
+ * with a in values, M or N times (K / 128 + 8) from 2^29 on, N from 2^27, more than 2^23
+ * tiles. */
+int ltx_op_linear_mx4(ltx_ctx* ctx, const void* a, const uint8_t* a_scales, const uint8_t* q, const uint8_t* scales,
+                      const float* bias, void* y, int out_f32, int M, int N, int K, int gelu, int mode, void* stream);
+
 /* ---- a key/value cache in 4 bits ---------------------------------------- */
 
 /* No counterpart in the reference: for streamed generation, where the keys and

@@ -11,7 +11,7 @@
 extern "C" {
 extern const unsigned char ltx_co_k_gemm[], ltx_co_k_gemm_s4[], ltx_co_k_gemm_f3[],
     ltx_co_k_gemm_x4h[], ltx_co_k_gemm_q8h[], ltx_co_k_attn[], ltx_co_k_norm[], ltx_co_k_f32[],
-    ltx_co_k_core[], ltx_co_k_kv[], ltx_co_k_q4[];
+    ltx_co_k_core[], ltx_co_k_kv[], ltx_co_k_q4[], ltx_co_k_mx4[], ltx_co_k_gemm_mx4[];
 }
 
 namespace ltx {
@@ -241,6 +241,10 @@ int ltx_init(int device, ltx_ctx** out) {
             c->side_early = std::strcmp(e, "off") == 0 ? 0 : std::strcmp(e, "all") == 0 ? 2 : 1;
         if (const char* e = std::getenv("LTX_KV_TILE"))  // 16, 128 or 256 columns of the 4-bit cache's attention
             c->kv_tile = std::strcmp(e, "16") == 0 ? 16 : std::strcmp(e, "128") == 0 ? 128 : std::strcmp(e, "256") == 0 ? 256 : 0;
+        if (const char* e = std::getenv("LTX_MX4_TILE")) {  // 16, 64, 128 or 256 rows of the 4-bit linear's tiles
+            const int t = std::atoi(e);
+            c->mx4_tile = t == 16 || t == 64 || t == 128 || t == 256 ? t : 0;
+        }
         if (const char* e = std::getenv("LTX_ATTN_VARIANT")) {
             c->attn_pp = std::strcmp(e, "w8") != 0;
             c->attn_kv = c->attn_pp && std::strcmp(e, "pp") != 0;
@@ -251,7 +255,8 @@ int ltx_init(int device, ltx_ctx** out) {
         for (auto& e : c->marks) HIPC(hipEventCreateWithFlags(&e, hipEventDisableTiming | hipEventDisableSystemFence));
         for (const unsigned char* co :
              {ltx_co_k_gemm, ltx_co_k_gemm_s4, ltx_co_k_gemm_f3, ltx_co_k_gemm_x4h, ltx_co_k_gemm_q8h, ltx_co_k_attn,
-              ltx_co_k_norm, ltx_co_k_f32, ltx_co_k_core, ltx_co_k_kv, ltx_co_k_q4}) {
+              ltx_co_k_norm, ltx_co_k_f32, ltx_co_k_core, ltx_co_k_kv, ltx_co_k_q4, ltx_co_k_mx4,
+              ltx_co_k_gemm_mx4}) {
             hipModule_t m;
             HIPC(hipModuleLoadData(&m, co));
             c->modules.push_back(m);

@@ -14,33 +14,8 @@
 // they turn into NaN.
 #include <type_traits>
 
-#include "ltx_device.h"
+#include "ltx_fp4.h"
 #include "ltx_kv_index.h"
-
-template <typename T>
-struct Fp4;
-template <>
-struct Fp4<_Float16> {
-    static constexpr int lo = 127 - 23, hi = 127 + 13;
-    template <int B>
-    static __device__ __forceinline__ uint32_t pair(uint32_t w, float s) {
-        return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, s, B));
-    }
-};
-template <>
-struct Fp4<__bf16> {
-    static constexpr int lo = 127 - 125, hi = 127 + 125;
-    template <int B>
-    static __device__ __forceinline__ uint32_t pair(uint32_t w, float s) {
-        return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, s, B));
-    }
-};
-
-// The scale whose code is byte i of w, as the conversions read it: the code at
-// bits 30 .. 23 (the bits around it take no part).
-__device__ __forceinline__ float scale_of(uint32_t w, int i) {
-    return __builtin_bit_cast(float, i == 0 ? w << 23 : i == 1 ? w << 15 : i == 2 ? w << 7 : w >> 1);
-}
 
 // ---- the batch ----------------------------------------------------------------
 // A sequence that is the same for all lanes, in scalar registers
@@ -89,52 +64,7 @@ __device__ __forceinline__ uint8_t* kv_place(const LtxKvBatchArgs& a, int row, i
     return a.data + kv_block(a, page, 0);
 }
 
-__device__ __forceinline__ uint32_t quad_max(uint32_t x) {  // over lanes 4 j .. 4 j + 3
-    x = max(x, (uint32_t)__builtin_amdgcn_mov_dpp((int)x, 0xB1, 0xf, 0xf, true));
-    return max(x, (uint32_t)__builtin_amdgcn_mov_dpp((int)x, 0x4E, 0xf, 0xf, true));
-}
-
-// Eight consecutive dims of a row -> their codes, and the scale code of their
-// group (four lanes hold its 32 dims).
-template <typename T>
-__device__ __forceinline__ uint32_t kv_encode(u32x4 w, uint32_t& code) {
-    float x[8];
-    uint32_t top = 0;
-#pragma unroll
-    for (int e = 0; e < 8; e++) {
-        x[e] = Op<T>::to_f32((uint16_t)(w[e >> 1] >> (16 * (e & 1))));
-        top = max(top, __builtin_bit_cast(uint32_t, x[e]) & 0x7fffffffu);
-    }
-    top = quad_max(top);
-    const int e = (int)(top >> 23) - 2 + ((top & 0x7fffffu) > 0x600000u ? 1 : 0);
-    code = top >= 0x7f800000u ? 255u : (uint32_t)min(max(e, Fp4<T>::lo), Fp4<T>::hi);
-    const float s = __builtin_bit_cast(float, code << 23);  // (255: codes of any value)
-    uint32_t q = 0;
-    q = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(q, x[0], x[1], s, 0);
-    q = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(q, x[2], x[3], s, 1);
-    q = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(q, x[4], x[5], s, 2);
-    q = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(q, x[6], x[7], s, 3);
-    return q;
-}
-
-// Dword j of lane i and dword i of lane j change places, over the lanes 4 q + 0 .. 3;
-__device__ __forceinline__ void quad_transpose(u32x4& x) {
-    const bool odd = threadIdx.x & 1, high = threadIdx.x & 2;
-    auto cross = [](bool upper, uint32_t& a, uint32_t& b, auto dpp) {
-        const uint32_t fa = dpp(a), fb = dpp(b);
-        a = upper ? fb : a;
-        b = upper ? b : fa;
-    };
-    uint32_t x0 = x[0], x1 = x[1], x2 = x[2], x3 = x[3];
-    auto one = [](uint32_t v) { return (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0xB1, 0xf, 0xf, true); };
-    auto two = [](uint32_t v) { return (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0x4E, 0xf, 0xf, true); };
-    cross(odd, x0, x1, one);
-    cross(odd, x2, x3, one);
-    cross(high, x0, x2, two);
-    cross(high, x1, x3, two);
-    x = u32x4{x0, x1, x2, x3};
-}
-// and over the lanes l, l + 16, l + 32, l + 48.
+// quad_transpose over the lanes l, l + 16, l + 32, l + 48.
 __device__ __forceinline__ void row_transpose(u32x4& x) {
     auto p = __builtin_amdgcn_permlane32_swap(x[0], x[2], false, false);
     const uint32_t a0 = p[0], a2 = p[1];
@@ -144,12 +74,6 @@ __device__ __forceinline__ void row_transpose(u32x4& x) {
     const uint32_t b0 = p[0], b1 = p[1];
     p = __builtin_amdgcn_permlane16_swap(a2, a3, false, false);
     x = u32x4{b0, b1, p[0], p[1]};
-}
-// x of the lane's place in its quad
-__device__ __forceinline__ uint32_t quad_pick(u32x4 x) {
-    const bool odd = threadIdx.x & 1, high = threadIdx.x & 2;
-    const uint32_t low = odd ? x[1] : x[0], up = odd ? x[3] : x[2];
-    return high ? up : low;
 }
 
 // Rows into the cache and out of it: a wave takes four rows of four heads, 16 lanes of
@@ -211,8 +135,8 @@ __device__ __forceinline__ void kv_rows(const LtxKvRowsArgs& a) {
 #pragma unroll
         for (int e = 0; e < KV_HB; e++) {
             uint32_t c0, c1;
-            qk[e] = kv_encode<T>(wk[e], c0);
-            qv[e] = kv_encode<T>(wv[e], c1);
+            qk[e] = fp4_encode<T>(wk[e], c0);
+            qv[e] = fp4_encode<T>(wv[e], c1);
             ek[e] = c0;
             ev[e] = c1;
         }

@@ -420,6 +420,34 @@ typedef struct {
 // Rows of a (mode F32) whose three planes are 15 of the 16 rows of one tile.
 #define LTX_Q4_PACKED 5
 
+// ---- microscaled 4-bit operands ----------------------------------------------
+// [rows][K] held as q [rows][K / 2], two e2m1 codes a byte (the even k low), and s
+// [K / 128][rows] words: byte g of word (k / 128, row) is the scale code e + 127 of the
+// row's group g of that 128 (255: not a number).
+typedef struct {
+    void* x;            // [rows][K] values, ldx elements apart (written by the way back)
+    uint8_t* q;
+    uint8_t* s;
+    int64_t ldx;
+    int rows, K;
+} LtxMx4RowsArgs;
+
+// y = a . w^T (+ bias, GELU)
+typedef struct {
+    const uint8_t* a;   // codes, or 16-bit rows (the kernels of few rows)
+    const uint8_t* as;
+    const uint8_t* w;
+    const uint8_t* ws;
+    const float* bias;  // [N] or NULL
+    void* y;            // [M][N] f32 or the 16-bit type
+    int M, N, K;
+    int gelu, out_f32;
+    int tiles_m, tiles_n;
+    int wide;           // rows of y start on 16 bytes
+} LtxMx4LinearArgs;
+// Rows of a that the linear of few rows takes in 16 bits.
+#define LTX_MX4_ROWS 64
+
 #ifdef __cplusplus
 }
 #endif

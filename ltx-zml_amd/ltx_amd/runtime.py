@@ -61,6 +61,9 @@ def lib() -> C.CDLL:
         "ltx_op_linear_q8_noalloc": (i32, [vp, vp, vp, vp, i32, vp, vp, i32, i32, i32, i32, i32, i32, vp]),
         "ltx_op_attention": (i32, [vp, vp, vp, vp, vp, vp, i32, i32, i32, vp]),
         "ltx_op_linear_q4": (i32, [vp, vp, vp, vp, i32, vp, vp, i32, i32, i32, i32, i32, i32, vp]),
+        "ltx_op_mx4_quantise": (i32, [vp, vp, i64, vp, vp, i32, i32, i32, vp]),
+        "ltx_op_mx4_values": (i32, [vp, vp, vp, vp, i64, i32, i32, i32, vp]),
+        "ltx_op_linear_mx4": (i32, [vp, vp, vp, vp, vp, vp, vp, i32, i32, i32, i32, i32, i32, vp]),
         "ltx_kv_cache_create": (i32, [vp, i32, i32, i32, C.POINTER(vp)]),
         "ltx_kv_cache_free": (None, [vp, vp]),
         "ltx_kv_cache_bytes": (u64, [vp]),
@@ -412,6 +415,52 @@ class Context:
                                            mode, st), "ltx_op_linear_q4")
         return y
 
+    # ---- microscaled 4-bit operands ----
+    def mx4_quantise(self, x, q, s, mode=MODE_F16, stream=None):
+        """x [rows, K] (rows may be strided) -> codes q uint8 [rows, K / 2] and scales s
+        uint8 [K / 128, rows, 4], which it returns (ltx_op_mx4_quantise)."""
+        st = stream.cuda_stream if stream is not None else _current_stream(self.device)
+        rows, K = self._mx4_rows("mx4_quantise", x, q, s, mode)
+        self._check(lib().ltx_op_mx4_quantise(self.handle, _ptr(x), x.stride(0), _ptr(q), _ptr(s), rows, K, mode, st),
+                    "ltx_op_mx4_quantise")
+        return q, s
+
+    def mx4_values(self, q, s, y, mode=MODE_F16, stream=None):
+        """What codes and scales stand for -> y [rows, K] (ltx_op_mx4_values)."""
+        st = stream.cuda_stream if stream is not None else _current_stream(self.device)
+        rows, K = self._mx4_rows("mx4_values", y, q, s, mode)
+        self._check(lib().ltx_op_mx4_values(self.handle, _ptr(q), _ptr(s), _ptr(y), y.stride(0), rows, K, mode, st),
+                    "ltx_op_mx4_values")
+        return y
+
+    def linear_mx4(self, a, a_s, q, s, bias, y, mode=MODE_F16, gelu=False, stream=None):
+        """a and a_s, q and s: M and N rows as mx4_quantise makes them, or a_s None and a at
+        most 64 rows [M, K] of the mode's type (ltx_op_linear_mx4)."""
+        import torch
+        (M, N), K = y.shape, 2 * q.shape[1]
+        x, f32 = _torch_dtype(mode), torch.float32
+        _mx4_held("linear_mx4", q, s, N, K, self.device)
+        if a_s is not None:
+            _mx4_held("linear_mx4", a, a_s, M, K, self.device)
+        elif not (a.shape == (M, K) and a.dtype == x and a.is_contiguous() and a.get_device() == self.device):
+            raise LtxError(f"linear_mx4: a contiguous a {[M, K]} of the mode's type on the context's device is needed")
+        if not (y.is_contiguous() and (y.dtype == x or y.dtype == f32) and y.get_device() == self.device):
+            raise LtxError("linear_mx4: a contiguous y of the mode's type or f32 on the context's device is needed")
+        if bias is not None and not (bias.shape == (N,) and bias.dtype == f32 and bias.is_contiguous()
+                                     and bias.get_device() == self.device):
+            raise LtxError(f"linear_mx4: bias must be f32 {[N]}, contiguous, on the context's device")
+        st = stream.cuda_stream if stream is not None else _current_stream(self.device)
+        self._check(lib().ltx_op_linear_mx4(self.handle, _ptr(a), _ptr(a_s), _ptr(q), _ptr(s), _ptr(bias), _ptr(y),
+                                            int(y.dtype == f32), M, N, K, int(gelu), mode, st), "ltx_op_linear_mx4")
+        return y
+
+    def _mx4_rows(self, name, x, q, s, mode):
+        rows, K = x.shape
+        if x.dtype != _torch_dtype(mode) or x.stride(1) != 1 or x.get_device() != self.device:
+            raise LtxError(f"{name}: rows of the mode's type on the context's device are needed")
+        _mx4_held(name, q, s, rows, K, self.device)
+        return rows, K
+
     # ---- the 4-bit key/value cache ----
     def kv_cache(self, kv_heads: int, pages: int, mode: int = MODE_F16) -> KvCache:
         h = C.c_void_p()
@@ -556,6 +605,17 @@ def _rows(name: str, batch: KvBatch, cache: KvCache, heads: int, *tensors):
             raise LtxError(f"{name}: tensors on the context's device are needed")
         if t.shape != shape or t.dtype != dt or t.stride(1) != 1:
             raise LtxError(f"{name}: {list(shape)} tensors of the cache's type are needed")
+
+
+def _mx4_held(name: str, q, s, rows: int, K: int, device: int):
+    """Codes [rows, K / 2] and scales [K / 128, rows, 4], uint8."""
+    if K % 128:
+        raise LtxError(f"{name}: K must be a multiple of 128")
+    for t, shape in ((q, (rows, K // 2)), (s, (K // 128, rows, 4))):
+        if t.shape != shape or t.element_size() != 1 or t.is_floating_point() or not t.is_contiguous():
+            raise LtxError(f"{name}: contiguous uint8 tensors {[rows, K // 2]} and {[K // 128, rows, 4]} are needed")
+        if t.get_device() != device:
+            raise LtxError(f"{name}: tensors on the context's device are needed")
 
 
 def _current_stream(device: int) -> int:
