@@ -317,6 +317,40 @@ int ltx_op_mx4_values(ltx_ctx* ctx, const uint8_t* q, const uint8_t* scales, voi
 int ltx_op_linear_mx4(ltx_ctx* ctx, const void* a, const uint8_t* a_scales, const uint8_t* q, const uint8_t* scales,
                       const float* bias, void* y, int out_f32, int M, int N, int K, int gelu, int mode, void* stream);
 
+/* ---- rotary positions on several axes ----------------------------------- */
+
+/* No counterpart in the reference as an operator of its own (the block forward's q and k
+ * norm and RoPE, ltx/block.zig:32-34, 69-77, 214-226, with the positions in place of host
+ * tables): for q and k between a projection and the cache below. A plan says what turns:
+ * pair j (values j and j + 64) of its head h turns by freq[h][j] * position on axis[h][j] +
+ * phase[h][j] radians. Host arrays [heads][64]; phase and axis may be NULL (zeros). heads: 1
+ * where all heads turn alike, or any divisor of the heads it is used with, which then share
+ * a head of the plan in runs. axes 1 .. 8; frequencies and phases finite. */
+typedef struct ltx_rope ltx_rope;
+int ltx_rope_create(ltx_ctx* ctx, int heads, int axes, const double* freq, const double* phase, const int32_t* axis,
+                    ltx_rope** out);
+/* The plan of this model's blocks (ltx_rope_tables): 32 heads; positions are the midpoints
+ * of a token's time, height and width ranges, in the grid's units. */
+int ltx_rope_create_grid(ltx_ctx* ctx, ltx_rope** out);
+/* Waits for the device's work; call it before ltx_destroy of the context. */
+void ltx_rope_free(ltx_ctx* ctx, ltx_rope* rope);
+
+/* q [rows][heads * 128] and k [rows][kv_heads * 128] (NULL: q alone), values of the mode's
+ * type, rows ldq .. elements apart (slices of fused q|k|v rows will do), into q_out and
+ * k_out, which may be q and k themselves (same address and stride), and overlap nothing
+ * else. q_norm, k_norm [heads * 128] f32 or NULL: each row is first divided by sqrt(mean of
+ * its squares + eps) and multiplied by these weights. Then head h's pairs turn as head h /
+ * (heads / plan heads) of the plan says, by pos [rows][axes] f64 (device memory): exact far
+ * into a stream, where f32 is not, for angles below 2^51 quarter turns. -pos turns back
+ * where phases are 0. f32 sums and products, one rounding to the mode's type, to infinity
+ * beyond its largest; a row with a position that is not finite is NaN in the pairs on its
+ * axis. rows may be 0. Refused: heads no multiples of the plan's, rows of q, k or their
+ * outputs not on 16 bytes or shorter than their heads, pos not on 8 bytes, weights not on
+ * 16, an unknown mode, a plan of another device. */
+int ltx_op_qk_rope(ltx_ctx* ctx, const ltx_rope* rope, const double* pos, int rows, const void* q, int64_t ldq,
+                   const float* q_norm, void* q_out, int64_t ldqo, int heads, const void* k, int64_t ldk,
+                   const float* k_norm, void* k_out, int64_t ldko, int kv_heads, float eps, int mode, void* stream);
+
 /* ---- a key/value cache in 4 bits ---------------------------------------- */
 
 /* No counterpart in the reference: for streamed generation, where the keys and

@@ -28,8 +28,8 @@ CEILING = PKG / "mfma_ceiling"
 INCLUDE = PKG.parent / "include"
 ROCM = pathlib.Path(os.environ.get("ROCM_PATH", "/opt/rocm"))
 KERNELS = ["k_gemm", "k_gemm_s4", "k_gemm_f3", "k_gemm_x4h", "k_gemm_q8h", "k_attn", "k_norm", "k_f32", "k_core",
-           "k_kv", "k_q4", "k_mx4", "k_gemm_mx4"]
-HOST = ["ltx_runtime", "ltx_forward", "ltx_weights", "ltx_rope", "ltx_loader", "ltx_core", "ltx_kv", "ltx_q4", "ltx_mx4",
+           "k_kv", "k_q4", "k_mx4", "k_gemm_mx4", "k_rope"]
+HOST = ["ltx_runtime", "ltx_forward", "ltx_weights", "ltx_rope", "ltx_loader", "ltx_core", "ltx_kv", "ltx_q4", "ltx_mx4", "ltx_qk_rope",
         "sha256"]
 
 HIPCC_FLAGS = [

@@ -245,6 +245,10 @@ uint16_t f32_to_f16_bits(float f);
 float bf16_bits_to_f32(uint16_t b);
 float f16_bits_to_f32(uint16_t h);
 
+// The block's rotary positions: frequency k of 682, and the axes' largest positions.
+double rope_frequency(int k);
+constexpr double kRopeMaxPos[3] = {20.0, 2048.0, 2048.0};
+
 // Device scratch of the isolated int8 GEMM: the weights as bytes q + 128
 // (N * K bytes) and the scale words [K/128][N] (4 N K / 128 bytes).
 struct LinearScratch {

@@ -12,32 +12,30 @@
 
 #include "ltx_internal.hpp"
 
+namespace ltx {
 namespace {
-
 constexpr int kNF = 682;
-constexpr double kMaxPos[3] = {20.0, 2048.0, 2048.0};
-
-void freqs(double* f) {
-    const double step = 1.0 / (double)(kNF - 1);
-    for (int k = 0; k < kNF; k++) {
-        const double x = k == kNF - 1 ? 1.0 : (double)k * step;  // numpy linspace
-        f[k] = (double)(float)(std::pow(10000.0, x) * (M_PI / 2.0));
-    }
 }
 
-}  // namespace
+double rope_frequency(int k) {
+    const double step = 1.0 / (double)(kNF - 1);
+    const double x = k == kNF - 1 ? 1.0 : (double)k * step;  // numpy linspace
+    return (double)(float)(std::pow(10000.0, x) * (M_PI / 2.0));
+}
+
+}  // namespace ltx
 
 extern "C" int ltx_rope_tables(const float* grid, int T, float* cos_out, float* sin_out, int graph_layout) {
     try {
         if (!grid || !cos_out || !sin_out || T <= 0) throw ltx::Error("ltx_rope_tables: bad arguments");
-        double f[kNF];
-        freqs(f);
+        double f[ltx::kNF];
+        for (int k = 0; k < ltx::kNF; k++) f[k] = ltx::rope_frequency(k);
         auto work = [&](int t0, int t1) {
             for (int t = t0; t < t1; t++) {
                 double arg[3];
                 for (int a = 0; a < 3; a++) {
                     const double s0 = grid[((size_t)a * T + t) * 2], s1 = grid[((size_t)a * T + t) * 2 + 1];
-                    arg[a] = (((s0 + s1) / 2.0) / kMaxPos[a]) * 2.0 - 1.0;
+                    arg[a] = (((s0 + s1) / 2.0) / ltx::kRopeMaxPos[a]) * 2.0 - 1.0;
                 }
                 for (int h = 0; h < LTX_H; h++)
                     for (int k = 0; k < 64; k++) {

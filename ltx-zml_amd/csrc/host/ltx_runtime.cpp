@@ -11,7 +11,8 @@
 extern "C" {
 extern const unsigned char ltx_co_k_gemm[], ltx_co_k_gemm_s4[], ltx_co_k_gemm_f3[],
     ltx_co_k_gemm_x4h[], ltx_co_k_gemm_q8h[], ltx_co_k_attn[], ltx_co_k_norm[], ltx_co_k_f32[],
-    ltx_co_k_core[], ltx_co_k_kv[], ltx_co_k_q4[], ltx_co_k_mx4[], ltx_co_k_gemm_mx4[];
+    ltx_co_k_core[], ltx_co_k_kv[], ltx_co_k_q4[], ltx_co_k_mx4[], ltx_co_k_gemm_mx4[],
+    ltx_co_k_rope[];
 }
 
 namespace ltx {
@@ -256,7 +257,7 @@ int ltx_init(int device, ltx_ctx** out) {
         for (const unsigned char* co :
              {ltx_co_k_gemm, ltx_co_k_gemm_s4, ltx_co_k_gemm_f3, ltx_co_k_gemm_x4h, ltx_co_k_gemm_q8h, ltx_co_k_attn,
               ltx_co_k_norm, ltx_co_k_f32, ltx_co_k_core, ltx_co_k_kv, ltx_co_k_q4, ltx_co_k_mx4,
-              ltx_co_k_gemm_mx4}) {
+              ltx_co_k_gemm_mx4, ltx_co_k_rope}) {
             hipModule_t m;
             HIPC(hipModuleLoadData(&m, co));
             c->modules.push_back(m);

@@ -1,0 +1,153 @@
+// Norm and rotary positions of q and k on several axes.
+#include "ltx_device.h"
+
+// Eight values of a row.
+template <typename T>
+struct RopeRow {
+    u32x4 x;
+    __device__ __forceinline__ void load(const void* p, size_t at) { x = *(const u32x4*)((const uint16_t*)p + at); }
+    __device__ __forceinline__ float get(int e) const { return Op<T>::to_f32((uint16_t)(x[e >> 1] >> (16 * (e & 1)))); }
+    static __device__ __forceinline__ void store(void* p, size_t at, const float (&v)[8]) {
+        *(u32x4*)((uint16_t*)p + at) = u32x4{Op<T>::cvt2(v[0], v[1]), Op<T>::cvt2(v[2], v[3]), Op<T>::cvt2(v[4], v[5]),
+                                             Op<T>::cvt2(v[6], v[7])};
+    }
+};
+template <>
+struct RopeRow<float> {
+    f32x4 x[2];
+    __device__ __forceinline__ void load(const void* p, size_t at) {
+        x[0] = *(const f32x4*)((const float*)p + at);
+        x[1] = *(const f32x4*)((const float*)p + at + 4);
+    }
+    __device__ __forceinline__ float get(int e) const { return x[e >> 2][e & 3]; }
+    static __device__ __forceinline__ void store(void* p, size_t at, const float (&v)[8]) {
+        *(f32x4*)((float*)p + at) = f32x4{v[0], v[1], v[2], v[3]};
+        *(f32x4*)((float*)p + at + 4) = f32x4{v[4], v[5], v[6], v[7]};
+    }
+};
+
+// What eight pairs of a plan's head turn by: quarter turns a unit of position, at position
+// 0, and the axes (a byte each).
+struct RopePairs {
+    double freq[8], phase[8];
+    uint32_t axis[2];
+    __device__ __forceinline__ void load(const LtxRopeArgs& a, int unit) {
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            freq[j] = a.freq[8 * unit + j];
+            phase[j] = a.phase[8 * unit + j];
+        }
+        const u32x2 x = *(const u32x2*)(a.axis + 8 * unit);
+        axis[0] = x[0];
+        axis[1] = x[1];
+    }
+};
+
+// cos and sin of t quarter turns. Angles go far (thousands of turns, where f32 holds no
+// fraction of one), so whole quarters are taken off in f64: adding 1.5 2^52 rounds t to
+// them, and leaves their last bits in the sum's (|t| below 2^51). What is left, within half a
+// quarter, takes the series of sin and cos: their next terms are 2e-9 and 2.5e-11 there.
+__device__ __forceinline__ void rope_turn(double t, float& c, float& s) {
+    const double up = t + 6755399441055744.0;
+    const uint32_t k = (uint32_t)__builtin_bit_cast(uint64_t, up);
+    const float x = (float)(t - (up - 6755399441055744.0)) * 1.57079632679489662f, z = x * x;
+    float p = __builtin_fmaf(z, 2.755731922e-6f, -1.984126984e-4f);
+    p = __builtin_fmaf(z, p, 8.333333333e-3f);
+    p = __builtin_fmaf(z, p, -1.666666667e-1f);
+    const float sx = __builtin_fmaf(x * z, p, x);
+    float r = __builtin_fmaf(z, -2.755731922e-7f, 2.480158730e-5f);
+    r = __builtin_fmaf(z, r, -1.388888889e-3f);
+    r = __builtin_fmaf(z, r, 4.166666667e-2f);
+    r = __builtin_fmaf(z, r, -0.5f);
+    const float cx = __builtin_fmaf(z, r, 1.0f);
+    // a quarter takes (c, s) to (-s, c)
+    const float c0 = k & 1 ? sx : cx, s0 = k & 1 ? cx : sx;
+    c = (k + 1) & 2 ? -c0 : c0;
+    s = k & 2 ? -s0 : s0;
+}
+
+__device__ __forceinline__ void rope_turns(const RopePairs& p, const double* pos, float (&c)[8], float (&s)[8]) {
+#pragma unroll
+    for (int j = 0; j < 8; j++)
+        rope_turn(__builtin_fma(p.freq[j], pos[(p.axis[j >> 2] >> (8 * (j & 3))) & 255u], p.phase[j]), c[j], s[j]);
+}
+
+// The sums of squares of two rows over the workgroup (256 threads).
+__device__ __forceinline__ void rope_sums(float& x, float& y, float (*red)[2]) {
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) {
+        x += __shfl_xor(x, o, 64);
+        y += __shfl_xor(y, o, 64);
+    }
+    if ((threadIdx.x & 63) == 0) {
+        red[threadIdx.x >> 6][0] = x;
+        red[threadIdx.x >> 6][1] = y;
+    }
+    __syncthreads();
+    x = red[0][0] + red[1][0] + red[2][0] + red[3][0];
+    y = red[0][1] + red[1][1] + red[2][1] + red[3][1];
+}
+
+// Thread t takes head t / 8 (and every 32nd after it) and pairs 8 (t % 8) .. + 7, so that
+// the two values of a pair are its own; a workgroup takes a.per rows, one after another.
+template <typename T>
+__device__ __forceinline__ void qk_rope(const LtxRopeArgs& a) {
+    __shared__ float red[2][4][2];
+    const int h0 = threadIdx.x >> 3, o = threadIdx.x & 7, at = 8 * o;
+    const int row0 = blockIdx.x * a.per, end = min(a.rows, row0 + a.per);
+    for (int row = row0; row < end; row++) {
+        const double* pos = a.pos + (size_t)row * a.axes;
+        float inv[2] = {1.f, 1.f};
+        if (a.norm[0] || a.norm[1]) {
+            float sum[2] = {0.f, 0.f};
+#pragma unroll
+            for (int m = 0; m < 2; m++)
+                if (a.norm[m])
+                    for (int h = h0; h < a.heads[m]; h += 32) {
+                        RopeRow<T> lo, hi;
+                        const size_t i = (size_t)row * a.ldx[m] + LTX_HD * h + at;
+                        lo.load(a.x[m], i);
+                        hi.load(a.x[m], i + 64);
+#pragma unroll
+                        for (int j = 0; j < 8; j++) {
+                            sum[m] = __builtin_fmaf(lo.get(j), lo.get(j), sum[m]);
+                            sum[m] = __builtin_fmaf(hi.get(j), hi.get(j), sum[m]);
+                        }
+                    }
+            rope_sums(sum[0], sum[1], red[row & 1]);
+#pragma unroll
+            for (int m = 0; m < 2; m++) inv[m] = 1.0f / sqrtf(sum[m] / (float)(LTX_HD * max(a.heads[m], 1)) + a.eps);
+        }
+#pragma unroll
+        for (int m = 0; m < 2; m++)
+            for (int h = h0; h < a.heads[m]; h += 32) {
+                RopePairs p;
+                p.load(a, 8 * (h / a.group[m]) + o);
+                float c[8], s[8], u[8], v[8];
+                rope_turns(p, pos, c, s);
+                RopeRow<T> lo, hi;
+                const size_t i = (size_t)row * a.ldx[m] + LTX_HD * h + at;
+                lo.load(a.x[m], i);
+                hi.load(a.x[m], i + 64);
+#pragma unroll
+                for (int j = 0; j < 8; j++) {
+                    float x = lo.get(j), y = hi.get(j);
+                    if (a.norm[m]) {
+                        x *= inv[m] * a.norm[m][LTX_HD * h + at + j];
+                        y *= inv[m] * a.norm[m][LTX_HD * h + at + 64 + j];
+                    }
+                    u[j] = x * c[j] - y * s[j];
+                    v[j] = y * c[j] + x * s[j];
+                }
+                const size_t d = (size_t)row * a.ldy[m] + LTX_HD * h + at;
+                RopeRow<T>::store(a.y[m], d, u);
+                RopeRow<T>::store(a.y[m], d + 64, v);
+            }
+    }
+}
+
+#define QK_ROPE(NAME, T) \
+    extern "C" __global__ void __launch_bounds__(256) NAME(const LtxRopeArgs a) { qk_rope<T>(a); }
+QK_ROPE(ltx_qk_rope_f16, _Float16)
+QK_ROPE(ltx_qk_rope_bf16, __bf16)
+QK_ROPE(ltx_qk_rope_f32, float)

@@ -448,6 +448,25 @@ typedef struct {
 // Rows of a that the linear of few rows takes in 16 bits.
 #define LTX_MX4_ROWS 64
 
+// ---- rotary positions on several axes ------------------------------------------
+// Two sets of rows (q and k; heads 0: none) of heads * 128 values, normed over the row
+// where there are weights, and turned: pair j of head h, values j and j + 64 of it, by
+// freq[p] * pos[row][axis[p]] + phase[p] quarter turns, p = 64 (h / group) + j.
+typedef struct {
+    const double* freq;
+    const double* phase;
+    const uint8_t* axis;
+    const double* pos;   // [rows][axes]
+    const void* x[2];
+    void* y[2];
+    const float* norm[2];  // [heads * 128] or NULL
+    int64_t ldx[2], ldy[2];
+    int heads[2], group[2];  // group heads share a head of the plan
+    int rows, axes;
+    int per;             // rows of a workgroup
+    float eps;
+} LtxRopeArgs;
+
 #ifdef __cplusplus
 }
 #endif

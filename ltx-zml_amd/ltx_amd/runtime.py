@@ -64,6 +64,11 @@ def lib() -> C.CDLL:
         "ltx_op_mx4_quantise": (i32, [vp, vp, i64, vp, vp, i32, i32, i32, vp]),
         "ltx_op_mx4_values": (i32, [vp, vp, vp, vp, i64, i32, i32, i32, vp]),
         "ltx_op_linear_mx4": (i32, [vp, vp, vp, vp, vp, vp, vp, i32, i32, i32, i32, i32, i32, vp]),
+        "ltx_rope_create": (i32, [vp, i32, i32, vp, vp, vp, C.POINTER(vp)]),
+        "ltx_rope_create_grid": (i32, [vp, C.POINTER(vp)]),
+        "ltx_rope_free": (None, [vp, vp]),
+        "ltx_op_qk_rope": (i32, [vp, vp, vp, i32, vp, i64, vp, vp, i64, i32, vp, i64, vp, vp, i64, i32, C.c_float, i32,
+                                 vp]),
         "ltx_kv_cache_create": (i32, [vp, i32, i32, i32, C.POINTER(vp)]),
         "ltx_kv_cache_free": (None, [vp, vp]),
         "ltx_kv_cache_bytes": (u64, [vp]),
@@ -272,6 +277,25 @@ class KvCache:
             pass
 
 
+class Rope:
+    """What the pairs of q and k turn by (ltx_rope)."""
+
+    def __init__(self, ctx: "Context", handle: int, heads: int, axes: int):
+        self.ctx, self.handle = ctx, handle
+        self.heads, self.axes = heads, axes
+
+    def free(self):
+        if self.handle:
+            lib().ltx_rope_free(self.ctx.handle, self.handle)
+            self.handle = None
+
+    def __del__(self):
+        try:
+            self.free()
+        except Exception:
+            pass
+
+
 class Context:
     """One device context (ltx_init). Not thread-safe."""
 
@@ -283,6 +307,7 @@ class Context:
         self.device = device
         self._graphs = weakref.WeakSet()
         self._caches = weakref.WeakSet()
+        self._ropes = weakref.WeakSet()
 
     def _check(self, ok: int, what: str):
         if not ok:
@@ -292,7 +317,7 @@ class Context:
         if self.handle:
             for g in list(self._graphs):  # graphs hold the context's workspace
                 g.free()
-            for k in list(self._caches):
+            for k in list(self._caches) + list(self._ropes):
                 k.free()
             lib().ltx_destroy(self.handle)
             self.handle = None
@@ -460,6 +485,59 @@ class Context:
             raise LtxError(f"{name}: rows of the mode's type on the context's device are needed")
         _mx4_held(name, q, s, rows, K, self.device)
         return rows, K
+
+    # ---- rotary positions on several axes ----
+    def rope(self, freq, phase=None, axis=None, axes: int = 1) -> Rope:
+        """freq, phase f64 and axis int32, host arrays [heads, 64] (ltx_rope_create)."""
+        f = np.ascontiguousarray(freq, np.float64)
+        if f.ndim != 2 or f.shape[1] != 64:
+            raise LtxError("rope: freq must be [heads, 64]")
+        p = None if phase is None else np.ascontiguousarray(phase, np.float64)
+        x = None if axis is None else np.ascontiguousarray(axis, np.int32)
+        if any(t is not None and t.shape != f.shape for t in (p, x)):
+            raise LtxError("rope: phase and axis must have freq's shape")
+        h = C.c_void_p()
+        self._check(lib().ltx_rope_create(self.handle, f.shape[0], axes, _ptr(f), _ptr(p), _ptr(x), C.byref(h)),
+                    "ltx_rope_create")
+        r = Rope(self, h.value, f.shape[0], axes)
+        self._ropes.add(r)
+        return r
+
+    def rope_grid(self) -> Rope:
+        """The plan of this model's blocks (ltx_rope_create_grid)."""
+        h = C.c_void_p()
+        self._check(lib().ltx_rope_create_grid(self.handle, C.byref(h)), "ltx_rope_create_grid")
+        r = Rope(self, h.value, 32, 3)
+        self._ropes.add(r)
+        return r
+
+    def qk_rope(self, rope: Rope, pos, q, q_out, k=None, k_out=None, q_norm=None, k_norm=None, eps: float = 1e-6,
+                mode=MODE_F16, stream=None):
+        """q, q_out [rows, heads * 128] and k, k_out [rows, kv_heads * 128] (rows may be
+        strided), pos f64 [rows, axes], norms f32 [heads * 128] or None (ltx_op_qk_rope)."""
+        import torch
+        rows, dt = q.shape[0], _torch_dtype(mode)
+        if (k is None) != (k_out is None):
+            raise LtxError("qk_rope: k and k_out belong together")
+        for x, y, w in ((q, q_out, q_norm), (k, k_out, k_norm)):
+            if x is None:
+                continue
+            for t in (x, y):
+                if t.dim() != 2 or t.shape[0] != rows or t.shape != x.shape or t.dtype != dt or t.stride(1) != 1:
+                    raise LtxError("qk_rope: rows of one shape and of the mode's type are needed")
+            if x.shape[1] % 128:
+                raise LtxError("qk_rope: rows of heads of 128 values are needed")
+            if w is not None and not (w.shape == x.shape[1:] and w.dtype == torch.float32 and w.is_contiguous()):
+                raise LtxError("qk_rope: norm weights must be f32, one for each value of a row")
+        if not (pos.shape == (rows, rope.axes) and pos.dtype == torch.float64 and pos.is_contiguous()):
+            raise LtxError(f"qk_rope: contiguous f64 positions {[rows, rope.axes]} are needed")
+        if any(t is not None and t.get_device() != self.device for t in (pos, q, q_out, k, k_out, q_norm, k_norm)):
+            raise LtxError("qk_rope: tensors on the context's device are needed")
+        st = stream.cuda_stream if stream is not None else _current_stream(self.device)
+        kl = (0, 0, 0) if k is None else (k.stride(0), k_out.stride(0), k.shape[1] // 128)
+        self._check(lib().ltx_op_qk_rope(self.handle, rope.handle, _ptr(pos), rows, _ptr(q), q.stride(0), _ptr(q_norm),
+                                         _ptr(q_out), q_out.stride(0), q.shape[1] // 128, _ptr(k), kl[0], _ptr(k_norm),
+                                         _ptr(k_out), kl[1], kl[2], eps, mode, st), "ltx_op_qk_rope")
 
     # ---- the 4-bit key/value cache ----
     def kv_cache(self, kv_heads: int, pages: int, mode: int = MODE_F16) -> KvCache:
