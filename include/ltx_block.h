@@ -441,6 +441,19 @@ int ltx_op_kv_attention(ltx_ctx* ctx, const ltx_kv_cache* cache, const ltx_kv_ba
                         int64_t ldq, int heads, int causal, const float* glog, void* out, int64_t ldo, void* work,
                         uint64_t work_bytes, void* stream);
 
+/* ltx_op_kv_attention with a sliding window and first keys that stay visible, for streams
+ * that run on: of the keys that a row would see there (up to its own position, or all kv_len),
+ * it sees the last `window` (at least 1) and the first `sinks` (0: none). Where causal is 0
+ * all rows of a sequence, a frame's, share one window. Only pages that hold such keys are
+ * read: entries of the table whose keys no row of the call sees may hold anything, and
+ * their pages may be in use elsewhere. Everything else is as in ltx_op_kv_attention; a window
+ * as wide as the table is that call. The workspace is of this call's mask. */
+int ltx_op_kv_attention_window_workspace(ltx_ctx* ctx, const ltx_kv_cache* cache, const ltx_kv_batch* batch, int heads,
+                                         int causal, int window, int sinks, uint64_t* bytes);
+int ltx_op_kv_attention_window(ltx_ctx* ctx, const ltx_kv_cache* cache, const ltx_kv_batch* batch, const void* q,
+                               int64_t ldq, int heads, int causal, int window, int sinks, const float* glog, void* out,
+                               int64_t ldo, void* work, uint64_t work_bytes, void* stream);
+
 /* ---- host utilities ---------------------------------------------------- */
 
 /* 3D RoPE tables, host f64 (ltx/block_conformance.zig:87-126). grid

@@ -1,5 +1,6 @@
 // The 4-bit key/value cache: its handle, rows written and read back, attention.
 #include <algorithm>
+#include <cstdio>
 #include <cstring>
 
 #include "ltx_internal.hpp"
@@ -58,10 +59,30 @@ void kv_rows(ltx_ctx* c, const ltx_kv_cache* k, const ltx_kv_batch* b, void* kp,
               (unsigned)(((size_t)b->rows + 15) / 16), (k->kv_heads + 3) / 4, 1, 256, &a, st);
 }
 
+// What rows see: causal or not, and with a window the last `window` of those keys and the
+// first `sinks` (window 0: none).
+struct AttnMask {
+    int causal = 1, window = 0, sinks = 0;
+};
+AttnMask mask_of(const ltx_kv_batch* b, int causal, int window, int sinks) {
+    if (window < 1 || sinks < 0) throw Error("window must be positive, sinks not negative");
+    const int64_t all = (int64_t)b->max_pages * LTX_KV_PAGE;  // (at most 2^30 keys)
+    if (window >= all) return {causal, 0, 0};
+    return {causal, window, (int)std::min<int64_t>(sinks, all)};
+}
+// Pages of a tile of `rows` rows, at most (the device's kv_range_units is no more).
+int64_t tile_pages(const ltx_kv_batch* b, const AttnMask& m, int64_t rows) {
+    if (!m.window) return b->max_pages;
+    const int64_t keys = (int64_t)m.window + (m.causal ? rows + 1 : 0);
+    return std::min<int64_t>(b->max_pages, ((int64_t)m.sinks + LTX_KV_PAGE - 1) / LTX_KV_PAGE +
+                                               (keys + LTX_KV_PAGE - 2) / LTX_KV_PAGE + 1);
+}
+
 struct AttnPlan {
     int tile = 16;  // columns (rows times query heads of a cached head) of a tile: 16, 128 or 256
     int least = 4, slots = 0, items = 0, parts = 0;
-    size_t bytes = 0;  // of partial results
+    int64_t width = 0;  // pages of a tile, at most
+    size_t bytes = 0;   // of partial results
 };
 
 // Tiles of 16 columns (eight waves that share a tile's pages), or of 128 or 256 (eight
@@ -81,10 +102,11 @@ struct AttnPlan {
 // The table's width stands for the lengths, which the host does not know. A call that
 // cannot split (captured, without a workspace) takes 256 columns only where they fill
 // the CUs: 256 rows of 32 heads on 8 over 28,672 keys 235 us on 16 columns, 815 on 256.
-int tile_columns(const ltx_ctx* c, const ltx_kv_cache* k, const ltx_kv_batch* b, int64_t columns, bool split) {
+int tile_columns(const ltx_ctx* c, const ltx_kv_cache* k, const ltx_kv_batch* b, const AttnMask& m, int64_t columns,
+                 bool split) {
     if (c->kv_tile) return c->kv_tile;
     const int64_t each = columns / b->nseq, wide = columns * k->kv_heads / 256;  // workgroups of 256 columns
-    const int64_t pages = wide * b->max_pages / c->num_cu;                       // of each, if split
+    const int64_t pages = wide * tile_pages(b, m, b->rows / b->nseq) / c->num_cu;  // of each, if split
     if (each >= 192 && wide >= c->num_cu) return 256;
     if (split && each >= 256 && pages >= 128) return 256;
     if (each >= 64 && (each + 127) / 128 * b->nseq * k->kv_heads >= c->num_cu) return 128;
@@ -92,10 +114,12 @@ int tile_columns(const ltx_ctx* c, const ltx_kv_cache* k, const ltx_kv_batch* b,
     return 16;
 }
 
-AttnPlan attn_plan(const ltx_ctx* c, const ltx_kv_cache* k, const ltx_kv_batch* b, int heads, bool split) {
+AttnPlan attn_plan(const ltx_ctx* c, const ltx_kv_cache* k, const ltx_kv_batch* b, int heads, const AttnMask& m,
+                   bool split) {
     const int64_t group = heads / k->kv_heads, columns = (int64_t)b->rows * group;
     AttnPlan p;
-    p.tile = tile_columns(c, k, b, columns, split);
+    p.tile = tile_columns(c, k, b, m, columns, split);
+    p.width = tile_pages(b, m, p.tile / group + 1);
     // tiles of the batch, at most
     const int64_t tiles = !b->row_start || b->nseq == 1
                               ? (int64_t)b->nseq * ((columns / b->nseq + p.tile - 1) / p.tile)
@@ -112,9 +136,9 @@ AttnPlan attn_plan(const ltx_ctx* c, const ltx_kv_cache* k, const ltx_kv_batch* 
     // ragged, 32 x 8 cached heads up to 8,192 keys 40 / 37, 8 x 32 up to 16,000 65 / 74.
     p.least = 8;
     const int64_t round = ((int64_t)c->num_cu + k->kv_heads - 1) / k->kv_heads;
-    const int64_t units = tiles * b->max_pages;
-    const bool few = p.tile == 16 ? tiles * k->kv_heads < c->num_cu && b->max_pages > 16
-                                  : p.tile == 256 && columns / 256 * k->kv_heads < c->num_cu && b->max_pages > p.least;
+    const int64_t units = tiles * p.width;
+    const bool few = p.tile == 16 ? tiles * k->kv_heads < c->num_cu && p.width > 16
+                                  : p.tile == 256 && columns / 256 * k->kv_heads < c->num_cu && p.width > p.least;
     if (split && few && units < 1ll << 31) p.slots = (int)std::min(round, (units + p.least - 1) / p.least);
     p.items = p.slots ? p.slots : (int)tiles;
     if (p.slots) {
@@ -127,6 +151,78 @@ AttnPlan attn_plan(const ltx_ctx* c, const ltx_kv_cache* k, const ltx_kv_batch* 
 void check_heads(const ltx_kv_cache* k, int heads) {
     if (heads <= 0 || heads % k->kv_heads) throw Error("heads must be a positive multiple of the cache's");
     if (heads > 65535) throw Error("heads must be at most 65535");
+}
+
+// Bytes of `work`: one size serves calls with row_start and without.
+uint64_t attn_workspace(const ltx_ctx* c, const ltx_kv_cache* cache, const ltx_kv_batch* batch, int heads,
+                        const AttnMask& m) {
+    uint64_t bytes = attn_plan(c, cache, batch, heads, m, true).bytes;
+    if (batch->rows == batch->nseq) {  // enough for the other form too: with row_start, or without
+        ltx_kv_batch other = *batch;
+        other.row_start = batch->row_start ? nullptr : batch->kv_len;  // (only whether there is one counts)
+        try {
+            bytes = std::max<uint64_t>(bytes, attn_plan(c, cache, &other, heads, m, true).bytes);
+        } catch (const Error&) {  // too many rows in that form: its calls are refused
+        }
+    }
+    return bytes;
+}
+
+struct AttnRows {
+    const void* q;
+    void* out;
+    const float* glog;
+    int64_t ldq, ldo;
+    int heads;
+};
+void attention(ltx_ctx* c, const ltx_kv_cache* cache, const ltx_kv_batch* batch, const AttnRows& r, const AttnMask& m,
+               void* work, uint64_t work_bytes, hipStream_t st) {
+    LtxKvAttnArgs a{};
+    a.b = batch_args(c, cache, batch);
+    check_heads(cache, r.heads);
+    check_rows(r.q, r.ldq, r.heads * LTX_HD, batch->rows, "q");
+    check_rows(r.out, r.ldo, r.heads * LTX_HD, batch->rows, "out");
+    if ((uintptr_t)r.glog & 3) throw Error("glog must start on 4 bytes");
+    if ((uintptr_t)work & 15) throw Error("work must start on 16 bytes");
+    AttnPlan p = attn_plan(c, cache, batch, r.heads, m, true);
+    if (work && work_bytes < p.bytes) throw Error("work is smaller than the workspace call says");
+    if (batch->rows == 0) return;
+    HIPC(hipSetDevice(c->device));
+    ScratchUse use(c->op_scratch, st);
+    if (p.bytes && !work && !(work = use.take(p.bytes))) p = attn_plan(c, cache, batch, r.heads, m, false);
+    a.q = r.q;
+    a.out = r.out;
+    a.glog = r.glog;
+    a.part = (float*)work;
+    a.ldq = r.ldq;
+    a.ldo = r.ldo;
+    a.heads = r.heads;
+    a.group = r.heads / cache->kv_heads;
+    a.causal = m.causal != 0;
+    a.window = m.window;
+    a.sinks = m.sinks;
+    a.tile = p.tile;
+    a.least = p.least;
+    a.slots = p.slots;
+    a.items = p.items;
+    a.parts = p.parts;
+    a.scale_log2 = 0.12751743f;  // log2(e) / sqrt(128)
+    // Streaming loads where the table spans more than the memory-side cache's 256 MB
+    // can help with: 499 MB (four sequences of 28,672 keys, 32 heads) 91 us against
+    // 102, 557 MB 95 against 108; 278 MB, called again and again, 53 against 50
+    const bool nt = (uint64_t)batch->nseq * p.width * cache->kv_heads * LTX_KV_BLOCK > 384u << 20;
+    char name[48];
+    auto launch = [&](const char* form, const char* end, unsigned gx, unsigned gy, unsigned threads) {
+        std::snprintf(name, sizeof(name), "ltx_kv_%s_%s%s%s", form, cache->mode == LTX_MODE_F16 ? "f16" : "bf16",
+                      m.window ? "_win" : "", end);
+        c->launch(name, gx, gy, 1, threads, &a, st);
+    };
+    if (p.tile == 16)
+        launch("attn", nt ? "_nt" : "", p.items, cache->kv_heads, 512);
+    else
+        launch("attn", p.tile == 128 ? "_rows1" : p.slots ? "_rows2_split" : "_rows2",
+               (unsigned)((int64_t)p.items * cache->kv_heads), 1, 512);
+    if (p.slots) launch("join", "", batch->rows, r.heads, 256);
 }
 
 }  // namespace
@@ -217,15 +313,7 @@ int ltx_op_kv_attention_workspace(ltx_ctx* c, const ltx_kv_cache* cache, const l
         if (!c || !bytes) throw ltx::Error("NULL argument");
         ltx::batch_args(c, cache, batch);
         ltx::check_heads(cache, heads);
-        *bytes = ltx::attn_plan(c, cache, batch, heads, true).bytes;
-        if (batch->rows == batch->nseq) {  // enough for the other form too: with row_start, or without
-            ltx_kv_batch other = *batch;
-            other.row_start = batch->row_start ? nullptr : batch->kv_len;  // (only whether there is one counts)
-            try {
-                *bytes = std::max<uint64_t>(*bytes, ltx::attn_plan(c, cache, &other, heads, true).bytes);
-            } catch (const ltx::Error&) {  // too many rows in that form: its calls are refused
-            }
-        }
+        *bytes = ltx::attn_workspace(c, cache, batch, heads, {});
     })
 }
 
@@ -234,50 +322,29 @@ int ltx_op_kv_attention(ltx_ctx* c, const ltx_kv_cache* cache, const ltx_kv_batc
                         uint64_t work_bytes, void* stream) {
     LTX_GUARD(c, {
         if (!c) throw ltx::Error("NULL context");
-        LtxKvAttnArgs a{};
-        a.b = ltx::batch_args(c, cache, batch);
+        ltx::attention(c, cache, batch, {q, out, glog, ldq, ldo, heads}, {causal, 0, 0}, work, work_bytes,
+                       (hipStream_t)stream);
+    })
+}
+
+int ltx_op_kv_attention_window_workspace(ltx_ctx* c, const ltx_kv_cache* cache, const ltx_kv_batch* batch, int heads,
+                                         int causal, int window, int sinks, uint64_t* bytes) {
+    LTX_GUARD(c, {
+        if (!c || !bytes) throw ltx::Error("NULL argument");
+        ltx::batch_args(c, cache, batch);
         ltx::check_heads(cache, heads);
-        ltx::check_rows(q, ldq, heads * LTX_HD, batch->rows, "q");
-        ltx::check_rows(out, ldo, heads * LTX_HD, batch->rows, "out");
-        if ((uintptr_t)glog & 3) throw ltx::Error("glog must start on 4 bytes");
-        if ((uintptr_t)work & 15) throw ltx::Error("work must start on 16 bytes");
-        ltx::AttnPlan p = ltx::attn_plan(c, cache, batch, heads, true);
-        if (work && work_bytes < p.bytes) throw ltx::Error("work is smaller than ltx_op_kv_attention_workspace says");
-        if (batch->rows == 0) return LTX_OK;
-        HIPC(hipSetDevice(c->device));
-        hipStream_t st = (hipStream_t)stream;
-        ltx::ScratchUse use(c->op_scratch, st);
-        if (p.bytes && !work && !(work = use.take(p.bytes))) p = ltx::attn_plan(c, cache, batch, heads, false);
-        a.q = q;
-        a.out = out;
-        a.glog = glog;
-        a.part = (float*)work;
-        a.ldq = ldq;
-        a.ldo = ldo;
-        a.heads = heads;
-        a.group = heads / cache->kv_heads;
-        a.causal = causal != 0;
-        a.tile = p.tile;
-        a.least = p.least;
-        a.slots = p.slots;
-        a.items = p.items;
-        a.parts = p.parts;
-        a.scale_log2 = 0.12751743f;  // log2(e) / sqrt(128)
-        const bool f16 = cache->mode == LTX_MODE_F16;
-        // Streaming loads where the table spans more than the memory-side cache's 256 MB
-        // can help with: 499 MB (four sequences of 28,672 keys, 32 heads) 91 us against
-        // 102, 557 MB 95 against 108; 278 MB, called again and again, 53 against 50
-        const bool nt = (uint64_t)batch->nseq * batch->max_pages * cache->kv_heads * LTX_KV_BLOCK > 384u << 20;
-        if (p.tile == 16)
-            c->launch(nt ? (f16 ? "ltx_kv_attn_f16_nt" : "ltx_kv_attn_bf16_nt") : (f16 ? "ltx_kv_attn_f16" : "ltx_kv_attn_bf16"),
-                      p.items, cache->kv_heads, 1, 512, &a, st);
-        else
-            c->launch(p.tile == 128 ? (f16 ? "ltx_kv_attn_f16_rows1" : "ltx_kv_attn_bf16_rows1")
-                      : p.slots     ? (f16 ? "ltx_kv_attn_f16_rows2_split" : "ltx_kv_attn_bf16_rows2_split")
-                                    : (f16 ? "ltx_kv_attn_f16_rows2" : "ltx_kv_attn_bf16_rows2"),
-                      (unsigned)((int64_t)p.items * cache->kv_heads), 1, 1, 512, &a, st);
-        if (p.slots)
-            c->launch(f16 ? "ltx_kv_join_f16" : "ltx_kv_join_bf16", batch->rows, heads, 1, 256, &a, st);
+        *bytes = ltx::attn_workspace(c, cache, batch, heads, ltx::mask_of(batch, causal, window, sinks));
+    })
+}
+
+int ltx_op_kv_attention_window(ltx_ctx* c, const ltx_kv_cache* cache, const ltx_kv_batch* batch, const void* q,
+                               int64_t ldq, int heads, int causal, int window, int sinks, const float* glog, void* out,
+                               int64_t ldo, void* work, uint64_t work_bytes, void* stream) {
+    LTX_GUARD(c, {
+        if (!c) throw ltx::Error("NULL context");
+        ltx::batch_args(c, cache, batch);
+        ltx::attention(c, cache, batch, {q, out, glog, ldq, ldo, heads}, ltx::mask_of(batch, causal, window, sinks),
+                       work, work_bytes, (hipStream_t)stream);
     })
 }
 

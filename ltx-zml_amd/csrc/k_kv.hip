@@ -233,18 +233,25 @@ __device__ __forceinline__ uint32_t wave_scan(uint32_t x) {  // inclusive sums o
     return x;
 }
 
+// Work of a tile of the sequence (WIN: with a window)
+template <bool WIN>
+__device__ __forceinline__ int kv_work(const LtxKvAttnArgs& a, const KvSeq& s) {
+    return WIN ? kv_range_units(a.window, a.sinks, a.causal, s, a.group, a.tile) : kv_units(s.L);
+}
+
 // Sequence base + lane, and what it adds to the tiles and units before the next one
 struct KvLane {
     KvSeq s;
     uint32_t tiles, units, tiles_to, units_to;  // its own, and inclusive sums from `base` on
 };
+template <bool WIN>
 __device__ __forceinline__ KvLane kv_lane(const LtxKvAttnArgs& a, int base) {
     const int b = base + (threadIdx.x & 63);
     KvLane k;
     k.s = KvSeq{0, 0, 0};
     if (b < a.b.nseq) k.s = kv_seq(a.b, b);
     k.tiles = kv_tiles(k.s.n, a.group, a.tile);
-    k.units = a.slots ? k.tiles * (uint32_t)kv_units(k.s.L) : k.tiles;
+    k.units = a.slots ? k.tiles * (uint32_t)kv_work<WIN>(a, k.s) : k.tiles;
     k.tiles_to = wave_scan(k.tiles);
     k.units_to = wave_scan(k.units);
     return k;
@@ -252,23 +259,25 @@ __device__ __forceinline__ KvLane kv_lane(const LtxKvAttnArgs& a, int base) {
 __device__ __forceinline__ uint32_t lane_of(uint32_t x, int l) { return __builtin_amdgcn_readlane(x, l); }
 
 // units an item: `first` is kv_lane(a, 0)
+template <bool WIN>
 __device__ __forceinline__ int kv_per(const LtxKvAttnArgs& a, const KvLane& first) {
     if (!a.slots) return 1;
     uint32_t units = lane_of(first.units_to, 63);
-    for (int base = 64; base < a.b.nseq; base += 64) units += lane_of(kv_lane(a, base).units_to, 63);
+    for (int base = 64; base < a.b.nseq; base += 64) units += lane_of(kv_lane<WIN>(a, base).units_to, 63);
     return kv_per_of(units, a.slots, a.least);
 }
 
 // The item's first span; false: there is none. Without a split an item is a tile, a
 // sequence's last one, which sees the most keys where the mask is causal, first.
+template <bool WIN>
 __device__ __forceinline__ bool kv_begin(const LtxKvAttnArgs& a, int item, KvSpan& it) {
-    KvLane k = kv_lane(a, 0);
-    it.left = kv_per(a, k);
+    KvLane k = kv_lane<WIN>(a, 0);
+    it.left = kv_per<WIN>(a, k);
     const uint64_t first = (uint64_t)item * it.left;
     if (first >> 32) return false;
     uint32_t u = (uint32_t)first, entities = 0;
     for (int base = 0; base < a.b.nseq; base += 64) {
-        if (base) k = kv_lane(a, base);
+        if (base) k = kv_lane<WIN>(a, base);
         const uint64_t here = __builtin_amdgcn_ballot_w64(u < k.units_to && u >= k.units_to - k.units);
         if (here) {
             const int l = __builtin_ctzll(here);
@@ -276,7 +285,7 @@ __device__ __forceinline__ bool kv_begin(const LtxKvAttnArgs& a, int item, KvSpa
             it.b = base + l;
             it.s = KvSeq{(int)lane_of(k.s.s0, l), (int)lane_of(k.s.n, l), (int)lane_of(k.s.L, l)};
             it.tiles = lane_of(k.tiles, l);
-            it.pages = kv_units(it.s.L);
+            it.pages = kv_work<WIN>(a, it.s);
             it.tile = a.slots ? (int)(u / (uint32_t)it.pages) : it.tiles - 1 - (int)u;
             it.page = a.slots ? (int)(u % (uint32_t)it.pages) : 0;
             it.entity = (int)(entities + lane_of(k.tiles_to - k.tiles, l)) + it.tile;
@@ -291,6 +300,7 @@ __device__ __forceinline__ bool kv_begin(const LtxKvAttnArgs& a, int item, KvSpa
 // units of the span
 __device__ __forceinline__ int kv_span(const KvSpan& it) { return min(it.left, it.pages - it.page); }
 // the next one
+template <bool WIN>
 __device__ __forceinline__ bool kv_next(const LtxKvAttnArgs& a, KvSpan& it) {
     it.left -= kv_span(it);
     if (it.left <= 0 || !a.slots) return false;
@@ -301,7 +311,7 @@ __device__ __forceinline__ bool kv_next(const LtxKvAttnArgs& a, KvSpan& it) {
     while (++it.b < a.b.nseq) {
         it.s = kv_seq_all(a.b, it.b);
         it.tiles = kv_tiles(it.s.n, a.group, a.tile);
-        it.pages = kv_units(it.s.L);
+        it.pages = kv_work<WIN>(a, it.s);
         if (it.tiles > 0) return true;
     }
     return false;
@@ -374,6 +384,37 @@ __device__ __forceinline__ void kv_mask(f32x4 (&s)[4], int p, int mine, int h) {
     for (int t = 0; t < 4; t++)
 #pragma unroll
         for (int i = 0; i < 4; i++) s[t][i] = kv_select((left - (16 * t + i + 1)) >> 31, s[t][i], 0xff800000u);
+}
+
+// And of those that a window and first keys leave out too: a column sees the keys below
+// `mine`, from `low` on or below `sinks`.
+__device__ __forceinline__ void kv_mask_range(f32x4 (&s)[4], int p, int mine, int low, int sinks, int h) {
+    const int first = p * LTX_KV_PAGE + 4 * h, left = mine - first, lo = low - first, sk = sinks - first;
+#pragma unroll
+    for (int t = 0; t < 4; t++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const int d = 16 * t + i;
+            s[t][i] = kv_select(((left - (d + 1)) | ((d - lo) & ~(d - sk))) >> 31, s[t][i], 0xff800000u);
+        }
+}
+// kv_seen with a window: of the pages kv_range_page(r, u0 .. u1 - 1), whether one in the pool
+// holds a key that the column sees.
+__device__ __forceinline__ void kv_seen_range(const LtxKvBatchArgs& a, int b, const KvRange& r, int u0, int u1, int mine,
+                                              int low, int sinks, float& m, float& sum) {
+    if (__builtin_amdgcn_ballot_w64(!(sum > 0.f)) == 0) return;
+    bool saw = false;
+    const int np = kv_pages(mine), ps = kv_pages(min(sinks, mine)), pw = low / LTX_KV_PAGE;
+    for (int base = u0; base < u1; base += 64) {
+        const int u = base + (threadIdx.x & 63);
+        uint64_t there = __builtin_amdgcn_ballot_w64(u < u1 && kv_in_pool(a, kv_page(a, b, kv_range_page(r, u))));
+        for (; there; there &= there - 1) {
+            const int p = kv_range_page(r, base + __builtin_ctzll(there));
+            saw |= p < np && (p >= pw || p < ps);
+        }
+    }
+    m = saw ? fmaxf(m, -__FLT_MAX__) : -__builtin_inff();
+    sum = saw ? sum : 0.f;
 }
 
 // Weights are formed and summed times 2^this (a factor that the division by their sum
@@ -479,7 +520,8 @@ __device__ __forceinline__ void kv_v_pair(const uint32_t (&x)[8], const uint32_t
 // memory-side cache holds much between calls) in 36. One short sequence is latency: a
 // page's index, its codes, two rounds of products and the waves' join, 8 us.
 // NT: the codes as streaming loads, for caches beyond what the memory-side cache holds.
-template <typename T, bool NT>
+// WIN: with a window, p counts the pages of the tile's range.
+template <typename T, bool NT, bool WIN>
 __device__ __forceinline__ void kv_attn(const LtxKvAttnArgs& a) {
     typedef typename Op<T>::v8 v8;
     __shared__ __attribute__((aligned(16))) float so[KV_WAVES][KV_TILE][LTX_HD + 4];
@@ -492,19 +534,22 @@ __device__ __forceinline__ void kv_attn(const LtxKvAttnArgs& a) {
     typedef const __attribute__((address_space(4))) uint32_t* scalar_ptr;
     const scalar_ptr flags = (scalar_ptr)(uintptr_t)a.b.flags;
     KvSpan it;
-    if (!kv_begin(a, blockIdx.x, it)) return;
+    if (!kv_begin<WIN>(a, blockIdx.x, it)) return;
     do {
-        const int limit = kv_tile_limit(a.causal, it.s, a.group, it.tile, KV_TILE), np = kv_pages(limit);
-        const int p0 = it.page, units = kv_span(it), p1 = min(np, p0 + units);
+        const int limit = kv_tile_limit(a.causal, it.s, a.group, it.tile, KV_TILE);
+        const int all = kv_limit(a.causal, it.s, it.tile * KV_TILE / a.group);  // keys that every column sees
+        const KvRange range = WIN ? kv_range(a.window, a.sinks, all, limit) : KvRange{0, 0, kv_pages(limit)};
+        auto real = [&](int p) { return WIN ? kv_range_page(range, p) : p; };
+        const int p0 = it.page, units = kv_span(it), p1 = min(range.count, p0 + units);
         const scalar_ptr table = (scalar_ptr)(uintptr_t)(a.b.pages + (size_t)it.b * a.b.max_pages);
-        uint32_t next = p0 + w < p1 ? table[p0 + w] : 0u;
+        uint32_t next = p0 + w < p1 ? table[real(p0 + w)] : 0u;
 
         // this lane's column: row, query head, keys it sees
         const int ncol = it.s.n * a.group, c0 = it.tile * KV_TILE;
         const int cols = min(KV_TILE, ncol - c0), c = min(c0 + r, ncol - 1);
         const int row = c / a.group, head = kh * a.group + c % a.group;
         const int mine = kv_limit(a.causal, it.s, row);
-        const int all = kv_limit(a.causal, it.s, c0 / a.group);  // keys that every column sees
+        const int low = WIN ? max(0, mine - a.window) : 0;
         v8 qf[4];
         const uint16_t* Q = (const uint16_t*)a.q + (size_t)(it.s.s0 + row) * a.ldq + (size_t)head * LTX_HD + 32 * h;
 #pragma unroll
@@ -537,7 +582,7 @@ __device__ __forceinline__ void kv_attn(const LtxKvAttnArgs& a) {
             for (int t = 0; t < 4; t++)
                 x.v[t] = codes(blk + LTX_KV_V + 1024 * t + 16 * lane);
             x.vs = *(const u32x4*)(blk + LTX_KV_VS + 64 * (r >> 2) + 16 * h);
-            next = p + KV_WAVES < p1 ? table[p + KV_WAVES] : 0u;
+            next = p + KV_WAVES < p1 ? table[real(p + KV_WAVES)] : 0u;
             __builtin_amdgcn_sched_barrier(0);
         };
         auto compute = [&](Page& x, int p) {
@@ -556,7 +601,12 @@ __device__ __forceinline__ void kv_attn(const LtxKvAttnArgs& a) {
             }
             __builtin_amdgcn_sched_barrier(0);
             if (x.flag) kv_set_nan(s, kv_drop_nan(x.vs));
-            if (x.none || (p + 1) * LTX_KV_PAGE > all) kv_mask(s, p, x.none ? 0 : mine, h);
+            if constexpr (WIN) {
+                const int key = real(p) * LTX_KV_PAGE, end = key + LTX_KV_PAGE;
+                if (x.none || end > all || (key < limit - a.window && end > a.sinks))
+                    kv_mask_range(s, real(p), x.none ? 0 : mine, low, a.sinks, h);
+            } else if (x.none || (p + 1) * LTX_KV_PAGE > all)
+                kv_mask(s, p, x.none ? 0 : mine, h);
             uint32_t pw[4][2];
             float corr;
             if (kv_softmax<T>(s, C, m, l, pw, corr))
@@ -599,7 +649,10 @@ __device__ __forceinline__ void kv_attn(const LtxKvAttnArgs& a) {
             l += kv_bad_query<T>(qf);
             l += __shfl_xor(l, 16, 64);
             l += __shfl_xor(l, 32, 64);
-            kv_seen(a.b, it.b, p0, p1, mine, m, l);
+            if constexpr (WIN)
+                kv_seen_range(a.b, it.b, range, p0, p1, mine, low, a.sinks, m, l);
+            else
+                kv_seen(a.b, it.b, p0, p1, mine, m, l);
         }
         if (h == 0) {
             sm[w][r] = m;
@@ -644,17 +697,21 @@ __device__ __forceinline__ void kv_attn(const LtxKvAttnArgs& a) {
             }
         }
         __syncthreads();
-    } while (kv_next(a, it));
+    } while (kv_next<WIN>(a, it));
 }
 
-#define KV_ATTN(NAME, T, NT)                                                                  \
+#define KV_ATTN(NAME, T, NT, WIN)                                                                  \
     extern "C" __global__ void __launch_bounds__(64 * KV_WAVES) NAME(const LtxKvAttnArgs a) { \
-        kv_attn<T, NT>(a);                                                                    \
+        kv_attn<T, NT, WIN>(a);                                                               \
     }
-KV_ATTN(ltx_kv_attn_f16, _Float16, false)
-KV_ATTN(ltx_kv_attn_bf16, __bf16, false)
-KV_ATTN(ltx_kv_attn_f16_nt, _Float16, true)
-KV_ATTN(ltx_kv_attn_bf16_nt, __bf16, true)
+KV_ATTN(ltx_kv_attn_f16, _Float16, false, false)
+KV_ATTN(ltx_kv_attn_bf16, __bf16, false, false)
+KV_ATTN(ltx_kv_attn_f16_nt, _Float16, true, false)
+KV_ATTN(ltx_kv_attn_bf16_nt, __bf16, true, false)
+KV_ATTN(ltx_kv_attn_f16_win, _Float16, false, true)
+KV_ATTN(ltx_kv_attn_bf16_win, __bf16, false, true)
+KV_ATTN(ltx_kv_attn_f16_win_nt, _Float16, true, true)
+KV_ATTN(ltx_kv_attn_bf16_win_nt, __bf16, true, true)
 
 // Many columns: a workgroup takes 128 NQ columns, its eight waves 16 NQ each, and a
 // run of pages. A page's codes become MFMA operands once for all eight waves, in LDS,
@@ -669,7 +726,7 @@ KV_ATTN(ltx_kv_attn_bf16_nt, __bf16, true)
 // operands 1,675 us, operands in LDS 1,176, two groups a phase apart 1,137, loads
 // without branches 1,100, one straight block of products without spills 900, staging
 // before the softmax 840.
-template <typename T, int NQ, bool SPLIT>
+template <typename T, int NQ, bool SPLIT, bool WIN>
 __device__ __forceinline__ void kv_attn_rows(const LtxKvAttnArgs& a) {
     typedef typename Op<T>::v8 v8;
     __shared__ __attribute__((aligned(1024))) uint8_t sk[2][16384];
@@ -685,9 +742,13 @@ __device__ __forceinline__ void kv_attn_rows(const LtxKvAttnArgs& a) {
     // the other over the XCDs, 32 heads 155 against 233.
     const int item = blockIdx.x / a.b.kvh, kh = blockIdx.x - item * a.b.kvh;
     KvSpan it;
-    if (!kv_begin(a, item, it)) return;
+    if (!kv_begin<WIN>(a, item, it)) return;
     do {
-        const int limit = kv_tile_limit(a.causal, it.s, a.group, it.tile, a.tile), np = kv_pages(limit);
+        const int limit = kv_tile_limit(a.causal, it.s, a.group, it.tile, a.tile);
+        const KvRange range = WIN ? kv_tile_range(a.window, a.sinks, a.causal, it.s, a.group, it.tile, a.tile)
+                                  : KvRange{0, 0, kv_pages(limit)};
+        auto real = [&](int p) { return WIN ? kv_range_page(range, p) : p; };
+        const int np = range.count;
         const int p0 = SPLIT ? it.page : 0, units = SPLIT ? kv_span(it) : np, p1 = min(np, p0 + units);
 
         const int ncol = it.s.n * a.group, c0 = it.tile * a.tile + 16 * NQ * w;  // the wave's first column
@@ -707,6 +768,8 @@ __device__ __forceinline__ void kv_attn_rows(const LtxKvAttnArgs& a) {
             for (int j = 0; j < 4; j++) qf[q][j] = __builtin_bit_cast(v8, *(const u32x4*)(Q + 8 * j));
         }
         const int all = kv_limit(a.causal, it.s, min(c0, ncol - 1) / a.group);  // keys that every column sees
+        // the wave's last window begins here: keys before it are not every column's
+        const int every = WIN ? kv_limit(a.causal, it.s, (min(c0 + 16 * NQ, ncol) - 1) / a.group) - a.window : 0;
 
         // Staging. A page's index is read two pages before its codes are used, its flag
         // beside them, by scalar loads (the constant address space: nothing writes them
@@ -715,7 +778,7 @@ __device__ __forceinline__ void kv_attn_rows(const LtxKvAttnArgs& a) {
         typedef const __attribute__((address_space(4))) uint32_t* scalar_ptr;
         const scalar_ptr table = (scalar_ptr)(uintptr_t)(a.b.pages + (size_t)it.b * a.b.max_pages);
         const scalar_ptr flags = (scalar_ptr)(uintptr_t)a.b.flags;
-        uint32_t next = p0 < p1 ? table[p0] : 0u;  // index of the page whose codes come next
+        uint32_t next = p0 < p1 ? table[real(p0)] : 0u;  // index of the page whose codes come next
         u32x4 x0, x1;                              // its codes and scales
         uint32_t y0, y1, flag = 0, none = 0;       // its flag, or that it is outside the pool
         uint32_t flag_s = 0, none_s = 0;           // those of the page in LDS
@@ -733,7 +796,7 @@ __device__ __forceinline__ void kv_attn_rows(const LtxKvAttnArgs& a) {
             y0 = *(const uint32_t*)(blk + at);
             y1 = *(const uint32_t*)(blk + at + 4);
             flag = flags[page];
-            next = p + 1 < p1 ? table[p + 1] : 0u;
+            next = p + 1 < p1 ? table[real(p + 1)] : 0u;
         };
         auto stage = [&](int buf) {
             const int lane = my_lane();
@@ -856,7 +919,15 @@ __device__ __forceinline__ void kv_attn_rows(const LtxKvAttnArgs& a) {
 #pragma unroll
                 for (int q = 0; q < NQ; q++) kv_set_nan(s[q], bits);
             }
-            if (none_s || (p + 1) * LTX_KV_PAGE > all)
+            if constexpr (WIN) {
+                const int page = real(p), key = page * LTX_KV_PAGE, end = key + LTX_KV_PAGE;
+                if (none_s || end > all || (key < every && end > a.sinks))
+#pragma unroll
+                    for (int q = 0; q < NQ; q++) {
+                        const int mine = limit_of(q);
+                        kv_mask_range(s[q], page, none_s ? 0 : mine, max(0, mine - a.window), a.sinks, my_lane() >> 4);
+                    }
+            } else if (none_s || (p + 1) * LTX_KV_PAGE > all)
 #pragma unroll
                 for (int q = 0; q < NQ; q++) kv_mask(s[q], p, none_s ? 0 : limit_of(q), my_lane() >> 4);
 #pragma unroll
@@ -926,7 +997,13 @@ __device__ __forceinline__ void kv_attn_rows(const LtxKvAttnArgs& a) {
             l[q] += kv_bad_query<T>(qf[q]);
             float lt = l[q] + __shfl_xor(l[q], 16, 64);
             lt += __shfl_xor(lt, 32, 64);
-            if (!idle) kv_seen(a.b, it.b, p0, p1, limit_of(q), m[q], lt);
+            if (!idle) {
+                const int mine = limit_of(q);
+                if constexpr (WIN)
+                    kv_seen_range(a.b, it.b, range, p0, p1, mine, max(0, mine - a.window), a.sinks, m[q], lt);
+                else
+                    kv_seen(a.b, it.b, p0, p1, mine, m[q], lt);
+            }
             if (c >= ncol || (!whole && part >= (size_t)a.parts)) continue;
             if (!whole) {
                 const size_t at = (part * a.b.kvh + kh) * a.tile + (c - it.tile * a.tile);
@@ -952,37 +1029,43 @@ __device__ __forceinline__ void kv_attn_rows(const LtxKvAttnArgs& a) {
             }
         }
         if (SPLIT) __syncthreads();
-    } while (SPLIT && kv_next(a, it));
+    } while (SPLIT && kv_next<WIN>(a, it));
 }
 
 // (the span loop costs the kernel that needs none 10 %: a kernel of its own)
-#define KV_ATTN_ROWS(NAME, T, NQ, SPLIT)                                            \
+#define KV_ATTN_ROWS(NAME, T, NQ, SPLIT, WIN)                                       \
     extern "C" __global__ void __launch_bounds__(512) NAME(const LtxKvAttnArgs a) { \
-        kv_attn_rows<T, NQ, SPLIT>(a);                                              \
+        kv_attn_rows<T, NQ, SPLIT, WIN>(a);                                         \
     }
-KV_ATTN_ROWS(ltx_kv_attn_f16_rows1, _Float16, 1, false)
-KV_ATTN_ROWS(ltx_kv_attn_bf16_rows1, __bf16, 1, false)
-KV_ATTN_ROWS(ltx_kv_attn_f16_rows2, _Float16, 2, false)
-KV_ATTN_ROWS(ltx_kv_attn_bf16_rows2, __bf16, 2, false)
-KV_ATTN_ROWS(ltx_kv_attn_f16_rows2_split, _Float16, 2, true)
-KV_ATTN_ROWS(ltx_kv_attn_bf16_rows2_split, __bf16, 2, true)
+KV_ATTN_ROWS(ltx_kv_attn_f16_rows1, _Float16, 1, false, false)
+KV_ATTN_ROWS(ltx_kv_attn_bf16_rows1, __bf16, 1, false, false)
+KV_ATTN_ROWS(ltx_kv_attn_f16_rows2, _Float16, 2, false, false)
+KV_ATTN_ROWS(ltx_kv_attn_bf16_rows2, __bf16, 2, false, false)
+KV_ATTN_ROWS(ltx_kv_attn_f16_rows2_split, _Float16, 2, true, false)
+KV_ATTN_ROWS(ltx_kv_attn_bf16_rows2_split, __bf16, 2, true, false)
+KV_ATTN_ROWS(ltx_kv_attn_f16_win_rows1, _Float16, 1, false, true)
+KV_ATTN_ROWS(ltx_kv_attn_bf16_win_rows1, __bf16, 1, false, true)
+KV_ATTN_ROWS(ltx_kv_attn_f16_win_rows2, _Float16, 2, false, true)
+KV_ATTN_ROWS(ltx_kv_attn_bf16_win_rows2, __bf16, 2, false, true)
+KV_ATTN_ROWS(ltx_kv_attn_f16_win_rows2_split, _Float16, 2, true, true)
+KV_ATTN_ROWS(ltx_kv_attn_bf16_win_rows2_split, __bf16, 2, true, true)
 
 // The runs of a tile into one, where items share tiles: a workgroup takes a row and query head, a wave every
 // fourth run, a lane two dims. In the runs' order: the same bits every time. Bound by
 // its launch: 5 us for four rows of 32 heads.
-template <typename T>
+template <typename T, bool WIN>
 __device__ __forceinline__ void kv_join(const LtxKvAttnArgs& a) {
     __shared__ float sx[4][LTX_HD], sml[4][2];
     const int lane = threadIdx.x & 63, row = blockIdx.x, head = blockIdx.y;
     const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     // the row's sequence, and the tiles and units of those before it
-    KvLane k = kv_lane(a, 0);
-    const int per = kv_per(a, k);
+    KvLane k = kv_lane<WIN>(a, 0);
+    const int per = kv_per<WIN>(a, k);
     uint32_t unit = 0, entity = 0;
     KvSeq s = {0, 0, 0};
     bool found = false;
     for (int base = 0; base < a.b.nseq; base += 64) {
-        if (base) k = kv_lane(a, base);
+        if (base) k = kv_lane<WIN>(a, base);
         const uint64_t here = __builtin_amdgcn_ballot_w64(row >= k.s.s0 && row < k.s.s0 + k.s.n);
         if (here) {
             const int l = __builtin_ctzll(here);
@@ -997,7 +1080,7 @@ __device__ __forceinline__ void kv_join(const LtxKvAttnArgs& a) {
     }
     if (!found) return;
     const int i = row - s.s0, kh = head / a.group;
-    const int c = i * a.group + head % a.group, tile = c / a.tile, col = c % a.tile, pages = kv_units(s.L);
+    const int c = i * a.group + head % a.group, tile = c / a.tile, col = c % a.tile, pages = kv_work<WIN>(a, s);
     unit += (uint32_t)tile * pages;
     entity += tile;
     const uint32_t i0 = unit / (uint32_t)per;
@@ -1058,5 +1141,9 @@ __device__ __forceinline__ void kv_join(const LtxKvAttnArgs& a) {
         Op<T>::cvt2(x0 * f, x1 * f);
 }
 
-extern "C" __global__ void __launch_bounds__(256) ltx_kv_join_f16(const LtxKvAttnArgs a) { kv_join<_Float16>(a); }
-extern "C" __global__ void __launch_bounds__(256) ltx_kv_join_bf16(const LtxKvAttnArgs a) { kv_join<__bf16>(a); }
+#define KV_JOIN(NAME, T, WIN) \
+    extern "C" __global__ void __launch_bounds__(256) NAME(const LtxKvAttnArgs a) { kv_join<T, WIN>(a); }
+KV_JOIN(ltx_kv_join_f16, _Float16, false)
+KV_JOIN(ltx_kv_join_bf16, __bf16, false)
+KV_JOIN(ltx_kv_join_f16_win, _Float16, true)
+KV_JOIN(ltx_kv_join_bf16_win, __bf16, true)

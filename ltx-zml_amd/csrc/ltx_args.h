@@ -405,6 +405,7 @@ typedef struct {
     int items;          // items of a cached head in the grid
     int parts;
     float scale_log2;   // log2(e) / sqrt(128)
+    int window, sinks;  // of the keys a row would see, the last and the first ones (the kernels with a window)
 } LtxKvAttnArgs;
 
 // y = a . (q s)^T (+ bias), 4-bit weights

@@ -65,3 +65,32 @@ KV_FN int kv_tile_limit(int causal, const KvSeq& s, int group, int t, int tile) 
     const int64_t c = kv_min((int64_t)(t + 1) * tile, (int64_t)s.n * group) - 1;
     return kv_limit(causal, s, (int)(c / group));
 }
+
+// ---- a window and first keys ----
+// A row that would see keys 0 .. e - 1 sees the last `window` of them and the first
+// `sinks`. Of a tile's rows, whose ends go from e0 up to e1, the first keys lie on pages 0 ..
+// ps - 1, the windows on ps + skip and on, `count` pages in all: u-th page kv_range_page.
+struct KvRange {
+    int ps, skip, count;
+};
+KV_FN KvRange kv_range(int window, int sinks, int e0, int e1) {
+    const int pw = (int)kv_max(0, (int64_t)e0 - window) / LTX_KV_PAGE, np = kv_pages(e1);
+    const int ps = (int)kv_min(pw, kv_pages((int)kv_min(sinks, e1)));
+    return {ps, pw - ps, ps + np - pw};
+}
+KV_FN int kv_range_page(const KvRange& r, int u) { return u + (u >= r.ps ? r.skip : 0); }
+KV_FN KvRange kv_tile_range(int window, int sinks, int causal, const KvSeq& s, int group, int t, int tile) {
+    return kv_range(window, sinks, kv_limit(causal, s, (int)((int64_t)t * tile / group)),
+                    kv_tile_limit(causal, s, group, t, tile));
+}
+// Work of a split call: the pages of any of the sequence's tiles, at most. With one tile, or
+// one range for all rows, they are that range's; else the ends of a tile's rows lie within
+// `rows` of each other.
+KV_FN int kv_range_units(int window, int sinks, int causal, const KvSeq& s, int group, int tile) {
+    if (s.n <= 0) return 1;
+    if (!causal || (int64_t)s.n * group <= tile)
+        return (int)kv_max(1, kv_tile_range(window, sinks, causal, s, group, 0, tile).count);
+    const int64_t rows = (int64_t)tile / group + 2;
+    const int64_t most = kv_pages((int)kv_min(sinks, s.L)) + (window + rows - 1 + LTX_KV_PAGE - 2) / LTX_KV_PAGE + 1;
+    return (int)kv_max(1, kv_min(kv_pages(s.L), most));
+}

@@ -77,6 +77,8 @@ def lib() -> C.CDLL:
         "ltx_op_kv_read": (i32, [vp, vp, vp, vp, i64, vp, i64, vp]),
         "ltx_op_kv_attention_workspace": (i32, [vp, vp, vp, i32, C.POINTER(u64)]),
         "ltx_op_kv_attention": (i32, [vp, vp, vp, vp, i64, i32, i32, vp, vp, i64, vp, u64, vp]),
+        "ltx_op_kv_attention_window_workspace": (i32, [vp, vp, vp, i32, i32, i32, i32, C.POINTER(u64)]),
+        "ltx_op_kv_attention_window": (i32, [vp, vp, vp, vp, i64, i32, i32, i32, i32, vp, vp, i64, vp, u64, vp]),
         "ltx_op_dequant": (i32, [vp, vp, vp, i32, i32, i32, vp, vp, i32, vp]),
         "ltx_rope_tables": (i32, [vp, i32, vp, vp, i32]),
         "ltx_profile_enable": (i32, [vp, i32]),
@@ -574,18 +576,44 @@ class Context:
         or None; work: a uint8 tensor of kv_attention_workspace bytes, or None
         (ltx_op_kv_attention)."""
         st = stream.cuda_stream if stream is not None else _current_stream(self.device)
-        _rows("kv_attention", batch, cache, heads, q, out)
-        if glog is not None and not (glog.shape == (batch.rows, heads) and glog.is_contiguous()
-                                     and glog.dtype == _torch_dtype(MODE_F32)
-                                     and glog.get_device() == self.device):
-            raise LtxError("kv_attention: glog must be f32 [rows, heads] on the context's device")
-        if work is not None and not (work.is_contiguous() and work.get_device() == self.device):
-            raise LtxError("kv_attention: work must be contiguous, on the context's device")
+        self._kv_attention_checks("kv_attention", cache, batch, q, out, heads, glog, work)
         self._check(lib().ltx_op_kv_attention(self.handle, cache.handle, batch.ref, _ptr(q), q.stride(0), heads,
                                               int(causal), _ptr(glog), _ptr(out), out.stride(0), _ptr(work),
                                               0 if work is None else work.numel() * work.element_size(), st),
                     "ltx_op_kv_attention")
         return out
+
+    def kv_attention_window_workspace(self, cache: KvCache, batch: KvBatch, heads: int, window: int, sinks: int = 0,
+                                      causal: bool = True) -> int:
+        """Bytes of `work` for kv_attention_window with this batch's nseq, rows and max_pages."""
+        n = C.c_uint64()
+        window, sinks = (min(x, 1 << 30) for x in (window, sinks))  # no table holds more keys
+        self._check(lib().ltx_op_kv_attention_window_workspace(self.handle, cache.handle, batch.ref, heads, int(causal),
+                                                               window, sinks, C.byref(n)),
+                    "ltx_op_kv_attention_window_workspace")
+        return n.value
+
+    def kv_attention_window(self, cache: KvCache, batch: KvBatch, q, out, heads: int, window: int, sinks: int = 0,
+                            causal: bool = True, glog=None, work=None, stream=None):
+        """kv_attention to the last `window` of the keys that a row would see and the first
+        `sinks` (ltx_op_kv_attention_window)."""
+        st = stream.cuda_stream if stream is not None else _current_stream(self.device)
+        self._kv_attention_checks("kv_attention_window", cache, batch, q, out, heads, glog, work)
+        window, sinks = (min(x, 1 << 30) for x in (window, sinks))  # no table holds more keys
+        self._check(lib().ltx_op_kv_attention_window(self.handle, cache.handle, batch.ref, _ptr(q), q.stride(0), heads,
+                                                     int(causal), window, sinks, _ptr(glog), _ptr(out), out.stride(0),
+                                                     _ptr(work), 0 if work is None else work.numel() * work.element_size(),
+                                                     st), "ltx_op_kv_attention_window")
+        return out
+
+    def _kv_attention_checks(self, name, cache, batch, q, out, heads, glog, work):
+        _rows(name, batch, cache, heads, q, out)
+        if glog is not None and not (glog.shape == (batch.rows, heads) and glog.is_contiguous()
+                                     and glog.dtype == _torch_dtype(MODE_F32)
+                                     and glog.get_device() == self.device):
+            raise LtxError(f"{name}: glog must be f32 [rows, heads] on the context's device")
+        if work is not None and not (work.is_contiguous() and work.get_device() == self.device):
+            raise LtxError(f"{name}: work must be contiguous, on the context's device")
 
     def dequant(self, q, s, out32, out16, mode=MODE_F16, stream=None):
         import torch
