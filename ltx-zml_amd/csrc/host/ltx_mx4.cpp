@@ -109,7 +109,7 @@ int ltx_op_linear_mx4(ltx_ctx* c, const void* a, const uint8_t* a_scales, const 
         g.tiles_n = (N + tile - 1) / tile;
         const int64_t n = tiles(tile);
         if (n >= 1 << 23) throw ltx::Error("too many rows or columns");  // (twice: past the last, an index stays in 31 bits)
-        std::snprintf(name, sizeof(name), "ltx_gemm_mx4_%s_%d", type, tile);
+        std::snprintf(name, sizeof(name), "ltx_gemm_mx4_%s%s_%d", out_f32 ? "f32" : type, gelu ? "_gelu" : "", tile);
         c->launch(name, (unsigned)(tile == 256 ? std::min(n, cu) : n), 1, 1, 256, &g, st);
     })
 }

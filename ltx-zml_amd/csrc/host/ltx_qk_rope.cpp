@@ -1,6 +1,7 @@
 // Rotary positions on several axes: their plan on the device, and the norm and rotation of
 // q and k. (The tables of the block forward are ltx_rope.cpp's.)
 #include <cmath>
+#include <cstdio>
 #include <algorithm>
 #include <vector>
 
@@ -140,8 +141,15 @@ int ltx_op_qk_rope(ltx_ctx* c, const ltx_rope* r, const double* pos, int rows, c
         a.rows = rows;
         a.axes = r->axes;
         a.eps = eps;
-        a.per = (int)std::max<int64_t>(1, ((int64_t)rows + (1 << 23) - 1) >> 23);  // (2^32 threads along x: one too many)
-        const char* name = mode == LTX_MODE_F16 ? "ltx_qk_rope_f16" : mode == LTX_MODE_BF16 ? "ltx_qk_rope_bf16" : "ltx_qk_rope_f32";
+        const int more = std::max(heads, kv_heads), fewer = std::min(heads, kv_heads);
+        const bool any = more > 32 || (fewer && more % fewer);
+        const bool norm = a.norm[0] || a.norm[1];
+        // workgroups that are all on the card at once (three a CU), each with its share of the rows
+        a.per = (int)std::max<int64_t>(1, any ? ((int64_t)rows + (1 << 23) - 1) >> 23
+                                              : ((int64_t)rows + 3 * c->num_cu - 1) / (3 * c->num_cu));
+        char name[32];
+        std::snprintf(name, sizeof(name), "ltx_qk_rope_%s%s",
+                      mode == LTX_MODE_F16 ? "f16" : mode == LTX_MODE_BF16 ? "bf16" : "f32", any ? "_any" : norm ? "_norm" : "");
         c->launch(name, (unsigned)(((int64_t)rows + a.per - 1) / a.per), 1, 1, 256, &a, (hipStream_t)stream);
     })
 }

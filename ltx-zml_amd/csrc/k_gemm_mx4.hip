@@ -1,9 +1,14 @@
-// GEMMs of microscaled 4-bit operands: ltx_gemm_mx4_{f16,bf16}_{256,128,64}.
+// GEMMs of microscaled 4-bit operands: ltx_gemm_mx4_{f16,bf16,f32}[_gelu]_{256,128,64}, by
+// the type of y and the tile.
 #include "gemm_mx4.h"
 
-MX4_GEMM_KERNEL(ltx_gemm_mx4_f16_256, _Float16, 8, 1)
-MX4_GEMM_KERNEL(ltx_gemm_mx4_bf16_256, __bf16, 8, 1)
-MX4_GEMM_KERNEL(ltx_gemm_mx4_f16_128, _Float16, 4, 2)
-MX4_GEMM_KERNEL(ltx_gemm_mx4_bf16_128, __bf16, 4, 2)
-MX4_GEMM_KERNEL(ltx_gemm_mx4_f16_64, _Float16, 2, 2)
-MX4_GEMM_KERNEL(ltx_gemm_mx4_bf16_64, __bf16, 2, 2)
+#define MX4_GEMM(TYPE, OUT)                                                \
+    MX4_GEMM_KERNEL(ltx_gemm_mx4_##TYPE##_256, OUT, 4, false, 1)           \
+    MX4_GEMM_KERNEL(ltx_gemm_mx4_##TYPE##_128, OUT, 2, false, 2)           \
+    MX4_GEMM_KERNEL(ltx_gemm_mx4_##TYPE##_64, OUT, 1, false, 2)            \
+    MX4_GEMM_KERNEL(ltx_gemm_mx4_##TYPE##_gelu_256, OUT, 4, true, 1)       \
+    MX4_GEMM_KERNEL(ltx_gemm_mx4_##TYPE##_gelu_128, OUT, 2, true, 2)       \
+    MX4_GEMM_KERNEL(ltx_gemm_mx4_##TYPE##_gelu_64, OUT, 1, true, 2)
+MX4_GEMM(f16, _Float16)
+MX4_GEMM(bf16, __bf16)
+MX4_GEMM(f32, float)

@@ -213,7 +213,7 @@ __device__ __forceinline__ void mx4_few(const LtxMx4LinearArgs& a) {
             u32x4 y = x.a[m][0];
             if constexpr (ROWS) y = mx4_group<T>(x.a[m], x.sa[m]);
 #pragma unroll
-            for (int t = 0; t < NT; t++) acc[m][t] = mx4_mfma(y, x.w[t], acc[m][t], x.sa[m], x.sw[t]);
+            for (int t = 0; t < NT; t++) acc[m][t] = mx4_mfma16(y, x.w[t], acc[m][t], x.sa[m], x.sw[t]);
         }
     };
     Step x[D];

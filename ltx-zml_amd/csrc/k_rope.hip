@@ -1,4 +1,6 @@
 // Norm and rotary positions of q and k on several axes.
+#include <type_traits>
+
 #include "ltx_device.h"
 
 // Eight values of a row.
@@ -88,8 +90,120 @@ __device__ __forceinline__ void rope_sums(float& x, float& y, float (*red)[2]) {
     y = red[0][1] + red[1][1] + red[2][1] + red[3][1];
 }
 
-// Thread t takes head t / 8 (and every 32nd after it) and pairs 8 (t % 8) .. + 7, so that
-// the two values of a pair are its own; a workgroup takes a.per rows, one after another.
+// The sum over a wave's lanes, for all of them.
+__device__ __forceinline__ float rope_wave_sum(float x) {
+    auto add = [&](auto C, auto M) {
+        const int y = __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), decltype(C)::value, decltype(M)::value, 0xf,
+                                                  false);
+        x += __builtin_bit_cast(float, y);
+    };
+    typedef std::integral_constant<int, 0xf> All;
+    add(std::integral_constant<int, 0x111>{}, All{});
+    add(std::integral_constant<int, 0x112>{}, All{});
+    add(std::integral_constant<int, 0x114>{}, All{});
+    add(std::integral_constant<int, 0x118>{}, All{});
+    add(std::integral_constant<int, 0x142>{}, std::integral_constant<int, 0xa>{});
+    add(std::integral_constant<int, 0x143>{}, std::integral_constant<int, 0xc>{});
+    return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, x), 63));
+}
+
+// Up to 32 heads, those of the set with fewer a divisor of the other's: thread t takes head
+// h = t / 8 of the larger set, pairs 8 (t % 8) .. + 7, and of the other set head h / r where
+// h is a multiple of r, their ratio: the plan's head of both, so one sine and cosine a pair
+// serve both, and what the pairs turn by stays in registers (the weights in LDS) while the
+// workgroup goes through its a.per rows. The next row's values are on their way while it
+// works on one.
+template <typename T, bool NORM>
+__device__ __forceinline__ void qk_rope_rows(const LtxRopeArgs& a) {
+    __shared__ double spos[4][2][8];
+    __shared__ float red[2][4][2];
+    __shared__ f32x4 wt[NORM ? 2 : 1][4][256];  // a thread's own weights: in registers they cost a third of the waves
+    const int h0 = threadIdx.x >> 3, o = threadIdx.x & 7, lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+    const int big = a.heads[1] > a.heads[0], ratio = a.heads[!big] ? a.heads[big] / a.heads[!big] : 1;
+    const bool mine[2] = {h0 < a.heads[big], a.heads[!big] && h0 < a.heads[big] && h0 % ratio == 0};
+    const int at[2] = {LTX_HD * h0 + 8 * o, LTX_HD * (h0 / ratio) + 8 * o};
+    const int row0 = blockIdx.x * a.per, end = min(a.rows, row0 + a.per);
+    RopePairs p;
+    if (mine[0]) p.load(a, 8 * (h0 / a.group[big]) + o);
+    if (NORM)
+#pragma unroll
+        for (int m = 0; m < 2; m++)
+            if (const float* n = a.norm[m ^ big]; mine[m] && n)
+#pragma unroll
+                for (int j = 0; j < 4; j++) wt[m][j][threadIdx.x] = *(const f32x4*)(n + at[m] + 4 * (j & 1) + 64 * (j >> 1));
+    RopeRow<T> x[2][2];
+    double pos = 0;
+    auto load = [&](int row) {
+#pragma unroll
+        for (int m = 0; m < 2; m++)
+            if (mine[m]) {
+                const size_t i = (size_t)row * a.ldx[m ^ big] + at[m];
+                x[m][0].load(a.x[m ^ big], i);
+                x[m][1].load(a.x[m ^ big], i + 64);
+            }
+        if (lane < a.axes) pos = a.pos[(size_t)row * a.axes + lane];
+    };
+    load(row0);
+    for (int row = row0; row < end; row++) {
+        float v[2][2][8], sum[2] = {0.f, 0.f};
+#pragma unroll
+        for (int m = 0; m < 2; m++)
+            if (mine[m])
+#pragma unroll
+                for (int j = 0; j < 8; j++) {
+                    v[m][0][j] = x[m][0].get(j);
+                    v[m][1][j] = x[m][1].get(j);
+                    if (NORM) {
+                        sum[m] = __builtin_fmaf(v[m][0][j], v[m][0][j], sum[m]);
+                        sum[m] = __builtin_fmaf(v[m][1][j], v[m][1][j], sum[m]);
+                    }
+                }
+        // (a wave's own copy: its LDS operations come in order)
+        if (lane < 8) spos[w][row & 1][lane] = pos;
+        if (row + 1 < end) load(row + 1);
+        if (NORM) {
+            sum[0] = rope_wave_sum(sum[0]);
+            sum[1] = rope_wave_sum(sum[1]);
+            if (lane == 0) {
+                red[row & 1][w][0] = sum[0];
+                red[row & 1][w][1] = sum[1];
+            }
+        }
+        float c[8], s[8];
+        if (mine[0]) rope_turns(p, spos[w][row & 1], c, s);
+        if (NORM) {
+            __syncthreads();
+#pragma unroll
+            for (int m = 0; m < 2; m++) {
+                if (!mine[m] || !a.norm[m ^ big]) continue;
+                const float all = red[row & 1][0][m] + red[row & 1][1][m] + red[row & 1][2][m] + red[row & 1][3][m];
+                const float inv = 1.0f / sqrtf(all / (float)(LTX_HD * a.heads[m ^ big]) + a.eps);
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    const f32x4 n = wt[m][j][threadIdx.x];
+#pragma unroll
+                    for (int e = 0; e < 4; e++) v[m][j >> 1][4 * (j & 1) + e] *= inv * n[e];
+                }
+            }
+        }
+#pragma unroll
+        for (int m = 0; m < 2; m++) {
+            if (!mine[m]) continue;
+            float y[2][8];
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                y[0][j] = v[m][0][j] * c[j] - v[m][1][j] * s[j];
+                y[1][j] = v[m][1][j] * c[j] + v[m][0][j] * s[j];
+            }
+            const size_t d = (size_t)row * a.ldy[m ^ big] + at[m];
+            RopeRow<T>::store(a.y[m ^ big], d, y[0]);
+            RopeRow<T>::store(a.y[m ^ big], d + 64, y[1]);
+        }
+    }
+}
+
+// Any heads: thread t takes head t / 8 and every 32nd after it. A row that is normed is read
+// twice.
 template <typename T>
 __device__ __forceinline__ void qk_rope(const LtxRopeArgs& a) {
     __shared__ float red[2][4][2];
@@ -146,8 +260,14 @@ __device__ __forceinline__ void qk_rope(const LtxRopeArgs& a) {
     }
 }
 
-#define QK_ROPE(NAME, T) \
-    extern "C" __global__ void __launch_bounds__(256) NAME(const LtxRopeArgs a) { qk_rope<T>(a); }
-QK_ROPE(ltx_qk_rope_f16, _Float16)
-QK_ROPE(ltx_qk_rope_bf16, __bf16)
-QK_ROPE(ltx_qk_rope_f32, float)
+#define QK_ROPE(NAME, ...) \
+    extern "C" __global__ void __launch_bounds__(256, 3) NAME(const LtxRopeArgs a) { __VA_ARGS__(a); }
+QK_ROPE(ltx_qk_rope_f16, qk_rope_rows<_Float16, false>)
+QK_ROPE(ltx_qk_rope_bf16, qk_rope_rows<__bf16, false>)
+QK_ROPE(ltx_qk_rope_f32, qk_rope_rows<float, false>)
+QK_ROPE(ltx_qk_rope_f16_norm, qk_rope_rows<_Float16, true>)
+QK_ROPE(ltx_qk_rope_bf16_norm, qk_rope_rows<__bf16, true>)
+QK_ROPE(ltx_qk_rope_f32_norm, qk_rope_rows<float, true>)
+QK_ROPE(ltx_qk_rope_f16_any, qk_rope<_Float16>)
+QK_ROPE(ltx_qk_rope_bf16_any, qk_rope<__bf16>)
+QK_ROPE(ltx_qk_rope_f32_any, qk_rope<float>)
