@@ -29,9 +29,9 @@ typedef __attribute__((address_space(3))) void* lds_vptr;
 typedef int i32x8 __attribute__((ext_vector_type(8)));
 
 #define MX4_RSRC_W3 0x00020000
-#define MX4_WAIT_VM0 ((7 << 4) | (15 << 8))
+// s_waitcnt: vmcnt(n) and lgkmcnt(0)
+#define MX4_WAIT(n) (((n) & 15) | (((n) >> 4) << 14) | (7 << 4))
 #define MX4_WAIT_LGKM0 (15 | (3 << 14) | (7 << 4))
-#define MX4_WAIT_ALL0 (7 << 4)
 
 // One __shared__ object per matrix and stage: the compiler's LDS-DMA alias tracking then
 // waits only for the stage that a read touches. KIND 0: A, 1: W, 2: scale words [A groups 0
@@ -67,16 +67,8 @@ __device__ __forceinline__ f32x16 mx4_mfma32(u32x4 a, u32x4 b, f32x16 c, uint32_
                                                            (int)sb);
 }
 
-template <typename Out>
-__device__ __forceinline__ void mx4_put(void* y, size_t at, float v) {
-    if constexpr (sizeof(Out) == 4)
-        ((float*)y)[at] = v;
-    else
-        ((uint16_t*)y)[at] = Op<Out>::bits(v);
-}
-
-// Out: the type of y, f32 or 16-bit.
-template <typename Out, int NB, bool GELU>
+// Out: the type of y, f32 or 16-bit. WIDE: its rows start on 16 bytes.
+template <typename Out, int NB, bool GELU, bool WIDE>
 struct Mx4Gemm {
     static constexpr int TM = 64 * NB;       // rows and columns of the output tile
     static constexpr int ND = 2 * NB;        // code DMA instructions of a K-tile, wave and matrix
@@ -85,11 +77,12 @@ struct Mx4Gemm {
     const LtxMx4LinearArgs& a;
     f32x16 acc[NB][NB];
     __amdgpu_buffer_rsrc_t ra_, rb_, rs_;
-    uint32_t ga[ND];            // per-lane source offsets of the DMA instructions, K-tile 0
+    uint32_t ga[2];             // per-lane source offsets of even and odd DMA instructions, K-tile 0
     uint32_t gs, gstep;         // of the scale words, and bytes to those of the next 128 k
     int lw, lsw;                // this wave's DMA destinations within a stage (codes, scale words)
-    uint32_t offa[4], offb[4];  // fragment reads of step t (row block i adds 4096 i)
-    uint32_t sa_, sb_, shift;   // of the scale words, steps 0 and 1 (row block i adds 128 i)
+    uint32_t off, soff;         // A's fragments of step 0 (row block i adds 4096 i) and scale words (128 i)
+    int ofw, sofw;              // from there to W's
+    uint32_t shift;
     u32x4 fa[2][NB], fb[2][NB];     // fragments of even and odd steps
     uint32_t xa[2][NB], xb[2][NB];  // scale words of the tile's first and last two steps
 
@@ -108,19 +101,21 @@ struct Mx4Gemm {
         return mx4_stage<2, S, 16 * TM>();
     }
 
-    // DMA instruction g of K-tile k into stage S: scale words first, then A, then W. The
-    // whole offset is the lane's, so that the bounds check covers it.
+    // DMA instruction g of K-tile k into stage S: scale words first, then A, then W. (The
+    // bounds check takes the scalar offset in.)
     template <int S>
     __device__ __forceinline__ void dma1(int g, int k, int l, int ls) {
         if (g < NS)
             __builtin_amdgcn_raw_ptr_buffer_load_lds(rs_, (lds_vptr)(stage_s<S>() + ls + 256 * g), 4,
-                                                     gs + 256 * g + 2 * k * gstep, 0, 0, 0);
+                                                     gs, 2 * k * gstep + 256 * g, 0, 0);
         else if (g < NS + ND)
             __builtin_amdgcn_raw_ptr_buffer_load_lds(ra_, (lds_vptr)(stage_a<S>() + l + 1024 * (g - NS)), 16,
-                                                     ga[g - NS] + 128 * k, 0, 0, 0);
+                                                     ga[(g - NS) & 1],
+                                                     128 * k + 16 * a.K * ((g - NS) >> 1 << 1) / 4, 0, 0);
         else
             __builtin_amdgcn_raw_ptr_buffer_load_lds(rb_, (lds_vptr)(stage_b<S>() + l + 1024 * (g - NS - ND)), 16,
-                                                     ga[g - NS - ND] + 128 * k, 0, 0, 0);
+                                                     ga[(g - NS) & 1],
+                                                     128 * k + 16 * a.K * ((g - NS - ND) >> 1 << 1) / 4, 0, 0);
     }
     template <int S>
     __device__ __forceinline__ void dma(int k) {
@@ -151,10 +146,12 @@ struct Mx4Gemm {
     template <int STEP, int RS, int RSTEP, int DS, bool FIRST = false>
     __device__ __forceinline__ void region(int g0, int g1, int kd) {
         constexpr int F = STEP & 1, X = (STEP >> 1) & 1, NM = NB * NB, NR = RSTEP < 4 ? 2 * NB : 0, R = RSTEP & 3;
-        const uint8_t* pa = stage_a<RS>() + mx4_vofs(offa[R]);
-        const uint8_t* pb = stage_b<RS>() + mx4_vofs(offb[R]);
-        const uint8_t* qa = stage_s<RS>() + mx4_vofs(sa_) + 4 * TM * (R >> 1);
-        const uint8_t* qb = stage_s<RS>() + mx4_vofs(sb_) + 4 * TM * (R >> 1);
+        // (chunk 2 t + h in its slot: the bits of 2 t flip)
+        const uint32_t at = mx4_vofs(off) ^ (32 * R), sat = mx4_vofs(soff);
+        const uint8_t* pa = stage_a<RS>() + at;
+        const uint8_t* pb = stage_b<RS>() + at + mx4_sofs(ofw);
+        const uint8_t* qa = stage_s<RS>() + sat + 4 * TM * (R >> 1);
+        const uint8_t* qb = stage_s<RS>() + sat + mx4_sofs(sofw) + 4 * TM * (R >> 1);
         const int l = mx4_sofs(lw), ls = mx4_sofs(lsw);
         if (STEP < 4 && F == 0) {  // the lane's bytes: 0 for this step, 2 for the next
 #pragma unroll
@@ -185,9 +182,23 @@ struct Mx4Gemm {
     template <bool WAIT = true>
     __device__ __forceinline__ void meet() {
         __builtin_amdgcn_sched_barrier(0);
-        __builtin_amdgcn_s_waitcnt(WAIT ? MX4_WAIT_ALL0 : MX4_WAIT_LGKM0);
+        __builtin_amdgcn_s_waitcnt(WAIT ? MX4_WAIT(0) : MX4_WAIT_LGKM0);
         __builtin_amdgcn_s_barrier();
         __builtin_amdgcn_sched_barrier(0);
+    }
+
+    // The products stay ahead of this: the compiler moved those of the last steps behind the
+    // epilogue's branches, away from the reads they run beside.
+    __device__ __forceinline__ void hold() {
+#pragma unroll
+        for (int i = 0; i < NB; i++)
+#pragma unroll
+            for (int j = 0; j < NB; j++) {
+                if constexpr (NB == 4)
+                    asm volatile("" : "+a"(acc[i][j]));
+                else
+                    asm volatile("" : "+v"(acc[i][j]));
+            }
     }
 
     // Tile k of stage S, from behind its step 2: entered after a barrier, the fragments of
@@ -202,52 +213,65 @@ struct Mx4Gemm {
         meet();
     }
 
-    // y of the wave's blocks. W's rows are the products' rows, so that a lane holds runs of four
-    // columns of one row of y; in 16 bits the lanes' halves exchange two runs, and each stores
-    // eight columns. Nothing goes through LDS, whose stages hold the next tile's operands.
-    // FULL: all of it is inside y, whose rows start on 16 bytes.
-    template <bool FULL>
-    __device__ __forceinline__ void store(int mw, int nw) {
+    // y of the wave's blocks, through a resource that begins at the tile's first row: rows
+    // behind the last, and columns (offset ~0), are not stored, without a branch. W's rows are
+    // the products' rows, so that a lane holds runs of four columns of one row of y; in 16 bits
+    // the lanes' halves exchange two runs, and each stores eight columns. Nothing goes through
+    // LDS, whose stages hold the next tile's operands.
+    __device__ __forceinline__ void store(__amdgpu_buffer_rsrc_t ry, int wm, int nw) {
         const int lane = opaque_tid() & 63, h = lane >> 5;
-        constexpr bool F32 = sizeof(Out) == 4;
-        typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));
+        constexpr int E = sizeof(Out);
 #pragma unroll
         for (int j = 0; j < NB; j++) {
             const int n = nw + 32 * j + 4 * h;
             f32x4 bias[4];
 #pragma unroll
-            for (int g = 0; g < 4; g++) {
-                bias[g] = f32x4{0, 0, 0, 0};
-                if (FULL) {
-                    if (a.bias) bias[g] = *(const f32x4u*)(a.bias + n + 8 * g);
-                } else {
+            for (int g = 0; g < 4; g++) bias[g] = f32x4{0, 0, 0, 0};
+            if (a.bias && nw + 32 * (j + 1) <= a.N) {
+                // scalar loads: a vector load's wait would be for the DMA ahead of it too
+                typedef const __attribute__((address_space(4))) float* scalar_ptr;
+                const scalar_ptr b = (scalar_ptr)(uintptr_t)(a.bias + nw + 32 * j);
 #pragma unroll
-                    for (int e = 0; e < 4; e++)
-                        if (a.bias && n + 8 * g + e < a.N) bias[g][e] = a.bias[n + 8 * g + e];
+                for (int r = 0; r < 16; r++) {
+                    const int c = 8 * (r >> 2) + (r & 3);
+                    const float lo = b[c], hi = b[c + 4];
+                    bias[r >> 2][r & 3] = h ? hi : lo;
                 }
+            } else if (a.bias && nw + 32 * j < a.N) {
+                const __amdgpu_buffer_rsrc_t rb =
+                    __builtin_amdgcn_make_buffer_rsrc((void*)(a.bias + nw), 0, 4 * (a.N - nw), MX4_RSRC_W3);
+#pragma unroll
+                for (int r = 0; r < 16; r++)
+                    bias[r >> 2][r & 3] = __builtin_bit_cast(
+                        float, __builtin_amdgcn_raw_buffer_load_b32(rb, 4 * (n - nw + 8 * (r >> 2) + (r & 3)), 0, 0));
+                __builtin_amdgcn_s_waitcnt(MX4_WAIT(0));  // (here, not where the sides meet)
             }
 #pragma unroll
             for (int i = 0; i < NB; i++) {
-                const int m = mw + 32 * i + (lane & 31);
+                const uint32_t at = (uint32_t)(wm + 32 * i + (lane & 31)) * (uint32_t)a.N;
                 float v[16];
 #pragma unroll
                 for (int r = 0; r < 16; r++) {
                     v[r] = acc[i][j][r] + bias[r >> 2][r & 3];
                     if (GELU) v[r] = gelu_tanh(v[r]);
                 }
-                if (!FULL) {
+                auto to = [&](int c) { return c < a.N ? (at + c) * E : ~0u; };
+                if constexpr (!WIDE) {
 #pragma unroll
                     for (int r = 0; r < 16; r++) {
-                        const int c = n + 8 * (r >> 2) + (r & 3);
-                        if (m < a.M && c < a.N) mx4_put<Out>(a.y, (size_t)m * a.N + c, v[r]);
+                        const uint32_t d = to(n + 8 * (r >> 2) + (r & 3));
+                        if constexpr (E == 4)
+                            __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(uint32_t, v[r]), ry, d, 0, 0);
+                        else
+                            __builtin_amdgcn_raw_buffer_store_b16(Op<Out>::bits(v[r]), ry, d, 0, 0);
                     }
-                } else if constexpr (F32) {
-                    float* y = (float*)a.y + (size_t)m * a.N + n;
+                } else if constexpr (E == 4) {
 #pragma unroll
                     for (int g = 0; g < 4; g++)
-                        *(f32x4*)(y + 8 * g) = f32x4{v[4 * g], v[4 * g + 1], v[4 * g + 2], v[4 * g + 3]};
+                        __builtin_amdgcn_raw_buffer_store_b128(
+                            __builtin_bit_cast(u32x4, (f32x4){v[4 * g], v[4 * g + 1], v[4 * g + 2], v[4 * g + 3]}), ry,
+                            to(n + 8 * g), 0, 0);
                 } else {
-                    uint16_t* y = (uint16_t*)a.y + (size_t)m * a.N + nw + 32 * j + 8 * h;
 #pragma unroll
                     for (int g = 0; g < 4; g += 2) {
                         const auto p = __builtin_amdgcn_permlane32_swap(
@@ -255,7 +279,9 @@ struct Mx4Gemm {
                         const auto q = __builtin_amdgcn_permlane32_swap(Op<Out>::cvt2(v[4 * g + 2], v[4 * g + 3]),
                                                                         Op<Out>::cvt2(v[4 * g + 6], v[4 * g + 7]), false,
                                                                         false);
-                        *(u32x4*)(y + 8 * g) = u32x4{(uint32_t)p[0], (uint32_t)q[0], (uint32_t)p[1], (uint32_t)q[1]};
+                        __builtin_amdgcn_raw_buffer_store_b128(
+                            u32x4{(uint32_t)p[0], (uint32_t)q[0], (uint32_t)p[1], (uint32_t)q[1]}, ry,
+                            to(n + 4 * h + 8 * g), 0, 0);
                     }
                 }
             }
@@ -263,17 +289,17 @@ struct Mx4Gemm {
     }
 
     // Resources that begin at the tile's first row (rows behind the last read as zeros), and
-    // the DMA of its first two K-tiles.
-    __device__ __forceinline__ void begin(int w, int m0, int n0) {
+    // the DMA of its first two K-tiles (there false: of nothing, zeros).
+    __device__ __forceinline__ void begin(int w, int m0, int n0, bool there) {
         const int G = a.K / 128, lane = threadIdx.x & 63;
         const uint32_t row = (uint32_t)a.K / 2;
         ra_ = __builtin_amdgcn_make_buffer_rsrc((void*)(a.a + (size_t)m0 * row), 0,
-                                                (int)((uint32_t)min(TM, a.M - m0) * row), MX4_RSRC_W3);
+                                                there ? (int)((uint32_t)min(TM, a.M - m0) * row) : 0, MX4_RSRC_W3);
         rb_ = __builtin_amdgcn_make_buffer_rsrc((void*)(a.w + (size_t)n0 * row), 0,
-                                                (int)((uint32_t)min(TM, a.N - n0) * row), MX4_RSRC_W3);
+                                                there ? (int)((uint32_t)min(TM, a.N - n0) * row) : 0, MX4_RSRC_W3);
         const int rows = w < 2 ? a.M : a.N, first = w < 2 ? m0 : n0;
         rs_ = __builtin_amdgcn_make_buffer_rsrc((void*)((w < 2 ? a.as : a.ws) + 4 * (size_t)first), 0,
-                                                (int)(4u * ((uint32_t)G * (uint32_t)rows - (uint32_t)first)),
+                                                there ? (int)(4u * ((uint32_t)G * (uint32_t)rows - (uint32_t)first)) : 0,
                                                 MX4_RSRC_W3);
         gstep = 4u * (uint32_t)rows;
         gs = 4 * lane + (w & 1) * gstep;
@@ -290,24 +316,25 @@ struct Mx4Gemm {
         lsw = 4 * TM * w;
         {
             const int h = lane >> 5, r = lane & 31;
-#pragma unroll
-            for (int t = 0; t < 4; t++) {
-                offa[t] = (wm + r) * 128 + 16 * ((2 * t + h) ^ ((r >> 1) & 7));
-                offb[t] = (wn + r) * 128 + 16 * ((2 * t + h) ^ ((r >> 1) & 7));
-            }
-            sa_ = 4 * (wm + r);
-            sb_ = 8 * TM + 4 * (wn + r);
+            off = (wm + r) * 128 + 16 * (h ^ ((r >> 1) & 7));
+            ofw = (wn - wm) * 128;
+            soff = 4 * (wm + r);
+            sofw = 8 * TM + 4 * (wn - wm);
             shift = 8 * h;
         }
 #pragma unroll
-        for (int i = 0; i < ND; i++) {
+        for (int i = 0; i < 2; i++) {
             const int tr = 8 * (ND * w + i) + (lane >> 3);
             ga[i] = (uint32_t)tr * ((uint32_t)a.K / 2) + 16u * ((lane & 7) ^ ((tr >> 1) & 7));
         }
         const int ntiles = a.tiles_m * a.tiles_n;
+        auto tile_at = [&](int i) {  // (in scalar registers, whatever the compiler makes of the loop)
+            const TileIdx t = tile_of(i, a.tiles_m, a.tiles_n);
+            return TileIdx{__builtin_amdgcn_readfirstlane(t.tm), __builtin_amdgcn_readfirstlane(t.tn)};
+        };
         int item = blockIdx.x;
-        TileIdx ti = tile_of(item, a.tiles_m, a.tiles_n);
-        begin(w, ti.tm * TM, ti.tn * TM);
+        TileIdx ti = tile_at(item);
+        begin(w, ti.tm * TM, ti.tn * TM, true);
         meet();
         while (true) {
             // the tile's first two K-tiles have landed for all waves
@@ -320,29 +347,34 @@ struct Mx4Gemm {
                 tile<0, true>(k);
                 tile<1, true>(k + 1);
             }
-            tile<0, false>(nk - 2);
-            // every wave has what is left in registers: the next tile's operands come in while
-            // it is multiplied and y is formed, and y's stores leave beside the next tile
-            const int m0 = ti.tm * TM + wm, n0 = ti.tn * TM + wn;
+            const int m0 = ti.tm * TM, n0 = ti.tn * TM + wn;
+            const __amdgpu_buffer_rsrc_t ry = __builtin_amdgcn_make_buffer_rsrc(
+                (void*)((Out*)a.y + (size_t)m0 * a.N), 0,
+                (int)((uint32_t)min(TM, a.M - m0) * (uint32_t)a.N * (uint32_t)sizeof(Out)), MX4_RSRC_W3);
             item += gridDim.x;
             const bool more = item < ntiles;
-            if (more) {
-                ti = tile_of(item, a.tiles_m, a.tiles_n);
-                begin(w, ti.tm * TM, ti.tn * TM);
-            }
+            ti = tile_at(more ? item : (int)blockIdx.x);
+            tile<0, false>(nk - 2);
+            // Every wave has what is left in registers: the next tile's operands come in while
+            // it is multiplied and y is formed, and y's stores leave beside the next tile.
+            // (Behind the last tile no operand is read.)
+            begin(w, ti.tm * TM, ti.tn * TM, more);
             region<3, 0, 4, 0>(0, 0, 0);
-            if (more) meet();
-            if (a.wide && m0 + 32 * NB <= a.M && n0 + 32 * NB <= a.N)
-                store<true>(m0, n0);
-            else
-                store<false>(m0, n0);
+            hold();
+            // the stores come behind the DMA, in order: it has landed when only they are left
+            constexpr int stores = NB * NB * (!WIDE ? 16 : sizeof(Out) == 4 ? 4 : 2);
+            store(ry, wm, n0);
+            __builtin_amdgcn_sched_barrier(0);
+            __builtin_amdgcn_s_waitcnt(MX4_WAIT(stores < 63 ? stores : 63));
+            __builtin_amdgcn_s_barrier();
+            __builtin_amdgcn_sched_barrier(0);
             if (!more) break;
         }
     }
 };
 
-#define MX4_GEMM_KERNEL(NAME, OUT_, NB_, GELU_, PER_)                                        \
+#define MX4_GEMM_KERNEL(NAME, OUT_, NB_, GELU_, WIDE_, PER_)                                 \
     extern "C" __global__ void __launch_bounds__(256, PER_) NAME(const LtxMx4LinearArgs a) { \
-        Mx4Gemm<OUT_, NB_, GELU_> k(a);                                                      \
+        Mx4Gemm<OUT_, NB_, GELU_, WIDE_> k(a);                                               \
         k.run();                                                                             \
     }

@@ -74,7 +74,8 @@ int ltx_op_linear_mx4(ltx_ctx* c, const void* a, const uint8_t* a_scales, const 
         if (((uintptr_t)a_scales | (uintptr_t)scales) & 3) throw ltx::Error("scales must start on 4 bytes");
         if ((uintptr_t)bias & 3 || (uintptr_t)y & (out_f32 ? 3 : 1))
             throw ltx::Error("bias and y must be aligned to their types");
-        if (K > ltx::kMaxK || !ltx::scales_fit(M, K) || !ltx::scales_fit(N, K) || N >= 1 << 27)
+        // (32-bit offsets of a tile's 256 rows of y)
+        if (K > ltx::kMaxK || !ltx::scales_fit(M, K) || !ltx::scales_fit(N, K) || N >= 1 << 21)
             throw ltx::Error("too many rows or columns");
         HIPC(hipSetDevice(c->device));
         hipStream_t st = (hipStream_t)stream;
@@ -91,7 +92,6 @@ int ltx_op_linear_mx4(ltx_ctx* c, const void* a, const uint8_t* a_scales, const 
         g.K = K;
         g.gelu = gelu != 0;
         g.out_f32 = out_f32 != 0;
-        g.wide = ((uintptr_t)y & 15) == 0 && N % (out_f32 ? 4 : 8) == 0;
         char name[48];
         const int64_t cu = c->num_cu;
         auto tiles = [&](int64_t t) { return (M + t - 1) / t * ((N + t - 1) / t); };
@@ -104,12 +104,14 @@ int ltx_op_linear_mx4(ltx_ctx* c, const void* a, const uint8_t* a_scales, const 
                       st);
             return LTX_OK;
         }
-        const int tile = c->mx4_tile > 16 ? c->mx4_tile : tiles(256) >= cu ? 256 : tiles(128) >= cu ? 128 : 64;
+        const bool odd = (uintptr_t)y & 15 || N % (out_f32 ? 4 : 8);  // rows of y that do not start on 16 bytes
+        const int tile = odd ? 128 : c->mx4_tile > 16 ? c->mx4_tile : tiles(256) >= cu ? 256 : tiles(128) >= cu ? 128 : 64;
         g.tiles_m = (M + tile - 1) / tile;
         g.tiles_n = (N + tile - 1) / tile;
         const int64_t n = tiles(tile);
         if (n >= 1 << 23) throw ltx::Error("too many rows or columns");  // (twice: past the last, an index stays in 31 bits)
-        std::snprintf(name, sizeof(name), "ltx_gemm_mx4_%s%s_%d", out_f32 ? "f32" : type, gelu ? "_gelu" : "", tile);
+        const char* form = odd ? "odd" : tile == 256 ? "256" : tile == 128 ? "128" : "64";
+        std::snprintf(name, sizeof(name), "ltx_gemm_mx4_%s%s_%s", out_f32 ? "f32" : type, gelu ? "_gelu" : "", form);
         c->launch(name, (unsigned)(tile == 256 ? std::min(n, cu) : n), 1, 1, 256, &g, st);
     })
 }

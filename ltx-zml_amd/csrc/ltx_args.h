@@ -444,7 +444,6 @@ typedef struct {
     int M, N, K;
     int gelu, out_f32;
     int tiles_m, tiles_n;
-    int wide;           // rows of y start on 16 bytes
 } LtxMx4LinearArgs;
 // Rows of a that the linear of few rows takes in 16 bits.
 #define LTX_MX4_ROWS 64
