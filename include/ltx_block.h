@@ -309,10 +309,12 @@ int ltx_op_mx4_values(ltx_ctx* ctx, const uint8_t* q, const uint8_t* scales, voi
  * from ltx_op_mx4_quantise). a_scales NULL: a holds at most 64 rows of 16-bit values of the
  * mode, [M][K], which the call quantises on its way, with the bits of
  * ltx_op_mx4_quantise. y f32 (out_f32, and always in mode F32) or 16-bit. A group that is
- * NaN makes its row of y, or column, NaN. No scratch: calls may overlap and be captured.
+ * NaN makes its row of y, or column, NaN. Calls may overlap and be captured. (More than 16
+ * rows in values go through scratch of the context, as in ltx_op_attention: a call being
+ * captured, or one that finds no memory, takes none, with the same bits, and longer.)
  * Refused: M, N or K not positive, K no multiple of 128 or above 2^23, a or q not on 16
  * bytes, scales not on 4, bias or y not aligned to their types, an unknown mode, mode F32
- * with a in values, M or N times (K / 128 + 8) from 2^29 on, N from 2^21, more than 2^23
+ * with a in values, M or N times (K / 128 + 8) from 2^29 on, N from 2^21, more than 2^22
  * tiles. */
 int ltx_op_linear_mx4(ltx_ctx* ctx, const void* a, const uint8_t* a_scales, const uint8_t* q, const uint8_t* scales,
                       const float* bias, void* y, int out_f32, int M, int N, int K, int gelu, int mode, void* stream);

@@ -67,8 +67,11 @@ __device__ __forceinline__ f32x16 mx4_mfma32(u32x4 a, u32x4 b, f32x16 c, uint32_
                                                            (int)sb);
 }
 
-// Out: the type of y, f32 or 16-bit. WIDE: its rows start on 16 bytes.
-template <typename Out, int NB, bool GELU, bool WIDE>
+// Out: the type of y, f32 or 16-bit. WIDE: its rows start on 16 bytes. KG: groups of four
+// waves that take a tile's K-tiles in turn, each with stages of its own, and whose sums are
+// added in the groups' order: where there are few tiles, a K-tile's latency is what counts
+// (64 x 64 tiles, K = 16,384: 0.5 us a K-tile, of which 0.05 are products).
+template <typename Out, int NB, bool GELU, bool WIDE, int KG>
 struct Mx4Gemm {
     static constexpr int TM = 64 * NB;       // rows and columns of the output tile
     static constexpr int ND = 2 * NB;        // code DMA instructions of a K-tile, wave and matrix
@@ -83,6 +86,7 @@ struct Mx4Gemm {
     uint32_t off, soff;         // A's fragments of step 0 (row block i adds 4096 i) and scale words (128 i)
     int ofw, sofw;              // from there to W's
     uint32_t shift;
+    int kg;                     // this wave's group
     u32x4 fa[2][NB], fb[2][NB];     // fragments of even and odd steps
     uint32_t xa[2][NB], xb[2][NB];  // scale words of the tile's first and last two steps
 
@@ -90,15 +94,15 @@ struct Mx4Gemm {
 
     template <int S>
     static __device__ __forceinline__ uint8_t* stage_a() {
-        return mx4_stage<0, S, 128 * TM>();
+        return mx4_stage<0, S, 128 * TM * KG>();
     }
     template <int S>
     static __device__ __forceinline__ uint8_t* stage_b() {
-        return mx4_stage<1, S, 128 * TM>();
+        return mx4_stage<1, S, 128 * TM * KG>();
     }
     template <int S>
     static __device__ __forceinline__ uint8_t* stage_s() {
-        return mx4_stage<2, S, 16 * TM>();
+        return mx4_stage<2, S, 16 * TM * KG>();
     }
 
     // DMA instruction g of K-tile k into stage S: scale words first, then A, then W. (The
@@ -107,15 +111,15 @@ struct Mx4Gemm {
     __device__ __forceinline__ void dma1(int g, int k, int l, int ls) {
         if (g < NS)
             __builtin_amdgcn_raw_ptr_buffer_load_lds(rs_, (lds_vptr)(stage_s<S>() + ls + 256 * g), 4,
-                                                     gs, 2 * k * gstep + 256 * g, 0, 0);
+                                                     gs, 2 * (KG * k + kg) * gstep + 256 * g, 0, 0);
         else if (g < NS + ND)
             __builtin_amdgcn_raw_ptr_buffer_load_lds(ra_, (lds_vptr)(stage_a<S>() + l + 1024 * (g - NS)), 16,
                                                      ga[(g - NS) & 1],
-                                                     128 * k + 16 * a.K * ((g - NS) >> 1 << 1) / 4, 0, 0);
+                                                     128 * (KG * k + kg) + 16 * a.K * ((g - NS) >> 1 << 1) / 4, 0, 0);
         else
             __builtin_amdgcn_raw_ptr_buffer_load_lds(rb_, (lds_vptr)(stage_b<S>() + l + 1024 * (g - NS - ND)), 16,
                                                      ga[(g - NS) & 1],
-                                                     128 * k + 16 * a.K * ((g - NS - ND) >> 1 << 1) / 4, 0, 0);
+                                                     128 * (KG * k + kg) + 16 * a.K * ((g - NS - ND) >> 1 << 1) / 4, 0, 0);
     }
     template <int S>
     __device__ __forceinline__ void dma(int k) {
@@ -211,6 +215,41 @@ struct Mx4Gemm {
         region<1, S ^ 1, 2, S>(0, 0, 0);
         region<2, S ^ 1, 3, S>(0, 0, 0);
         meet();
+    }
+
+    // The groups' sums into the first one's, through the stages, which are free; true there.
+    __device__ __forceinline__ bool sum_groups(int w) {
+        const int lane = threadIdx.x & 63;
+        auto place = [&](int g, int b) {  // 16 KB a block of a group
+            constexpr int each = TM * KG / 128;
+            const int s = (g - 1) * NB * NB + b;
+            uint8_t* at = s / each == 0 ? stage_a<0>() : s / each == 1 ? stage_a<1>() : s / each == 2 ? stage_b<0>() : stage_b<1>();
+            return (f32x4*)(at + 16384 * (s % each) + 4096 * w) + lane;
+        };
+#pragma unroll
+        for (int g = 1; g < KG; g++) {
+            if (kg != g) continue;
+#pragma unroll
+            for (int b = 0; b < NB * NB; b++)
+#pragma unroll
+                for (int q = 0; q < 4; q++) {
+                    const f32x16& x = acc[b / NB][b % NB];
+                    place(g, b)[64 * q] = f32x4{x[4 * q], x[4 * q + 1], x[4 * q + 2], x[4 * q + 3]};
+                }
+        }
+        __syncthreads();
+        if (kg > 0) return false;
+#pragma unroll
+        for (int g = 1; g < KG; g++)
+#pragma unroll
+            for (int b = 0; b < NB * NB; b++)
+#pragma unroll
+                for (int q = 0; q < 4; q++) {
+                    const f32x4 x = place(g, b)[64 * q];
+#pragma unroll
+                    for (int e = 0; e < 4; e++) acc[b / NB][b % NB][4 * q + e] += x[e];
+                }
+        return true;
     }
 
     // y of the wave's blocks, through a resource that begins at the tile's first row: rows
@@ -309,16 +348,17 @@ struct Mx4Gemm {
 
     __device__ __forceinline__ void run() {
         const int tid = threadIdx.x, lane = tid & 63;
-        const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+        const int w = __builtin_amdgcn_readfirstlane(tid >> 6) & 3;  // within the group
+        kg = __builtin_amdgcn_readfirstlane(tid >> 8);
         const int wm = 32 * NB * (w >> 1), wn = 32 * NB * (w & 1);
-        const int nk = 2 * ((a.K / 128 + 3) / 4);
-        lw = 1024 * ND * w;
-        lsw = 4 * TM * w;
+        const int nk = 2 * ((a.K / 128 + 4 * KG - 1) / (4 * KG));
+        lw = 1024 * ND * w + 128 * TM * kg;
+        lsw = 4 * TM * w + 16 * TM * kg;
         {
             const int h = lane >> 5, r = lane & 31;
-            off = (wm + r) * 128 + 16 * (h ^ ((r >> 1) & 7));
+            off = (wm + r) * 128 + 16 * (h ^ ((r >> 1) & 7)) + 128 * TM * kg;
             ofw = (wn - wm) * 128;
-            soff = 4 * (wm + r);
+            soff = 4 * (wm + r) + 16 * TM * kg;
             sofw = 8 * TM + 4 * (wn - wm);
             shift = 8 * h;
         }
@@ -351,6 +391,13 @@ struct Mx4Gemm {
             const __amdgpu_buffer_rsrc_t ry = __builtin_amdgcn_make_buffer_rsrc(
                 (void*)((Out*)a.y + (size_t)m0 * a.N), 0,
                 (int)((uint32_t)min(TM, a.M - m0) * (uint32_t)a.N * (uint32_t)sizeof(Out)), MX4_RSRC_W3);
+            if constexpr (KG > 1) {  // (a tile a workgroup)
+                tile<0, false>(nk - 2);
+                region<3, 0, 4, 0>(0, 0, 0);
+                if (!sum_groups(w)) return;
+                store(ry, wm, n0);
+                return;
+            }
             item += gridDim.x;
             const bool more = item < ntiles;
             ti = tile_at(more ? item : (int)blockIdx.x);
@@ -373,8 +420,8 @@ struct Mx4Gemm {
     }
 };
 
-#define MX4_GEMM_KERNEL(NAME, OUT_, NB_, GELU_, WIDE_, PER_)                                 \
-    extern "C" __global__ void __launch_bounds__(256, PER_) NAME(const LtxMx4LinearArgs a) { \
-        Mx4Gemm<OUT_, NB_, GELU_, WIDE_> k(a);                                               \
-        k.run();                                                                             \
+#define MX4_GEMM_KERNEL(NAME, OUT_, NB_, GELU_, WIDE_, KG_, PER_)                                   \
+    extern "C" __global__ void __launch_bounds__(256 * KG_, PER_) NAME(const LtxMx4LinearArgs a) { \
+        Mx4Gemm<OUT_, NB_, GELU_, WIDE_, KG_> k(a);                                                \
+        k.run();                                                                                   \
     }

@@ -170,7 +170,8 @@ struct ltx_ctx {
     bool attn_pp = true;
     bool attn_kv = true;
     int kv_tile = 0;  // columns of a tile of the 4-bit cache's attention: 0 by the rule, or 16, 128 or 256 (tests)
-    int mx4_tile = 0;  // tile of the microscaled 4-bit linear: 0 by the rule, 16 the kernel of few rows, or 64, 128 or 256 (tests)
+    int mx4_tile = 0;  // tile of the microscaled 4-bit linear: 0 by the rule, 16 the kernel of few rows, or 64,
+                       // 128 or 256 (tests)
     // side stream of a forward: work off the main chain (gate logits, the
     // cross-attention K/V) overlaps it, ordered by the events
     hipStream_t side = nullptr;

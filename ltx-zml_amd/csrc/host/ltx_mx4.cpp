@@ -38,6 +38,42 @@ void rows_call(ltx_ctx* c, bool quantise, void* x, int64_t ldx, uint8_t* q, uint
     c->launch(name, (unsigned)blocks, 1, 1, 256, &a, st);
 }
 
+struct Mx4Form {
+    int tile, groups;  // 16: the kernel of few rows
+    const char* name;
+};
+
+// Tiles of 256 x 256 where they come near to filling the CUs; of 128, two workgroups a CU; and
+// where few tiles leave a K-tile's latency to count, several groups of waves on one tile. us
+// at K = 4,096, few rows / 64k2 / 64k4 / 128 / 128k2 / 256:
+//   M   16 x N  4,096    4.4 /  5.9 /  5.8 /  9.6 /  9.1 /   -
+//       32 x    4,096    5.5 /  5.8 /  5.9 /  9.6 /  9.2 /   -
+//       64 x    4,096    8.2 /  5.9 /  6.0 /  9.8 /  9.3 /   -
+//       16 x    8,192    6.1 /  5.8 /  5.9 /  9.5 /  9.2 /   -
+//       16 x   12,288    8.5 /  6.4 /  6.2 / 10.5 /  9.3 /   -
+//      128 x   16,384   27   / 10.5 / 14.0 / 14.9 / 12.8 /   -
+//      256 x   12,288    -   / 15.5 / 19.0 / 14.0 / 12.3 /   -
+//      512 x    4,096    -   /  9.9 / 11.8 / 10.6 / 10.1 /   -
+//      640 x   12,288    -   / 37   / 49   / 23   / 28   / 29
+//    1,024 x    4,096    -   / 20   / 26   / 14.1 / 13.5 / 27
+//    1,024 x   12,288    -   / 54   / 71   / 36   / 39   / 32
+//    2,048 x    8,192    -   / 69   / 94   / 44   / 52   / 37
+// K = 16,384, N = 4,096: 16 rows 12 / 22 / 17 / 41 / 32, 64 26 / 23 / 19 / 42 / 33, 256 - / 24 /
+// 21 / 44 / 35, 512 - / 31 / 39 / 44 / 35, 2,970 - / 165 / 220 / 114 / 123 / 96; K = 1,024, 64
+// rows 4.0 / 3.6 / 4.7 / 5.2 / 5.2.
+Mx4Form mx4_form(const ltx_ctx* c, int64_t M, int64_t N, int K, bool rows, bool odd) {
+    auto tiles = [&](int64_t t) { return (M + t - 1) / t * ((N + t - 1) / t); };
+    const int64_t cu = c->num_cu;
+    const Mx4Form few{16, 1, ""};
+    if (rows || c->mx4_tile == 16 || (!c->mx4_tile && ((M <= 32 && N <= 16 * cu) || (M <= 16 && N <= 32 * cu)))) return few;
+    if (odd) return {128, 1, "odd"};
+    const int t = c->mx4_tile;
+    if (t ? t == 64 : tiles(64) <= 2 * cu)
+        return tiles(64) <= cu && K >= 4096 ? Mx4Form{64, 4, "64k4"} : Mx4Form{64, 2, "64k2"};
+    if (t ? t == 128 : tiles(256) < 3 * cu / 4) return tiles(128) <= cu ? Mx4Form{128, 2, "128k2"} : Mx4Form{128, 1, "128"};
+    return {256, 1, "256"};
+}
+
 }  // namespace
 }  // namespace ltx
 
@@ -92,27 +128,36 @@ int ltx_op_linear_mx4(ltx_ctx* c, const void* a, const uint8_t* a_scales, const 
         g.K = K;
         g.gelu = gelu != 0;
         g.out_f32 = out_f32 != 0;
+        // Rows in values: up to 16 are quantised by every workgroup that multiplies them, more
+        // once, by a launch of their own, into scratch. us, in the product / in a launch: 16
+        // rows of 4,096 x 4,096 7.4 / 7.3, 17 7.8 / 7.8, 64 18.5 / 8.8; 16 of 16,384 x 4,096
+        // 12.0 / 12.1, 33 17.3 / 11.7; 48 of 4,096 x 16,384 50 / 23.
+        ltx::ScratchUse use(c->op_scratch, st);
+        if (!a_scales && M > 16) {
+            const size_t codes = (size_t)M * K / 2;
+            if (uint8_t* s = (uint8_t*)use.take(codes + (size_t)M * K / 32)) {
+                ltx::rows_call(c, true, (void*)a, K, s, s + codes, M, K, mode, st);
+                g.a = s;
+                g.as = s + codes;
+            }
+        }
+        const ltx::Mx4Form form = ltx::mx4_form(c, M, N, K, !g.as, (uintptr_t)y & 15 || N % (out_f32 ? 4 : 8));
         char name[48];
-        const int64_t cu = c->num_cu;
-        auto tiles = [&](int64_t t) { return (M + t - 1) / t * ((N + t - 1) / t); };
-        if (!a_scales || (c->mx4_tile ? c->mx4_tile == 16 && M <= 1 << 20 : M <= LTX_MX4_ROWS)) {
-            const int mt = std::min((M + 15) / 16, 4);
-            int nt = 1;
-            while (nt < (mt > 2 ? 2 : 4) && ((int64_t)N + 16 * nt - 1) / (16 * nt) > cu) nt *= 2;
-            std::snprintf(name, sizeof(name), "ltx_linear_mx4_%s_%s%d_%d", type, a_scales ? "" : "rows_", mt, nt);
+        if (form.tile == 16) {
+            const int mt = std::min((M + 15) / 16, g.as ? 2 : 4);
+            int nt = 1;  // the fewest columns of 16, 32 or 64 whose workgroups are at most one a CU
+            while (nt < 4 && ((int64_t)N + 16 * nt - 1) / (16 * nt) > c->num_cu) nt *= 2;
+            std::snprintf(name, sizeof(name), "ltx_linear_mx4_%s_%s%d_%d", type, g.as ? "" : "rows_", mt, nt);
             c->launch(name, (unsigned)((N + 16 * nt - 1) / (16 * nt)), (unsigned)((M + 16 * mt - 1) / (16 * mt)), 1, 512, &g,
                       st);
             return LTX_OK;
         }
-        const bool odd = (uintptr_t)y & 15 || N % (out_f32 ? 4 : 8);  // rows of y that do not start on 16 bytes
-        const int tile = odd ? 128 : c->mx4_tile > 16 ? c->mx4_tile : tiles(256) >= cu ? 256 : tiles(128) >= cu ? 128 : 64;
-        g.tiles_m = (M + tile - 1) / tile;
-        g.tiles_n = (N + tile - 1) / tile;
-        const int64_t n = tiles(tile);
-        if (n >= 1 << 23) throw ltx::Error("too many rows or columns");  // (twice: past the last, an index stays in 31 bits)
-        const char* form = odd ? "odd" : tile == 256 ? "256" : tile == 128 ? "128" : "64";
-        std::snprintf(name, sizeof(name), "ltx_gemm_mx4_%s%s_%s", out_f32 ? "f32" : type, gelu ? "_gelu" : "", form);
-        c->launch(name, (unsigned)(tile == 256 ? std::min(n, cu) : n), 1, 1, 256, &g, st);
+        g.tiles_m = (M + form.tile - 1) / form.tile;
+        g.tiles_n = (N + form.tile - 1) / form.tile;
+        const int64_t n = (int64_t)g.tiles_m * g.tiles_n;
+        if (n >= 1 << 22) throw ltx::Error("too many rows or columns");  // (2^32 threads along x)
+        std::snprintf(name, sizeof(name), "ltx_gemm_mx4_%s%s_%s", out_f32 ? "f32" : type, gelu ? "_gelu" : "", form.name);
+        c->launch(name, (unsigned)(form.tile == 256 ? std::min<int64_t>(n, c->num_cu) : n), 1, 1, 256 * form.groups, &g, st);
     })
 }
 

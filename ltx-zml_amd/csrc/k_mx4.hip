@@ -159,8 +159,7 @@ __device__ __forceinline__ u32x4 mx4_group(const u32x4 (&x)[4], uint32_t& code) 
 
 template <typename T, bool ROWS, int MT, int NT>
 __device__ __forceinline__ void mx4_few(const LtxMx4LinearArgs& a) {
-    // what of a's step is in flight: the sooner it is asked for, the more registers wait
-    constexpr int D = MT == 1 ? 4 : ROWS && MT > 2 ? 1 : 2, NA = ROWS ? 4 : 1;
+    constexpr int D = MT == 1 ? 4 : ROWS && MT * NT == 16 ? 1 : 2, NA = ROWS ? 4 : 1;  // steps in flight
     __shared__ __attribute__((aligned(16))) float sums[MX4_WAVES][MT * NT][64][4];
     const int tid = threadIdx.x, lane = tid & 63, r = lane & 15, h = lane >> 4;
     const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -177,54 +176,61 @@ __device__ __forceinline__ void mx4_few(const LtxMx4LinearArgs& a) {
     const __amdgpu_buffer_rsrc_t rsa =
         rsrc(ROWS ? a.w : a.as + 4 * (size_t)m0, ROWS ? 0 : 4u * ((uint32_t)G * a.M - m0));
     const __amdgpu_buffer_rsrc_t rsw = rsrc(a.ws + 4 * (size_t)n0, 4u * ((uint32_t)G * a.N - n0));
-    struct Step {
-        u32x4 a[MT][NA], w[NT];
-        uint32_t sa[MT], sw[NT];
-    };
+    // Steps in flight: w's of D, a's of as many where they are codes or one tile, else of one,
+    // whose tiles make way for the next step's one by one.
+    constexpr int DA = ROWS && MT > 1 ? 1 : D;
+    u32x4 xa[DA][MT][NA], xw[D][NT];
+    uint32_t sa[DA][MT], sw[D][NT];
     auto step = [&](int i) { return 2 * (w + MX4_WAVES * (i >> 1)) + (i & 1); };
-    auto load = [&](Step& x, int g) {
+    auto load_a = [&](int d, int m, int g) {
+        if (g >= G) return;
+#pragma unroll
+        for (int j = 0; j < NA; j++)
+            xa[d][m][j] = __builtin_bit_cast(
+                u32x4, __builtin_amdgcn_raw_buffer_load_b128(ra, (16 * m + r) * la + (ROWS ? 64 : 16) * h + 16 * j,
+                                                             (ROWS ? 256 : 64) * g, 0));
+        if (!ROWS) sa[d][m] = __builtin_amdgcn_raw_buffer_load_b8(rsa, 4 * (16 * m + r) + h + 4 * g * a.M, 0, 0);
+    };
+    auto load_w = [&](int d, int g) {
         if (g >= G) return;
 #pragma unroll
         for (int t = 0; t < NT; t++) {
-            x.w[t] = __builtin_bit_cast(
+            xw[d][t] = __builtin_bit_cast(
                 u32x4, __builtin_amdgcn_raw_buffer_load_b128(rw, (16 * t + r) * lw + 16 * h, 64 * g, 0));
-            x.sw[t] = __builtin_amdgcn_raw_buffer_load_b8(rsw, 4 * (16 * t + r) + h + 4 * g * a.N, 0, 0);
+            sw[d][t] = __builtin_amdgcn_raw_buffer_load_b8(rsw, 4 * (16 * t + r) + h + 4 * g * a.N, 0, 0);
         }
-#pragma unroll
-        for (int t = 0; t < MT; t++) {
-#pragma unroll
-            for (int j = 0; j < NA; j++)
-                x.a[t][j] = __builtin_bit_cast(
-                    u32x4, __builtin_amdgcn_raw_buffer_load_b128(ra, (16 * t + r) * la + (ROWS ? 64 : 16) * h + 16 * j,
-                                                                 (ROWS ? 256 : 64) * g, 0));
-            if (!ROWS) x.sa[t] = __builtin_amdgcn_raw_buffer_load_b8(rsa, 4 * (16 * t + r) + h + 4 * g * a.M, 0, 0);
-        }
-        __builtin_amdgcn_sched_barrier(0);
     };
     f32x4 acc[MT][NT];
 #pragma unroll
     for (int m = 0; m < MT; m++)
 #pragma unroll
         for (int t = 0; t < NT; t++) acc[m][t] = f32x4{0, 0, 0, 0};
-    auto compute = [&](Step& x, int g) {
-        if (g >= G) return;
 #pragma unroll
-        for (int m = 0; m < MT; m++) {
-            u32x4 y = x.a[m][0];
-            if constexpr (ROWS) y = mx4_group<T>(x.a[m], x.sa[m]);
+    for (int i = 0; i < D; i++) {
+        load_w(i, step(i));
+        if (i < DA)
 #pragma unroll
-            for (int t = 0; t < NT; t++) acc[m][t] = mx4_mfma16(y, x.w[t], acc[m][t], x.sa[m], x.sw[t]);
-        }
-    };
-    Step x[D];
-#pragma unroll
-    for (int i = 0; i < D; i++) load(x[i], step(i));
+            for (int m = 0; m < MT; m++) load_a(i, m, step(i));
+    }
 #pragma nounroll
     for (int i = 0; step(i) < G; i += D) {
 #pragma unroll
         for (int d = 0; d < D; d++) {
-            compute(x[d], step(i + d));
-            load(x[d], step(i + d + D));
+            if (step(i + d) >= G) break;
+#pragma unroll
+            for (int m = 0; m < MT; m++) {
+                constexpr int last = DA - 1;
+                const int e = d < DA ? d : last;
+                u32x4 y = xa[e][m][0];
+                if constexpr (ROWS) y = mx4_group<T>(xa[e][m], sa[e][m]);
+                const uint32_t s = sa[e][m];
+                __builtin_amdgcn_sched_barrier(0);
+                load_a(e, m, step(i + d + DA));
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int t = 0; t < NT; t++) acc[m][t] = mx4_mfma16(y, xw[d][t], acc[m][t], s, sw[d][t]);
+            }
+            load_w(d, step(i + d + D));
         }
     }
 #pragma unroll
@@ -249,26 +255,17 @@ __device__ __forceinline__ void mx4_few(const LtxMx4LinearArgs& a) {
     }
 }
 
-#define MX4_FEW(MT, NT)                                                                                              \
-    extern "C" __global__ void __launch_bounds__(512) ltx_linear_mx4_f16_rows_##MT##_##NT(const LtxMx4LinearArgs a) { \
-        mx4_few<_Float16, true, MT, NT>(a);                                                                          \
-    }                                                                                                                \
-    extern "C" __global__ void __launch_bounds__(512) ltx_linear_mx4_bf16_rows_##MT##_##NT(const LtxMx4LinearArgs a) { \
-        mx4_few<__bf16, true, MT, NT>(a);                                                                            \
-    }                                                                                                                \
-    extern "C" __global__ void __launch_bounds__(512) ltx_linear_mx4_f16_##MT##_##NT(const LtxMx4LinearArgs a) {     \
-        mx4_few<_Float16, false, MT, NT>(a);                                                                         \
-    }                                                                                                                \
-    extern "C" __global__ void __launch_bounds__(512) ltx_linear_mx4_bf16_##MT##_##NT(const LtxMx4LinearArgs a) {    \
-        mx4_few<__bf16, false, MT, NT>(a);                                                                           \
+#define MX4_FEW(NAME, T, ROWS, MT, NT)                                                                     \
+    extern "C" __global__ void __launch_bounds__(512) NAME##MT##_##NT(const LtxMx4LinearArgs a) {          \
+        mx4_few<T, ROWS, MT, NT>(a);                                                                       \
     }
-MX4_FEW(1, 1)
-MX4_FEW(1, 2)
-MX4_FEW(1, 4)
-MX4_FEW(2, 1)
-MX4_FEW(2, 2)
-MX4_FEW(2, 4)
-MX4_FEW(3, 1)
-MX4_FEW(3, 2)
-MX4_FEW(4, 1)
-MX4_FEW(4, 2)
+#define MX4_FEW_TILES(NAME, T, ROWS, MT) MX4_FEW(NAME, T, ROWS, MT, 1) MX4_FEW(NAME, T, ROWS, MT, 2) MX4_FEW(NAME, T, ROWS, MT, 4)
+#define MX4_FEW_TYPE(TYPE, T)                             \
+    MX4_FEW_TILES(ltx_linear_mx4_##TYPE##_, T, false, 1)      \
+    MX4_FEW_TILES(ltx_linear_mx4_##TYPE##_, T, false, 2)      \
+    MX4_FEW_TILES(ltx_linear_mx4_##TYPE##_rows_, T, true, 1)  \
+    MX4_FEW_TILES(ltx_linear_mx4_##TYPE##_rows_, T, true, 2)  \
+    MX4_FEW_TILES(ltx_linear_mx4_##TYPE##_rows_, T, true, 3)  \
+    MX4_FEW_TILES(ltx_linear_mx4_##TYPE##_rows_, T, true, 4)
+MX4_FEW_TYPE(f16, _Float16)
+MX4_FEW_TYPE(bf16, __bf16)
