@@ -102,12 +102,17 @@ struct AttnPlan {
 // The table's width stands for the lengths, which the host does not know. A call that
 // cannot split (captured, without a workspace) takes 256 columns only where they fill
 // the CUs: 256 rows of 32 heads on 8 over 28,672 keys 235 us on 16 columns, 815 on 256.
+// A window of few pages leaves the wide tiles' starts and ends to count, which two
+// workgroups of 128 columns on a CU overlap. us on 128 / 256, causal: 32 heads on 8, 8,192
+// rows, windows of 300, 1,000, 2,000 and 3,000 keys 115 / 116, 192 / 189, 294 / 304, 374 /
+// 365; 32 heads, three times 4,096 rows 169 / 229, 313 / 352, 519 / 534, 699 / 706.
 int tile_columns(const ltx_ctx* c, const ltx_kv_cache* k, const ltx_kv_batch* b, const AttnMask& m, int64_t columns,
                  bool split) {
     if (c->kv_tile) return c->kv_tile;
+    const int64_t group = std::max<int64_t>(1, columns / std::max(b->rows, 1));
     const int64_t each = columns / b->nseq, wide = columns * k->kv_heads / 256;  // workgroups of 256 columns
     const int64_t pages = wide * tile_pages(b, m, b->rows / b->nseq) / c->num_cu;  // of each, if split
-    if (each >= 192 && wide >= c->num_cu) return 256;
+    if (each >= 192 && wide >= c->num_cu && !(m.window && tile_pages(b, m, 256 / group) <= 32)) return 256;
     if (split && each >= 256 && pages >= 128) return 256;
     if (each >= 64 && (each + 127) / 128 * b->nseq * k->kv_heads >= c->num_cu) return 128;
     if (split && each >= 256 && pages >= 24) return 256;
@@ -136,8 +141,12 @@ AttnPlan attn_plan(const ltx_ctx* c, const ltx_kv_cache* k, const ltx_kv_batch* 
     // ragged, 32 x 8 cached heads up to 8,192 keys 40 / 37, 8 x 32 up to 16,000 65 / 74.
     p.least = 8;
     const int64_t round = ((int64_t)c->num_cu + k->kv_heads - 1) / k->kv_heads;
-    const int64_t units = tiles * p.width;
-    const bool few = p.tile == 16 ? tiles * k->kv_heads < c->num_cu && p.width > 16
+    // With a window, whose range is worked out for every sequence in turn: us split / not, 32
+    // cached heads, one sequence, 1,000 keys 12.1 / 10.0, 1,500 12.1 / 11.7, 2,000 12.3 / 13.3;
+    // four of them, 1,000 16.3 / 10.4, 2,500 22.6 / 16.6, 4,096 24.3 / 22.4; four of 8 cached
+    // heads, 2,000 15.8 / 13.4, 2,500 16.0 / 15.3, 4,096 16.1 / 20.5.
+    const int64_t units = tiles * p.width, least = m.window ? 28 + (tiles - 1) * k->kv_heads * 3 / 8 : 16;
+    const bool few = p.tile == 16 ? tiles * k->kv_heads < c->num_cu && p.width > least
                                   : p.tile == 256 && columns / 256 * k->kv_heads < c->num_cu && p.width > p.least;
     if (split && few && units < 1ll << 31) p.slots = (int)std::min(round, (units + p.least - 1) / p.least);
     p.items = p.slots ? p.slots : (int)tiles;

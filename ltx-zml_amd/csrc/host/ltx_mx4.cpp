@@ -145,8 +145,10 @@ int ltx_op_linear_mx4(ltx_ctx* c, const void* a, const uint8_t* a_scales, const 
         char name[48];
         if (form.tile == 16) {
             const int mt = std::min((M + 15) / 16, g.as ? 2 : 4);
-            int nt = 1;  // the fewest columns of 16, 32 or 64 whose workgroups are at most one a CU
-            while (nt < 4 && ((int64_t)N + 16 * nt - 1) / (16 * nt) > c->num_cu) nt *= 2;
+            // the fewest columns of 16, 32 or 64 whose workgroups are at most one a CU (codes: where
+            // these kernels are taken, 16 or, up to 16 rows, 32)
+            int nt = 1;
+            while (nt < (!g.as ? 4 : mt == 1 ? 2 : 1) && ((int64_t)N + 16 * nt - 1) / (16 * nt) > c->num_cu) nt *= 2;
             std::snprintf(name, sizeof(name), "ltx_linear_mx4_%s_%s%d_%d", type, g.as ? "" : "rows_", mt, nt);
             c->launch(name, (unsigned)((N + 16 * nt - 1) / (16 * nt)), (unsigned)((M + 16 * mt - 1) / (16 * mt)), 1, 512, &g,
                       st);

@@ -261,8 +261,9 @@ __device__ __forceinline__ void mx4_few(const LtxMx4LinearArgs& a) {
     }
 #define MX4_FEW_TILES(NAME, T, ROWS, MT) MX4_FEW(NAME, T, ROWS, MT, 1) MX4_FEW(NAME, T, ROWS, MT, 2) MX4_FEW(NAME, T, ROWS, MT, 4)
 #define MX4_FEW_TYPE(TYPE, T)                             \
-    MX4_FEW_TILES(ltx_linear_mx4_##TYPE##_, T, false, 1)      \
-    MX4_FEW_TILES(ltx_linear_mx4_##TYPE##_, T, false, 2)      \
+    MX4_FEW(ltx_linear_mx4_##TYPE##_, T, false, 1, 1)         \
+    MX4_FEW(ltx_linear_mx4_##TYPE##_, T, false, 1, 2)         \
+    MX4_FEW(ltx_linear_mx4_##TYPE##_, T, false, 2, 1)         \
     MX4_FEW_TILES(ltx_linear_mx4_##TYPE##_rows_, T, true, 1)  \
     MX4_FEW_TILES(ltx_linear_mx4_##TYPE##_rows_, T, true, 2)  \
     MX4_FEW_TILES(ltx_linear_mx4_##TYPE##_rows_, T, true, 3)  \
