@@ -297,7 +297,7 @@ int ltx_op_linear_q4(ltx_ctx* ctx, const void* a, const uint8_t* q, const void* 
  * type (exact in the mode that it came from, and in F32; beyond f16's largest: infinity).
  * rows may be 0. Refused: K not a positive multiple of 128 or above 2^23, x or q not on 16
  * bytes, scales not on 4, rows of x not on 16 bytes or shorter than K, an unknown mode,
- * rows (K / 128 + 8) from 2^29 on. */
+ * rows (K / 128 + 16) from 2^29 on. */
 int ltx_op_mx4_quantise(ltx_ctx* ctx, const void* x, int64_t ldx, uint8_t* q, uint8_t* scales, int rows, int K,
                         int mode, void* stream);
 int ltx_op_mx4_values(ltx_ctx* ctx, const uint8_t* q, const uint8_t* scales, void* y, int64_t ldy, int rows, int K,
@@ -314,7 +314,7 @@ int ltx_op_mx4_values(ltx_ctx* ctx, const uint8_t* q, const uint8_t* scales, voi
  * captured, or one that finds no memory, takes none, with the same bits, and longer.)
  * Refused: M, N or K not positive, K no multiple of 128 or above 2^23, a or q not on 16
  * bytes, scales not on 4, bias or y not aligned to their types, an unknown mode, mode F32
- * with a in values, M or N times (K / 128 + 8) from 2^29 on, N from 2^21, more than 2^22
+ * with a in values, M or N times (K / 128 + 16) from 2^29 on, N from 2^21, more than 2^22
  * tiles. */
 int ltx_op_linear_mx4(ltx_ctx* ctx, const void* a, const uint8_t* a_scales, const uint8_t* q, const uint8_t* scales,
                       const float* bias, void* y, int out_f32, int M, int N, int K, int gelu, int mode, void* stream);

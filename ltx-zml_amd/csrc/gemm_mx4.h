@@ -406,6 +406,7 @@ struct Mx4Gemm {
             // it is multiplied and y is formed, and y's stores leave beside the next tile.
             // (Behind the last tile no operand is read.)
             begin(w, ti.tm * TM, ti.tn * TM, more);
+            __builtin_amdgcn_sched_barrier(0);
             region<3, 0, 4, 0>(0, 0, 0);
             hold();
             // the stores come behind the DMA, in order: it has landed when only they are left

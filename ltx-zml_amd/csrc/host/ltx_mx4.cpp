@@ -16,8 +16,8 @@ const char* mode_name(int mode) {
     throw Error("unknown mode");
 }
 
-// 32-bit offsets of the scale words, eight groups of 128 behind the last among them
-bool scales_fit(int64_t rows, int K) { return 4 * rows * (K / 128 + 8) < 1ll << 31; }
+// 32-bit offsets of the scale words, sixteen groups of 128 behind the last among them
+bool scales_fit(int64_t rows, int K) { return 4 * rows * (K / 128 + 16) < 1ll << 31; }
 
 void rows_call(ltx_ctx* c, bool quantise, void* x, int64_t ldx, uint8_t* q, uint8_t* s, int rows, int K, int mode,
                hipStream_t st) {

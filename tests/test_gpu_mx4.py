@@ -316,6 +316,44 @@ def test_y_anywhere(any_tile, M, N, out):
     assert bool((buf[:17] == 7).all()) and bool((buf[17 + M * N:] == 7).all())
 
 
+@pytest.mark.parametrize("K", [128, 512, 640, 2176])
+@pytest.mark.parametrize("M,N,mode,out_f32,bias,gelu", [
+    (4369, 4880, "f16", False, True, False), (4096, 4608, "bf16", False, True, True), (5000, 4100, "f16", True, True, False),
+    (4600, 4999, "bf16", False, False, False),
+])
+def test_many_tiles(ctx, M, N, mode, out_f32, bias, gelu, K):
+    """More tiles than CUs: a workgroup's next tile comes in while the last one leaves.
+    Called again and again, the same bits. (f64 on the GPU)"""
+    say(f"linear_mx4 many tiles M={M} N={N} K={K} {mode} out_f32={out_f32}")
+    g = torch.Generator(device="cuda").manual_seed(M + K)
+    a = torch.randn(M, K, generator=g, device="cuda").to(MODES[mode][1])
+    w = torch.randn(N, K, generator=g, device="cuda") * 0.05
+    b = torch.randn(N, generator=g, device="cuda") if bias else None
+    qa, qw = quantise(ctx, a, mode), quantise(ctx, w, "f32")
+    ax, wx = torch.empty(M, K, device="cuda"), torch.empty(N, K, device="cuda")
+    ctx.mx4_values(*qa, ax, mode=rt.MODE_F32)
+    ctx.mx4_values(*qw, wx, mode=rt.MODE_F32)
+    out = torch.float32 if out_f32 else MODES[mode][1]
+    y = torch.full((M, N), 7.0, dtype=out, device="cuda")
+    ctx.linear_mx4(*qa, *qw, b, y, mode=MODES[mode][0], gelu=gelu)
+    want = ax.double() @ wx.double().T
+    size = ax.double().abs() @ wx.double().abs().T
+    bx = torch.zeros((), dtype=torch.float64, device="cuda") if b is None else b.double()
+    want = want + bx
+    tol = 2 * 2.0 ** -24 * (128 + K // 128 + 8) * size + 2.0 ** -24 * (want.abs() + bx.abs())
+    if gelu:
+        tol = 1.13 * tol + 2.0 ** -20 * want.abs()
+        want = want / (1 + torch.exp(-2 * math.sqrt(2 / math.pi) * (want + 0.044715 * want ** 3)))
+    if not out_f32:
+        tol = tol + torch.finfo(out).eps / 2 * (want.abs() + tol) + 2.0 ** -25
+    off = (y.double() - want).abs()
+    assert bool((off <= tol).all()), (int((off > tol).sum()), float((off / tol).max()))
+    for _ in range(10):
+        z = torch.full_like(y, 7.0)
+        ctx.linear_mx4(*qa, *qw, b, z, mode=MODES[mode][0], gelu=gelu)
+        assert torch.equal(y, z)
+
+
 def test_captured_and_on_another_stream(ctx):
     """Quantise and multiply, replayed with other inputs, and beside it on a stream."""
     say("linear_mx4 graph and stream")
