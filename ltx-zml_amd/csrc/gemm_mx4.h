@@ -144,9 +144,9 @@ struct Mx4Gemm {
         }
     }
 
-    // The products of step STEP (4: none; FIRST: the tile's first, onto zero) with the reads of step RSTEP of stage RS (4: none)
-    // and the DMA instructions g0 .. g1 - 1 of tile kd into stage DS, spread evenly between
-    // them.
+    // The products of step STEP (4: none; FIRST: the tile's first, onto zero) with the reads of
+    // step RSTEP of stage RS (4: none) and the DMA instructions g0 .. g1 - 1 of tile kd into
+    // stage DS, spread evenly between them.
     template <int STEP, int RS, int RSTEP, int DS, bool FIRST = false>
     __device__ __forceinline__ void region(int g0, int g1, int kd) {
         constexpr int F = STEP & 1, X = (STEP >> 1) & 1, NM = NB * NB, NR = RSTEP < 4 ? 2 * NB : 0, R = RSTEP & 3;
@@ -410,10 +410,11 @@ struct Mx4Gemm {
             region<3, 0, 4, 0>(0, 0, 0);
             hold();
             // the stores come behind the DMA, in order: it has landed when only they are left
+            // (the counter's 63 would be no wait)
             constexpr int stores = NB * NB * (!WIDE ? 16 : sizeof(Out) == 4 ? 4 : 2);
             store(ry, wm, n0);
             __builtin_amdgcn_sched_barrier(0);
-            __builtin_amdgcn_s_waitcnt(MX4_WAIT(stores < 63 ? stores : 63));
+            __builtin_amdgcn_s_waitcnt(MX4_WAIT(stores < 62 ? stores : 62));
             __builtin_amdgcn_s_barrier();
             __builtin_amdgcn_sched_barrier(0);
             if (!more) break;

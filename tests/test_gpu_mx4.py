@@ -388,6 +388,45 @@ def test_captured_and_on_another_stream(ctx):
         assert torch.equal(y, eager)
 
 
+def test_rows_in_values_at_once(ctx):
+    """Calls that share the context's scratch on four streams, and two graphs, which take
+    none: the bits of each call alone."""
+    say("linear_mx4 rows in values at once")
+    K, cases = 1024, [(17, 272), (64, 4112), (33, 96), (48, 528)]
+    w = [quantise(ctx, torch.randn(N, K, device="cuda") * 0.02, "f32") for _, N in cases]
+    x = [torch.randn(M, K, device="cuda").bfloat16() for M, _ in cases]
+    want = [torch.empty(M, N, device="cuda") for M, N in cases]
+    got = [torch.zeros_like(t) for t in want]
+
+    def call(i, y, **kw):
+        ctx.linear_mx4(x[i], None, *w[i], None, y, mode=rt.MODE_BF16, **kw)
+
+    for i, y in enumerate(want):
+        call(i, y)
+    streams = [torch.cuda.Stream() for _ in cases]
+    torch.cuda.synchronize()
+    for _ in range(10):
+        for i, st in enumerate(streams):
+            call(i, got[i], stream=st)
+    torch.cuda.synchronize()
+    assert all(torch.equal(g, t) for g, t in zip(got, want))
+    graphs = [torch.cuda.CUDAGraph() for _ in range(2)]
+    for i, graph in enumerate(graphs):
+        with torch.cuda.graph(graph):
+            call(i, got[i])
+    for _ in range(3):
+        for g in got:
+            g.zero_()
+        torch.cuda.synchronize()
+        for graph, st in zip(graphs, streams):
+            with torch.cuda.stream(st):
+                graph.replay()
+        for i in (2, 3):
+            call(i, got[i])
+        torch.cuda.synchronize()
+        assert all(torch.equal(g, t) for g, t in zip(got, want))
+
+
 def test_empty_and_refused(ctx):
     say("mx4 refusals")
     q, s = room(0, 256)
