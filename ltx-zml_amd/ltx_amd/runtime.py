@@ -447,46 +447,46 @@ class Context:
         """x [rows, K] (rows may be strided) -> codes q uint8 [rows, K / 2] and scales s
         uint8 [K / 128, rows, 4], which it returns (ltx_op_mx4_quantise)."""
         st = stream.cuda_stream if stream is not None else _current_stream(self.device)
-        rows, K = self._mx4_rows("mx4_quantise", x, q, s, mode)
-        self._check(lib().ltx_op_mx4_quantise(self.handle, _ptr(x), x.stride(0), _ptr(q), _ptr(s), rows, K, mode, st),
+        rows, K, ld = self._mx4_rows("mx4_quantise", x, q, s, mode)
+        self._check(lib().ltx_op_mx4_quantise(self.handle, x.data_ptr(), ld, q.data_ptr(), s.data_ptr(), rows, K, mode, st),
                     "ltx_op_mx4_quantise")
         return q, s
 
     def mx4_values(self, q, s, y, mode=MODE_F16, stream=None):
         """What codes and scales stand for -> y [rows, K] (ltx_op_mx4_values)."""
         st = stream.cuda_stream if stream is not None else _current_stream(self.device)
-        rows, K = self._mx4_rows("mx4_values", y, q, s, mode)
-        self._check(lib().ltx_op_mx4_values(self.handle, _ptr(q), _ptr(s), _ptr(y), y.stride(0), rows, K, mode, st),
+        rows, K, ld = self._mx4_rows("mx4_values", y, q, s, mode)
+        self._check(lib().ltx_op_mx4_values(self.handle, q.data_ptr(), s.data_ptr(), y.data_ptr(), ld, rows, K, mode, st),
                     "ltx_op_mx4_values")
         return y
 
     def linear_mx4(self, a, a_s, q, s, bias, y, mode=MODE_F16, gelu=False, stream=None):
         """a and a_s, q and s: M and N rows as mx4_quantise makes them, or a_s None and a at
         most 64 rows [M, K] of the mode's type (ltx_op_linear_mx4)."""
-        import torch
-        (M, N), K = y.shape, 2 * q.shape[1]
-        x, f32 = _torch_dtype(mode), torch.float32
-        _mx4_held("linear_mx4", q, s, N, K, self.device)
+        (M, N), K, device = y.shape, 2 * q.shape[1], self.device
+        x, f32, out = _torch_dtype(mode), _torch_dtype(MODE_F32), y.dtype
+        _mx4_held("linear_mx4", q, s, N, K, device)
         if a_s is not None:
-            _mx4_held("linear_mx4", a, a_s, M, K, self.device)
-        elif not (a.shape == (M, K) and a.dtype == x and a.is_contiguous() and a.get_device() == self.device):
+            _mx4_held("linear_mx4", a, a_s, M, K, device)
+        elif not (a.shape == (M, K) and a.dtype == x and a.is_contiguous() and a.get_device() == device):
             raise LtxError(f"linear_mx4: a contiguous a {[M, K]} of the mode's type on the context's device is needed")
-        if not (y.is_contiguous() and (y.dtype == x or y.dtype == f32) and y.get_device() == self.device):
+        if not (y.is_contiguous() and (out == x or out == f32) and y.get_device() == device):
             raise LtxError("linear_mx4: a contiguous y of the mode's type or f32 on the context's device is needed")
         if bias is not None and not (bias.shape == (N,) and bias.dtype == f32 and bias.is_contiguous()
-                                     and bias.get_device() == self.device):
+                                     and bias.get_device() == device):
             raise LtxError(f"linear_mx4: bias must be f32 {[N]}, contiguous, on the context's device")
-        st = stream.cuda_stream if stream is not None else _current_stream(self.device)
-        self._check(lib().ltx_op_linear_mx4(self.handle, _ptr(a), _ptr(a_s), _ptr(q), _ptr(s), _ptr(bias), _ptr(y),
-                                            int(y.dtype == f32), M, N, K, int(gelu), mode, st), "ltx_op_linear_mx4")
+        st = stream.cuda_stream if stream is not None else _current_stream(device)
+        self._check(lib().ltx_op_linear_mx4(self.handle, a.data_ptr(), _ptr(a_s), q.data_ptr(), s.data_ptr(), _ptr(bias),
+                                            y.data_ptr(), int(out == f32), M, N, K, int(gelu), mode, st),
+                    "ltx_op_linear_mx4")
         return y
 
     def _mx4_rows(self, name, x, q, s, mode):
-        rows, K = x.shape
-        if x.dtype != _torch_dtype(mode) or x.stride(1) != 1 or x.get_device() != self.device:
+        (rows, K), (ld, unit) = x.shape, x.stride()
+        if x.dtype != _torch_dtype(mode) or unit != 1 or x.get_device() != self.device:
             raise LtxError(f"{name}: rows of the mode's type on the context's device are needed")
         _mx4_held(name, q, s, rows, K, self.device)
-        return rows, K
+        return rows, K, ld
 
     # ---- rotary positions on several axes ----
     def rope(self, freq, phase=None, axis=None, axes: int = 1) -> Rope:
@@ -517,29 +517,32 @@ class Context:
                 mode=MODE_F16, stream=None):
         """q, q_out [rows, heads * 128] and k, k_out [rows, kv_heads * 128] (rows may be
         strided), pos f64 [rows, axes], norms f32 [heads * 128] or None (ltx_op_qk_rope)."""
-        import torch
-        rows, dt = q.shape[0], _torch_dtype(mode)
+        rows, dt, f32, device = q.shape[0], _torch_dtype(mode), _torch_dtype(MODE_F32), self.device
         if (k is None) != (k_out is None):
             raise LtxError("qk_rope: k and k_out belong together")
-        for x, y, w in ((q, q_out, q_norm), (k, k_out, k_norm)):
-            if x is None:
-                continue
-            for t in (x, y):
-                if t.dim() != 2 or t.shape[0] != rows or t.shape != x.shape or t.dtype != dt or t.stride(1) != 1:
-                    raise LtxError("qk_rope: rows of one shape and of the mode's type are needed")
-            if x.shape[1] % 128:
+
+        def strides(x, y, w):  # of x and y, and the heads (a row's call costs a few us: each question once)
+            shape, sx, sy = x.shape, x.stride(), y.stride()
+            if not (len(shape) == 2 and shape == y.shape and shape[0] == rows and x.dtype == dt and y.dtype == dt
+                    and sx[1] == 1 and sy[1] == 1):
+                raise LtxError("qk_rope: rows of one shape and of the mode's type are needed")
+            if shape[1] % 128:
                 raise LtxError("qk_rope: rows of heads of 128 values are needed")
-            if w is not None and not (w.shape == x.shape[1:] and w.dtype == torch.float32 and w.is_contiguous()):
+            if w is not None and not (w.shape == shape[1:] and w.dtype == f32 and w.is_contiguous()):
                 raise LtxError("qk_rope: norm weights must be f32, one for each value of a row")
-        if not (pos.shape == (rows, rope.axes) and pos.dtype == torch.float64 and pos.is_contiguous()):
-            raise LtxError(f"qk_rope: contiguous f64 positions {[rows, rope.axes]} are needed")
-        if any(t is not None and t.get_device() != self.device for t in (pos, q, q_out, k, k_out, q_norm, k_norm)):
-            raise LtxError("qk_rope: tensors on the context's device are needed")
-        st = stream.cuda_stream if stream is not None else _current_stream(self.device)
-        kl = (0, 0, 0) if k is None else (k.stride(0), k_out.stride(0), k.shape[1] // 128)
-        self._check(lib().ltx_op_qk_rope(self.handle, rope.handle, _ptr(pos), rows, _ptr(q), q.stride(0), _ptr(q_norm),
-                                         _ptr(q_out), q_out.stride(0), q.shape[1] // 128, _ptr(k), kl[0], _ptr(k_norm),
-                                         _ptr(k_out), kl[1], kl[2], eps, mode, st), "ltx_op_qk_rope")
+            if not (x.get_device() == device and y.get_device() == device and (w is None or w.get_device() == device)):
+                raise LtxError("qk_rope: tensors on the context's device are needed")
+            return sx[0], sy[0], shape[1] // 128
+
+        ql = strides(q, q_out, q_norm)
+        kl = (0, 0, 0) if k is None else strides(k, k_out, k_norm)
+        if not (pos.shape == (rows, rope.axes) and pos.is_floating_point() and pos.element_size() == 8 and pos.is_contiguous()
+                and pos.get_device() == device):
+            raise LtxError(f"qk_rope: contiguous f64 positions {[rows, rope.axes]} on the context's device are needed")
+        st = stream.cuda_stream if stream is not None else _current_stream(device)
+        self._check(lib().ltx_op_qk_rope(self.handle, rope.handle, pos.data_ptr(), rows, q.data_ptr(), ql[0], _ptr(q_norm),
+                                         q_out.data_ptr(), ql[1], ql[2], _ptr(k), kl[0], _ptr(k_norm), _ptr(k_out), kl[1],
+                                         kl[2], eps, mode, st), "ltx_op_qk_rope")
 
     # ---- the 4-bit key/value cache ----
     def kv_cache(self, kv_heads: int, pages: int, mode: int = MODE_F16) -> KvCache:
@@ -717,11 +720,11 @@ def _mx4_held(name: str, q, s, rows: int, K: int, device: int):
     """Codes [rows, K / 2] and scales [K / 128, rows, 4], uint8."""
     if K % 128:
         raise LtxError(f"{name}: K must be a multiple of 128")
-    for t, shape in ((q, (rows, K // 2)), (s, (K // 128, rows, 4))):
-        if t.shape != shape or t.element_size() != 1 or t.is_floating_point() or not t.is_contiguous():
-            raise LtxError(f"{name}: contiguous uint8 tensors {[rows, K // 2]} and {[K // 128, rows, 4]} are needed")
-        if t.get_device() != device:
-            raise LtxError(f"{name}: tensors on the context's device are needed")
+    if not (q.shape == (rows, K // 2) and s.shape == (K // 128, rows, 4) and q.element_size() == 1 and s.element_size() == 1
+            and not (q.is_floating_point() or s.is_floating_point()) and q.is_contiguous() and s.is_contiguous()):
+        raise LtxError(f"{name}: contiguous uint8 tensors {[rows, K // 2]} and {[K // 128, rows, 4]} are needed")
+    if not q.get_device() == s.get_device() == device:
+        raise LtxError(f"{name}: tensors on the context's device are needed")
 
 
 def _current_stream(device: int) -> int:
