@@ -21,6 +21,12 @@
 // row (or zeros behind the last), which are numbers whatever they are; their scale words lie
 // behind the resource's end and read as zeros, 2^-127 on both sides, and what such products
 // add is below f32's smallest number.
+//
+// Bound: 28,672 x 4,096 x 16,384 (f32 out) 830 us, 4.63 PFLOP/s, where the instruction with
+// its LDS reads comes to 5.7; the K loop alone runs at about 5.0 (an operand byte is read
+// from LDS once a wave and row or column block), and a 256 x 256 tile costs about 5 us beside
+// it, y's stores, which the next tile's operands overlap. 2,048 x 12,288 x 4,096 is 1.5
+// rounds of tiles: 61 us, 3.4 PFLOP/s.
 #pragma once
 #include "gemm_common.h"
 #include "ltx_fp4.h"

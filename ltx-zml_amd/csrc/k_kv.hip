@@ -239,19 +239,20 @@ __device__ __forceinline__ int kv_work(const LtxKvAttnArgs& a, const KvSeq& s) {
     return WIN ? kv_range_units(a.window, a.sinks, a.causal, s, a.group, a.tile) : kv_units(s.L);
 }
 
-// Sequence base + lane, and what it adds to the tiles and units before the next one
+// Sequence base + lane, and what it adds to the tiles and units before the next one. (SPLIT
+// false: a kernel whose calls never split, a.slots 0.)
 struct KvLane {
     KvSeq s;
     uint32_t tiles, units, tiles_to, units_to;  // its own, and inclusive sums from `base` on
 };
-template <bool WIN>
+template <bool WIN, bool SPLIT = true>
 __device__ __forceinline__ KvLane kv_lane(const LtxKvAttnArgs& a, int base) {
     const int b = base + (threadIdx.x & 63);
     KvLane k;
     k.s = KvSeq{0, 0, 0};
     if (b < a.b.nseq) k.s = kv_seq(a.b, b);
     k.tiles = kv_tiles(k.s.n, a.group, a.tile);
-    k.units = a.slots ? k.tiles * (uint32_t)kv_work<WIN>(a, k.s) : k.tiles;
+    k.units = SPLIT && a.slots ? k.tiles * (uint32_t)kv_work<WIN>(a, k.s) : k.tiles;
     k.tiles_to = wave_scan(k.tiles);
     k.units_to = wave_scan(k.units);
     return k;
@@ -259,25 +260,25 @@ __device__ __forceinline__ KvLane kv_lane(const LtxKvAttnArgs& a, int base) {
 __device__ __forceinline__ uint32_t lane_of(uint32_t x, int l) { return __builtin_amdgcn_readlane(x, l); }
 
 // units an item: `first` is kv_lane(a, 0)
-template <bool WIN>
+template <bool WIN, bool SPLIT = true>
 __device__ __forceinline__ int kv_per(const LtxKvAttnArgs& a, const KvLane& first) {
-    if (!a.slots) return 1;
+    if (!SPLIT || !a.slots) return 1;
     uint32_t units = lane_of(first.units_to, 63);
-    for (int base = 64; base < a.b.nseq; base += 64) units += lane_of(kv_lane<WIN>(a, base).units_to, 63);
+    for (int base = 64; base < a.b.nseq; base += 64) units += lane_of(kv_lane<WIN, SPLIT>(a, base).units_to, 63);
     return kv_per_of(units, a.slots, a.least);
 }
 
 // The item's first span; false: there is none. Without a split an item is a tile, a
 // sequence's last one, which sees the most keys where the mask is causal, first.
-template <bool WIN>
+template <bool WIN, bool SPLIT = true>
 __device__ __forceinline__ bool kv_begin(const LtxKvAttnArgs& a, int item, KvSpan& it) {
-    KvLane k = kv_lane<WIN>(a, 0);
-    it.left = kv_per<WIN>(a, k);
+    KvLane k = kv_lane<WIN, SPLIT>(a, 0);
+    it.left = kv_per<WIN, SPLIT>(a, k);
     const uint64_t first = (uint64_t)item * it.left;
     if (first >> 32) return false;
     uint32_t u = (uint32_t)first, entities = 0;
     for (int base = 0; base < a.b.nseq; base += 64) {
-        if (base) k = kv_lane<WIN>(a, base);
+        if (base) k = kv_lane<WIN, SPLIT>(a, base);
         const uint64_t here = __builtin_amdgcn_ballot_w64(u < k.units_to && u >= k.units_to - k.units);
         if (here) {
             const int l = __builtin_ctzll(here);
@@ -285,11 +286,11 @@ __device__ __forceinline__ bool kv_begin(const LtxKvAttnArgs& a, int item, KvSpa
             it.b = base + l;
             it.s = KvSeq{(int)lane_of(k.s.s0, l), (int)lane_of(k.s.n, l), (int)lane_of(k.s.L, l)};
             it.tiles = lane_of(k.tiles, l);
-            it.pages = kv_work<WIN>(a, it.s);
-            it.tile = a.slots ? (int)(u / (uint32_t)it.pages) : it.tiles - 1 - (int)u;
-            it.page = a.slots ? (int)(u % (uint32_t)it.pages) : 0;
+            it.pages = SPLIT ? kv_work<WIN>(a, it.s) : 1;
+            it.tile = SPLIT && a.slots ? (int)(u / (uint32_t)it.pages) : it.tiles - 1 - (int)u;
+            it.page = SPLIT && a.slots ? (int)(u % (uint32_t)it.pages) : 0;
             it.entity = (int)(entities + lane_of(k.tiles_to - k.tiles, l)) + it.tile;
-            if (!a.slots) it.left = it.pages;
+            if (!SPLIT || !a.slots) it.left = it.pages;
             return true;
         }
         u -= lane_of(k.units_to, 63);
@@ -520,7 +521,12 @@ __device__ __forceinline__ void kv_v_pair(const uint32_t (&x)[8], const uint32_t
 // memory-side cache holds much between calls) in 36. One short sequence is latency: a
 // page's index, its codes, two rounds of products and the waves' join, 8 us.
 // NT: the codes as streaming loads, for caches beyond what the memory-side cache holds.
-// WIN: with a window, p counts the pages of the tile's range.
+// WIN: with a window, p counts the pages of the tile's range, which is worked out from the
+// lengths as the split is: pages in front of the window are never read. One row of 32 heads
+// with a window of 1,000 keys behind 28,000 9.5 us; 32 ragged
+// sequences of 8 heads, windows of 4,096 (109 MB), 24.5. Sixteen waves of one page each in
+// place of eight: 10.9 and no less for longer windows; a CU's conversions count, 1.7 us for
+// eight pages.
 template <typename T, bool NT, bool WIN>
 __device__ __forceinline__ void kv_attn(const LtxKvAttnArgs& a) {
     typedef typename Op<T>::v8 v8;
@@ -600,13 +606,16 @@ __device__ __forceinline__ void kv_attn(const LtxKvAttnArgs& a) {
                 }
             }
             __builtin_amdgcn_sched_barrier(0);
-            if (x.flag) kv_set_nan(s, kv_drop_nan(x.vs));
             if constexpr (WIN) {
-                const int key = real(p) * LTX_KV_PAGE, end = key + LTX_KV_PAGE;
-                if (x.none || end > all || (key < limit - a.window && end > a.sinks))
-                    kv_mask_range(s, real(p), x.none ? 0 : mine, low, a.sinks, h);
-            } else if (x.none || (p + 1) * LTX_KV_PAGE > all)
-                kv_mask(s, p, x.none ? 0 : mine, h);
+                const int page = real(p), key = page * LTX_KV_PAGE, end = key + LTX_KV_PAGE;
+                if (x.flag || x.none || end > all || (key < limit - a.window && end > a.sinks)) {
+                    kv_set_nan(s, x.flag ? kv_drop_nan(x.vs) : 0u);
+                    kv_mask_range(s, page, x.none ? 0 : mine, low, a.sinks, h);
+                }
+            } else {
+                if (x.flag) kv_set_nan(s, kv_drop_nan(x.vs));
+                if (x.none || (p + 1) * LTX_KV_PAGE > all) kv_mask(s, p, x.none ? 0 : mine, h);
+            }
             uint32_t pw[4][2];
             float corr;
             if (kv_softmax<T>(s, C, m, l, pw, corr))
@@ -742,7 +751,7 @@ __device__ __forceinline__ void kv_attn_rows(const LtxKvAttnArgs& a) {
     // the other over the XCDs, 32 heads 155 against 233.
     const int item = blockIdx.x / a.b.kvh, kh = blockIdx.x - item * a.b.kvh;
     KvSpan it;
-    if (!kv_begin<WIN>(a, item, it)) return;
+    if (!kv_begin<WIN, SPLIT || !WIN>(a, item, it)) return;
     do {
         const int limit = kv_tile_limit(a.causal, it.s, a.group, it.tile, a.tile);
         const KvRange range = WIN ? kv_tile_range(a.window, a.sinks, a.causal, it.s, a.group, it.tile, a.tile)
@@ -768,8 +777,16 @@ __device__ __forceinline__ void kv_attn_rows(const LtxKvAttnArgs& a) {
             for (int j = 0; j < 4; j++) qf[q][j] = __builtin_bit_cast(v8, *(const u32x4*)(Q + 8 * j));
         }
         const int all = kv_limit(a.causal, it.s, min(c0, ncol - 1) / a.group);  // keys that every column sees
-        // the wave's last window begins here: keys before it are not every column's
-        const int every = WIN ? kv_limit(a.causal, it.s, (min(c0 + 16 * NQ, ncol) - 1) / a.group) - a.window : 0;
+        // With a window, pages with keys that a column of the wave does not see: from `tail` on,
+        // and `head_n` from `head` on (behind the first keys, before the last column's window).
+        int tail = 0, head = 0;
+        uint32_t head_n = 0;
+        if constexpr (WIN) {
+            const int first = kv_limit(a.causal, it.s, (min(c0 + 16 * NQ, ncol) - 1) / a.group) - a.window;
+            tail = __builtin_amdgcn_readfirstlane(kv_range_find(range, all / LTX_KV_PAGE));
+            head = __builtin_amdgcn_readfirstlane(kv_range_find(range, a.sinks / LTX_KV_PAGE));
+            head_n = __builtin_amdgcn_readfirstlane(max(0, kv_range_find(range, kv_pages(max(0, first))) - head));
+        }
 
         // Staging. A page's index is read two pages before its codes are used, its flag
         // beside them, by scalar loads (the constant address space: nothing writes them
@@ -913,23 +930,32 @@ __device__ __forceinline__ void kv_attn_rows(const LtxKvAttnArgs& a) {
         auto softmax = [&](int t) {
             const int p = p0 + t;
             if (idle) return;
-            if (flag_s) {
-                const int h = my_lane() >> 4;
-                const uint32_t bits = snan[t & 1][0][h] | snan[t & 1][1][h] << 8;
-#pragma unroll
-                for (int q = 0; q < NQ; q++) kv_set_nan(s[q], bits);
-            }
             if constexpr (WIN) {
-                const int page = real(p), key = page * LTX_KV_PAGE, end = key + LTX_KV_PAGE;
-                if (none_s || end > all || (key < every && end > a.sinks))
+                // (one branch for both: with two the compiler moves the scores to other registers
+                // and back on every page, 6 % of the frame's time)
+                const uint32_t none_p = __builtin_amdgcn_readfirstlane(none_s);
+                if ((flag_s | none_p) || p >= tail || (uint32_t)(p - head) < head_n) {
+                    const int page = real(p);
+                    const int h = my_lane() >> 4;
+                    const uint32_t bits = flag_s ? snan[t & 1][0][h] | snan[t & 1][1][h] << 8 : 0u;
 #pragma unroll
                     for (int q = 0; q < NQ; q++) {
                         const int mine = limit_of(q);
-                        kv_mask_range(s[q], page, none_s ? 0 : mine, max(0, mine - a.window), a.sinks, my_lane() >> 4);
+                        kv_set_nan(s[q], bits);
+                        kv_mask_range(s[q], page, none_p ? 0 : mine, max(0, mine - a.window), a.sinks, h);
                     }
-            } else if (none_s || (p + 1) * LTX_KV_PAGE > all)
+                }
+            } else {
+                if (flag_s) {
+                    const int h = my_lane() >> 4;
+                    const uint32_t bits = snan[t & 1][0][h] | snan[t & 1][1][h] << 8;
 #pragma unroll
-                for (int q = 0; q < NQ; q++) kv_mask(s[q], p, none_s ? 0 : limit_of(q), my_lane() >> 4);
+                    for (int q = 0; q < NQ; q++) kv_set_nan(s[q], bits);
+                }
+                if (none_s || (p + 1) * LTX_KV_PAGE > all)
+#pragma unroll
+                    for (int q = 0; q < NQ; q++) kv_mask(s[q], p, none_s ? 0 : limit_of(q), my_lane() >> 4);
+            }
 #pragma unroll
             for (int q = 0; q < NQ; q++) {
                 // weights with the maximum so far; only where a column's sum of them is

@@ -79,6 +79,10 @@ KV_FN KvRange kv_range(int window, int sinks, int e0, int e1) {
     return {ps, pw - ps, ps + np - pw};
 }
 KV_FN int kv_range_page(const KvRange& r, int u) { return u + (u >= r.ps ? r.skip : 0); }
+// the first u whose page is `page` or behind it
+KV_FN int kv_range_find(const KvRange& r, int page) {
+    return page < r.ps ? page : (int)kv_max(r.ps, (int64_t)page - r.skip);
+}
 KV_FN KvRange kv_tile_range(int window, int sinks, int causal, const KvSeq& s, int group, int t, int tile) {
     return kv_range(window, sinks, kv_limit(causal, s, (int)((int64_t)t * tile / group)),
                     kv_tile_limit(causal, s, group, t, tile));

@@ -425,6 +425,12 @@ static void window_index(unsigned seed) {
                     if (j >= (int64_t)e - window || j < sinks) want.insert(j / 64);
             }
             for (int u = 0; u < r.count; u++) got.insert(kv_range_page(r, u));
+            for (int page = 0; page <= kv_pages(s.L) + 1; page++) {  // the first u from that page on
+                int u = 0;
+                while (u < r.count && kv_range_page(r, u) < page) u++;
+                const int found = kv_range_find(r, page);
+                CHECK(u < r.count ? found == u : found >= r.count, "page %d: %d for %d", page, found, u);
+            }
             CHECK((int)got.size() == r.count, "pages twice");
             CHECK(got == want || (!all && std::includes(got.begin(), got.end(), want.begin(), want.end())), "%zu and %zu",
                   got.size(), want.size());
