@@ -103,19 +103,28 @@ struct AttnPlan {
 // cannot split (captured, without a workspace) takes 256 columns only where they fill
 // the CUs: 256 rows of 32 heads on 8 over 28,672 keys 235 us on 16 columns, 815 on 256.
 // A window of few pages leaves the wide tiles' starts and ends to count, which two
-// workgroups of 128 columns on a CU overlap. us on 128 / 256, causal: 32 heads on 8, 8,192
-// rows, windows of 300, 1,000, 2,000 and 3,000 keys 115 / 116, 192 / 189, 294 / 304, 374 /
-// 365; 32 heads, three times 4,096 rows 169 / 229, 313 / 352, 519 / 534, 699 / 706.
+// workgroups of 128 columns on a CU overlap, and the more so the more rows, each with its own
+// end, a tile has. us on 128 / 256, causal, windows of 300, 1,000, 2,000 and 3,000 keys: 32
+// heads on 8, 8,192 rows 97 / 107, 184 / 180, 287 / 281, 376 / 340; 32 heads, three times 4,096
+// rows 165 / 225, 328 / 342, 524 / 507, 718 / 663.
+// And there the 16 columns' higher cost of a page counts less than their filling of the CUs:
+// about (42 + 1.9 pages) us times the share of the CUs that 128 columns would fill, those 9.5 +
+// 1.4 pages. us on 16 / 128, 32 heads, windows of 300, 700, 1,400 and 2,000: 256 rows 15.5 / 15.8,
+// 18 / 25, 25 / 40, 30 / 55; 512 rows 27 / 17, 32 / 25, 44 / 41, 55 / 56; 768 rows 40 / 17, 47 / 27,
+// 63 / 43, 78 / 58.
 int tile_columns(const ltx_ctx* c, const ltx_kv_cache* k, const ltx_kv_batch* b, const AttnMask& m, int64_t columns,
                  bool split) {
     if (c->kv_tile) return c->kv_tile;
     const int64_t group = std::max<int64_t>(1, columns / std::max(b->rows, 1));
     const int64_t each = columns / b->nseq, wide = columns * k->kv_heads / 256;  // workgroups of 256 columns
-    const int64_t pages = wide * tile_pages(b, m, b->rows / b->nseq) / c->num_cu;  // of each, if split
-    if (each >= 192 && wide >= c->num_cu && !(m.window && tile_pages(b, m, 256 / group) <= 32)) return 256;
-    if (split && each >= 256 && pages >= 128) return 256;
-    if (each >= 64 && (each + 127) / 128 * b->nseq * k->kv_heads >= c->num_cu) return 128;
-    if (split && each >= 256 && pages >= 24) return 256;
+    const int64_t rows = std::min<int64_t>(256 / group, b->rows / b->nseq), width = tile_pages(b, m, rows);
+    const int64_t pages = wide * width / c->num_cu;  // of each, if split
+    if (each >= 192 && wide >= c->num_cu && !(m.window && width <= 12 + rows / 11)) return 256;
+    if (split && each >= 256 && wide < c->num_cu && pages >= 128) return 256;
+    const int64_t some = (each + 127) / 128 * b->nseq * k->kv_heads;  // workgroups of 128
+    if (each >= 64 && some >= c->num_cu) return 128;
+    if (m.window && each >= 128 && some * (90 + 4 * width) >= c->num_cu * (20 + 3 * width)) return 128;
+    if (split && each >= 256 && wide < c->num_cu && pages >= 24) return 256;
     return 16;
 }
 
