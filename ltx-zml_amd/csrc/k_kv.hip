@@ -736,7 +736,7 @@ KV_ATTN(ltx_kv_attn_bf16_win_nt, __bf16, true, true)
 // without branches 1,100, one straight block of products without spills 900, staging
 // before the softmax 840.
 // WIN: with a window, over the pages of the tile's range. 2,048 rows of 32 f16 heads that see
-// 12,288 of 28,672 keys 350 us, 1.18 PFLOP/s, as long as without a window for as many pages;
+// 12,288 of 28,672 keys 350 us, 1.18 PFLOP/s (360 without a window, as many pages);
 // causal, ragged prompts of up to 2,970 tokens, 701 keys, 32 heads on 8 125, of which 7 us a
 // workgroup are no pages.
 template <typename T, int NQ, bool SPLIT, bool WIN>
