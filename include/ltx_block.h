@@ -310,8 +310,9 @@ int ltx_op_mx4_values(ltx_ctx* ctx, const uint8_t* q, const uint8_t* scales, voi
  * mode, [M][K], which the call quantises on its way, with the bits of
  * ltx_op_mx4_quantise. y f32 (out_f32, and always in mode F32) or 16-bit. A group that is
  * NaN makes its row of y, or column, NaN. Calls may overlap and be captured. (More than 16
- * rows in values go through scratch of the context, as in ltx_op_attention: a call being
- * captured, or one that finds no memory, takes none, with the same bits, and longer.)
+ * rows and 2^17 values go through scratch of the context, as in ltx_op_attention: a call being
+ * captured, or one that finds no memory, takes none, and longer; the order of the f32 sums may
+ * differ then, as it does with M.)
  * Refused: M, N or K not positive, K no multiple of 128 or above 2^23, a or q not on 16
  * bytes, scales not on 4, bias or y not aligned to their types, an unknown mode, mode F32
  * with a in values, M or N times (K / 128 + 16) from 2^29 on, N from 2^21, more than 2^22

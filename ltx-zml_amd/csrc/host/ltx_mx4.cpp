@@ -128,12 +128,14 @@ int ltx_op_linear_mx4(ltx_ctx* c, const void* a, const uint8_t* a_scales, const 
         g.K = K;
         g.gelu = gelu != 0;
         g.out_f32 = out_f32 != 0;
-        // Rows in values: up to 16 are quantised by every workgroup that multiplies them, more
-        // once, by a launch of their own, into scratch. us, in the product / in a launch: 16
-        // rows of 4,096 x 4,096 7.4 / 7.3, 17 7.8 / 7.8, 64 18.5 / 8.8; 16 of 16,384 x 4,096
-        // 12.0 / 12.1, 33 17.3 / 11.7; 48 of 4,096 x 16,384 50 / 23.
+        // Rows in values: up to 16, and few values, are quantised by every workgroup that
+        // multiplies them, others once, by a launch of their own, into scratch (whose order
+        // behind other calls takes 3 us). us, in the product / in a launch: K = 1,024, N =
+        // 16,384, 17 rows 5.6 / 10.8, 64 10.8 / 11.3; K = 4,096, N = 4,096, 17 rows 8.1 / 11.9, 32
+        // 10.9 / 12.6, 48 15.2 / 13.8, 64 18.7 / 14.3, and N = 16,384 12.9 / 14.9, 16.3 / 15.2, 21.0
+        // / 16.5, 25.6 / 16.3; K = 16,384, N = 4,096, 17 rows 25 / 20, 64 65 / 27.
         ltx::ScratchUse use(c->op_scratch, st);
-        if (!a_scales && M > 16) {
+        if (!a_scales && M > 16 && (int64_t)M * K > 1 << 17) {
             const size_t codes = (size_t)M * K / 2;
             if (uint8_t* s = (uint8_t*)use.take(codes + (size_t)M * K / 32)) {
                 ltx::rows_call(c, true, (void*)a, K, s, s + codes, M, K, mode, st);

@@ -20,6 +20,7 @@ torch = pytest.importorskip("torch")
 pytestmark = pytest.mark.gpu
 
 from ltx_amd import runtime as rt  # noqa: E402
+from test_gpu_mx4 import streams  # noqa: E402
 
 MODES = {"f16": (rt.MODE_F16, torch.float16), "bf16": (rt.MODE_BF16, torch.bfloat16),
          "f32": (rt.MODE_F32, torch.float32)}
@@ -216,7 +217,7 @@ def test_captured_and_on_another_stream(ctx):
     graph = torch.cuda.CUDAGraph()
     with torch.cuda.graph(graph):
         ctx.qk_rope(r, pos, q, qo, k, ko, w, w, mode=rt.MODE_BF16)
-    st = torch.cuda.Stream()
+    st, = streams(1)
     for i in range(4):
         pos.copy_(torch.rand(70, 3, dtype=torch.float64, device="cuda") * 100 * i)
         ctx.qk_rope(r, pos, q, qo, k, ko, w, w, mode=rt.MODE_BF16)

@@ -19,6 +19,7 @@ pytestmark = pytest.mark.gpu
 
 from ltx_amd import runtime as rt  # noqa: E402
 from test_gpu_kv import HD, MODES, PAGE, SHAPES, Setup, any_tile, check, ints  # noqa: E402, F401
+from test_gpu_mx4 import streams  # noqa: E402
 
 
 class Windowed(Setup):
@@ -319,10 +320,10 @@ def test_strides_streams_and_captures(ctx):
     assert n > 0
     outs = [torch.zeros_like(out) for _ in range(4)]
     works = [torch.empty(n, dtype=torch.uint8, device="cuda") for _ in outs]
-    streams = [torch.cuda.Stream() for _ in outs]
+    sts = streams(len(outs))
     torch.cuda.synchronize()
     for _ in range(5):
-        for o, w, st in zip(outs, works, streams):
+        for o, w, st in zip(outs, works, sts):
             call(o, work=w, stream=st)
     torch.cuda.synchronize()
     for o in outs:
