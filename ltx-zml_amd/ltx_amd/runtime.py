@@ -445,7 +445,9 @@ class Context:
     # ---- microscaled 4-bit operands ----
     def mx4_quantise(self, x, q, s, mode=MODE_F16, stream=None):
         """x [rows, K] (rows may be strided) -> codes q uint8 [rows, K / 2] and scales s
-        uint8 [K / 128, rows, 4], which it returns (ltx_op_mx4_quantise)."""
+        uint8 [K / 128, rows, 4], which it returns (ltx_op_mx4_quantise). Here and below
+        torch's float4_e2m1fn_x2 and float8_e8m0fnu will do for codes and scales: the same
+        bytes."""
         st = stream.cuda_stream if stream is not None else _current_stream(self.device)
         rows, K, ld = self._mx4_rows("mx4_quantise", x, q, s, mode)
         self._check(lib().ltx_op_mx4_quantise(self.handle, x.data_ptr(), ld, q.data_ptr(), s.data_ptr(), rows, K, mode, st),
@@ -716,13 +718,24 @@ def _rows(name: str, batch: KvBatch, cache: KvCache, heads: int, *tensors):
             raise LtxError(f"{name}: {list(shape)} tensors of the cache's type are needed")
 
 
+def _mx4_bytes(t, own: str) -> bool:
+    """Whether t is of plain bytes, or of torch's own type for the same bytes."""
+    if t.element_size() != 1:
+        return False
+    if not t.is_floating_point():
+        return True
+    import torch
+    return t.dtype == getattr(torch, own, None)
+
+
 def _mx4_held(name: str, q, s, rows: int, K: int, device: int):
-    """Codes [rows, K / 2] and scales [K / 128, rows, 4], uint8."""
+    """Codes [rows, K / 2] and scales [K / 128, rows, 4], uint8 or float4_e2m1fn_x2 and float8_e8m0fnu."""
     if K % 128:
         raise LtxError(f"{name}: K must be a multiple of 128")
-    if not (q.shape == (rows, K // 2) and s.shape == (K // 128, rows, 4) and q.element_size() == 1 and s.element_size() == 1
-            and not (q.is_floating_point() or s.is_floating_point()) and q.is_contiguous() and s.is_contiguous()):
-        raise LtxError(f"{name}: contiguous uint8 tensors {[rows, K // 2]} and {[K // 128, rows, 4]} are needed")
+    if not (q.shape == (rows, K // 2) and s.shape == (K // 128, rows, 4) and _mx4_bytes(q, "float4_e2m1fn_x2")
+            and _mx4_bytes(s, "float8_e8m0fnu") and q.is_contiguous() and s.is_contiguous()):
+        raise LtxError(f"{name}: contiguous tensors {[rows, K // 2]} and {[K // 128, rows, 4]} of uint8, or of torch's "
+                       "float4_e2m1fn_x2 and float8_e8m0fnu, are needed")
     if not q.get_device() == s.get_device() == device:
         raise LtxError(f"{name}: tensors on the context's device are needed")
 

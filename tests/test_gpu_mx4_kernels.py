@@ -125,3 +125,26 @@ def test_long_k_by_the_rule(ctx, M, N, form):
     count = launched(ctx, lambda: ctx.linear_mx4(*qa, *qw, None, y))
     assert count(f"ltx_gemm_mx4_f16_{form}") >= 1 and count("") == 1
     right(y, want, tol)
+
+
+@pytest.mark.skipif(not hasattr(torch, "float4_e2m1fn_x2"), reason="torch has no 4-bit type")
+@pytest.mark.parametrize("M", [5, 90])
+def test_torchs_own_types(ctx, M):
+    """Codes and scales as torch's types for these bytes, out of rows and into a linear: the
+    same bits."""
+    say(f"linear_mx4 torch's types M={M}")
+    own = torch.float4_e2m1fn_x2, torch.float8_e8m0fnu
+    x, w = torch.randn(M, 256, device="cuda").half(), torch.randn(48, 256, device="cuda")
+    q, s = quantise(ctx, x, "f16")
+    qo, so = torch.zeros_like(q).view(own[0]), torch.zeros_like(s).view(own[1])
+    ctx.mx4_quantise(x, qo, so)
+    assert torch.equal(qo.view(torch.uint8), q) and torch.equal(so.view(torch.uint8), s)
+    a, b = torch.empty_like(x), torch.empty_like(x)
+    ctx.mx4_values(q, s, a)
+    ctx.mx4_values(qo, so, b)
+    assert torch.equal(a, b)
+    qw, sw = quantise(ctx, w, "f32")
+    y, z = torch.empty(M, 48, device="cuda"), torch.empty(M, 48, device="cuda")
+    ctx.linear_mx4(q, s, qw, sw, None, y)
+    ctx.linear_mx4(qo, so, qw.view(own[0]), sw.view(own[1]), None, z)
+    assert torch.equal(y, z)
