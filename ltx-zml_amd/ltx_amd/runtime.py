@@ -497,9 +497,12 @@ class Context:
         if f.ndim != 2 or f.shape[1] != 64:
             raise LtxError("rope: freq must be [heads, 64]")
         p = None if phase is None else np.ascontiguousarray(phase, np.float64)
-        x = None if axis is None else np.ascontiguousarray(axis, np.int32)
-        if any(t is not None and t.shape != f.shape for t in (p, x)):
+        a = np.zeros(f.shape, np.int32) if axis is None else np.asarray(axis)
+        if a.shape != f.shape or (p is not None and p.shape != f.shape):
             raise LtxError("rope: phase and axis must have freq's shape")
+        if not 1 <= axes <= 8 or not ((a >= 0) & (a < axes) & (a == np.floor(a))).all():
+            raise LtxError("rope: axes must be 1 .. 8, axis whole numbers of 0 .. axes - 1")
+        x = np.ascontiguousarray(a, np.int32)
         h = C.c_void_p()
         self._check(lib().ltx_rope_create(self.handle, f.shape[0], axes, _ptr(f), _ptr(p), _ptr(x), C.byref(h)),
                     "ltx_rope_create")
@@ -592,7 +595,7 @@ class Context:
                                       causal: bool = True) -> int:
         """Bytes of `work` for kv_attention_window with this batch's nseq, rows and max_pages."""
         n = C.c_uint64()
-        window, sinks = (min(x, 1 << 30) for x in (window, sinks))  # no table holds more keys
+        window, sinks = _keys(window), _keys(sinks)
         self._check(lib().ltx_op_kv_attention_window_workspace(self.handle, cache.handle, batch.ref, heads, int(causal),
                                                                window, sinks, C.byref(n)),
                     "ltx_op_kv_attention_window_workspace")
@@ -604,7 +607,7 @@ class Context:
         `sinks` (ltx_op_kv_attention_window)."""
         st = stream.cuda_stream if stream is not None else _current_stream(self.device)
         self._kv_attention_checks("kv_attention_window", cache, batch, q, out, heads, glog, work)
-        window, sinks = (min(x, 1 << 30) for x in (window, sinks))  # no table holds more keys
+        window, sinks = _keys(window), _keys(sinks)
         self._check(lib().ltx_op_kv_attention_window(self.handle, cache.handle, batch.ref, _ptr(q), q.stride(0), heads,
                                                      int(causal), window, sinks, _ptr(glog), _ptr(out), out.stride(0),
                                                      _ptr(work), 0 if work is None else work.numel() * work.element_size(),
@@ -716,6 +719,11 @@ def _rows(name: str, batch: KvBatch, cache: KvCache, heads: int, *tensors):
             raise LtxError(f"{name}: tensors on the context's device are needed")
         if t.shape != shape or t.dtype != dt or t.stride(1) != 1:
             raise LtxError(f"{name}: {list(shape)} tensors of the cache's type are needed")
+
+
+def _keys(n: int) -> int:
+    """A count of keys within 32 bits: no table holds more than 2^30, and less than 0 is refused."""
+    return max(-1, min(n, 1 << 30))
 
 
 def _mx4_bytes(t, own: str) -> bool:

@@ -1,0 +1,63 @@
+"""Numbers that the bindings of rotary plans and windowed attention hand on, without a GPU:
+what 32 bits do not hold is refused or limited, not wrapped."""
+import ctypes as C
+import types
+
+import numpy as np
+import pytest
+
+torch = pytest.importorskip("torch")
+
+from ltx_amd import runtime as rt  # noqa: E402
+
+
+@pytest.fixture
+def calls(monkeypatch):
+    """A context on the host whose library notes the calls that it gets: (name, arguments)."""
+    seen = []
+
+    class Lib:
+        def __getattr__(self, name):
+            def call(*args):
+                seen.append((name, args))
+                return 1
+            return call
+    monkeypatch.setattr(rt, "lib", lambda: Lib())
+    ctx = rt.Context.__new__(rt.Context)
+    ctx.handle, ctx.device = 1, -1
+    ctx._graphs, ctx._caches, ctx._ropes = set(), set(), set()
+    yield ctx, seen
+    ctx._ropes.clear()
+    ctx.handle = None
+
+
+@pytest.mark.parametrize("window,sinks", [(5, 3), (2 ** 31 + 7, 2 ** 40), (-(2 ** 32) + 5, 0), (7, -(2 ** 32) + 5), (0, -1),
+                                          (2 ** 32 + 5, 2 ** 32 + 1)])
+def test_windows_beyond_32_bits(calls, window, sinks):
+    """What the library is asked has the same sign, and more keys than a table holds stay more."""
+    ctx, seen = calls
+    kv = torch.zeros(1, dtype=torch.int32)
+    batch = rt.KvBatch(kv, kv[None])
+    cache = types.SimpleNamespace(handle=1, mode=rt.MODE_F16, ctx=ctx)
+    q = torch.zeros(1, 128, dtype=torch.float16)
+    ctx.kv_attention_window_workspace(cache, batch, 1, window, sinks)
+    ctx.kv_attention_window(cache, batch, q, q, 1, window, sinks, stream=types.SimpleNamespace(cuda_stream=0))
+    asked = [a[5:7] for n, a in seen if n.endswith("workspace")] + [a[7:9] for n, a in seen if n.endswith("window")]
+    assert len(asked) == 2
+    for pair in asked:
+        for want, got in zip((window, sinks), pair):
+            got = C.c_int32(got).value
+            assert got == want if abs(want) <= 2 ** 30 else got >= 2 ** 30 if want > 0 else got < 0
+
+
+def test_plans_beyond_32_bits(calls):
+    ctx, seen = calls
+    freq = np.ones((2, 64))
+    for bad in [dict(axes=2 ** 32 + 1), dict(axes=-(2 ** 32) + 2), dict(axis=np.full((2, 64), 2 ** 32)),
+                dict(axis=np.full((2, 64), 0.5)), dict(axis=np.full((2, 64), np.nan))]:
+        with pytest.raises(rt.LtxError):
+            ctx.rope(freq, **dict(dict(axes=2), **bad))
+    assert not seen
+    for axis in (None, np.ones((2, 64)), np.ones((2, 64), np.int64), torch.ones(2, 64, dtype=torch.int32)):
+        ctx.rope(freq, axis=axis, axes=2).handle = None
+    assert len(seen) == 4
