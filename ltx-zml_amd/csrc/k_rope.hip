@@ -90,6 +90,31 @@ __device__ __forceinline__ void rope_sums(float& x, float& y, float (*red)[2]) {
     y = red[0][1] + red[1][1] + red[2][1] + red[3][1];
 }
 
+// A normed row is multiplied by 1 / sqrt(mean square + eps). Sums of squares are f32's; where that
+// leaves it (f16's never do), the row's mean square is formed again in f64, and the row multiplied
+// by a power of two near the root's inverse (`first`), then by the rest of it. `ms`: the same for
+// the whole workgroup. What this costs where no row needs it: nothing up to 32 heads (28,672 rows of
+// 32 + 32 bf16 heads 207 us with and without), beyond between 5 % (40 + 8 bf16 heads 468 -> 491)
+// and -3 % (48 + 48 f32 heads, 14,336 rows, 625 -> 605).
+template <typename T>
+__device__ __forceinline__ bool rope_far(float ms) {
+    return !__is_same(T, _Float16) && !(ms >= 0x1p-90f && ms <= __FLT_MAX__);
+}
+__device__ __forceinline__ float rope_far_factor(double sum, int n, float eps, float& first) {
+    const double root = sqrt(sum / (double)n + (double)eps);
+    const int e = -__builtin_amdgcn_frexp_exp(root), near = min(max(e, -126), 126);
+    first = ldexpf(1.f, near);
+    return ldexpf((float)(1.0 / __builtin_amdgcn_frexp_mant(root)), e - near);
+}
+// The sum over the workgroup of each thread's x.
+__device__ __forceinline__ double rope_far_sum(double x, double* red) {
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) x += __shfl_xor(x, o, 64);
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = x;
+    __syncthreads();
+    return red[0] + red[1] + red[2] + red[3];
+}
+
 // The sum over a wave's lanes, for all of them.
 __device__ __forceinline__ float rope_wave_sum(float x) {
     auto add = [&](auto C, auto M) {
@@ -120,6 +145,7 @@ template <typename T, bool NORM>
 __device__ __forceinline__ void qk_rope_rows(const LtxRopeArgs& a) {
     __shared__ double spos[4][2][8];
     __shared__ float red[2][4][2];
+    __shared__ double far[2][4];
     __shared__ f32x4 wt[NORM ? 2 : 1][4][256];  // a thread's own weights: in registers they cost a third of the waves
     const int h0 = threadIdx.x >> 3, o = threadIdx.x & 7, lane = threadIdx.x & 63, w = threadIdx.x >> 6;
     const int big = a.heads[1] > a.heads[0], ratio = a.heads[!big] ? a.heads[big] / a.heads[!big] : 1;
@@ -178,9 +204,26 @@ __device__ __forceinline__ void qk_rope_rows(const LtxRopeArgs& a) {
             __syncthreads();
 #pragma unroll
             for (int m = 0; m < 2; m++) {
-                if (!mine[m] || !a.norm[m ^ big]) continue;
+                if (!a.norm[m ^ big]) continue;
                 const float all = red[row & 1][0][m] + red[row & 1][1][m] + red[row & 1][2][m] + red[row & 1][3][m];
-                const float inv = 1.0f / sqrtf(all / (float)(LTX_HD * a.heads[m ^ big]) + a.eps);
+                const float ms = all / (float)(LTX_HD * a.heads[m ^ big]) + a.eps;
+                float inv = 1.0f / sqrtf(ms);
+                if (rope_far<T>(ms)) {
+                    double sum = 0;
+                    if (mine[m])
+#pragma unroll
+                        for (int j = 0; j < 16; j++) {
+                            const double x = v[m][j >> 3][j & 7];
+                            sum = __builtin_fma(x, x, sum);
+                        }
+                    float first;
+                    // (the next row's sums come behind its barrier above)
+                    inv = rope_far_factor(rope_far_sum(sum, far[m]), LTX_HD * a.heads[m ^ big], a.eps, first);
+                    if (mine[m])
+#pragma unroll
+                        for (int j = 0; j < 16; j++) v[m][j >> 3][j & 7] *= first;
+                }
+                if (!mine[m]) continue;
 #pragma unroll
                 for (int j = 0; j < 4; j++) {
                     const f32x4 n = wt[m][j][threadIdx.x];
@@ -210,11 +253,12 @@ __device__ __forceinline__ void qk_rope_rows(const LtxRopeArgs& a) {
 template <typename T>
 __device__ __forceinline__ void qk_rope(const LtxRopeArgs& a) {
     __shared__ float red[2][4][2];
+    __shared__ double far[2][4];
     const int h0 = threadIdx.x >> 3, o = threadIdx.x & 7, at = 8 * o;
     const int row0 = blockIdx.x * a.per, end = min(a.rows, row0 + a.per);
     for (int row = row0; row < end; row++) {
         const double* pos = a.pos + (size_t)row * a.axes;
-        float inv[2] = {1.f, 1.f};
+        float inv[2] = {1.f, 1.f}, first[2] = {1.f, 1.f};
         if (a.norm[0] || a.norm[1]) {
             float sum[2] = {0.f, 0.f};
 #pragma unroll
@@ -233,7 +277,25 @@ __device__ __forceinline__ void qk_rope(const LtxRopeArgs& a) {
                     }
             rope_sums(sum[0], sum[1], red[row & 1]);
 #pragma unroll
-            for (int m = 0; m < 2; m++) inv[m] = 1.0f / sqrtf(sum[m] / (float)(LTX_HD * max(a.heads[m], 1)) + a.eps);
+            for (int m = 0; m < 2; m++) {
+                const int n = LTX_HD * max(a.heads[m], 1);
+                const float ms = sum[m] / (float)n + a.eps;
+                inv[m] = 1.0f / sqrtf(ms);
+                if (!a.norm[m] || !rope_far<T>(ms)) continue;
+                double all = 0;
+                for (int h = h0; h < a.heads[m]; h += 32) {
+                    RopeRow<T> x[2];
+                    const size_t i = (size_t)row * a.ldx[m] + LTX_HD * h + at;
+                    x[0].load(a.x[m], i);
+                    x[1].load(a.x[m], i + 64);
+#pragma unroll
+                    for (int j = 0; j < 16; j++) {
+                        const double y = x[j >> 3].get(j & 7);
+                        all = __builtin_fma(y, y, all);
+                    }
+                }
+                inv[m] = rope_far_factor(rope_far_sum(all, far[m]), n, a.eps, first[m]);
+            }
         }
 #pragma unroll
         for (int m = 0; m < 2; m++)
@@ -250,6 +312,10 @@ __device__ __forceinline__ void qk_rope(const LtxRopeArgs& a) {
                 for (int j = 0; j < 8; j++) {
                     float x = lo.get(j), y = hi.get(j);
                     if (a.norm[m]) {
+                        if (!__is_same(T, _Float16)) {
+                            x *= first[m];
+                            y *= first[m];
+                        }
                         x *= inv[m] * a.norm[m][LTX_HD * h + at + j];
                         y *= inv[m] * a.norm[m][LTX_HD * h + at + 64 + j];
                     }
