@@ -382,8 +382,9 @@ struct AttnPP {
     // Group 0 (waves 0-3) issues every DMA: wave w fills its own 2 KB slice
     // of a stage and that of wave w + 4 (8 KB further, K rows + 32 = keys
     // + 32, V^T rows + 64), 4 instructions per K or V tile.
-    // K rows past the last repeat it where the tile may be the last one (CLAMP;
-    // the scalar offset takes no part in the buffer's range check).
+    // K rows past the last repeat it where the tile may be the last one (CLAMP:
+    // the whole offset is the lane's then, so that it can be limited. The buffer's
+    // range check, which takes the scalar offset in, would give zeros).
     template <bool CLAMP>
     __device__ __forceinline__ void dma_k1(uint8_t* d, int t, int h, int i) {
         const uint32_t o = (uint32_t)(64 * t + 32 * h) * kr;

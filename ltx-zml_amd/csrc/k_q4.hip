@@ -33,8 +33,9 @@ __device__ __forceinline__ u32x4 q4_operand(uint32_t w) {
 
 // Operands come through buffer resources that begin at the workgroup's first row:
 // rows past the last read as zeros without an access. The group goes into the scalar
-// offset, which takes no part in that check; for a group that is not there the
-// resource is empty instead. So the loads need no branch and no vector arithmetic.
+// offset; one that is not there would lie in the next row for that check (which takes
+// both offsets in), so the resource is empty then. So the loads need no branch and no
+// vector arithmetic.
 typedef __amdgpu_buffer_rsrc_t q4_rsrc;
 struct Q4Buffer {
     const void* base;
