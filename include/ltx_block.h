@@ -343,9 +343,10 @@ void ltx_rope_free(ltx_ctx* ctx, ltx_rope* rope);
  * k_out, which may be q and k themselves (same address and stride), and overlap nothing
  * else. q_norm, k_norm [heads * 128] f32 or NULL: each row is first divided by sqrt(mean of
  * its squares + eps) and multiplied by these weights. Then head h's pairs turn as head h /
- * (heads / plan heads) of the plan says, by pos [rows][axes] f64 (device memory): exact far
- * into a stream, where f32 is not, for angles below 2^51 quarter turns. -pos turns back
- * where phases are 0. f32 sums (f64 for a row whose squares leave f32) and products, one
+ * (heads / plan heads) of the plan says, by pos [rows][axes] f64 (device memory). Angles are
+ * f64: off by at most 2^-51 of |freq pos| + |phase|, which is below f32's rounding of the
+ * result up to 10^8 radians; they must stay below 2^51 quarter turns. -pos turns back where
+ * phases are 0. f32 sums (f64 for a row whose squares leave f32) and products, one
  * rounding to the mode's type, to infinity beyond its largest; a row with a position that is not finite is NaN in the pairs on its
  * axis. rows may be 0. Refused: heads no multiples of the plan's, rows of q, k or their
  * outputs not on 16 bytes or shorter than their heads, pos not on 8 bytes, weights not on
