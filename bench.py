@@ -48,9 +48,8 @@ def log(msg: str) -> None:
 
 def mfma_ceiling():
     """The practical MFMA rate of this GPU, measured beside the benchmark by
-    ltx-zml_amd/mfma_ceiling (a child process): v_mfma_f32_32x32x16 loops on
-    random f16 / bf16 operands, A from registers or from one LDS read per
-    MFMA. The board's power limit holds these well below the published
+    ltx-zml_amd/mfma_ceiling (a child process): MFMA loops on random f16,
+    bf16 and 4-bit operands, A from registers or from LDS. The board's power limit holds these well below the published
     dense peak; None when the tool is not built."""
     exe = ROOT / "ltx-zml_amd" / "mfma_ceiling"
     if not exe.exists():

@@ -2,7 +2,8 @@
 // the form of ltx_args.h, on v_mfma_scale_f32_32x32x64_f8f6f4: a lane's operand is a group
 // of 32 codes (16 bytes) and its scale, which the instruction applies, so nothing is
 // unpacked. f32 accumulation. (From registers and on random operands 32 x 32 x 64 runs at
-// 6.5 PFLOP/s, 16 x 16 x 128 at 5.1; with an LDS read for every two of the former, 5.7.)
+// 6.4 PFLOP/s, 16 x 16 x 128 at 7.2; with an LDS read for every two products 5.7 and 5.5, twice
+// the reads a flop in the latter: csrc/tools/mfma_ceiling.hip.)
 //
 // Workgroup: 4 waves in a 2 x 2 grid, output tile 64 NB x 64 NB, a wave NB x NB blocks of
 // 32 x 32. K goes in tiles of 256 (128 bytes of a row) through LDS by LDS DMA in two stages,
