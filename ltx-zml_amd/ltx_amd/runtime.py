@@ -488,7 +488,7 @@ class Context:
         if x.dtype != _torch_dtype(mode) or unit != 1 or x.get_device() != self.device:
             raise LtxError(f"{name}: rows of the mode's type on the context's device are needed")
         _mx4_held(name, q, s, rows, K, self.device)
-        return rows, K, ld
+        return rows, K, ld if rows > 1 else K
 
     # ---- rotary positions on several axes ----
     def rope(self, freq, phase=None, axis=None, axes: int = 1) -> Rope:
@@ -537,7 +537,7 @@ class Context:
                 raise LtxError("qk_rope: norm weights must be f32, one for each value of a row")
             if not (x.get_device() == device and y.get_device() == device and (w is None or w.get_device() == device)):
                 raise LtxError("qk_rope: tensors on the context's device are needed")
-            return sx[0], sy[0], shape[1] // 128
+            return *((sx[0], sy[0]) if rows > 1 else 2 * (shape[1],)), shape[1] // 128
 
         ql = strides(q, q_out, q_norm)
         kl = (0, 0, 0) if k is None else strides(k, k_out, k_norm)
@@ -561,15 +561,15 @@ class Context:
         """k, v [rows, kv_heads * 128] (rows may be strided) -> the cache (ltx_op_kv_write)."""
         st = stream.cuda_stream if stream is not None else _current_stream(self.device)
         _rows("kv_write", batch, cache, cache.kv_heads, k, v)
-        self._check(lib().ltx_op_kv_write(self.handle, cache.handle, batch.ref, _ptr(k), k.stride(0), _ptr(v),
-                                          v.stride(0), st), "ltx_op_kv_write")
+        self._check(lib().ltx_op_kv_write(self.handle, cache.handle, batch.ref, _ptr(k), _ld(k), _ptr(v),
+                                          _ld(v), st), "ltx_op_kv_write")
 
     def kv_read(self, cache: KvCache, batch: KvBatch, k, v, stream=None):
         """What the cache holds of the batch's rows -> k, v (ltx_op_kv_read)."""
         st = stream.cuda_stream if stream is not None else _current_stream(self.device)
         _rows("kv_read", batch, cache, cache.kv_heads, k, v)
-        self._check(lib().ltx_op_kv_read(self.handle, cache.handle, batch.ref, _ptr(k), k.stride(0), _ptr(v),
-                                         v.stride(0), st), "ltx_op_kv_read")
+        self._check(lib().ltx_op_kv_read(self.handle, cache.handle, batch.ref, _ptr(k), _ld(k), _ptr(v),
+                                         _ld(v), st), "ltx_op_kv_read")
 
     def kv_attention_workspace(self, cache: KvCache, batch: KvBatch, heads: int) -> int:
         """Bytes of `work` for kv_attention with this batch's nseq, rows and max_pages."""
@@ -585,8 +585,8 @@ class Context:
         (ltx_op_kv_attention)."""
         st = stream.cuda_stream if stream is not None else _current_stream(self.device)
         self._kv_attention_checks("kv_attention", cache, batch, q, out, heads, glog, work)
-        self._check(lib().ltx_op_kv_attention(self.handle, cache.handle, batch.ref, _ptr(q), q.stride(0), heads,
-                                              int(causal), _ptr(glog), _ptr(out), out.stride(0), _ptr(work),
+        self._check(lib().ltx_op_kv_attention(self.handle, cache.handle, batch.ref, _ptr(q), _ld(q), heads,
+                                              int(causal), _ptr(glog), _ptr(out), _ld(out), _ptr(work),
                                               0 if work is None else work.numel() * work.element_size(), st),
                     "ltx_op_kv_attention")
         return out
@@ -608,8 +608,8 @@ class Context:
         st = stream.cuda_stream if stream is not None else _current_stream(self.device)
         self._kv_attention_checks("kv_attention_window", cache, batch, q, out, heads, glog, work)
         window, sinks = _keys(window), _keys(sinks)
-        self._check(lib().ltx_op_kv_attention_window(self.handle, cache.handle, batch.ref, _ptr(q), q.stride(0), heads,
-                                                     int(causal), window, sinks, _ptr(glog), _ptr(out), out.stride(0),
+        self._check(lib().ltx_op_kv_attention_window(self.handle, cache.handle, batch.ref, _ptr(q), _ld(q), heads,
+                                                     int(causal), window, sinks, _ptr(glog), _ptr(out), _ld(out),
                                                      _ptr(work), 0 if work is None else work.numel() * work.element_size(),
                                                      st), "ltx_op_kv_attention_window")
         return out
@@ -707,6 +707,11 @@ def _torch_dtype(mode: int):
         import torch
         _DTYPES.update({MODE_F16: torch.float16, MODE_BF16: torch.bfloat16, MODE_F32: torch.float32})
     return _DTYPES.get(mode)
+
+
+def _ld(t) -> int:
+    """Elements from a row to the next: the length of one that is alone, whose stride says nothing."""
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
 
 
 def _rows(name: str, batch: KvBatch, cache: KvCache, heads: int, *tensors):

@@ -61,3 +61,34 @@ def test_plans_beyond_32_bits(calls):
     for axis in (None, np.ones((2, 64)), np.ones((2, 64), np.int64), torch.ones(2, 64, dtype=torch.int32)):
         ctx.rope(freq, axis=axis, axes=2).handle = None
     assert len(seen) == 4
+
+
+def test_one_row_has_no_stride(calls):
+    """A single row's stride says nothing (that of a transposed column is 1): its length is handed on."""
+    ctx, seen = calls
+    st = types.SimpleNamespace(cuda_stream=0)
+
+    def row(n, dt=torch.float16):
+        t = torch.zeros(n, 1, dtype=dt).T
+        assert t.stride() == (1, 1)
+        return t
+    u8 = dict(dtype=torch.uint8)
+    q, s = torch.zeros(1, 128, **u8), torch.zeros(2, 1, 4, **u8)
+    ctx.mx4_quantise(row(256), q, s, stream=st)
+    ctx.mx4_values(q, s, row(256), stream=st)
+    plan = types.SimpleNamespace(handle=1, axes=1)
+    ctx.qk_rope(plan, torch.zeros(1, 1, dtype=torch.float64), row(256), row(256), row(128), row(128), stream=st)
+    kv = torch.zeros(1, dtype=torch.int32)
+    batch = rt.KvBatch(kv, kv[None])
+    cache = types.SimpleNamespace(handle=1, mode=rt.MODE_F16, ctx=ctx, kv_heads=2)
+    ctx.kv_write(cache, batch, row(256), row(256), stream=st)
+    ctx.kv_read(cache, batch, row(256), row(256), stream=st)
+    ctx.kv_attention(cache, batch, row(256), row(256), 2, stream=st)
+    ctx.kv_attention_window(cache, batch, row(256), row(256), 2, 9, stream=st)
+    where = {"ltx_op_mx4_quantise": (2,), "ltx_op_mx4_values": (4,), "ltx_op_qk_rope": (5, 8, 11, 14),
+             "ltx_op_kv_write": (4, 6), "ltx_op_kv_read": (4, 6), "ltx_op_kv_attention": (4, 9),
+             "ltx_op_kv_attention_window": (4, 11)}
+    assert {n for n, _ in seen} == set(where)
+    for name, args in seen:
+        widths = [128 if (name, i) in {("ltx_op_qk_rope", 11), ("ltx_op_qk_rope", 14)} else 256 for i in where[name]]
+        assert [args[i] for i in where[name]] == widths, name
