@@ -61,6 +61,10 @@ struct Mx4Form {
 // K = 16,384, N = 4,096: 16 rows 12 / 22 / 17 / 41 / 32, 64 26 / 23 / 19 / 42 / 33, 256 - / 24 /
 // 21 / 44 / 35, 512 - / 31 / 39 / 44 / 35, 2,970 - / 165 / 220 / 114 / 123 / 96; K = 1,024, 64
 // rows 4.0 / 3.6 / 4.7 / 5.2 / 5.2.
+// Rows of y that do not start on 16 bytes (`odd`) have one form, 128 x 128 with narrow stores,
+// whatever the sizes: the others exist for whole 16-byte stores only. us at N = 4,097 / 4,104, f16:
+// K = 4,096, 64 rows 12.5 / 6.3, 300 19.3 / 11.1, 2,048 56 / 34, 28,672 478 / 238; K = 16,384, 64
+// rows 45 / 20, 300 51 / 30, 2,048 133 / 112.
 Mx4Form mx4_form(const ltx_ctx* c, int64_t M, int64_t N, int K, bool rows, bool odd) {
     auto tiles = [&](int64_t t) { return (M + t - 1) / t * ((N + t - 1) / t); };
     const int64_t cu = c->num_cu;
@@ -133,7 +137,8 @@ int ltx_op_linear_mx4(ltx_ctx* c, const void* a, const uint8_t* a_scales, const 
         // behind other calls takes 3 us). us, in the product / in a launch: K = 1,024, N =
         // 16,384, 17 rows 5.6 / 10.8, 64 10.8 / 11.3; K = 4,096, N = 4,096, 17 rows 8.1 / 11.9, 32
         // 10.9 / 12.6, 48 15.2 / 13.8, 64 18.7 / 14.3, and N = 16,384 12.9 / 14.9, 16.3 / 15.2, 21.0
-        // / 16.5, 25.6 / 16.3; K = 16,384, N = 4,096, 17 rows 25 / 20, 64 65 / 27.
+        // / 16.5, 25.6 / 16.3; K = 16,384, N = 4,096, 17 rows 25 / 20, 64 65 / 27. (N is not in the
+        // rule: its worst case among these, 32 rows of 16,384 x 4,096, is 7 % slower than a launch.)
         ltx::ScratchUse use(c->op_scratch, st);
         if (!a_scales && M > 16 && (int64_t)M * K > 1 << 17) {
             const size_t codes = (size_t)M * K / 2;
